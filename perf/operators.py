@@ -5,8 +5,8 @@ key/value cache with the position rotation, and attention over such a cache.
 
 Cache pages.  A cache is one tensor of pages; sequence b keeps its entry n in page ``page_table[b, n // page]``, slot
 ``n % page``.  16 bits: ``[pages, kv_heads, 2, page, dim]`` (keys, then values).  4 bits: uint8 ``[pages, kv_heads,
-page * (dim + dim / 4)]``: key codes ``[page, dim / 2]``, value codes, then for keys and for values bf16 (step, low)
-``[page, dim / 32, 2]``; a value is ``low + step * code``, dimension 2 j in the low half of byte j.
+page, dim + dim / 4]``, of which each kv head's bytes are key codes ``[page, dim / 2]``, value codes, then for keys and
+for values bf16 (step, low) ``[page, dim / 32, 2]``; a value is ``low + step * code``, dimension 2 j in the low half of byte j.
 """
 
 import math
@@ -148,11 +148,10 @@ def _packed_bytes(codes):
 def _parts(data, page, dim):
     """Views of a 4-bit cache: key codes, value codes, key (step, low), value (step, low)."""
     n, g = page * dim // 2, page * dim // GROUP * 4
-    lead = data.shape[:-1]
+    data = data.flatten(-2)
     codes = [data[..., i * n : (i + 1) * n].unflatten(-1, (page, dim // 2)) for i in (0, 1)]
     pairs = [data[..., 2 * n + i * g : 2 * n + (i + 1) * g].view(torch.bfloat16).unflatten(-1, (page, dim // GROUP, 2))
              for i in (0, 1)]
-    assert codes[0].shape[:-2] == lead
     return codes + pairs
 
 
@@ -163,7 +162,7 @@ def _cache(case, gen, pages):
         data[:, :, 0] = _rows(gen, pages * hkv, page, dim, outliers=True).view(pages, hkv, page, dim).to(dtype)
         data[:, :, 1] = _rows(gen, pages * hkv, page, dim).view(pages, hkv, page, dim).to(dtype)
         return data
-    data = torch.empty(pages, hkv, page * (dim + dim // 4), dtype=torch.uint8, device="cuda")
+    data = torch.empty(pages, hkv, page, dim + dim // 4, dtype=torch.uint8, device="cuda")
     parts = _parts(data, page, dim)
     for i in (0, 1):
         x = _rows(gen, pages * hkv, page, dim, outliers=i == 0).view(pages, hkv, page, dim)
@@ -400,7 +399,7 @@ def _exact_rows(case, cache, pages, count):
     head = torch.arange(hkv, device="cuda")
     if case["bits"] == 16:
         return cache[at, head, 0, slot].double(), cache[at, head, 1, slot].double()
-    both, codes = [], page * dim // 2
+    both, codes, cache = [], page * dim // 2, cache.flatten(-2)
     for i in (0, 1):
         first = i * codes + slot * (dim // 2)
         raw = cache[at[..., None], head[:, None], first[..., None] + torch.arange(dim // 2, device="cuda")]
