@@ -296,6 +296,84 @@ int32_t svla_fused_rope_attention_f32_mask_implicit_pos(const float* q_raw, cons
                                                         svla_stream_t stream);
 
 /* -------------------------------------------------------------------------------------------------
+ * Serving: prompts of different lengths packed back to back, and a cache made of pages.  No counterpart in the
+ * reference, whose engine holds one prompt of fixed length and a dense cache per call
+ * (deploy/trt_sample_actions_core_deploy.py:108-237).
+ *
+ * Packed tensors are [rows, heads * head_dim] with a row stride (elements, a multiple of 8, rows 16-byte aligned):
+ * sequence b owns rows cu[b] .. cu[b + 1] - 1 of a non-decreasing int32 [batch + 1]; rows behind cu[batch] are neither
+ * read nor written.  head_dim 64 or 128; dtype SVLA_DT_BF16 or SVLA_DT_HALF; query head h reads kv head
+ * h / (hq / hkv).  A query with no key to see gives zeros.
+ *
+ * Cache pages (page_size a multiple of 16, 16 to 256): entry n of sequence b is slot n % page_size of page
+ * page_table[b, n / page_size].  bits 16: [n_pages, hkv, 2, page_size, head_dim] of the dtype (keys, values).  bits 4:
+ * bytes [n_pages, hkv][page_size * (head_dim + head_dim / 4)]: key codes [page_size, head_dim / 2], value codes, then for
+ * keys and for values bf16 (step, low) pairs [page_size, head_dim / 32]; an entry is low + step * code, dimension 2 j in
+ * the low half of byte j.  An index outside the table or a page outside the cache is neither written nor read, and
+ * device error 104 is recorded (svla_device_error).
+ * ------------------------------------------------------------------------------------------------*/
+
+/* cs[p][i] = (cos, sin)(p / max_wavelength^(2 i / head_dim)), p < max_pos, i < head_dim / 2, from angles in 64 bits
+ * (svla_rope_table keeps the reference's fp32 angles, which far positions outgrow).  cs 16-byte aligned. */
+int32_t svla_rope_table_wide(float* cs, int32_t max_pos, int32_t head_dim, double max_wavelength, svla_stream_t stream);
+
+/* Appends the new tokens' keys and values to a paged cache, rotated on the way; token i of the n_b new ones of
+ * sequence b becomes entry kv_len[b] - n_b + i (kv_len counts them).  With rope_cs ([max_pos][head_dim / 2] (cos, sin),
+ * svla_rope_table_wide) keys and, if given, queries are rotated (rotate-half, fp32) at position pos[t], or the entry's
+ * index without pos; positions are clamped to 0 .. max_pos - 1.  4 bits, per 32 dimensions: low = bf16(min), step =
+ * bf16((max - min) / 15), code = round((x - low) / step) clamped to 0 .. 15; a group with an infinity or a NaN reads
+ * back as NaN.  k_out / v_out (or NULL): the appended rows as the cache holds them, rounded to the dtype, packed like
+ * k / v.  q_out, k_out, v_out may alias q, k, v.  Two tokens must not share an entry. */
+typedef struct svla_kv_append_desc {
+  const void* q; const void* k; const void* v;   /* packed; q may be NULL */
+  void* q_out; void* k_out; void* v_out;
+  void* cache;
+  const int32_t* cu_q;        /* [batch + 1] */
+  const int32_t* kv_len;      /* [batch] */
+  const int32_t* page_table;  /* [batch, page_table_rs], the first max_pages columns */
+  const int32_t* pos;         /* [total_q] or NULL */
+  const float* rope_cs;       /* or NULL: no rotation */
+  int64_t q_rs, k_rs, v_rs, q_out_rs, k_out_rs, v_out_rs, page_table_rs;
+  int32_t batch, total_q, hq, hkv, head_dim, dtype;
+  int32_t bits, page_size, n_pages, max_pages, max_pos;
+} svla_kv_append_desc;
+
+int32_t svla_kv_append(const svla_kv_append_desc* desc, svla_stream_t stream);
+
+/* Attention over packed prompts: query i of sequence b (n_q queries, n_k keys) sees key j iff !causal or
+ * j <= n_k - n_q + i.  What stands outside a sequence never enters its results.  Every total fits 31 bits. */
+typedef struct svla_packed_attn_desc {
+  const void* q; const void* k; const void* v;
+  void* o;
+  const int32_t* cu_q; const int32_t* cu_k;  /* [batch + 1] */
+  int64_t q_rs, k_rs, v_rs, o_rs;
+  int32_t batch, total_q, total_k;           /* rows of q / o and of k / v */
+  int32_t hq, hkv, head_dim, dtype, causal;  /* hq / hkv <= 64 */
+  float scale;                               /* 0 = head_dim^-1/2 */
+} svla_packed_attn_desc;
+
+int32_t svla_packed_attention(const svla_packed_attn_desc* desc, svla_stream_t stream);
+
+/* Attention of a few new tokens per sequence (one, or several drafted ones) over a paged cache: query i of the n_b new
+ * ones sees entries n <= kv_len[b] - n_b + i, so the tokens themselves are appended first (svla_kv_append).  The
+ * workspace (256-byte aligned, at least svla_paged_attention_workspace_size bytes) needs no initialisation; calls that
+ * overlap on the GPU must not share one. */
+size_t svla_paged_attention_workspace_size(int32_t batch, int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim);
+
+typedef struct svla_paged_attn_desc {
+  const void* q; const void* cache;
+  void* o;
+  const int32_t* cu_q; const int32_t* kv_len; const int32_t* page_table;
+  void* workspace; size_t workspace_bytes;
+  int64_t q_rs, o_rs, page_table_rs;
+  int32_t batch, total_q, hq, hkv, head_dim, dtype;
+  int32_t bits, page_size, n_pages, max_pages;
+  float scale;                               /* 0 = head_dim^-1/2 */
+} svla_paged_attn_desc;
+
+int32_t svla_paged_attention(const svla_paged_attn_desc* desc, svla_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------------
  * sample_actions glue
  * ------------------------------------------------------------------------------------------------*/
 /* Policy-side processing around sample_actions (lerobot SmolVLA prepare_images / prepare_state and the

@@ -65,7 +65,8 @@ class AttnDesc(ctypes.Structure):
 
 
 FLOW_MAX_LAYERS, FLOW_MAX_ROWS = 32, 64
-ERR_MBAR_TIMEOUT, ERR_BAD_SHAPE, ERR_FLOW_BARRIER = 101, 102, 103  # device error word codes
+# device error word codes
+ERR_MBAR_TIMEOUT, ERR_BAD_SHAPE, ERR_FLOW_BARRIER, ERR_BAD_PAGE = 101, 102, 103, 104
 
 
 class FlowLayer(ctypes.Structure):
@@ -109,6 +110,36 @@ ENGINE_NO_GRAPH, ENGINE_NO_SPLIT_K, ENGINE_NO_FLOW = 1, 2, 4  # SVLA_ENGINE_* fl
 DT_FLOAT, DT_HALF, DT_INT32, DT_BF16, DT_INT64 = 0, 1, 3, 7, 8
 
 
+class KvAppendDesc(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p), ("v_out", c_void_p),
+        ("cache", c_void_p), ("cu_q", c_void_p), ("kv_len", c_void_p), ("page_table", c_void_p), ("pos", c_void_p),
+        ("rope_cs", c_void_p), ("q_rs", c_int64), ("k_rs", c_int64), ("v_rs", c_int64), ("q_out_rs", c_int64),
+        ("k_out_rs", c_int64), ("v_out_rs", c_int64), ("page_table_rs", c_int64), ("batch", c_int32),
+        ("total_q", c_int32), ("hq", c_int32), ("hkv", c_int32), ("head_dim", c_int32), ("dtype", c_int32),
+        ("bits", c_int32), ("page_size", c_int32), ("n_pages", c_int32), ("max_pages", c_int32), ("max_pos", c_int32),
+    ]
+
+
+class PackedAttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("o", c_void_p), ("cu_q", c_void_p), ("cu_k", c_void_p),
+        ("q_rs", c_int64), ("k_rs", c_int64), ("v_rs", c_int64), ("o_rs", c_int64), ("batch", c_int32),
+        ("total_q", c_int32), ("total_k", c_int32), ("hq", c_int32), ("hkv", c_int32), ("head_dim", c_int32),
+        ("dtype", c_int32), ("causal", c_int32), ("scale", c_float),
+    ]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("cache", c_void_p), ("o", c_void_p), ("cu_q", c_void_p), ("kv_len", c_void_p),
+        ("page_table", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("q_rs", c_int64),
+        ("o_rs", c_int64), ("page_table_rs", c_int64), ("batch", c_int32), ("total_q", c_int32), ("hq", c_int32),
+        ("hkv", c_int32), ("head_dim", c_int32), ("dtype", c_int32), ("bits", c_int32), ("page_size", c_int32),
+        ("n_pages", c_int32), ("max_pages", c_int32), ("scale", c_float),
+    ]
+
+
 class RopeParams(ctypes.Structure):
     _fields_ = [("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("max_wavelength", c_float)]
 
@@ -149,6 +180,11 @@ SIGNATURES = {
     "svla_unnormalize_actions": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_int32, c_void_p,
                                            c_void_p]),
     "svla_rope_table": (c_int32, [c_void_p, c_int32, c_float, c_void_p]),
+    "svla_rope_table_wide": (c_int32, [c_void_p, c_int32, c_int32, ctypes.c_double, c_void_p]),
+    "svla_kv_append": (c_int32, [POINTER(KvAppendDesc), c_void_p]),
+    "svla_packed_attention": (c_int32, [POINTER(PackedAttnDesc), c_void_p]),
+    "svla_paged_attention_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "svla_paged_attention": (c_int32, [POINTER(PagedAttnDesc), c_void_p]),
     "svla_build_masks": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "svla_embed_tokens": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_int32, c_int32, c_float, c_void_p,

@@ -34,8 +34,12 @@ FLAGS = [*ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 
 def units() -> list[tuple[Path, list[Path]]]:
     """(source, the files its object depends on) for every translation unit of the library."""
-    kernels = [CSRC / "svla.cu", *sorted(CSRC.glob("*.cuh")), HEADER]
-    return [(CSRC / "svla.cu", kernels), (CSRC / "engine.cpp", [CSRC / "engine.cpp", HEADER])]
+    shared = [CSRC / "host.cuh", CSRC / "ptx.cuh", HEADER]
+    serving = [CSRC / f"{n}.cuh" for n in ("kv_append", "paged_attention", "packed_attention", "serving_common")]
+    path = [p for p in sorted(CSRC.glob("*.cuh")) if p not in serving]
+    return [(CSRC / "svla.cu", [CSRC / "svla.cu", *path, HEADER]),
+            (CSRC / "serving.cu", [CSRC / "serving.cu", *serving, *shared]),
+            (CSRC / "engine.cpp", [CSRC / "engine.cpp", HEADER])]
 
 
 def sources() -> list[Path]:

@@ -1,0 +1,715 @@
+// Attention over a paged key / value cache (layouts in kv_append.cuh), 16-bit or 4-bit entries, for a few new tokens
+// per sequence: query i of sequence b (of n_b) sees the cache entries n <= kv_len[b] - n_b + i,
+//   o_i = sum_n softmax_n(scale q_i . k_n) v_n          (no entry to see: zeros).
+//
+// Bound by the bytes of the live cache; the work around them has to stay below what an SM issues in the time they
+// take (4 bits, D = 64: 1280 bytes, 55 cycles, per 16 entries of one head).
+//
+// Shape of the products.  Keys are the M side: S^T (16 entries x 8 query rows) = K Q^T, O^T (16 dimensions x 8 query
+// rows) += V^T P^T.  A query row is a (token, head) of one kv head, packed token-major, so grouped heads and several
+// tokens share every key that is read; 8 rows fit one MMA column block, and single tokens of up to 8 grouped heads
+// waste half of what 16 query rows would.
+//
+// 4-bit entries are never expanded to 16-bit values.  A nibble c masked out of a word, as it stands, is the fp16
+// subnormal c 2^-24 (or 16 c 2^-24 for the second nibble of a byte): tensor cores take subnormals exactly, so one AND
+// makes two MMA operands.  With k = low + step c per group of 32 dimensions
+//   q . k = sum_g step_g (sum_{d in g} q_d c_d) + low_g (sum_{d in g} q_d)
+// needs one accumulator per group and two FMAs per score, and
+//   sum_n p_n v_n = sum_n (p_n step_n) c_n + sum_n p_n low_n
+// takes p_n step_n as the other operand.  Query rows are scaled by a power of two to the top of fp16's range (exact but
+// for components below 2^-25 of the row's largest), so bf16 queries lose nothing.  p_n step_n is rounded to fp16
+// (2^-12 relative); to keep it in fp16's range whatever the steps are, the running maximum is taken over
+// score + exponent(largest step of the entry) instead of the score.  Products with low_n stay in fp32.
+//
+// Every warp works alone: its own tiles of 32 entries through its own ring of asynchronous copies, its own running
+// maximum, sum and O, no barrier in the loop.  The maximum is lazy: it moves (and O is rescaled) only when a score
+// passes it by more than 8 in log2 units, one vote per tile instead of shuffles.
+//
+// Work split.  All tiles of all (sequence, kv head, query tile) items form one line; every CTA takes an equal piece of
+// it, whatever the sequences' lengths are, and finds its place from cu_q and kv_len on the device.  An item that lies in
+// one CTA is finished there; one cut by a piece's border leaves partials (maximum, sum, O in fp32) in the workspace,
+// which the combine kernel joins in the line's order, so results do not depend on timing.
+#pragma once
+
+#include "serving_common.cuh"
+
+namespace svla {
+
+struct PagedAttnArgs {
+  const void* q;
+  const uint8_t* cache;
+  void* o;
+  const int *cu_q, *kv_len, *table;
+  float* part;             // workspace: 2 slots per CTA
+  int4* meta;              // workspace, per CTA: {b, kv head, query tile, CTA of its last tile} of a cut item that starts
+                           // there, or {-1, ..}; then per CTA that item's first slot
+  long long q_rs, o_rs, table_rs;
+  int batch, total, hq, hkv, g, page, n_pages, max_pages;
+  unsigned long long page_magic;  // ceil(2^32 / (page / 16)): 16-entry slab -> page
+  int split;               // 0: items are not cut
+  int min_share;           // tiles a piece has at least
+  float scale_log2;
+  int* err;
+};
+
+namespace paged_detail {
+constexpr int kWarps = 4;
+constexpr int kKeys = 32;  // entries per tile: two 16-entry slabs, each inside one page
+constexpr int kStages = 3;
+
+template <int D, int BITS>
+struct Tile {
+  static constexpr int kRow = BITS == 16 ? D * 2 : D / 2;  // bytes of an entry's key (or value)
+  static constexpr int kPairs = BITS == 16 ? 0 : D / 8;    // bytes of its (step, low) pairs
+  static constexpr int kK = 0, kV = kKeys * kRow, kKP = 2 * kKeys * kRow, kVP = kKP + kKeys * kPairs;
+  static constexpr int kBytes = 2 * kKeys * (kRow + kPairs);
+};
+
+// rows of a (sequence, kv head) and their tiles
+template <int NT>
+__device__ __forceinline__ int query_tiles(int n_new, int g) {
+  return (n_new * g + 8 * NT - 1) / (8 * NT);
+}
+}  // namespace paged_detail
+
+template <typename T, int D, int BITS, int NT>
+struct PagedSmem {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kRing = paged_detail::kStages * paged_detail::Tile<D, BITS>::kBytes;  // per warp
+  static constexpr int kJoin = kRows * (D + 1 + 2) * 4;  // per warp: O, maximum, sum
+  static constexpr int kPerWarp = kRing > kJoin ? kRing : (kJoin + 15) / 16 * 16;
+  static constexpr int kBytes = paged_detail::kWarps * kPerWarp;
+};
+
+template <typename T, int D, int BITS, int NT>
+__global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_kernel(const PagedAttnArgs a) {
+  using namespace paged_detail;
+  using serving::copy16;
+  using Tl = Tile<D, BITS>;
+  using Sm = PagedSmem<T, D, BITS, NT>;
+  using serving::mma16816;
+  constexpr int kRows = 8 * NT, kGroups = D / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int place[2];         // first sequence of this CTA's piece, and ...
+  __shared__ long long place64[3]; // its start on the line; the piece
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+  uint8_t* ring = smem + warp * Sm::kPerWarp;
+  pdl_wait();
+  pdl_trigger();
+
+  // entries a sequence really has: its table's reach bounds them
+  const long long reach = static_cast<long long>(a.max_pages) * a.page;
+  auto entries = [&](int b) { return static_cast<int>(min(static_cast<long long>(max(__ldg(a.kv_len + b), 0)), reach)); };
+  auto tiles_of = [&](int len) { return a.split ? max((len + kKeys - 1) / kKeys, 1) : 1; };  // on the line, per item
+  auto weight = [&](int b) -> long long {
+    const serving::Span s = serving::span_of(a.cu_q, b, a.total);
+    return static_cast<long long>(tiles_of(entries(b))) * query_tiles<NT>(s.end - s.begin, a.g) * a.hkv;
+  };
+  // ---- this CTA's piece of the line and the sequence where it starts
+  if (warp == 0) {
+    long long sum = 0;
+    for (int b = lane; b < a.batch; b += 32) sum += weight(b);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    long long share = (sum + gridDim.x - 1) / gridDim.x;
+    if (share < a.min_share) share = a.min_share;
+    const long long from = share * blockIdx.x, to = min(from + share, sum);
+    int b0 = a.batch;
+    long long at = 0, base = 0;
+    for (int c = 0; c < a.batch && from < to; c += 32) {
+      const long long w = c + lane < a.batch ? weight(c + lane) : 0;
+      long long upto = w;  // inclusive prefix
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += y;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, base + upto > from);
+      if (past) {
+        const int l = __ffs(past) - 1;
+        b0 = c + l;
+        at = base + __shfl_sync(0xffffffffu, upto - w, l);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) {
+      place[0] = b0;
+      place64[0] = at;
+      place64[1] = from;
+      place64[2] = to;
+      if (a.split) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    }
+  }
+  __syncthreads();
+  int b = place[0];
+  long long at = place64[0];  // start of sequence b on the line
+  long long cur = place64[1];
+  const long long from = cur, to = place64[2];
+  const long long share = to - from;
+  const long long full_share = from > 0 ? from / blockIdx.x : share;
+  const long long page_bytes = BITS == 16 ? 4ll * a.page * D : static_cast<long long>(a.page) * (D + D / 4);
+
+  while (cur < to) {
+    // ---- the item at `cur`
+    const serving::Span sq = serving::span_of(a.cu_q, b, a.total);
+    const int n_new = sq.end - sq.begin, len = entries(b), n_tiles = tiles_of(len);
+    const int qt_n = query_tiles<NT>(n_new, a.g);
+    const long long w = static_cast<long long>(n_tiles) * qt_n * a.hkv;
+    if (cur >= at + w) {
+      at += w;
+      ++b;
+      continue;
+    }
+    if (threadIdx.x == 0 && __ldg(a.kv_len + b) > reach) record_error(a.err, serving::kErrBadPage);
+    const int item = static_cast<int>((cur - at) / n_tiles);
+    const long long item_at = at + static_cast<long long>(item) * n_tiles;
+    const int kh = item % a.hkv, qt = item / a.hkv;
+    const long long seg_end = min(item_at + n_tiles, to);
+    const bool whole = cur == item_at && seg_end == item_at + n_tiles;
+    // tiles of the sequence in this segment (an uncut item: all of them)
+    const int real_tiles = (len + kKeys - 1) / kKeys;
+    const int tile0 = a.split ? static_cast<int>(cur - item_at) : 0;
+    int tile1 = a.split ? min(static_cast<int>(seg_end - item_at), real_tiles) : real_tiles;
+    const int row0 = qt * kRows, rows = min(kRows, n_new * a.g - row0);
+    // entries the last / first row of this query tile sees
+    const int sees_last = min(max(len - n_new + (row0 + rows - 1) / a.g + 1, 0), len);
+    const int sees_first = min(max(len - n_new + row0 / a.g + 1, 0), len);
+    tile1 = min(tile1, (sees_last + kKeys - 1) / kKeys);
+
+    // ---- Q^T operands: column g8 of block nt is row row0 + nt * 8 + g8
+    constexpr int kQRegs = BITS == 16 ? D / 16 * 2 : kGroups * 4;
+    uint32_t qb[NT][kQRegs];
+    float qf[NT][2];            // 4 bits: factor of this thread's two score columns (queries 2 t4, 2 t4 + 1)
+    float qs[NT][kGroups][2];   // 4 bits: sums of their components, per group, times scale
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + nt * 8 + g8;
+      const bool in = nt * 8 + g8 < rows;
+      const T* src = static_cast<const T*>(a.q) + static_cast<size_t>(sq.begin + (in ? r / a.g : 0)) * a.q_rs +
+                     (kh * a.g + (in ? r % a.g : 0)) * D;
+      if constexpr (BITS == 16) {
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          qb[nt][2 * kk] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 2 * t4)) : 0u;
+          qb[nt][2 * kk + 1] = in ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + 8 + 2 * t4)) : 0u;
+        }
+        qf[nt][0] = qf[nt][1] = a.scale_log2;
+      } else {
+        float x[kGroups][8];
+        float top = 0.f, sum[kGroups];
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          const uint4 u = in ? __ldg(reinterpret_cast<const uint4*>(src + gr * 32 + t4 * 8)) : make_uint4(0, 0, 0, 0);
+          const uint32_t uu[4] = {u.x, u.y, u.z, u.w};
+          sum[gr] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = serving::unpack2<T>(uu[i]);
+            x[gr][2 * i] = f.x;
+            x[gr][2 * i + 1] = f.y;
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+            sum[gr] += f.x + f.y;
+          }
+        }
+#pragma unroll
+        for (int d = 1; d < 4; d <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], d);
+        }
+        // up = 2^(14 - exponent of the largest component): the row then fills fp16's range (largest in [2^14, 2^15))
+        int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+        e = (top > 0.f && e < 128) ? max(e, -100) : 14;
+        const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
+        const float f = ldexpf(a.scale_log2, 24 + e - 14);  // undoes 2^-24 of the codes and `up`
+#pragma unroll
+        for (int gr = 0; gr < kGroups; ++gr) {
+          // step 0 of the group: (n0, n4 | n1, n5), step 1: (n2, n6 | n3, n7); odd nibbles count 16 times
+          qb[nt][4 * gr + 0] = serving::pack2<__half>(x[gr][0] * up, x[gr][4] * up);
+          qb[nt][4 * gr + 1] = serving::pack2<__half>(x[gr][1] * (up * 0.0625f), x[gr][5] * (up * 0.0625f));
+          qb[nt][4 * gr + 2] = serving::pack2<__half>(x[gr][2] * up, x[gr][6] * up);
+          qb[nt][4 * gr + 3] = serving::pack2<__half>(x[gr][3] * (up * 0.0625f), x[gr][7] * (up * 0.0625f));
+        }
+        // the score columns of this thread are queries 2 t4 and 2 t4 + 1: take their factors from lanes 8 t4, 8 t4 + 4
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          qf[nt][u] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4 * u);
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr)
+            qs[nt][gr][u] = __shfl_sync(0xffffffffu, sum[gr] * a.scale_log2, 8 * t4 + 4 * u);
+        }
+      }
+    }
+    // entries that this thread's two score columns see
+    int sees[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int r = row0 + nt * 8 + 2 * t4 + u;
+        sees[nt][u] = min(max(len - n_new + r / a.g + 1, 0), len);
+      }
+
+    // ---- this warp's tiles: tile0 + warp, + 4, ...
+    const int mine = tile1 - tile0 - warp > 0 ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;
+    // page of slab s of the warp's i-th tile: lane 2 (i % 16) + s of `pages` (this batch of 16 tiles) or `pages_next`
+    auto load_pages = [&](int i0) -> int {
+      const int i = i0 + (lane >> 1);
+      if (i >= mine) return -1;
+      const int slab = (tile0 + warp + i * kWarps) * (kKeys / 16) + (lane & 1);
+      if (slab * 16 >= sees_last) return -1;
+      const int pg = static_cast<int>((static_cast<unsigned long long>(slab) * a.page_magic) >> 32);
+      const int id = __ldg(a.table + static_cast<size_t>(b) * a.table_rs + pg);
+      if (id >= 0 && id < a.n_pages) return id;
+      record_error(a.err, serving::kErrBadPage);
+      return -1;
+    };
+    int pages = load_pages(0), pages_next = load_pages(16);
+    const int slabs_per_page = a.page / 16;
+    // copies tile i of the warp into its ring stage; returns nothing, the validity is read again from the page ids
+    auto issue = [&](int i, int ids) {
+      uint8_t* st = ring + (i % kStages) * Tl::kBytes;
+      const int tile = tile0 + warp + i * kWarps;
+#pragma unroll
+      for (int s = 0; s < kKeys / 16; ++s) {
+        const int id = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + s);
+        const int slab = tile * (kKeys / 16) + s;
+        const int pg = static_cast<int>((static_cast<unsigned long long>(slab) * a.page_magic) >> 32);
+        const int slot = (slab - pg * slabs_per_page) * 16;
+        const uint8_t* base = a.cache + (static_cast<size_t>(id < 0 ? 0 : id) * a.hkv + kh) * page_bytes;
+        if constexpr (BITS == 16) {
+          constexpr int kChunks = D / 8;  // 16-byte chunks of a row; chunk c of row r sits at c ^ (r % 8)
+#pragma unroll
+          for (int u = 0; u < kChunks / 2; ++u) {
+            const int idx = lane + u * 32, r = idx / kChunks, c = idx % kChunks;
+            // entries past the sequence are zeros, whatever the page holds there
+            const int n = (id >= 0 && slab * 16 + r < len) ? 16 : 0;
+            const uint8_t* src = base + static_cast<size_t>(slot + r) * (2 * D) + c * 16;
+            const int dst = (s * 16 + r) * Tl::kRow + ((c ^ (r & 7)) * 16);
+            copy16(st + Tl::kK + dst, src, n);
+            copy16(st + Tl::kV + dst, src + static_cast<size_t>(a.page) * (2 * D), n);
+          }
+        } else {
+          constexpr int kChunks = D / 32;  // chunk c (one group's codes) of row r sits at c ^ swizzle(r): no bank conflicts
+          const int n = id >= 0 ? 16 : 0;
+#pragma unroll
+          for (int u = 0; u < kChunks / 2; ++u) {
+            const int idx = lane + u * 32, r = idx / kChunks, c = idx % kChunks;
+            const int sw = D == 64 ? (r >> 2) & 1 : (r >> 1) & 3;
+            const uint8_t* src = base + static_cast<size_t>(slot + r) * (D / 2) + c * 16;
+            const int dst = (s * 16 + r) * Tl::kRow + ((c ^ sw) * 16);
+            copy16(st + Tl::kK + dst, src, n);
+            copy16(st + Tl::kV + dst, src + static_cast<size_t>(a.page) * (D / 2), n);
+          }
+          if (lane < D / 4) {  // 16 entries' pairs: D / 8 chunks for keys, D / 8 for values
+            const int is_v = lane / (D / 8), c = lane % (D / 8);
+            const uint8_t* src = base + static_cast<size_t>(a.page) * D +
+                                 (static_cast<size_t>(is_v ? a.page : 0) + slot) * (D / 8) + c * 16;
+            copy16(st + (is_v ? Tl::kVP : Tl::kKP) + s * 16 * Tl::kPairs + c * 16, src, n);
+          }
+        }
+      }
+    };
+
+    float o[NT][D / 16][4];     // O^T: see the P.V product for which dimensions a thread holds
+    float om[NT][kGroups][2];   // 4 bits: sum of p low
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
+#pragma unroll
+      for (int gr = 0; gr < kGroups; ++gr) om[nt][gr][0] = om[nt][gr][1] = 0.f;
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+    }
+
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (i < mine) issue(i, pages);
+      serving::copy_commit();
+    }
+    for (int i = 0; i < mine; ++i) {
+      // refill the stage that tile i - 1 used (every lane has passed the __syncwarp that ends tile i - 1)
+      const int ahead = i + kStages - 1;
+      if (ahead < mine) issue(ahead, (ahead >> 4) == (i >> 4) ? pages : pages_next);
+      serving::copy_commit();
+      serving::copy_wait<kStages - 1>();
+      __syncwarp();
+      const uint8_t* st = ring + (i % kStages) * Tl::kBytes;
+      const int key0 = (tile0 + warp + i * kWarps) * kKeys;
+      int ids[2];
+      ids[0] = __shfl_sync(0xffffffffu, pages, 2 * (i & 15));
+      ids[1] = __shfl_sync(0xffffffffu, pages, 2 * (i & 15) + 1);
+      if ((i & 15) == 15) {
+        pages = pages_next;
+        pages_next = load_pages(i + 17);
+      }
+      // some entry of the tile is hidden from some row (warp-uniform)
+      const bool edge = key0 + kKeys > sees_first || ids[0] < 0 || ids[1] < 0;
+
+      // ---- scores, in log2 units: s[nt][slab][e]: entry slab * 16 + g8 + 8 (e / 2), query column 2 t4 + e % 2
+      float s[NT][2][4];
+      float vstep[2][2][kGroups], vlow[2][2][kGroups];  // [slab][row half][group] of this thread's entries
+      float lift[2][2];  // log2 bound of the entry's steps (0 for 16 bits)
+#pragma unroll
+      for (int sl = 0; sl < 2; ++sl) {
+        if constexpr (BITS == 16) {
+          float acc[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t ka[4];  // entries (lane & 15), dimensions kk * 16 + 8 (lane >> 4)
+            const int r = sl * 16 + (lane & 15), ch = kk * 2 + (lane >> 4);
+            serving::ldsm_x4(ka, st + Tl::kK + r * Tl::kRow + ((ch ^ (r & 7)) * 16));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma16816<T>(acc[nt], ka, qb[nt][2 * kk], qb[nt][2 * kk + 1]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[nt][sl][e] = acc[nt][e] * qf[nt][e & 1];
+          lift[sl][0] = lift[sl][1] = 0.f;
+        } else {
+          float acc[NT][kGroups][4];
+          const int r0 = sl * 16 + g8;
+          const int sw0 = D == 64 ? (r0 >> 2) & 1 : (r0 >> 1) & 3, sw1 = D == 64 ? ((r0 + 8) >> 2) & 1 : ((r0 + 8) >> 1) & 3;
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) {
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + Tl::kK + r0 * Tl::kRow + ((gr ^ sw0) * 16) + t4 * 4);
+            const uint32_t w1 =
+                *reinterpret_cast<const uint32_t*>(st + Tl::kK + (r0 + 8) * Tl::kRow + ((gr ^ sw1) * 16) + t4 * 4);
+            const uint32_t x0 = w0 >> 8, x1 = w1 >> 8;
+            const uint32_t a0[4] = {w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u};
+            const uint32_t a1[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              acc[nt][gr][0] = acc[nt][gr][1] = acc[nt][gr][2] = acc[nt][gr][3] = 0.f;
+              mma16816<__half>(acc[nt][gr], a0, qb[nt][4 * gr], qb[nt][4 * gr + 1]);
+              mma16816<__half>(acc[nt][gr], a1, qb[nt][4 * gr + 2], qb[nt][4 * gr + 3]);
+            }
+          }
+#pragma unroll
+          for (int hr = 0; hr < 2; ++hr) {
+            const int r = r0 + 8 * hr;
+            uint32_t kp[kGroups], vp[kGroups];
+            if constexpr (kGroups == 2) {
+              const uint2 ku = *reinterpret_cast<const uint2*>(st + Tl::kKP + r * Tl::kPairs);
+              const uint2 vu = *reinterpret_cast<const uint2*>(st + Tl::kVP + r * Tl::kPairs);
+              kp[0] = ku.x, kp[1] = ku.y, vp[0] = vu.x, vp[1] = vu.y;
+            } else {
+              const uint4 ku = *reinterpret_cast<const uint4*>(st + Tl::kKP + r * Tl::kPairs);
+              const uint4 vu = *reinterpret_cast<const uint4*>(st + Tl::kVP + r * Tl::kPairs);
+              kp[0] = ku.x, kp[1] = ku.y, kp[2] = ku.z, kp[3] = ku.w;
+              vp[0] = vu.x, vp[1] = vu.y, vp[2] = vu.z, vp[3] = vu.w;
+            }
+            uint32_t big = 0u;
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) {
+              vstep[sl][hr][gr] = __uint_as_float(vp[gr] << 16);
+              vlow[sl][hr][gr] = __uint_as_float(vp[gr] & 0xFFFF0000u);
+              const uint32_t ex = (vp[gr] >> 7) & 0xFFu;  // exponent of the step; a NaN or infinity does not count
+              big = max(big, ex == 255u ? 0u : ex);
+            }
+            // steps below 2^-60 would push p beyond fp32's range: their products lose nothing that matters
+            lift[sl][hr] = static_cast<float>(max(static_cast<int>(big) - 127, -60));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                float dot = 0.f, add = 0.f;
+#pragma unroll
+                for (int gr = 0; gr < kGroups; ++gr) {
+                  dot = fmaf(__uint_as_float(kp[gr] << 16), acc[nt][gr][2 * hr + u], dot);
+                  add = fmaf(__uint_as_float(kp[gr] & 0xFFFF0000u), qs[nt][gr][u], add);
+                }
+                s[nt][sl][2 * hr + u] = fmaf(dot, qf[nt][u], add);
+              }
+          }
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int n = key0 + sl * 16 + g8 + 8 * (e >> 1);
+              if (n >= sees[nt][e & 1] || ids[sl] < 0) s[nt][sl][e] = -INFINITY;
+            }
+      }
+      // ---- lazy running maximum
+      bool pass = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pass |= s[nt][sl][e] + lift[sl][e >> 1] > m[nt][e & 1] + 8.f;
+      if (__any_sync(0xffffffffu, pass)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float top = m[nt][u];
+#pragma unroll
+            for (int sl = 0; sl < 2; ++sl)
+              top = fmaxf(top, fmaxf(s[nt][sl][u] + lift[sl][0], s[nt][sl][2 + u] + lift[sl][1]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float alpha = m[nt][u] == -INFINITY ? 0.f : ex2_approx(m[nt][u] - top);
+            m[nt][u] = top;
+            l[nt][u] *= alpha;
+#pragma unroll
+            for (int i2 = 0; i2 < D / 16; ++i2) {
+              o[nt][i2][u] *= alpha;
+              o[nt][i2][2 + u] *= alpha;
+            }
+            if constexpr (BITS == 4) {
+#pragma unroll
+              for (int gr = 0; gr < kGroups; ++gr) om[nt][gr][u] *= alpha;
+            }
+          }
+        }
+      }
+      // ---- probabilities
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[nt][sl][e] = ex2_approx(s[nt][sl][e] - ((e & 1) ? m1 : m0));
+            l[nt][e & 1] += s[nt][sl][e];
+          }
+      }
+      // ---- O^T += V^T P^T
+      if constexpr (BITS == 16) {
+        // an infinity or a NaN in the value of an entry that some row does not see would reach that row as 0 * inf
+        bool odd = false;
+        if (edge && n_new > 1) {
+          for (int idx = lane; idx < kKeys * (D / 8); idx += 32) {
+            const uint4 u = *reinterpret_cast<const uint4*>(st + Tl::kV + idx * 16);
+            odd |= serving::any_nonfinite<T>(u.x) || serving::any_nonfinite<T>(u.y) ||
+                   serving::any_nonfinite<T>(u.z) || serving::any_nonfinite<T>(u.w);
+          }
+          odd = __any_sync(0xffffffffu, odd);
+        }
+        if (!odd) {
+#pragma unroll
+          for (int sl = 0; sl < 2; ++sl) {
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              pb[nt][0] = serving::movmatrix_trans(serving::pack2<T>(s[nt][sl][0], s[nt][sl][1]));
+              pb[nt][1] = serving::movmatrix_trans(serving::pack2<T>(s[nt][sl][2], s[nt][sl][3]));
+            }
+#pragma unroll
+            for (int mt = 0; mt < D / 16; ++mt) {
+              // V^T: rows = dimensions mt * 16 .. + 15, columns = the slab's entries; transposed 8 x 8 blocks
+              uint32_t va[4];
+              const int r = sl * 16 + (lane & 7) + ((lane >> 4) << 3), ch = mt * 2 + ((lane >> 3) & 1);
+              serving::ldsm_x4_trans(va, st + Tl::kV + r * Tl::kRow + ((ch ^ (r & 7)) * 16));
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma16816<T>(o[nt][mt], va, pb[nt][0], pb[nt][1]);
+            }
+          }
+        } else {  // rare: one entry after the other, hidden ones left out
+          for (int n = 0; n < kKeys; ++n) {
+            const int r = n;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              float p[2];
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                // entry n's row of the score block: slab n / 16, half (n / 8) % 2, lane group n % 8
+                const float v0 = (n >> 4) ? ((n >> 3) & 1 ? s[nt][1][2 + u] : s[nt][1][u])
+                                          : ((n >> 3) & 1 ? s[nt][0][2 + u] : s[nt][0][u]);
+                p[u] = __shfl_sync(0xffffffffu, v0, (n & 7) * 4 + t4);
+              }
+#pragma unroll
+              for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                  const int d = mt * 16 + hf * 8 + g8;
+                  const T* vp = reinterpret_cast<const T*>(st + Tl::kV + r * Tl::kRow + (((d >> 3) ^ (r & 7)) * 16)) + (d & 7);
+                  const float v = static_cast<float>(*vp);
+#pragma unroll
+                  for (int u = 0; u < 2; ++u)
+                    if (key0 + n < sees[nt][u]) o[nt][mt][2 * hf + u] = fmaf(p[u], v, o[nt][mt][2 * hf + u]);
+                }
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int sl = 0; sl < 2; ++sl) {
+          uint32_t pb[NT][kGroups][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr)
+#pragma unroll
+              for (int hr = 0; hr < 2; ++hr) {
+                float w0 = s[nt][sl][2 * hr] * vstep[sl][hr][gr], w1 = s[nt][sl][2 * hr + 1] * vstep[sl][hr][gr];
+                float a0 = s[nt][sl][2 * hr] * vlow[sl][hr][gr], a1 = s[nt][sl][2 * hr + 1] * vlow[sl][hr][gr];
+                if (edge) {  // what stands in a hidden entry's pair (NaN too) does not count
+                  const int n = key0 + sl * 16 + g8 + 8 * hr;
+                  if (n >= sees[nt][0] || ids[sl] < 0) w0 = a0 = 0.f;
+                  if (n >= sees[nt][1] || ids[sl] < 0) w1 = a1 = 0.f;
+                }
+                om[nt][gr][0] += a0;
+                om[nt][gr][1] += a1;
+                pb[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(w0, w1));
+              }
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) {
+            // this lane's entries 2 t4, 2 t4 + 1 (and + 8): the half word g8 of the group's codes, dimensions 4 g8 .. + 3
+            uint32_t x[2];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const int r = sl * 16 + 2 * t4 + 8 * hf;
+              const int sw = D == 64 ? (r >> 2) & 1 : (r >> 1) & 3;  // the same for r and r + 1
+              const uint8_t* src = st + Tl::kV + r * Tl::kRow + ((gr ^ sw) * 16) + (g8 >> 1) * 4;
+              const uint32_t w0 = *reinterpret_cast<const uint32_t*>(src);
+              const uint32_t w1 = *reinterpret_cast<const uint32_t*>(src + Tl::kRow);
+              x[hf] = __byte_perm(w0, w1, (g8 & 1) ? 0x7632 : 0x5410);
+            }
+            const uint32_t y0 = x[0] >> 8, y1 = x[1] >> 8;
+            // rows g8 of the first product: dimension 4 g8, rows g8 + 8: 4 g8 + 1 (16 times); second: 4 g8 + 2, + 3
+            const uint32_t a0[4] = {x[0] & 0x000F000Fu, x[0] & 0x00F000F0u, x[1] & 0x000F000Fu, x[1] & 0x00F000F0u};
+            const uint32_t a1[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<__half>(o[nt][2 * gr], a0, pb[nt][gr][0], pb[nt][gr][1]);
+              mma16816<__half>(o[nt][2 * gr + 1], a1, pb[nt][gr][0], pb[nt][gr][1]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+    serving::copy_wait<0>();
+    __syncthreads();  // every warp is done with its ring
+
+    // ---- join the four warps
+    float* js = reinterpret_cast<float*>(smem + warp * Sm::kPerWarp);  // [kRows][D + 1], then maxima, sums
+    float* jm = js + kRows * (D + 1);
+    float* jl = jm + kRows;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          l[nt][u] += __shfl_xor_sync(0xffffffffu, l[nt][u], d);
+          if constexpr (BITS == 4) {
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) om[nt][gr][u] += __shfl_xor_sync(0xffffffffu, om[nt][gr][u], d);
+          }
+        }
+        const int r = nt * 8 + 2 * t4 + u;
+        if (g8 == 0) {
+          jm[r] = m[nt][u];
+          jl[r] = l[nt][u];
+        }
+#pragma unroll
+        for (int mt = 0; mt < D / 16; ++mt) {
+          if constexpr (BITS == 16) {
+            js[r * (D + 1) + mt * 16 + g8] = o[nt][mt][u];
+            js[r * (D + 1) + mt * 16 + 8 + g8] = o[nt][mt][2 + u];
+          } else {
+            // 2^24 undoes the codes' subnormals, odd dimensions counted 16 times
+            const int d = (mt >> 1) * 32 + 4 * g8 + 2 * (mt & 1);
+            js[r * (D + 1) + d] = fmaf(o[nt][mt][u], 16777216.f, om[nt][mt >> 1][u]);
+            js[r * (D + 1) + d + 1] = fmaf(o[nt][mt][2 + u], 1048576.f, om[nt][mt >> 1][u]);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const bool starts_here = cur == item_at;
+    const int slot_id = 2 * blockIdx.x + (cur > from ? 1 : 0);
+    for (int idx = threadIdx.x; idx < kRows * (D / 2); idx += kWarps * 32) {
+      const int r = idx / (D / 2), d = (idx % (D / 2)) * 2;
+      if (r >= rows) break;
+      float top = -INFINITY;
+#pragma unroll
+      for (int wv = 0; wv < kWarps; ++wv)
+        top = fmaxf(top, reinterpret_cast<const float*>(smem + wv * Sm::kPerWarp)[kRows * (D + 1) + r]);
+      float sum = 0.f, o0 = 0.f, o1 = 0.f;
+#pragma unroll
+      for (int wv = 0; wv < kWarps; ++wv) {
+        const float* p = reinterpret_cast<const float*>(smem + wv * Sm::kPerWarp);
+        const float pm = p[kRows * (D + 1) + r];
+        // a warp without entries (or with nothing visible) has sum 0; one whose scores are all NaN keeps its NaN
+        const float f = pm == -INFINITY ? 1.f : ex2_approx(pm - top);
+        sum = fmaf(f, p[kRows * (D + 1) + kRows + r], sum);
+        o0 = fmaf(f, p[r * (D + 1) + d], o0);
+        o1 = fmaf(f, p[r * (D + 1) + d + 1], o1);
+      }
+      if (whole) {
+        const int row = row0 + r;
+        const bool sees_some = len - n_new + row / a.g + 1 > 0 && len > 0;
+        const float inv = sees_some ? __frcp_rn(sum) : 0.f;
+        T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + d;
+        *reinterpret_cast<uint32_t*>(dst) = sees_some ? serving::pack2<T>(o0 * inv, o1 * inv) : 0u;
+      } else {
+        float* p = a.part + static_cast<size_t>(slot_id) * kRows * (D + 2);
+        *reinterpret_cast<float2*>(p + r * D + d) = make_float2(o0, o1);
+        if (d == 0) *reinterpret_cast<float2*>(p + kRows * D + 2 * r) = make_float2(top, sum);
+      }
+    }
+    if (!whole && starts_here && threadIdx.x == 0) {
+      // the item's last piece: the CTA whose piece holds the item's last tile
+      const long long last = (item_at + n_tiles - 1) / full_share;
+      a.meta[blockIdx.x] = make_int4(b, kh, qt, static_cast<int>(last));
+      a.meta[gridDim.x + blockIdx.x].x = slot_id;
+    }
+    cur = seg_end;
+    __syncthreads();  // the join buffers are the next item's ring
+  }
+}
+
+// Joins the partials of the items that the pieces' borders cut; CTA c takes the one that starts in piece c.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs a) {
+  constexpr int kRows = 8 * NT;
+  pdl_wait();
+  pdl_trigger();
+  const int4 meta = a.meta[blockIdx.x];
+  if (meta.x < 0) return;
+  const int b = meta.x, kh = meta.y, row0 = meta.z * kRows, last = meta.w;
+  const serving::Span sq = serving::span_of(a.cu_q, b, a.total);
+  const int n_new = sq.end - sq.begin, rows = min(kRows, n_new * a.g - row0);
+  const long long reach = static_cast<long long>(a.max_pages) * a.page;
+  const int len = static_cast<int>(min(static_cast<long long>(max(__ldg(a.kv_len + b), 0)), reach));
+  const int first_slot = a.meta[gridDim.x + blockIdx.x].x;
+  for (int idx = threadIdx.x; idx < rows * (D / 2); idx += blockDim.x) {
+    const int r = idx / (D / 2), d = (idx % (D / 2)) * 2;
+    float top = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
+    for (int c = blockIdx.x; c <= last; ++c) {
+      const int slot = c == static_cast<int>(blockIdx.x) ? first_slot : 2 * c;
+      const float* p = a.part + static_cast<size_t>(slot) * kRows * (D + 2);
+      const float2 ml = *reinterpret_cast<const float2*>(p + kRows * D + 2 * r);
+      const float2 ov = *reinterpret_cast<const float2*>(p + r * D + d);
+      const float nt = fmaxf(top, ml.x);
+      const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - nt), f1 = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - nt);
+      sum = fmaf(f1, ml.y, f0 * sum);
+      o0 = fmaf(f1, ov.x, f0 * o0);
+      o1 = fmaf(f1, ov.y, f0 * o1);
+      top = nt;
+    }
+    const int row = row0 + r;
+    const bool sees_some = len - n_new + row / a.g + 1 > 0 && len > 0;
+    const float inv = sees_some ? __frcp_rn(sum) : 0.f;
+    T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + d;
+    *reinterpret_cast<uint32_t*>(dst) = sees_some ? serving::pack2<T>(o0 * inv, o1 * inv) : 0u;
+  }
+}
+
+}  // namespace svla

@@ -354,7 +354,7 @@ __device__ __forceinline__ int8_t smooth_quant(float x, float s, float a) {
   return static_cast<int8_t>(quant_rn_clamp(__fdiv_rn(__fdiv_rn(x, s), a), -128, 127));
 }
 // the same, kept out of line: the rare fallback of smooth_quant_fast (one copy instead of one per element)
-__device__ __noinline__ int smooth_quant_slow(float x, float s, float a) { return smooth_quant(x, s, a); }
+inline __device__ __noinline__ int smooth_quant_slow(float x, float s, float a) { return smooth_quant(x, s, a); }
 
 // The same result as smooth_quant, cheaper: y = (x * rs) * ra with rs = 1/s, ra = 1/a (correctly rounded
 // reciprocals) differs from fl(fl(x / s) / a) by at most 6 * 2^-24 * |y| (< 1e-4 for |y| < 256).  Away

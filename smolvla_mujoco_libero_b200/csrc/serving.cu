@@ -1,0 +1,243 @@
+// C-ABI entry points of the serving operators (include/svla.h): attention over packed prompts, appending to a paged
+// cache, attention over a paged cache.  Argument checks, template dispatch and launches; nothing allocates memory.
+#include <cmath>
+#include <cstring>
+
+#include "host.cuh"
+#include "kv_append.cuh"
+#include "packed_attention.cuh"
+#include "paged_attention.cuh"
+
+namespace svla {
+namespace {
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int32_t check_heads(const char* who, int32_t hq, int32_t hkv, int32_t head_dim, int32_t dtype) {
+  if (hq <= 0 || hkv <= 0 || hq % hkv) return fail(SVLA_ERR_ARG, "%s: hq must be a positive multiple of hkv", who);
+  if (head_dim != 64 && head_dim != 128) return fail(SVLA_ERR_ARG, "%s: head_dim must be 64 or 128 (got %d)", who, head_dim);
+  if (dtype != SVLA_DT_BF16 && dtype != SVLA_DT_HALF) return fail(SVLA_ERR_ARG, "%s: dtype must be BF16 or HALF (got %d)", who, dtype);
+  return SVLA_OK;
+}
+
+// a packed tensor [rows][heads * head_dim]: 16-byte aligned rows that hold all heads
+int32_t check_rows(const char* who, const char* name, const void* p, int64_t rs, int64_t width) {
+  if (!p) return fail(SVLA_ERR_ARG, "%s: %s is null", who, name);
+  if (!aligned(p, 16) || rs % 8 || rs < width)
+    return fail(SVLA_ERR_ARG, "%s: %s must be 16-byte aligned with a row stride that is a multiple of 8 and >= %lld", who,
+                name, static_cast<long long>(width));
+  return SVLA_OK;
+}
+
+int32_t check_cache(const char* who, const void* cache, int32_t bits, int32_t page, int32_t n_pages, const int32_t* table,
+                    int64_t table_rs, int32_t max_pages, const int32_t* kv_len) {
+  if (!cache || !table || !kv_len) return fail(SVLA_ERR_ARG, "%s: null cache, page_table or kv_len", who);
+  if (!aligned(cache, 16)) return fail(SVLA_ERR_ARG, "%s: cache must be 16-byte aligned", who);
+  if (bits != 4 && bits != 16) return fail(SVLA_ERR_ARG, "%s: bits must be 4 or 16 (got %d)", who, bits);
+  if (page < 16 || page > 256 || page % 16)
+    return fail(SVLA_ERR_ARG, "%s: page_size must be a multiple of 16, 16 to 256 (got %d)", who, page);
+  if (n_pages <= 0 || max_pages <= 0 || table_rs < max_pages)
+    return fail(SVLA_ERR_ARG, "%s: n_pages and max_pages must be positive, page_table rows at least max_pages", who);
+  return SVLA_OK;
+}
+
+template <typename Kern>
+int32_t allow_smem(Kern kern, int bytes, bool (&configured)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return fail(SVLA_ERR_ARG, "device index %d out of range", dev);
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return fail(SVLA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    configured[dev] = true;
+  }
+  return SVLA_OK;
+}
+
+// ---------------------------------------------------------------- append
+template <typename T, int D>
+int32_t launch_append(const KvAppendArgs& a, int bits, dim3 grid, cudaStream_t st) {
+  const dim3 block(append_detail::kWarps * 32);
+  if (bits == 16) return launch(kv_append_kernel<T, D, 16>, grid, block, 0, st, "kv_append_kernel", a);
+  return launch(kv_append_kernel<T, D, 4>, grid, block, 0, st, "kv_append_kernel", a);
+}
+
+// ---------------------------------------------------------------- packed prompts
+template <typename T, int D>
+int32_t launch_packed(const PackedAttnArgs& a, long long items, cudaStream_t st) {
+  static bool configured[64] = {false};
+  auto kern = packed_attention_kernel<T, D>;
+  if (int32_t rc = allow_smem(kern, PackedSmem<T, D>::kBytes, configured)) return rc;
+  return launch(kern, dim3(static_cast<unsigned>(items)), dim3(packed_detail::kWarps * 32), PackedSmem<T, D>::kBytes, st,
+                "packed_attention_kernel", a);
+}
+
+// ---------------------------------------------------------------- paged
+constexpr int kPagedCtas = 4;  // most CTAs per SM
+
+// rows of a query tile / 8: single tokens of up to 8 grouped heads, or more
+int paged_nt(int batch, int total_q, int g) { return static_cast<long long>(total_q) * g <= 8ll * batch ? 1 : 2; }
+
+size_t paged_part_bytes(long long ctas, int nt, int d) { return static_cast<size_t>(2 * ctas) * 8 * nt * (d + 2) * 4; }
+
+template <typename T, int D, int BITS, int NT>
+int32_t launch_paged_inst(PagedAttnArgs a, cudaStream_t st) {
+  using Sm = PagedSmem<T, D, BITS, NT>;
+  static bool configured[64] = {false};
+  static int ctas[64] = {0};
+  auto kern = paged_attention_kernel<T, D, BITS, NT>;
+  if (int32_t rc = allow_smem(kern, Sm::kBytes, configured)) return rc;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (ctas[dev] == 0) {
+    int n = 0;
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, paged_detail::kWarps * 32, Sm::kBytes);
+    if (e != cudaSuccess) return fail(SVLA_ERR_CUDA, "cudaOccupancyMaxActiveBlocksPerMultiprocessor: %s", cudaGetErrorString(e));
+    ctas[dev] = (n < 1 ? 1 : (n > kPagedCtas ? kPagedCtas : n)) * sm_count();
+  }
+  const int grid = ctas[dev];
+  a.meta = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(a.part) + paged_part_bytes(grid, NT, D));
+  int32_t rc = launch(kern, dim3(grid), dim3(paged_detail::kWarps * 32), Sm::kBytes, st, "paged_attention_kernel", a);
+  if (rc || !a.split) return rc;
+  return launch(paged_combine_kernel<T, D, NT>, dim3(grid), dim3(128), 0, st, "paged_combine_kernel", a);
+}
+
+template <typename T, int D>
+int32_t launch_paged(const PagedAttnArgs& a, int bits, int nt, cudaStream_t st) {
+  if (bits == 16) return nt == 1 ? launch_paged_inst<T, D, 16, 1>(a, st) : launch_paged_inst<T, D, 16, 2>(a, st);
+  return nt == 1 ? launch_paged_inst<T, D, 4, 1>(a, st) : launch_paged_inst<T, D, 4, 2>(a, st);
+}
+
+}  // namespace
+}  // namespace svla
+
+using namespace svla;
+
+extern "C" {
+
+int32_t svla_rope_table_wide(float* c, int32_t max_pos, int32_t head_dim, double max_wavelength, svla_stream_t stream) {
+  if (!c || !aligned(c, 16) || max_pos <= 0 || head_dim <= 0 || head_dim % 2 || !(max_wavelength > 0))
+    return fail(SVLA_ERR_ARG, "svla_rope_table_wide: bad args");
+  const long long n = static_cast<long long>(max_pos) * (head_dim / 2);
+  return launch(rope_table_wide_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, cs(stream),
+                "rope_table_wide_kernel", reinterpret_cast<float2*>(c), max_pos, head_dim / 2, max_wavelength);
+}
+
+int32_t svla_kv_append(const svla_kv_append_desc* d, svla_stream_t stream) {
+  const char* who = "svla_kv_append";
+  if (!d) return fail(SVLA_ERR_ARG, "%s: null descriptor", who);
+  if (d->batch < 0 || d->total_q < 0) return fail(SVLA_ERR_ARG, "%s: negative batch or total_q", who);
+  const int32_t hq = d->q ? d->hq : d->hkv;  // without queries hq is not read
+  if (int32_t rc = check_heads(who, hq, d->hkv, d->head_dim, d->dtype)) return rc;
+  if (int32_t rc = check_cache(who, d->cache, d->bits, d->page_size, d->n_pages, d->page_table, d->page_table_rs, d->max_pages, d->kv_len)) return rc;
+  if (!d->cu_q) return fail(SVLA_ERR_ARG, "%s: cu_q is null", who);
+  const int64_t qw = static_cast<int64_t>(hq) * d->head_dim, kw = static_cast<int64_t>(d->hkv) * d->head_dim;
+  if (int32_t rc = check_rows(who, "k", d->k, d->k_rs, kw)) return rc;
+  if (int32_t rc = check_rows(who, "v", d->v, d->v_rs, kw)) return rc;
+  if (d->q) {
+    if (int32_t rc = check_rows(who, "q", d->q, d->q_rs, qw)) return rc;
+    if (int32_t rc = check_rows(who, "q_out", d->q_out, d->q_out_rs, qw)) return rc;
+  }
+  if (d->k_out) if (int32_t rc = check_rows(who, "k_out", d->k_out, d->k_out_rs, kw)) return rc;
+  if (d->v_out) if (int32_t rc = check_rows(who, "v_out", d->v_out, d->v_out_rs, kw)) return rc;
+  if (d->rope_cs && (!aligned(d->rope_cs, 16) || d->max_pos <= 0))
+    return fail(SVLA_ERR_ARG, "%s: rope_cs must be 16-byte aligned with max_pos > 0", who);
+  if (d->batch == 0 || d->total_q == 0) return SVLA_OK;
+  KvAppendArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.q = d->q, a.k = d->k, a.v = d->v;
+  a.qo = d->q_out, a.ko = d->k_out, a.vo = d->v_out;
+  a.cache = static_cast<uint8_t*>(d->cache);
+  a.cu_q = d->cu_q, a.kv_len = d->kv_len, a.table = d->page_table, a.pos = d->pos;
+  a.cs = reinterpret_cast<const float2*>(d->rope_cs);
+  a.q_rs = d->q_rs, a.k_rs = d->k_rs, a.v_rs = d->v_rs;
+  a.qo_rs = d->q_out_rs, a.ko_rs = d->k_out_rs, a.vo_rs = d->v_out_rs, a.table_rs = d->page_table_rs;
+  a.batch = d->batch, a.total = d->total_q, a.hq = d->hq, a.hkv = d->hkv;
+  a.page = d->page_size, a.n_pages = d->n_pages, a.max_pages = d->max_pages, a.max_pos = d->max_pos;
+  a.err = device_error_ptr();
+  // few tokens: several warps share a token's heads, so that a call fills the GPU and its rows are fetched at once
+  const int slots = 32 / (d->head_dim / 16), rounds = ((d->q ? d->hq : 0) + 2 * d->hkv + slots - 1) / slots;
+  long long parts = 16ll * sm_count() / d->total_q;
+  a.parts = static_cast<int>(parts < 1 ? 1 : (parts > rounds ? rounds : parts));
+  const long long warps = static_cast<long long>(d->total_q) * a.parts;
+  const dim3 grid(static_cast<unsigned>((warps + append_detail::kWarps - 1) / append_detail::kWarps));
+  const bool h = d->dtype == SVLA_DT_HALF;
+  if (d->head_dim == 64) return h ? launch_append<__half, 64>(a, d->bits, grid, cs(stream)) : launch_append<__nv_bfloat16, 64>(a, d->bits, grid, cs(stream));
+  return h ? launch_append<__half, 128>(a, d->bits, grid, cs(stream)) : launch_append<__nv_bfloat16, 128>(a, d->bits, grid, cs(stream));
+}
+
+int32_t svla_packed_attention(const svla_packed_attn_desc* d, svla_stream_t stream) {
+  const char* who = "svla_packed_attention";
+  if (!d) return fail(SVLA_ERR_ARG, "%s: null descriptor", who);
+  if (d->batch < 0 || d->total_q < 0 || d->total_k < 0) return fail(SVLA_ERR_ARG, "%s: negative batch, total_q or total_k", who);
+  if (int32_t rc = check_heads(who, d->hq, d->hkv, d->head_dim, d->dtype)) return rc;
+  const int g = d->hq / d->hkv;
+  if (g > packed_detail::kRows) return fail(SVLA_ERR_ARG, "%s: at most %d query heads per kv head (got %d)", who, packed_detail::kRows, g);
+  if (!d->cu_q || !d->cu_k) return fail(SVLA_ERR_ARG, "%s: cu_q or cu_k is null", who);
+  if (d->batch == 0 || d->total_q == 0) return SVLA_OK;
+  const int64_t qw = static_cast<int64_t>(d->hq) * d->head_dim, kw = static_cast<int64_t>(d->hkv) * d->head_dim;
+  if (int32_t rc = check_rows(who, "q", d->q, d->q_rs, qw)) return rc;
+  if (int32_t rc = check_rows(who, "o", d->o, d->o_rs, qw)) return rc;
+  if (d->total_k > 0) {
+    if (int32_t rc = check_rows(who, "k", d->k, d->k_rs, kw)) return rc;
+    if (int32_t rc = check_rows(who, "v", d->v, d->v_rs, kw)) return rc;
+  }
+  PackedAttnArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.q = d->q, a.k = d->k, a.v = d->v, a.o = d->o;
+  a.cu_q = d->cu_q, a.cu_k = d->cu_k;
+  a.q_rs = d->q_rs, a.k_rs = d->k_rs, a.v_rs = d->v_rs, a.o_rs = d->o_rs;
+  a.batch = d->batch, a.total_q = d->total_q, a.total_k = d->total_k, a.hq = d->hq, a.hkv = d->hkv, a.g = g;
+  a.causal = d->causal != 0;
+  a.scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt(static_cast<float>(d->head_dim))) * serving::kLog2e;
+  a.qt = packed_detail::kRows / g;
+  // the lengths are on the device: as many items as the sequences can have (each one's last tile may be short)
+  const long long items = (static_cast<long long>(d->total_q) / a.qt + d->batch) * d->hkv;
+  if (items > 0x7fffffffll) return fail(SVLA_ERR_ARG, "%s: too many query tiles", who);
+  const bool h = d->dtype == SVLA_DT_HALF;
+  if (d->head_dim == 64) return h ? launch_packed<__half, 64>(a, items, cs(stream)) : launch_packed<__nv_bfloat16, 64>(a, items, cs(stream));
+  return h ? launch_packed<__half, 128>(a, items, cs(stream)) : launch_packed<__nv_bfloat16, 128>(a, items, cs(stream));
+}
+
+size_t svla_paged_attention_workspace_size(int32_t batch, int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim) {
+  if (batch <= 0 || total_q <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || head_dim <= 0) return 0;
+  const long long ctas = static_cast<long long>(kPagedCtas) * sm_count();
+  return paged_part_bytes(ctas, paged_nt(batch, total_q, hq / hkv), head_dim) + static_cast<size_t>(2 * ctas) * sizeof(int4);
+}
+
+int32_t svla_paged_attention(const svla_paged_attn_desc* d, svla_stream_t stream) {
+  const char* who = "svla_paged_attention";
+  if (!d) return fail(SVLA_ERR_ARG, "%s: null descriptor", who);
+  if (d->batch < 0 || d->total_q < 0) return fail(SVLA_ERR_ARG, "%s: negative batch or total_q", who);
+  if (int32_t rc = check_heads(who, d->hq, d->hkv, d->head_dim, d->dtype)) return rc;
+  if (int32_t rc = check_cache(who, d->cache, d->bits, d->page_size, d->n_pages, d->page_table, d->page_table_rs, d->max_pages, d->kv_len)) return rc;
+  if (!d->cu_q) return fail(SVLA_ERR_ARG, "%s: cu_q is null", who);
+  if (d->batch == 0 || d->total_q == 0) return SVLA_OK;
+  const int64_t qw = static_cast<int64_t>(d->hq) * d->head_dim;
+  if (int32_t rc = check_rows(who, "q", d->q, d->q_rs, qw)) return rc;
+  if (int32_t rc = check_rows(who, "o", d->o, d->o_rs, qw)) return rc;
+  const size_t need = svla_paged_attention_workspace_size(d->batch, d->total_q, d->hq, d->hkv, d->head_dim);
+  if (!d->workspace || !aligned(d->workspace, 256) || d->workspace_bytes < need)
+    return fail(SVLA_ERR_ARG, "%s: workspace must be 256-byte aligned with at least %zu bytes (got %zu)", who, need, d->workspace_bytes);
+  PagedAttnArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.q = d->q, a.o = d->o, a.cache = static_cast<const uint8_t*>(d->cache);
+  a.cu_q = d->cu_q, a.kv_len = d->kv_len, a.table = d->page_table;
+  a.part = static_cast<float*>(d->workspace);
+  a.q_rs = d->q_rs, a.o_rs = d->o_rs, a.table_rs = d->page_table_rs;
+  a.batch = d->batch, a.total = d->total_q, a.hq = d->hq, a.hkv = d->hkv, a.g = d->hq / d->hkv;
+  a.page = d->page_size, a.n_pages = d->n_pages, a.max_pages = d->max_pages;
+  a.page_magic = ((1ull << 32) + a.page / 16 - 1) / (a.page / 16);
+  a.scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt(static_cast<float>(d->head_dim))) * serving::kLog2e;
+  a.err = device_error_ptr();
+  // items of at most 16 tiles (4 a warp) are not worth a second launch to join their parts
+  const long long most = (static_cast<long long>(d->max_pages) * d->page_size + paged_detail::kKeys - 1) / paged_detail::kKeys;
+  a.split = most > 16;
+  a.min_share = a.split ? 8 : 1;
+  const int nt = paged_nt(d->batch, d->total_q, a.g);
+  const bool h = d->dtype == SVLA_DT_HALF;
+  if (d->head_dim == 64) return h ? launch_paged<__half, 64>(a, d->bits, nt, cs(stream)) : launch_paged<__nv_bfloat16, 64>(a, d->bits, nt, cs(stream));
+  return h ? launch_paged<__half, 128>(a, d->bits, nt, cs(stream)) : launch_paged<__nv_bfloat16, 128>(a, d->bits, nt, cs(stream));
+}
+
+}  // extern "C"

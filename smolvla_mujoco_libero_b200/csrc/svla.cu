@@ -23,6 +23,7 @@
 #include "misc.cuh"
 #include "norm.cuh"
 #include "flow.cuh"
+#include "host.cuh"
 #include "process.cuh"
 #include "rope.cuh"
 
@@ -33,113 +34,6 @@ __device__ int g_device_error = 0;
 namespace {
 
 thread_local std::string t_last_error;
-
-int32_t fail(int32_t code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
-int32_t fail(int32_t code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  t_last_error = buf;
-  return code;
-}
-
-int32_t check_launch(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(SVLA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-  return SVLA_OK;
-}
-
-// Programmatic dependent launch (see pdl_wait in ptx.cuh): on by default, SVLA_PDL=0 turns it off.
-bool pdl_enabled() {
-  static int v = -1;
-  if (v < 0) {
-    const char* e = std::getenv("SVLA_PDL");
-    v = (e != nullptr && e[0] == '0') ? 0 : 1;
-  }
-  return v == 1;
-}
-
-template <typename... KArgs, typename... Args>
-int32_t launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                       const char* name, unsigned cluster_x, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int na = 0;
-  if (pdl_enabled()) {
-    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[na].val.programmaticStreamSerializationAllowed = 1;
-    ++na;
-  }
-  if (cluster_x > 1) {  // CTA pairs: clusters of cluster_x consecutive CTAs along x
-    attr[na].id = cudaLaunchAttributeClusterDimension;
-    attr[na].val.clusterDim.x = cluster_x;
-    attr[na].val.clusterDim.y = 1;
-    attr[na].val.clusterDim.z = 1;
-    ++na;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = na;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-  if (e != cudaSuccess) return fail(SVLA_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
-  return check_launch(name);
-}
-
-template <typename... KArgs, typename... Args>
-int32_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, const char* name,
-               Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-  if (e != cudaSuccess) return fail(SVLA_ERR_CUDA, "%s: %s", name, cudaGetErrorString(e));
-  return check_launch(name);
-}
-
-int* device_error_ptr() {
-  // one device-error word per device; the symbol address is per device
-  static int* ptrs[64] = {nullptr};
-  static std::mutex mu;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  std::lock_guard<std::mutex> lk(mu);
-  if (!ptrs[dev]) {
-    void* p = nullptr;
-    if (cudaGetSymbolAddress(&p, g_device_error) != cudaSuccess) return nullptr;
-    ptrs[dev] = static_cast<int*>(p);
-  }
-  return ptrs[dev];
-}
-
-// ---------------------------------------------------------------- TMA descriptors
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
 
 // 2D row-major [rows, cols] tensor, box [box_rows, box_cols]; cols is the contiguous dimension.
 int32_t make_tmap(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem_bytes, uint64_t cols,
@@ -226,19 +120,6 @@ int32_t dispatch_bn(int bn, int pair, Epi e, const GemmArgs& args, dim3 grid, cu
   return fail(SVLA_ERR_ARG, "block_n must be 64, 128 or 256 (got %d)", bn);
 }
 
-int sm_count() {
-  static int counts[64] = {0};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return 148;
-  if (counts[dev] == 0) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    counts[dev] = n;
-  }
-  return counts[dev];
-}
-
 // Tile width.  A k-stage costs about the same time at 64, 128 and 256 columns (measured), so a GEMM takes
 // about (rounds of tiles over the SMs) x (k-stages): take the width with the fewest rounds, the wider one on
 // a tie (pairs: at most 128 so two accumulator buffers fit TMEM).  When even 64-column tiles leave half of
@@ -263,7 +144,22 @@ int choose_block_n(const svla_gemm_desc* d, int sms) {
 
 }  // namespace
 
-// the last-error message of the calling thread, for the library's other translation units (engine.cpp)
+int* device_error_ptr() {
+  // one device-error word per device; the symbol address is per device
+  static int* ptrs[64] = {nullptr};
+  static std::mutex mu;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lk(mu);
+  if (!ptrs[dev]) {
+    void* p = nullptr;
+    if (cudaGetSymbolAddress(&p, g_device_error) != cudaSuccess) return nullptr;
+    ptrs[dev] = static_cast<int*>(p);
+  }
+  return ptrs[dev];
+}
+
+// the last-error message of the calling thread, for the library's other translation units
 int32_t set_error(int32_t code, const std::string& msg) {
   t_last_error = msg;
   return code;
@@ -468,8 +364,6 @@ int32_t run_gemm(const svla_gemm_desc* d, cudaStream_t stream) {
 }  // namespace svla
 
 using namespace svla;
-
-static inline cudaStream_t cs(svla_stream_t s) { return reinterpret_cast<cudaStream_t>(s); }
 
 extern "C" {
 

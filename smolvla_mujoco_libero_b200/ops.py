@@ -335,10 +335,219 @@ def rope_attention(q_raw: torch.Tensor, k_raw: torch.Tensor, v_raw: torch.Tensor
     return ctx
 
 
+def rope_table_wide(max_pos: int, max_wavelength: float, device, head_dim: int = 64) -> torch.Tensor:
+    """(cos, sin) [max_pos, head_dim / 2, 2] from angles in 64 bits: the table of ``kv_append`` (``rope_table`` keeps the
+    reference's fp32 angles and its width of 64)."""
+    cs = torch.empty(max_pos, head_dim // 2, 2, dtype=torch.float32, device=device)
+    check(lib().svla_rope_table_wide(_p(cs), max_pos, head_dim, float(max_wavelength), _stream()), "rope_table_wide")
+    return cs
+
+
 def rope_table(max_pos: int, max_wavelength: float, device) -> torch.Tensor:
     cs = torch.empty(max_pos, 32, 2, dtype=torch.float32, device=device)
     check(lib().svla_rope_table(_p(cs), max_pos, float(max_wavelength), _stream()), "rope_table")
     return cs
+
+
+# ----------------------------------------------------------------------------- serving: packed prompts, paged cache
+
+_DT16 = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_HALF}
+
+
+def _packed(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> None:
+    """t: [rows, heads, head_dim] bf16 / fp16 on the current device, heads next to each other (any row stride)."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
+    if t.dim() != 3 or t.dtype not in _DT16:
+        raise ValueError(f"{name} must be bf16 or fp16 [rows, heads, head_dim], got {t.dtype} {tuple(t.shape)}")
+    h, d = t.shape[1], t.shape[2]
+    rs, hs, es = t.stride()
+    if t.numel() and ((es != 1 and d > 1) or (hs != d and h > 1)):
+        raise ValueError(f"{name}: the heads of a row must lie next to each other (strides {t.stride()})")
+    if like is None:
+        if t.device.index != torch.cuda.current_device():
+            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    elif t.dtype != like.dtype or t.device != like.device or d != like.shape[2]:
+        raise ValueError(f"{name} must be {like.dtype} with head_dim {like.shape[2]} on {like.device}")
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between rows; a single row's stride does not matter to torch, so it is not taken from it."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _ints(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> None:
+    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 {list(shape)} on {device}, got {t.dtype} {list(t.shape)} "
+                         f"on {t.device}")
+
+
+def _batch_of(cu: torch.Tensor, name: str, device: torch.device) -> int:
+    if cu.dim() != 1 or cu.shape[0] < 1:
+        raise ValueError(f"{name} must be int32 [batch + 1]")
+    _ints(cu, name, (cu.shape[0],), device)
+    return cu.shape[0] - 1
+
+
+def kv_cache(n_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 16,
+             dtype: torch.dtype = torch.bfloat16, device="cuda") -> torch.Tensor:
+    """An empty paged cache of one layer: ``[n_pages, kv_heads, 2, page_size, head_dim]`` of the dtype, or with
+    ``bits=4`` uint8 ``[n_pages, kv_heads, page_size, head_dim + head_dim / 4]`` (svla.h describes a page's bytes)."""
+    if bits not in (4, 16) or page_size < 16 or page_size > 256 or page_size % 16 or head_dim not in (64, 128):
+        raise ValueError(f"kv_cache: bits 4 or 16, page_size a multiple of 16 up to 256, head_dim 64 or 128 "
+                         f"(got {bits}, {page_size}, {head_dim})")
+    if bits == 4:
+        return torch.zeros(n_pages, kv_heads, page_size, head_dim + head_dim // 4, dtype=torch.uint8, device=device)
+    if dtype not in _DT16:
+        raise ValueError(f"kv_cache: dtype must be bf16 or fp16, got {dtype}")
+    return torch.zeros(n_pages, kv_heads, 2, page_size, head_dim, dtype=dtype, device=device)
+
+
+def _cache(cache: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, batch: int, like: torch.Tensor,
+           hkv: int) -> tuple[int, int]:
+    """(bits, page_size) of a cache that fits packed rows like ``like``."""
+    d, dev = like.shape[2], like.device
+    if cache.device != dev or not cache.is_contiguous():
+        raise ValueError(f"cache must be contiguous on {dev}")
+    if cache.dim() == 5:
+        bits, page = 16, cache.shape[3]
+        ok = cache.dtype == like.dtype and cache.shape[2] == 2 and cache.shape[4] == d
+    else:
+        bits, page = 4, (cache.shape[2] if cache.dim() == 4 else 0)
+        ok = cache.dtype == torch.uint8 and page > 0 and cache.shape[3] == d + d // 4
+    if not ok or cache.shape[1] != hkv:
+        raise ValueError(f"cache {cache.dtype} {list(cache.shape)} does not hold {hkv} kv heads of {like.dtype} "
+                         f"[{d}] (see kv_cache)")
+    _ints(kv_len, "kv_len", (batch,), dev)
+    if (page_table.dtype != torch.int32 or page_table.device != dev or page_table.dim() != 2
+            or page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+        raise ValueError(f"page_table must be int32 [{batch}, max_pages] on {dev} with unit column stride")
+    return bits, page
+
+
+def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+              page_table: torch.Tensor, q: torch.Tensor | None = None, rope_cs: torch.Tensor | None = None,
+              pos: torch.Tensor | None = None, q_out: torch.Tensor | None = None, want_rows: bool = False,
+              k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None):
+    """Append packed keys / values ([rows, kv_heads, head_dim], sequence b's in rows cu_q[b] .. cu_q[b + 1] - 1) to a
+    paged cache; kv_len [B] counts them.  With ``rope_cs`` ([max_pos, head_dim / 2, 2], ``rope_table_wide``) keys and the
+    queries ``q`` are rotated at ``pos`` [rows], or at the entry's index.  Returns the rotated queries (None without q), or
+    with ``want_rows`` (q, k, v): the appended rows as the cache holds them, which prompt attention takes.  The outputs may
+    be the inputs (in place)."""
+    _packed(k, "k")
+    _packed(v, "v", k)
+    rows, hkv, d = k.shape
+    dev = k.device
+    if v.shape != k.shape:
+        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    batch = _batch_of(cu_q, "cu_q", dev)
+    bits, page = _cache(cache, page_table, kv_len, batch, k, hkv)
+    hq = 0
+    if q is not None:
+        _packed(q, "q", k)
+        hq = q.shape[1]
+        if q.shape[0] != rows:
+            raise ValueError(f"q has {q.shape[0]} rows, k {rows}")
+        if q_out is None:
+            q_out = torch.empty(rows, hq, d, dtype=q.dtype, device=dev)
+        else:
+            _packed(q_out, "q_out", k)
+            if q_out.shape != q.shape:
+                raise ValueError("q_out must have q's shape")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    if want_rows:
+        k_out = torch.empty(rows, hkv, d, dtype=k.dtype, device=dev) if k_out is None else k_out
+        v_out = torch.empty(rows, hkv, d, dtype=k.dtype, device=dev) if v_out is None else v_out
+    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
+        if t is not None:
+            _packed(t, name, k)
+            if t.shape != k.shape:
+                raise ValueError(f"{name} must have k's shape")
+    max_pos = 0
+    if rope_cs is not None:
+        if (rope_cs.dtype != torch.float32 or rope_cs.device != dev or rope_cs.dim() != 3
+                or rope_cs.shape[1:] != (d // 2, 2) or not rope_cs.is_contiguous()):
+            raise ValueError(f"rope_cs must be contiguous fp32 [max_pos, {d // 2}, 2] on {dev}")
+        max_pos = rope_cs.shape[0]
+    if pos is not None:
+        _ints(pos, "pos", (rows,), dev)
+    if rows:
+        desc = L.KvAppendDesc(_p(q), k.data_ptr(), v.data_ptr(), _p(q_out), _p(k_out), _p(v_out), cache.data_ptr(),
+                              cu_q.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), _p(pos), _p(rope_cs),
+                              0 if q is None else _row_stride(q), _row_stride(k), _row_stride(v),
+                              0 if q is None else _row_stride(q_out), 0 if k_out is None else _row_stride(k_out),
+                              0 if v_out is None else _row_stride(v_out),
+                              page_table.stride(0) if batch > 1 else page_table.shape[1], batch, rows, hq, hkv, d,
+                              _DT16[k.dtype], bits, page, cache.shape[0], page_table.shape[1], max_pos)
+        check(lib().svla_kv_append(ctypes.byref(desc), _stream()), "svla_kv_append")
+    return (q_out, k_out, v_out) if want_rows else q_out
+
+
+def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                     cu_k: torch.Tensor | None = None, causal: bool = True, scale: float = 0.0,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention over prompts of different lengths packed back to back: q [rows, heads, head_dim], k / v
+    [rows_k, kv_heads, head_dim] (views of one projection's output are fine), sequence b in rows cu_q[b] ..
+    cu_q[b + 1] - 1 of q and cu_k[b] .. of k and v (cu_k None: the same).  Causal: the queries are the last tokens of
+    their sequence.  Returns [rows, heads, head_dim]; rows behind the last sequence are left as they are in ``out``
+    (undefined without it)."""
+    _packed(q, "q")
+    _packed(k, "k", q)
+    _packed(v, "v", q)
+    if v.shape != k.shape:
+        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    dev = q.device
+    batch = _batch_of(cu_q, "cu_q", dev)
+    if cu_k is None:
+        cu_k = cu_q
+    else:
+        _ints(cu_k, "cu_k", (batch + 1,), dev)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _packed(out, "out", q)
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+    rows, hq, d = q.shape
+    desc = L.PackedAttnDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
+                            _row_stride(q), _row_stride(k), _row_stride(v), _row_stride(out), batch, rows, k.shape[0],
+                            hq, k.shape[1], d, _DT16[q.dtype], int(causal), float(scale))
+    check(lib().svla_packed_attention(ctypes.byref(desc), _stream()), "svla_packed_attention")
+    return out
+
+
+def paged_attention(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+                    page_table: torch.Tensor, scale: float = 0.0, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the newest tokens (q [rows, heads, head_dim], sequence b's in rows cu_q[b] .. cu_q[b + 1] - 1, already
+    appended) over a paged cache of 16 or 4 bits; kv_len [B] entries, pages in page_table [B, max_pages].  Returns
+    [rows, heads, head_dim].  ``workspace``: uint8 of svla_paged_attention_workspace_size bytes, taken from torch's
+    allocator when None."""
+    _packed(q, "q")
+    dev = q.device
+    batch = _batch_of(cu_q, "cu_q", dev)
+    rows, hq, d = q.shape
+    hkv = cache.shape[1] if cache.dim() > 1 else 0
+    bits, page = _cache(cache, page_table, kv_len, batch, q, hkv)
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    else:
+        _packed(out, "out", q)
+        if out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+    handle = lib()
+    if workspace is None:
+        need = handle.svla_paged_attention_workspace_size(batch, rows, hq, hkv, d)
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous uint8 on {dev}")
+    desc = L.PagedAttnDesc(q.data_ptr(), cache.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(),
+                           page_table.data_ptr(), workspace.data_ptr(), workspace.numel(), _row_stride(q),
+                           _row_stride(out), page_table.stride(0) if batch > 1 else page_table.shape[1], batch, rows, hq,
+                           hkv, d, _DT16[q.dtype], bits, page, cache.shape[0], page_table.shape[1], float(scale))
+    check(handle.svla_paged_attention(ctypes.byref(desc), _stream()), "svla_paged_attention")
+    return out
 
 
 # ----------------------------------------------------------------------------- torch custom ops
