@@ -183,7 +183,7 @@ SIGNATURES = {
     "svla_rope_table_wide": (c_int32, [c_void_p, c_int32, c_int32, ctypes.c_double, c_void_p]),
     "svla_kv_append": (c_int32, [POINTER(KvAppendDesc), c_void_p]),
     "svla_packed_attention": (c_int32, [POINTER(PackedAttnDesc), c_void_p]),
-    "svla_paged_attention_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "svla_paged_attention_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int64]),
     "svla_paged_attention": (c_int32, [POINTER(PagedAttnDesc), c_void_p]),
     "svla_build_masks": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),

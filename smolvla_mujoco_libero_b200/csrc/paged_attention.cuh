@@ -5,10 +5,11 @@
 // Bound by the bytes of the live cache; the work around them has to stay below what an SM issues in the time they
 // take (4 bits, D = 64: 1280 bytes, 55 cycles, per 16 entries of one head).
 //
-// Shape of the products.  Keys are the M side: S^T (16 entries x 8 query rows) = K Q^T, O^T (16 dimensions x 8 query
+// Shape of the products.  Entries are the M side: S^T (16 entries x 8 query rows) = K Q^T, O^T (16 dimensions x 8 query
 // rows) += V^T P^T.  A query row is a (token, head) of one kv head, packed token-major, so grouped heads and several
-// tokens share every key that is read; 8 rows fit one MMA column block, and single tokens of up to 8 grouped heads
-// waste half of what 16 query rows would.
+// tokens share every entry that is read; 8 rows fit one MMA column block, and single tokens of up to 8 grouped heads
+// waste half of what 16 query rows would (that form, without the transposition of P, takes twice the products and
+// registers and measured 60 us where this one takes 50).
 //
 // 4-bit entries are never expanded to 16-bit values.  A nibble c masked out of a word, as it stands, is the fp16
 // subnormal c 2^-24 (or 16 c 2^-24 for the second nibble of a byte): tensor cores take subnormals exactly, so one AND
@@ -18,15 +19,19 @@
 //   sum_n p_n v_n = sum_n (p_n step_n) c_n + sum_n p_n low_n
 // takes p_n step_n as the other operand.  Query rows are scaled by a power of two to the top of fp16's range (exact but
 // for components below 2^-25 of the row's largest), so bf16 queries lose nothing.  p_n step_n is rounded to fp16
-// (2^-12 relative); to keep it in fp16's range whatever the steps are, the running maximum is taken over
-// score + exponent(largest step of the entry) instead of the score.  Products with low_n stay in fp32.
+// (2^-11 relative); to keep it in fp16's range whatever the steps are, p_n carries the factor 2^-e of the largest step
+// seen so far, 2^e <= step < 2^(e + 1), besides that of the running maximum (both cancel in O / l).  Products with low_n
+// stay in fp32.
 //
 // Every warp works alone: its own tiles of 32 entries through its own ring of asynchronous copies, its own running
 // maximum, sum and O, no barrier in the loop.  The maximum is lazy: it moves (and O is rescaled) only when a score
-// passes it by more than 8 in log2 units, one vote per tile instead of shuffles.
+// passes it by more than 8 in log2 units (or a step 2^(e + 1)), one vote per tile instead of shuffles.  Instruction issue
+// is what stands beside the memory system: the two query columns of a thread go through packed fp32 operations, a page's
+// address is worked out once by one lane for 16 tiles, and the masks are in a branch that only a sequence's end takes.
 //
-// Work split.  All tiles of all (sequence, kv head, query tile) items form one line; every CTA takes an equal piece of
-// it, whatever the sequences' lengths are, and finds its place from cu_q and kv_len on the device.  An item that lies in
+// Work split.  All tiles of all (sequence, kv head, query tile) items form one line, each item 512 entries longer than it
+// is (what its start and its join cost: without that, pieces of many short items came last, 58 us where 44 do); every CTA
+// takes an equal piece of it, whatever the sequences' lengths are, and finds its place from cu_q and kv_len on the device.  An item that lies in
 // one CTA is finished there; one cut by a piece's border leaves partials (maximum, sum, O in fp32) in the workspace,
 // which the combine kernel joins in the line's order, so results do not depend on timing.
 #pragma once
@@ -48,22 +53,42 @@ struct PagedAttnArgs {
   unsigned long long page_magic;  // ceil(2^32 / (page / 16)): 16-entry slab -> page
   int split;               // 0: items are not cut
   int min_share;           // tiles a piece has at least
+  int item_cost;           // what an item costs beside its tiles, in tiles
   float scale_log2;
   int* err;
 };
 
 namespace paged_detail {
 constexpr int kWarps = 4;
-constexpr int kKeys = 32;  // entries per tile: two 16-entry slabs, each inside one page
-constexpr int kStages = 3;
 
 template <int D, int BITS>
 struct Tile {
+  // entries per tile, in 16-entry slabs that lie inside one page each: enough independent work per warp to cover the
+  // latency of the chain from scores to products, and 5 to 8 KB per copy
+  static constexpr int kKeys = BITS == 4 ? (D == 64 ? 64 : 32) : (D == 64 ? 32 : 16);
+  static constexpr int kSlabs = kKeys / 16;
+  static constexpr int kStages = 3;                        // tiles in a warp's ring
   static constexpr int kRow = BITS == 16 ? D * 2 : D / 2;  // bytes of an entry's key (or value)
   static constexpr int kPairs = BITS == 16 ? 0 : D / 8;    // bytes of its (step, low) pairs
   static constexpr int kK = 0, kV = kKeys * kRow, kKP = 2 * kKeys * kRow, kVP = kKP + kKeys * kPairs;
   static constexpr int kBytes = 2 * kKeys * (kRow + kPairs);
 };
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// an entry's (step, low) pairs
+__device__ __forceinline__ void load_pairs(uint32_t (&p)[2], const uint8_t* src) {
+  const uint2 u = *reinterpret_cast<const uint2*>(src);
+  p[0] = u.x, p[1] = u.y;
+}
+__device__ __forceinline__ void load_pairs(uint32_t (&p)[4], const uint8_t* src) {
+  const uint4 u = *reinterpret_cast<const uint4*>(src);
+  p[0] = u.x, p[1] = u.y, p[2] = u.z, p[3] = u.w;
+}
 
 // rows of a (sequence, kv head) and their tiles
 template <int NT>
@@ -75,20 +100,23 @@ __device__ __forceinline__ int query_tiles(int n_new, int g) {
 template <typename T, int D, int BITS, int NT>
 struct PagedSmem {
   static constexpr int kRows = 8 * NT;
-  static constexpr int kRing = paged_detail::kStages * paged_detail::Tile<D, BITS>::kBytes;  // per warp
+  static constexpr int kRing = paged_detail::Tile<D, BITS>::kStages * paged_detail::Tile<D, BITS>::kBytes;  // per warp
   static constexpr int kJoin = kRows * (D + 1 + 2) * 4;  // per warp: O, maximum, sum
   static constexpr int kPerWarp = kRing > kJoin ? kRing : (kJoin + 15) / 16 * 16;
   static constexpr int kBytes = paged_detail::kWarps * kPerWarp;
 };
 
+// single tokens at D = 64: three CTAs per SM (four, at 128 registers, measured 51 us where three take 48)
 template <typename T, int D, int BITS, int NT>
-__global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_kernel(const PagedAttnArgs a) {
+__global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1) ? 3 : 1)
+    paged_attention_kernel(const PagedAttnArgs a) {
   using namespace paged_detail;
   using serving::copy16;
   using Tl = Tile<D, BITS>;
   using Sm = PagedSmem<T, D, BITS, NT>;
   using serving::mma16816;
-  constexpr int kRows = 8 * NT, kGroups = D / 32;
+  constexpr int kRows = 8 * NT, kGroups = D / 32, kStages = Tl::kStages, kKeys = Tl::kKeys, kSlabs = Tl::kSlabs;
+  constexpr int kBatch = 32 / kSlabs;  // tiles whose pages a warp holds
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int place[2];         // first sequence of this CTA's piece, and ...
   __shared__ long long place64[3]; // its start on the line; the piece
@@ -100,7 +128,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
   // entries a sequence really has: its table's reach bounds them
   const long long reach = static_cast<long long>(a.max_pages) * a.page;
   auto entries = [&](int b) { return static_cast<int>(min(static_cast<long long>(max(__ldg(a.kv_len + b), 0)), reach)); };
-  auto tiles_of = [&](int len) { return a.split ? max((len + kKeys - 1) / kKeys, 1) : 1; };  // on the line, per item
+  auto tiles_of = [&](int len) { return a.split ? (len + kKeys - 1) / kKeys + a.item_cost : 1; };  // on the line, per item
   auto weight = [&](int b) -> long long {
     const serving::Span s = serving::span_of(a.cu_q, b, a.total);
     return static_cast<long long>(tiles_of(entries(b))) * query_tiles<NT>(s.end - s.begin, a.g) * a.hkv;
@@ -150,6 +178,25 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
   const long long full_share = from > 0 ? from / blockIdx.x : share;
   const long long page_bytes = BITS == 16 ? 4ll * a.page * D : static_cast<long long>(a.page) * (D + D / 4);
 
+  const int slabs_per_page = a.page / 16;
+  // where a lane finds its words of a slab (4 bits; the swizzles of `issue`)
+  int k_at[kGroups], k_at2[kGroups], v_at[kGroups], v_at2[kGroups];
+  if constexpr (BITS == 4) {
+    auto swz = [](int r) { return D == 64 ? (r >> 2) & 1 : (r >> 1) & 3; };
+#pragma unroll
+    for (int gr = 0; gr < kGroups; ++gr) {
+      k_at[gr] = g8 * Tl::kRow + ((gr ^ swz(g8)) * 16) + t4 * 4;
+      k_at2[gr] = (g8 + 8) * Tl::kRow + ((gr ^ swz(g8 + 8)) * 16) + t4 * 4;
+      v_at[gr] = 2 * t4 * Tl::kRow + ((gr ^ swz(2 * t4)) * 16) + (g8 >> 1) * 4;
+      v_at2[gr] = (2 * t4 + 8) * Tl::kRow + ((gr ^ swz(2 * t4 + 8)) * 16) + (g8 >> 1) * 4;
+    }
+  }
+  const uint32_t v_sel = (g8 & 1) ? 0x7632u : 0x5410u;
+  // 4 bits: this lane's chunk of a slab's (step, low) pairs, first the keys', then the values'
+  const int pair_is_v = lane / (D / 8), pair_c = lane % (D / 8);
+  const int pair_dst = (pair_is_v ? Tl::kVP : Tl::kKP) + pair_c * 16;
+  const int pair_src = a.page * D + (pair_is_v ? a.page * (D / 8) : 0) + pair_c * 16;
+
   while (cur < to) {
     // ---- the item at `cur`
     const serving::Span sq = serving::span_of(a.cu_q, b, a.total);
@@ -169,19 +216,90 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
     const bool whole = cur == item_at && seg_end == item_at + n_tiles;
     // tiles of the sequence in this segment (an uncut item: all of them)
     const int real_tiles = (len + kKeys - 1) / kKeys;
-    const int tile0 = a.split ? static_cast<int>(cur - item_at) : 0;
-    int tile1 = a.split ? min(static_cast<int>(seg_end - item_at), real_tiles) : real_tiles;
+    const int tile0 = a.split ? max(static_cast<int>(cur - item_at) - a.item_cost, 0) : 0;
+    int tile1 = a.split ? min(static_cast<int>(seg_end - item_at) - a.item_cost, real_tiles) : real_tiles;
     const int row0 = qt * kRows, rows = min(kRows, n_new * a.g - row0);
     // entries the last / first row of this query tile sees
     const int sees_last = min(max(len - n_new + (row0 + rows - 1) / a.g + 1, 0), len);
     const int sees_first = min(max(len - n_new + row0 / a.g + 1, 0), len);
     tile1 = min(tile1, (sees_last + kKeys - 1) / kKeys);
 
-    // ---- Q^T operands: column g8 of block nt is row row0 + nt * 8 + g8
+    // ---- this warp's tiles: tile0 + warp, + 4, ...
+    const int mine = tile1 - tile0 - warp > 0 ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;
+    // Slab s of the warp's i-th tile: lane kSlabs (i % kBatch) + s holds the byte offset of this kv head's part of its
+    // page, with slot / 16 in the low four bits (parts are multiples of 16 bytes); -1: there is nothing to read.
+    auto load_pages = [&](int i0, unsigned& bad) -> long long {
+      const int i = i0 + lane / kSlabs;
+      long long off = -1;
+      bool wrong = false;
+      if (i < mine) {
+        const int slab = (tile0 + warp + i * kWarps) * kSlabs + lane % kSlabs;
+        if (slab * 16 < sees_last) {
+          const int pg = static_cast<int>((static_cast<unsigned long long>(slab) * a.page_magic) >> 32);
+          const int id = __ldg(a.table + static_cast<size_t>(b) * a.table_rs + pg);
+          wrong = id < 0 || id >= a.n_pages;
+          if (!wrong) off = (static_cast<long long>(id) * a.hkv + kh) * page_bytes + (slab - pg * slabs_per_page);
+        }
+      }
+      if (wrong) record_error(a.err, serving::kErrBadPage);
+      bad = __ballot_sync(0xffffffffu, wrong);
+      return off;
+    };
+    unsigned bad, bad_next;
+    long long pages = load_pages(0, bad), pages_next = load_pages(kBatch, bad_next);
+    // copies tile i of the warp into its ring stage
+    auto issue = [&](int i, long long offs) {
+      uint8_t* st = ring + (i % kStages) * Tl::kBytes;
+#pragma unroll
+      for (int s = 0; s < kSlabs; ++s) {
+        const long long off = __shfl_sync(0xffffffffu, offs, kSlabs * (i % kBatch) + s);
+        const bool have = off >= 0;
+        const uint8_t* base = a.cache + (have ? off & ~15ll : 0);
+        const int slot = (static_cast<int>(off) & 15) * 16;
+        if constexpr (BITS == 16) {
+          constexpr int kChunks = D / 8;  // 16-byte chunks of a row; chunk c of row r sits at c ^ (r % 8)
+          // entries past the sequence are zeros, whatever the page holds there
+          const int left = have ? len - ((tile0 + warp + i * kWarps) * kKeys + s * 16) : 0;
+          const uint8_t* src = base + slot * (2 * D) + lane * 16;
+          const int v_off = a.page * (2 * D);
+#pragma unroll
+          for (int u = 0; u < kChunks / 2; ++u) {
+            const int idx = lane + u * 32, r = idx / kChunks, c = idx % kChunks;
+            const int n = r < left ? 16 : 0;
+            const int dst = (s * 16 + r) * Tl::kRow + ((c ^ (r & 7)) * 16);
+            copy16(st + Tl::kK + dst, src + u * 512, n);
+            copy16(st + Tl::kV + dst, src + u * 512 + v_off, n);
+          }
+        } else {
+          constexpr int kChunks = D / 32;  // chunk c (one group's codes) of row r sits at c ^ swizzle(r): no bank conflicts
+          const int n = have ? 16 : 0;
+          const uint8_t* src = base + slot * (D / 2) + lane * 16;
+          const int v_off = a.page * (D / 2);
+#pragma unroll
+          for (int u = 0; u < kChunks / 2; ++u) {
+            const int idx = lane + u * 32, r = idx / kChunks, c = idx % kChunks;
+            const int sw = D == 64 ? (r >> 2) & 1 : (r >> 1) & 3;
+            const int dst = (s * 16 + r) * Tl::kRow + ((c ^ sw) * 16);
+            copy16(st + Tl::kK + dst, src + u * 512, n);
+            copy16(st + Tl::kV + dst, src + u * 512 + v_off, n);
+          }
+          if (lane < D / 4)  // 16 entries' pairs: D / 8 chunks for keys, D / 8 for values
+            copy16(st + pair_dst + s * 16 * Tl::kPairs, base + pair_src + slot * (D / 8), n);
+        }
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+      if (i < mine) issue(i, pages);
+      serving::copy_commit();
+    }
+
+    // ---- Q^T operands: column g8 of block nt is row row0 + nt * 8 + g8; a missing row is zeros
     constexpr int kQRegs = BITS == 16 ? D / 16 * 2 : kGroups * 4;
     uint32_t qb[NT][kQRegs];
-    float qf[NT][2];            // 4 bits: factor of this thread's two score columns (queries 2 t4, 2 t4 + 1)
+    float qf[NT][2];            // factors of this thread's two score columns (queries 2 t4, 2 t4 + 1)
     float qs[NT][kGroups][2];   // 4 bits: sums of their components, per group, times scale
+    float big_limit = 0.f;      // 4 bits: a step from here on moves the exponent e
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = row0 + nt * 8 + g8;
@@ -219,10 +337,10 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
           for (int gr = 0; gr < kGroups; ++gr) sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], d);
         }
         // up = 2^(14 - exponent of the largest component): the row then fills fp16's range (largest in [2^14, 2^15))
-        int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-        e = (top > 0.f && e < 128) ? max(e, -100) : 14;
-        const float up = __uint_as_float(static_cast<uint32_t>(14 - e + 127) << 23);
-        const float f = ldexpf(a.scale_log2, 24 + e - 14);  // undoes 2^-24 of the codes and `up`
+        int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
+        ex = (top > 0.f && ex < 128) ? max(ex, -100) : 14;
+        const float up = __uint_as_float(static_cast<uint32_t>(14 - ex + 127) << 23);
+        const float f = ldexpf(a.scale_log2, 24 + ex - 14);  // undoes 2^-24 of the codes and `up`
 #pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) {
           // step 0 of the group: (n0, n4 | n1, n5), step 1: (n2, n6 | n3, n7); odd nibbles count 16 times
@@ -251,110 +369,42 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
         sees[nt][u] = min(max(len - n_new + r / a.g + 1, 0), len);
       }
 
-    // ---- this warp's tiles: tile0 + warp, + 4, ...
-    const int mine = tile1 - tile0 - warp > 0 ? (tile1 - tile0 - warp + kWarps - 1) / kWarps : 0;
-    // page of slab s of the warp's i-th tile: lane 2 (i % 16) + s of `pages` (this batch of 16 tiles) or `pages_next`
-    auto load_pages = [&](int i0) -> int {
-      const int i = i0 + (lane >> 1);
-      if (i >= mine) return -1;
-      const int slab = (tile0 + warp + i * kWarps) * (kKeys / 16) + (lane & 1);
-      if (slab * 16 >= sees_last) return -1;
-      const int pg = static_cast<int>((static_cast<unsigned long long>(slab) * a.page_magic) >> 32);
-      const int id = __ldg(a.table + static_cast<size_t>(b) * a.table_rs + pg);
-      if (id >= 0 && id < a.n_pages) return id;
-      record_error(a.err, serving::kErrBadPage);
-      return -1;
-    };
-    int pages = load_pages(0), pages_next = load_pages(16);
-    const int slabs_per_page = a.page / 16;
-    // copies tile i of the warp into its ring stage; returns nothing, the validity is read again from the page ids
-    auto issue = [&](int i, int ids) {
-      uint8_t* st = ring + (i % kStages) * Tl::kBytes;
-      const int tile = tile0 + warp + i * kWarps;
-#pragma unroll
-      for (int s = 0; s < kKeys / 16; ++s) {
-        const int id = __shfl_sync(0xffffffffu, ids, 2 * (i & 15) + s);
-        const int slab = tile * (kKeys / 16) + s;
-        const int pg = static_cast<int>((static_cast<unsigned long long>(slab) * a.page_magic) >> 32);
-        const int slot = (slab - pg * slabs_per_page) * 16;
-        const uint8_t* base = a.cache + (static_cast<size_t>(id < 0 ? 0 : id) * a.hkv + kh) * page_bytes;
-        if constexpr (BITS == 16) {
-          constexpr int kChunks = D / 8;  // 16-byte chunks of a row; chunk c of row r sits at c ^ (r % 8)
-#pragma unroll
-          for (int u = 0; u < kChunks / 2; ++u) {
-            const int idx = lane + u * 32, r = idx / kChunks, c = idx % kChunks;
-            // entries past the sequence are zeros, whatever the page holds there
-            const int n = (id >= 0 && slab * 16 + r < len) ? 16 : 0;
-            const uint8_t* src = base + static_cast<size_t>(slot + r) * (2 * D) + c * 16;
-            const int dst = (s * 16 + r) * Tl::kRow + ((c ^ (r & 7)) * 16);
-            copy16(st + Tl::kK + dst, src, n);
-            copy16(st + Tl::kV + dst, src + static_cast<size_t>(a.page) * (2 * D), n);
-          }
-        } else {
-          constexpr int kChunks = D / 32;  // chunk c (one group's codes) of row r sits at c ^ swizzle(r): no bank conflicts
-          const int n = id >= 0 ? 16 : 0;
-#pragma unroll
-          for (int u = 0; u < kChunks / 2; ++u) {
-            const int idx = lane + u * 32, r = idx / kChunks, c = idx % kChunks;
-            const int sw = D == 64 ? (r >> 2) & 1 : (r >> 1) & 3;
-            const uint8_t* src = base + static_cast<size_t>(slot + r) * (D / 2) + c * 16;
-            const int dst = (s * 16 + r) * Tl::kRow + ((c ^ sw) * 16);
-            copy16(st + Tl::kK + dst, src, n);
-            copy16(st + Tl::kV + dst, src + static_cast<size_t>(a.page) * (D / 2), n);
-          }
-          if (lane < D / 4) {  // 16 entries' pairs: D / 8 chunks for keys, D / 8 for values
-            const int is_v = lane / (D / 8), c = lane % (D / 8);
-            const uint8_t* src = base + static_cast<size_t>(a.page) * D +
-                                 (static_cast<size_t>(is_v ? a.page : 0) + slot) * (D / 8) + c * 16;
-            copy16(st + (is_v ? Tl::kVP : Tl::kKP) + s * 16 * Tl::kPairs + c * 16, src, n);
-          }
-        }
-      }
-    };
-
     float o[NT][D / 16][4];     // O^T: see the P.V product for which dimensions a thread holds
-    float om[NT][kGroups][2];   // 4 bits: sum of p low
-    float m[NT][2], l[NT][2];
+    float om[NT][kGroups][2];   // 4 bits: sums of p low
+    float m[NT][2], ref[NT][2], l[NT][2];
+    float e = -60.f;            // 4 bits: exponent of the largest step so far (not below 2^-60: see below)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
 #pragma unroll
       for (int gr = 0; gr < kGroups; ++gr) om[nt][gr][0] = om[nt][gr][1] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) m[nt][u] = -INFINITY, ref[nt][u] = 0.f, l[nt][u] = 0.f;
     }
 
-#pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-      if (i < mine) issue(i, pages);
-      serving::copy_commit();
-    }
     for (int i = 0; i < mine; ++i) {
       // refill the stage that tile i - 1 used (every lane has passed the __syncwarp that ends tile i - 1)
       const int ahead = i + kStages - 1;
-      if (ahead < mine) issue(ahead, (ahead >> 4) == (i >> 4) ? pages : pages_next);
+      if (ahead < mine) issue(ahead, ahead / kBatch == i / kBatch ? pages : pages_next);
       serving::copy_commit();
       serving::copy_wait<kStages - 1>();
       __syncwarp();
       const uint8_t* st = ring + (i % kStages) * Tl::kBytes;
       const int key0 = (tile0 + warp + i * kWarps) * kKeys;
-      int ids[2];
-      ids[0] = __shfl_sync(0xffffffffu, pages, 2 * (i & 15));
-      ids[1] = __shfl_sync(0xffffffffu, pages, 2 * (i & 15) + 1);
-      if ((i & 15) == 15) {
+      const unsigned gone = (bad >> (kSlabs * (i % kBatch))) & ((1u << kSlabs) - 1u);  // slabs without a page
+      if (i % kBatch == kBatch - 1) {
         pages = pages_next;
-        pages_next = load_pages(i + 17);
+        bad = bad_next;
+        pages_next = load_pages(i + 1 + kBatch, bad_next);
       }
       // some entry of the tile is hidden from some row (warp-uniform)
-      const bool edge = key0 + kKeys > sees_first || ids[0] < 0 || ids[1] < 0;
+      const bool edge = key0 + kKeys > sees_first || gone != 0u;
 
       // ---- scores, in log2 units: s[nt][slab][e]: entry slab * 16 + g8 + 8 (e / 2), query column 2 t4 + e % 2
-      float s[NT][2][4];
-      float vstep[2][2][kGroups], vlow[2][2][kGroups];  // [slab][row half][group] of this thread's entries
-      float lift[2][2];  // log2 bound of the entry's steps (0 for 16 bits)
+      float s[NT][kSlabs][4];
 #pragma unroll
-      for (int sl = 0; sl < 2; ++sl) {
+      for (int sl = 0; sl < kSlabs; ++sl) {
         if constexpr (BITS == 16) {
           float acc[NT][4];
 #pragma unroll
@@ -370,51 +420,27 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[nt][sl][e] = acc[nt][e] * qf[nt][e & 1];
-          lift[sl][0] = lift[sl][1] = 0.f;
+            for (int x = 0; x < 4; ++x) s[nt][sl][x] = acc[nt][x] * qf[nt][x & 1];
         } else {
           float acc[NT][kGroups][4];
-          const int r0 = sl * 16 + g8;
-          const int sw0 = D == 64 ? (r0 >> 2) & 1 : (r0 >> 1) & 3, sw1 = D == 64 ? ((r0 + 8) >> 2) & 1 : ((r0 + 8) >> 1) & 3;
+          const uint8_t* kt = st + Tl::kK + sl * 16 * Tl::kRow;
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr) {
-            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(st + Tl::kK + r0 * Tl::kRow + ((gr ^ sw0) * 16) + t4 * 4);
-            const uint32_t w1 =
-                *reinterpret_cast<const uint32_t*>(st + Tl::kK + (r0 + 8) * Tl::kRow + ((gr ^ sw1) * 16) + t4 * 4);
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kt + k_at[gr]);
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kt + k_at2[gr]);
             const uint32_t x0 = w0 >> 8, x1 = w1 >> 8;
             const uint32_t a0[4] = {w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u};
             const uint32_t a1[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              acc[nt][gr][0] = acc[nt][gr][1] = acc[nt][gr][2] = acc[nt][gr][3] = 0.f;
-              mma16816<__half>(acc[nt][gr], a0, qb[nt][4 * gr], qb[nt][4 * gr + 1]);
+              serving::mma16816_first<__half>(acc[nt][gr], a0, qb[nt][4 * gr], qb[nt][4 * gr + 1]);
               mma16816<__half>(acc[nt][gr], a1, qb[nt][4 * gr + 2], qb[nt][4 * gr + 3]);
             }
           }
 #pragma unroll
           for (int hr = 0; hr < 2; ++hr) {
-            const int r = r0 + 8 * hr;
-            uint32_t kp[kGroups], vp[kGroups];
-            if constexpr (kGroups == 2) {
-              const uint2 ku = *reinterpret_cast<const uint2*>(st + Tl::kKP + r * Tl::kPairs);
-              const uint2 vu = *reinterpret_cast<const uint2*>(st + Tl::kVP + r * Tl::kPairs);
-              kp[0] = ku.x, kp[1] = ku.y, vp[0] = vu.x, vp[1] = vu.y;
-            } else {
-              const uint4 ku = *reinterpret_cast<const uint4*>(st + Tl::kKP + r * Tl::kPairs);
-              const uint4 vu = *reinterpret_cast<const uint4*>(st + Tl::kVP + r * Tl::kPairs);
-              kp[0] = ku.x, kp[1] = ku.y, kp[2] = ku.z, kp[3] = ku.w;
-              vp[0] = vu.x, vp[1] = vu.y, vp[2] = vu.z, vp[3] = vu.w;
-            }
-            uint32_t big = 0u;
-#pragma unroll
-            for (int gr = 0; gr < kGroups; ++gr) {
-              vstep[sl][hr][gr] = __uint_as_float(vp[gr] << 16);
-              vlow[sl][hr][gr] = __uint_as_float(vp[gr] & 0xFFFF0000u);
-              const uint32_t ex = (vp[gr] >> 7) & 0xFFu;  // exponent of the step; a NaN or infinity does not count
-              big = max(big, ex == 255u ? 0u : ex);
-            }
-            // steps below 2^-60 would push p beyond fp32's range: their products lose nothing that matters
-            lift[sl][hr] = static_cast<float>(max(static_cast<int>(big) - 127, -60));
+            uint32_t kp[kGroups];
+            load_pairs(kp, st + Tl::kKP + (sl * 16 + g8 + 8 * hr) * Tl::kPairs);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -430,38 +456,70 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
           }
         }
       }
+      // 4 bits: largest step of the tile's values, a lane's share of the pairs at a time
+      float big = 0.f;
+      if constexpr (BITS == 4) {
+        constexpr int kWords = kKeys * kGroups / 32;  // 4
+        static_assert(kWords == 4, "a lane takes 16 bytes of the pairs");
+        const uint4 v = *reinterpret_cast<const uint4*>(st + Tl::kVP + lane * 16);
+        big = max3(max3(big, __uint_as_float(v.x << 16), __uint_as_float(v.y << 16)), __uint_as_float(v.z << 16),
+                   __uint_as_float(v.w << 16));
+        if (edge) {  // whatever stands in entries that nobody sees does not count
+          const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+          big = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int n = (lane * 4 + w) / kGroups;
+            if (key0 + n < sees_last && !((gone >> (n / 16)) & 1u)) big = fmaxf(big, __uint_as_float(vv[w] << 16));
+          }
+        }
+      }
       if (edge) {
 #pragma unroll
-        for (int sl = 0; sl < 2; ++sl)
+        for (int sl = 0; sl < kSlabs; ++sl)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int x = 0; x < 4; ++x) {
+            const int n = (gone >> sl) & 1u ? 0x7fffffff : key0 + sl * 16 + g8 + 8 * (x >> 1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int n = key0 + sl * 16 + g8 + 8 * (e >> 1);
-              if (n >= sees[nt][e & 1] || ids[sl] < 0) s[nt][sl][e] = -INFINITY;
-            }
+            for (int nt = 0; nt < NT; ++nt)
+              if (n >= sees[nt][x & 1]) s[nt][sl][x] = -INFINITY;
+          }
       }
       // ---- lazy running maximum
-      bool pass = false;
+      float top[NT][2];
+      bool pass = BITS == 4 && big >= big_limit;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int sl = 0; sl < 2; ++sl)
+        for (int u = 0; u < 2; ++u) {
+          float t = fmaxf(s[nt][0][u], s[nt][0][2 + u]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) pass |= s[nt][sl][e] + lift[sl][e >> 1] > m[nt][e & 1] + 8.f;
+          for (int sl = 1; sl < kSlabs; ++sl) t = max3(t, s[nt][sl][u], s[nt][sl][2 + u]);
+          top[nt][u] = t;
+          pass |= t > m[nt][u] + 8.f;
+        }
       if (__any_sync(0xffffffffu, pass)) {
+        float e_new = e;
+        if constexpr (BITS == 4) {
+          // steps that are no number do not count; below 2^-60 the factor would push p beyond fp32's range, and what
+          // fp16 loses there is nothing beside any other entry
+          big = big < 1.7e38f ? big : 0.f;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+          for (int d = 1; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+          e_new = fmaxf(e, static_cast<float>(static_cast<int>(__float_as_uint(big) >> 23) - 127));
+          big_limit = exp2f(e_new + 1.f);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            float top = m[nt][u];
+            float t = fmaxf(top[nt][u], m[nt][u]);
 #pragma unroll
-            for (int sl = 0; sl < 2; ++sl)
-              top = fmaxf(top, fmaxf(s[nt][sl][u] + lift[sl][0], s[nt][sl][2 + u] + lift[sl][1]));
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float alpha = m[nt][u] == -INFINITY ? 0.f : ex2_approx(m[nt][u] - top);
-            m[nt][u] = top;
+            for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
+            // nothing seen so far: O and the sums are zeros, any factor will do
+            const float alpha = m[nt][u] == -INFINITY ? 1.f : ex2_approx((m[nt][u] - t) + (e - e_new));
+            m[nt][u] = t;
+            ref[nt][u] = t == -INFINITY ? 0.f : t + (BITS == 4 ? e_new : 0.f);
             l[nt][u] *= alpha;
 #pragma unroll
             for (int i2 = 0; i2 < D / 16; ++i2) {
@@ -473,20 +531,18 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
               for (int gr = 0; gr < kGroups; ++gr) om[nt][gr][u] *= alpha;
             }
           }
-        }
+        e = e_new;
       }
       // ---- probabilities
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const float m0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int sl = 0; sl < 2; ++sl)
+        for (int sl = 0; sl < kSlabs; ++sl)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[nt][sl][e] = ex2_approx(s[nt][sl][e] - ((e & 1) ? m1 : m0));
-            l[nt][e & 1] += s[nt][sl][e];
+          for (int x = 0; x < 4; ++x) {
+            s[nt][sl][x] = ex2_approx(s[nt][sl][x] - ref[nt][x & 1]);
+            l[nt][x & 1] += s[nt][sl][x];
           }
-      }
       // ---- O^T += V^T P^T
       if constexpr (BITS == 16) {
         // an infinity or a NaN in the value of an entry that some row does not see would reach that row as 0 * inf
@@ -501,13 +557,13 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
         }
         if (!odd) {
 #pragma unroll
-          for (int sl = 0; sl < 2; ++sl) {
+          for (int sl = 0; sl < kSlabs; ++sl) {
             uint32_t pb[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              pb[nt][0] = serving::movmatrix_trans(serving::pack2<T>(s[nt][sl][0], s[nt][sl][1]));
-              pb[nt][1] = serving::movmatrix_trans(serving::pack2<T>(s[nt][sl][2], s[nt][sl][3]));
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int hr = 0; hr < 2; ++hr)
+                pb[nt][hr] = serving::movmatrix_trans(serving::pack2<T>(s[nt][sl][2 * hr], s[nt][sl][2 * hr + 1]));
 #pragma unroll
             for (int mt = 0; mt < D / 16; ++mt) {
               // V^T: rows = dimensions mt * 16 .. + 15, columns = the slab's entries; transposed 8 x 8 blocks
@@ -519,69 +575,77 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
             }
           }
         } else {  // rare: one entry after the other, hidden ones left out
-          for (int n = 0; n < kKeys; ++n) {
-            const int r = n;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              float p[2];
+          for (int sl = 0; sl < kSlabs; ++sl)
+            for (int n = 0; n < 16; ++n) {
+              const int r = sl * 16 + n;
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                // entry n's row of the score block: slab n / 16, half (n / 8) % 2, lane group n % 8
-                const float v0 = (n >> 4) ? ((n >> 3) & 1 ? s[nt][1][2 + u] : s[nt][1][u])
-                                          : ((n >> 3) & 1 ? s[nt][0][2 + u] : s[nt][0][u]);
-                p[u] = __shfl_sync(0xffffffffu, v0, (n & 7) * 4 + t4);
-              }
+              for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int mt = 0; mt < D / 16; ++mt)
+                for (int u = 0; u < 2; ++u) {
+                  // entry n's row of the score block: half n / 8, lane group n % 8
+                  const float p = __shfl_sync(0xffffffffu, n >> 3 ? s[nt][sl][2 + u] : s[nt][sl][u], (n & 7) * 4 + t4);
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                  const int d = mt * 16 + hf * 8 + g8;
-                  const T* vp = reinterpret_cast<const T*>(st + Tl::kV + r * Tl::kRow + (((d >> 3) ^ (r & 7)) * 16)) + (d & 7);
-                  const float v = static_cast<float>(*vp);
+                  for (int mt = 0; mt < D / 16; ++mt)
 #pragma unroll
-                  for (int u = 0; u < 2; ++u)
-                    if (key0 + n < sees[nt][u]) o[nt][mt][2 * hf + u] = fmaf(p[u], v, o[nt][mt][2 * hf + u]);
+                    for (int hf = 0; hf < 2; ++hf) {
+                      const int d = mt * 16 + hf * 8 + g8;
+                      const float v = static_cast<float>(*(reinterpret_cast<const T*>(st + Tl::kV + r * Tl::kRow + (((d >> 3) ^ (r & 7)) * 16)) + (d & 7)));
+                      if (key0 + r < sees[nt][u]) o[nt][mt][2 * hf + u] = fmaf(p, v, o[nt][mt][2 * hf + u]);
+                    }
                 }
             }
-          }
         }
       } else {
 #pragma unroll
-        for (int sl = 0; sl < 2; ++sl) {
+        for (int sl = 0; sl < kSlabs; ++sl) {
           uint32_t pb[NT][kGroups][2];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int hr = 0; hr < 2; ++hr) {
+            uint32_t vp[kGroups];
+            load_pairs(vp, st + Tl::kVP + (sl * 16 + g8 + 8 * hr) * Tl::kPairs);
+            if (edge) {
+              const int n = key0 + sl * 16 + g8 + 8 * hr;
 #pragma unroll
-            for (int gr = 0; gr < kGroups; ++gr)
+              for (int gr = 0; gr < kGroups; ++gr) {
+                // whatever stands in an entry that nobody sees counts nothing; a pair that is no number, of an entry
+                // that some rows see: those get their NaN through the sum of p low (p = 0 would not keep it from the
+                // others), and the codes count nothing
+                const bool none = n >= sees_last || ((gone >> sl) & 1u);
+                const bool fine = isfinite(__uint_as_float(vp[gr] << 16)) && isfinite(__uint_as_float(vp[gr] & 0xFFFF0000u));
+                if (!none && !fine) {
 #pragma unroll
-              for (int hr = 0; hr < 2; ++hr) {
-                float w0 = s[nt][sl][2 * hr] * vstep[sl][hr][gr], w1 = s[nt][sl][2 * hr + 1] * vstep[sl][hr][gr];
-                float a0 = s[nt][sl][2 * hr] * vlow[sl][hr][gr], a1 = s[nt][sl][2 * hr + 1] * vlow[sl][hr][gr];
-                if (edge) {  // what stands in a hidden entry's pair (NaN too) does not count
-                  const int n = key0 + sl * 16 + g8 + 8 * hr;
-                  if (n >= sees[nt][0] || ids[sl] < 0) w0 = a0 = 0.f;
-                  if (n >= sees[nt][1] || ids[sl] < 0) w1 = a1 = 0.f;
+                  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                      if (n < sees[nt][u]) om[nt][gr][u] = NAN;
                 }
-                om[nt][gr][0] += a0;
-                om[nt][gr][1] += a1;
-                pb[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(w0, w1));
+                if (none || !fine) vp[gr] = 0u;
               }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int gr = 0; gr < kGroups; ++gr) {
+                const float step = __uint_as_float(vp[gr] << 16), low = __uint_as_float(vp[gr] & 0xFFFF0000u);
+                const float p0 = s[nt][sl][2 * hr], p1 = s[nt][sl][2 * hr + 1];
+                om[nt][gr][0] = fmaf(p0, low, om[nt][gr][0]);
+                om[nt][gr][1] = fmaf(p1, low, om[nt][gr][1]);
+                pb[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(p0 * step, p1 * step));
+              }
+          }
+          const uint8_t* vt = st + Tl::kV + sl * 16 * Tl::kRow;
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr) {
             // this lane's entries 2 t4, 2 t4 + 1 (and + 8): the half word g8 of the group's codes, dimensions 4 g8 .. + 3
-            uint32_t x[2];
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              const int r = sl * 16 + 2 * t4 + 8 * hf;
-              const int sw = D == 64 ? (r >> 2) & 1 : (r >> 1) & 3;  // the same for r and r + 1
-              const uint8_t* src = st + Tl::kV + r * Tl::kRow + ((gr ^ sw) * 16) + (g8 >> 1) * 4;
-              const uint32_t w0 = *reinterpret_cast<const uint32_t*>(src);
-              const uint32_t w1 = *reinterpret_cast<const uint32_t*>(src + Tl::kRow);
-              x[hf] = __byte_perm(w0, w1, (g8 & 1) ? 0x7632 : 0x5410);
-            }
-            const uint32_t y0 = x[0] >> 8, y1 = x[1] >> 8;
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vt + v_at[gr]);
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(vt + v_at[gr] + Tl::kRow);
+            const uint32_t w2 = *reinterpret_cast<const uint32_t*>(vt + v_at2[gr]);
+            const uint32_t w3 = *reinterpret_cast<const uint32_t*>(vt + v_at2[gr] + Tl::kRow);
+            const uint32_t x0 = __byte_perm(w0, w1, v_sel), x1 = __byte_perm(w2, w3, v_sel);
+            const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
             // rows g8 of the first product: dimension 4 g8, rows g8 + 8: 4 g8 + 1 (16 times); second: 4 g8 + 2, + 3
-            const uint32_t a0[4] = {x[0] & 0x000F000Fu, x[0] & 0x00F000F0u, x[1] & 0x000F000Fu, x[1] & 0x00F000F0u};
+            const uint32_t a0[4] = {x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu, x1 & 0x00F000F0u};
             const uint32_t a1[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -601,7 +665,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
     float* jm = js + kRows * (D + 1);
     float* jl = jm + kRows;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
@@ -614,7 +678,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
         }
         const int r = nt * 8 + 2 * t4 + u;
         if (g8 == 0) {
-          jm[r] = m[nt][u];
+          jm[r] = m[nt][u] == -INFINITY ? -INFINITY : ref[nt][u];
           jl[r] = l[nt][u];
         }
 #pragma unroll
@@ -630,7 +694,6 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
           }
         }
       }
-    }
     __syncthreads();
     const bool starts_here = cur == item_at;
     const int slot_id = 2 * blockIdx.x + (cur > from ? 1 : 0);
@@ -675,40 +738,80 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32) paged_attention_ker
   }
 }
 
-// Joins the partials of the items that the pieces' borders cut; CTA c takes the one that starts in piece c.
+// Joins the partials of the items that the pieces' borders cut; CTA c takes the one that starts in piece c.  The parts'
+// maxima and sums are read by a warp per row, all at once, and turned into factors in shared memory; then a thread per
+// two dimensions of a row adds the parts up in the line's order.
+constexpr int kPagedJoinThreads = 256;
+constexpr int kPagedJoinChunk = 128;  // parts whose factors are held at a time
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const PagedAttnArgs a) {
-  constexpr int kRows = 8 * NT;
+__global__ void __launch_bounds__(kPagedJoinThreads) paged_combine_kernel(const PagedAttnArgs a) {
+  constexpr int kRows = 8 * NT, kSlot = kRows * (D + 2), kPer = kRows * (D / 2) / kPagedJoinThreads;
+  __shared__ float factor[kPagedJoinChunk][kRows], tops[kRows], sums[kRows];
   pdl_wait();
   pdl_trigger();
   const int4 meta = a.meta[blockIdx.x];
+  const int first_slot = a.meta[gridDim.x + blockIdx.x].x;
   if (meta.x < 0) return;
-  const int b = meta.x, kh = meta.y, row0 = meta.z * kRows, last = meta.w;
+  const int b = meta.x, kh = meta.y, row0 = meta.z * kRows, parts = meta.w - static_cast<int>(blockIdx.x) + 1;
   const serving::Span sq = serving::span_of(a.cu_q, b, a.total);
   const int n_new = sq.end - sq.begin, rows = min(kRows, n_new * a.g - row0);
   const long long reach = static_cast<long long>(a.max_pages) * a.page;
   const int len = static_cast<int>(min(static_cast<long long>(max(__ldg(a.kv_len + b), 0)), reach));
-  const int first_slot = a.meta[gridDim.x + blockIdx.x].x;
-  for (int idx = threadIdx.x; idx < rows * (D / 2); idx += blockDim.x) {
-    const int r = idx / (D / 2), d = (idx % (D / 2)) * 2;
-    float top = -INFINITY, sum = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int c = blockIdx.x; c <= last; ++c) {
-      const int slot = c == static_cast<int>(blockIdx.x) ? first_slot : 2 * c;
-      const float* p = a.part + static_cast<size_t>(slot) * kRows * (D + 2);
-      const float2 ml = *reinterpret_cast<const float2*>(p + kRows * D + 2 * r);
-      const float2 ov = *reinterpret_cast<const float2*>(p + r * D + d);
-      const float nt = fmaxf(top, ml.x);
-      const float f0 = top == -INFINITY ? 1.f : ex2_approx(top - nt), f1 = ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - nt);
-      sum = fmaf(f1, ml.y, f0 * sum);
-      o0 = fmaf(f1, ov.x, f0 * o0);
-      o1 = fmaf(f1, ov.y, f0 * o1);
-      top = nt;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto part = [&](int c) { return a.part + static_cast<size_t>(c == 0 ? first_slot : 2 * (static_cast<int>(blockIdx.x) + c)) * kSlot; };
+  for (int r = warp; r < rows; r += kPagedJoinThreads / 32) {
+    float top = -INFINITY;
+    for (int c = lane; c < parts; c += 32) top = fmaxf(top, part(c)[kRows * D + 2 * r]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float sum = 0.f;
+    for (int c = lane; c < parts; c += 32) {
+      const float2 ml = *reinterpret_cast<const float2*>(part(c) + kRows * D + 2 * r);
+      // a part without anything to see has sum 0; one whose scores are all NaN keeps its NaN
+      sum = fmaf(ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - top), ml.y, sum);
     }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) {
+      tops[r] = top;
+      sums[r] = sum;
+    }
+  }
+  __syncthreads();
+  float2 o[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) o[i] = make_float2(0.f, 0.f);
+  for (int c0 = 0; c0 < parts; c0 += kPagedJoinChunk) {
+    const int n = min(kPagedJoinChunk, parts - c0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * rows; i += kPagedJoinThreads) {
+      const int c = i / rows, r = i % rows;
+      const float m = part(c0 + c)[kRows * D + 2 * r];
+      factor[c][r] = m == -INFINITY ? 1.f : ex2_approx(m - tops[r]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int idx = threadIdx.x + i * kPagedJoinThreads, r = idx / (D / 2), d = (idx % (D / 2)) * 2;
+      if (r >= rows) continue;
+#pragma unroll 8
+      for (int c = 0; c < n; ++c) {
+        const float2 x = *reinterpret_cast<const float2*>(part(c0 + c) + r * D + d);
+        o[i].x = fmaf(factor[c][r], x.x, o[i].x);
+        o[i].y = fmaf(factor[c][r], x.y, o[i].y);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int idx = threadIdx.x + i * kPagedJoinThreads, r = idx / (D / 2), d = (idx % (D / 2)) * 2;
+    if (r >= rows) continue;
     const int row = row0 + r;
     const bool sees_some = len - n_new + row / a.g + 1 > 0 && len > 0;
-    const float inv = sees_some ? __frcp_rn(sum) : 0.f;
+    const float inv = sees_some ? __frcp_rn(sums[r]) : 0.f;
     T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + d;
-    *reinterpret_cast<uint32_t*>(dst) = sees_some ? serving::pack2<T>(o0 * inv, o1 * inv) : 0u;
+    *reinterpret_cast<uint32_t*>(dst) = sees_some ? serving::pack2<T>(o[i].x * inv, o[i].y * inv) : 0u;
   }
 }
 

@@ -78,6 +78,9 @@ constexpr int kPagedCtas = 4;  // most CTAs per SM
 // rows of a query tile / 8: single tokens of up to 8 grouped heads, or more
 int paged_nt(int batch, int total_q, int g) { return static_cast<long long>(total_q) * g <= 8ll * batch ? 1 : 2; }
 
+// items of at most 512 entries are not worth a second launch to join their parts
+bool paged_split(long long max_entries) { return max_entries > 512; }
+
 size_t paged_part_bytes(long long ctas, int nt, int d) { return static_cast<size_t>(2 * ctas) * 8 * nt * (d + 2) * 4; }
 
 template <typename T, int D, int BITS, int NT>
@@ -96,10 +99,13 @@ int32_t launch_paged_inst(PagedAttnArgs a, cudaStream_t st) {
     ctas[dev] = (n < 1 ? 1 : (n > kPagedCtas ? kPagedCtas : n)) * sm_count();
   }
   const int grid = ctas[dev];
-  a.meta = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(a.part) + paged_part_bytes(grid, NT, D));
+  // a piece is worth at least 256 entries (64 a warp); an item's start and join cost about as much as 512
+  a.min_share = a.split ? 256 / paged_detail::Tile<D, BITS>::kKeys : 1;
+  a.item_cost = 512 / paged_detail::Tile<D, BITS>::kKeys;
+  if (a.split) a.meta = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(a.part) + paged_part_bytes(grid, NT, D));
   int32_t rc = launch(kern, dim3(grid), dim3(paged_detail::kWarps * 32), Sm::kBytes, st, "paged_attention_kernel", a);
   if (rc || !a.split) return rc;
-  return launch(paged_combine_kernel<T, D, NT>, dim3(grid), dim3(128), 0, st, "paged_combine_kernel", a);
+  return launch(paged_combine_kernel<T, D, NT>, dim3(grid), dim3(kPagedJoinThreads), 0, st, "paged_combine_kernel", a);
 }
 
 template <typename T, int D>
@@ -199,8 +205,9 @@ int32_t svla_packed_attention(const svla_packed_attn_desc* d, svla_stream_t stre
   return h ? launch_packed<__half, 128>(a, items, cs(stream)) : launch_packed<__nv_bfloat16, 128>(a, items, cs(stream));
 }
 
-size_t svla_paged_attention_workspace_size(int32_t batch, int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim) {
-  if (batch <= 0 || total_q <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || head_dim <= 0) return 0;
+size_t svla_paged_attention_workspace_size(int32_t batch, int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim,
+                                           int64_t max_entries) {
+  if (batch <= 0 || total_q <= 0 || hq <= 0 || hkv <= 0 || hq % hkv || head_dim <= 0 || !paged_split(max_entries)) return 0;
   const long long ctas = static_cast<long long>(kPagedCtas) * sm_count();
   return paged_part_bytes(ctas, paged_nt(batch, total_q, hq / hkv), head_dim) + static_cast<size_t>(2 * ctas) * sizeof(int4);
 }
@@ -216,8 +223,9 @@ int32_t svla_paged_attention(const svla_paged_attn_desc* d, svla_stream_t stream
   const int64_t qw = static_cast<int64_t>(d->hq) * d->head_dim;
   if (int32_t rc = check_rows(who, "q", d->q, d->q_rs, qw)) return rc;
   if (int32_t rc = check_rows(who, "o", d->o, d->o_rs, qw)) return rc;
-  const size_t need = svla_paged_attention_workspace_size(d->batch, d->total_q, d->hq, d->hkv, d->head_dim);
-  if (!d->workspace || !aligned(d->workspace, 256) || d->workspace_bytes < need)
+  const long long max_entries = static_cast<long long>(d->max_pages) * d->page_size;
+  const size_t need = svla_paged_attention_workspace_size(d->batch, d->total_q, d->hq, d->hkv, d->head_dim, max_entries);
+  if (need && (!d->workspace || !aligned(d->workspace, 256) || d->workspace_bytes < need))
     return fail(SVLA_ERR_ARG, "%s: workspace must be 256-byte aligned with at least %zu bytes (got %zu)", who, need, d->workspace_bytes);
   PagedAttnArgs a;
   std::memset(&a, 0, sizeof(a));
@@ -230,10 +238,7 @@ int32_t svla_paged_attention(const svla_paged_attn_desc* d, svla_stream_t stream
   a.page_magic = ((1ull << 32) + a.page / 16 - 1) / (a.page / 16);
   a.scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt(static_cast<float>(d->head_dim))) * serving::kLog2e;
   a.err = device_error_ptr();
-  // items of at most 16 tiles (4 a warp) are not worth a second launch to join their parts
-  const long long most = (static_cast<long long>(d->max_pages) * d->page_size + paged_detail::kKeys - 1) / paged_detail::kKeys;
-  a.split = most > 16;
-  a.min_share = a.split ? 8 : 1;
+  a.split = paged_split(max_entries);
   const int nt = paged_nt(d->batch, d->total_q, a.g);
   const bool h = d->dtype == SVLA_DT_HALF;
   if (d->head_dim == 64) return h ? launch_paged<__half, 64>(a, d->bits, nt, cs(stream)) : launch_paged<__nv_bfloat16, 64>(a, d->bits, nt, cs(stream));

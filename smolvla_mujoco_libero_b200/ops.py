@@ -18,7 +18,7 @@ from ._lib import check, lib
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(t: torch.Tensor | None) -> int | None:
@@ -354,39 +354,41 @@ def rope_table(max_pos: int, max_wavelength: float, device) -> torch.Tensor:
 _DT16 = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_HALF}
 
 
-def _packed(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> None:
-    """t: [rows, heads, head_dim] bf16 / fp16 on the current device, heads next to each other (any row stride)."""
+def _packed_first(t: torch.Tensor, name: str) -> tuple[torch.dtype, int, int]:
+    """(dtype, device index, head_dim) of the tensor that the call's other tensors have to fit."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
     if t.dim() != 3 or t.dtype not in _DT16:
         raise ValueError(f"{name} must be bf16 or fp16 [rows, heads, head_dim], got {t.dtype} {tuple(t.shape)}")
-    h, d = t.shape[1], t.shape[2]
+    dev = t.get_device()
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"{name} is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
+    return t.dtype, dev, t.shape[2]
+
+
+def _packed(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int, d: int) -> tuple[int, int, int]:
+    """(rows, heads, row stride) of t [rows, heads, d], whose heads lie next to each other (any row stride; a single
+    row's does not matter to torch, so it is not taken from it)."""
+    if t.dtype is not dtype or t.get_device() != dev or t.dim() != 3:
+        raise ValueError(f"{name} must be {dtype} [rows, heads, {d}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    rows, h, dd = t.shape
     rs, hs, es = t.stride()
-    if t.numel() and ((es != 1 and d > 1) or (hs != d and h > 1)):
-        raise ValueError(f"{name}: the heads of a row must lie next to each other (strides {t.stride()})")
-    if like is None:
-        if t.device.index != torch.cuda.current_device():
-            raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    elif t.dtype != like.dtype or t.device != like.device or d != like.shape[2]:
-        raise ValueError(f"{name} must be {like.dtype} with head_dim {like.shape[2]} on {like.device}")
+    if dd != d or (rows and (es != 1 or (hs != d and h > 1))):
+        raise ValueError(f"{name} must be [rows, heads, {d}] with the heads of a row next to each other, got "
+                         f"{tuple(t.shape)} with strides {t.stride()}")
+    return rows, h, (rs if rows > 1 else h * d)
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements between rows; a single row's stride does not matter to torch, so it is not taken from it."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+def _ints(t: torch.Tensor, name: str, n: int, dev: int) -> None:
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.dim() != 1 or len(t) != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{n}] on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
-def _ints(t: torch.Tensor, name: str, shape: tuple, device: torch.device) -> None:
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32 {list(shape)} on {device}, got {t.dtype} {list(t.shape)} "
-                         f"on {t.device}")
-
-
-def _batch_of(cu: torch.Tensor, name: str, device: torch.device) -> int:
-    if cu.dim() != 1 or cu.shape[0] < 1:
-        raise ValueError(f"{name} must be int32 [batch + 1]")
-    _ints(cu, name, (cu.shape[0],), device)
-    return cu.shape[0] - 1
+def _batch_of(cu: torch.Tensor, name: str, dev: int) -> int:
+    if cu.dim() != 1 or len(cu) < 1:
+        raise ValueError(f"{name} must be int32 [batch + 1], got {list(cu.shape)}")
+    _ints(cu, name, len(cu), dev)
+    return len(cu) - 1
 
 
 def kv_cache(n_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 16,
@@ -403,26 +405,25 @@ def kv_cache(n_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: i
     return torch.zeros(n_pages, kv_heads, 2, page_size, head_dim, dtype=dtype, device=device)
 
 
-def _cache(cache: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, batch: int, like: torch.Tensor,
-           hkv: int) -> tuple[int, int]:
-    """(bits, page_size) of a cache that fits packed rows like ``like``."""
-    d, dev = like.shape[2], like.device
-    if cache.device != dev or not cache.is_contiguous():
-        raise ValueError(f"cache must be contiguous on {dev}")
-    if cache.dim() == 5:
-        bits, page = 16, cache.shape[3]
-        ok = cache.dtype == like.dtype and cache.shape[2] == 2 and cache.shape[4] == d
+def _cache(cache: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, batch: int, dtype: torch.dtype,
+           dev: int, d: int) -> tuple[int, int, int, int, int, int]:
+    """(bits, page_size, n_pages, kv heads, max_pages, page_table's row stride)."""
+    shape = cache.shape
+    if len(shape) == 5 and cache.dtype is dtype and shape[2] == 2 and shape[4] == d:
+        bits, page = 16, shape[3]
+    elif len(shape) == 4 and cache.dtype is torch.uint8 and shape[3] == d + d // 4:
+        bits, page = 4, shape[2]
     else:
-        bits, page = 4, (cache.shape[2] if cache.dim() == 4 else 0)
-        ok = cache.dtype == torch.uint8 and page > 0 and cache.shape[3] == d + d // 4
-    if not ok or cache.shape[1] != hkv:
-        raise ValueError(f"cache {cache.dtype} {list(cache.shape)} does not hold {hkv} kv heads of {like.dtype} "
-                         f"[{d}] (see kv_cache)")
-    _ints(kv_len, "kv_len", (batch,), dev)
-    if (page_table.dtype != torch.int32 or page_table.device != dev or page_table.dim() != 2
-            or page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
-        raise ValueError(f"page_table must be int32 [{batch}, max_pages] on {dev} with unit column stride")
-    return bits, page
+        raise ValueError(f"cache {cache.dtype} {list(shape)} does not hold entries of {dtype} [{d}] (see kv_cache)")
+    if cache.get_device() != dev or not cache.is_contiguous():
+        raise ValueError(f"cache must be contiguous on cuda:{dev}")
+    _ints(kv_len, "kv_len", batch, dev)
+    if (page_table.dtype is not torch.int32 or page_table.get_device() != dev or page_table.dim() != 2
+            or len(page_table) != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
+        raise ValueError(f"page_table must be int32 [{batch}, max_pages] on cuda:{dev} with unit column stride, got "
+                         f"{page_table.dtype} {list(page_table.shape)} on {page_table.device}")
+    max_pages = page_table.shape[1]
+    return bits, page, shape[0], shape[1], max_pages, (page_table.stride(0) if batch > 1 else max_pages)
 
 
 def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
@@ -434,52 +435,56 @@ def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch
     queries ``q`` are rotated at ``pos`` [rows], or at the entry's index.  Returns the rotated queries (None without q), or
     with ``want_rows`` (q, k, v): the appended rows as the cache holds them, which prompt attention takes.  The outputs may
     be the inputs (in place)."""
-    _packed(k, "k")
-    _packed(v, "v", k)
-    rows, hkv, d = k.shape
-    dev = k.device
-    if v.shape != k.shape:
+    dtype, dev, d = _packed_first(k, "k")
+    rows, hkv, k_rs = _packed(k, "k", dtype, dev, d)
+    v_rows, v_heads, v_rs = _packed(v, "v", dtype, dev, d)
+    if v_rows != rows or v_heads != hkv:
         raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
     batch = _batch_of(cu_q, "cu_q", dev)
-    bits, page = _cache(cache, page_table, kv_len, batch, k, hkv)
-    hq = 0
+    bits, page, n_pages, cache_heads, max_pages, table_rs = _cache(cache, page_table, kv_len, batch, dtype, dev, d)
+    if cache_heads != hkv:
+        raise ValueError(f"the cache holds {cache_heads} kv heads, k has {hkv}")
+    hq = q_rs = qo_rs = ko_rs = vo_rs = max_pos = 0
+    q_ptr = qo_ptr = ko_ptr = vo_ptr = cs_ptr = pos_ptr = None
     if q is not None:
-        _packed(q, "q", k)
-        hq = q.shape[1]
-        if q.shape[0] != rows:
-            raise ValueError(f"q has {q.shape[0]} rows, k {rows}")
+        q_rows, hq, q_rs = _packed(q, "q", dtype, dev, d)
+        if q_rows != rows:
+            raise ValueError(f"q has {q_rows} rows, k {rows}")
         if q_out is None:
-            q_out = torch.empty(rows, hq, d, dtype=q.dtype, device=dev)
+            q_out, qo_rs = q.new_empty(rows, hq, d), hq * d
         else:
-            _packed(q_out, "q_out", k)
-            if q_out.shape != q.shape:
+            qo_rows, qo_heads, qo_rs = _packed(q_out, "q_out", dtype, dev, d)
+            if qo_rows != rows or qo_heads != hq:
                 raise ValueError("q_out must have q's shape")
+        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
     if want_rows:
-        k_out = torch.empty(rows, hkv, d, dtype=k.dtype, device=dev) if k_out is None else k_out
-        v_out = torch.empty(rows, hkv, d, dtype=k.dtype, device=dev) if v_out is None else v_out
-    for t, name in ((k_out, "k_out"), (v_out, "v_out")):
-        if t is not None:
-            _packed(t, name, k)
-            if t.shape != k.shape:
-                raise ValueError(f"{name} must have k's shape")
-    max_pos = 0
+        k_out = k.new_empty(rows, hkv, d) if k_out is None else k_out
+        v_out = k.new_empty(rows, hkv, d) if v_out is None else v_out
+    if k_out is not None:
+        o_rows, o_heads, ko_rs = _packed(k_out, "k_out", dtype, dev, d)
+        if o_rows != rows or o_heads != hkv:
+            raise ValueError("k_out must have k's shape")
+        ko_ptr = k_out.data_ptr()
+    if v_out is not None:
+        o_rows, o_heads, vo_rs = _packed(v_out, "v_out", dtype, dev, d)
+        if o_rows != rows or o_heads != hkv:
+            raise ValueError("v_out must have v's shape")
+        vo_ptr = v_out.data_ptr()
     if rope_cs is not None:
-        if (rope_cs.dtype != torch.float32 or rope_cs.device != dev or rope_cs.dim() != 3
-                or rope_cs.shape[1:] != (d // 2, 2) or not rope_cs.is_contiguous()):
-            raise ValueError(f"rope_cs must be contiguous fp32 [max_pos, {d // 2}, 2] on {dev}")
-        max_pos = rope_cs.shape[0]
+        if (rope_cs.dtype is not torch.float32 or rope_cs.get_device() != dev or rope_cs.dim() != 3
+                or rope_cs.shape[1] != d // 2 or rope_cs.shape[2] != 2 or not rope_cs.is_contiguous()):
+            raise ValueError(f"rope_cs must be contiguous fp32 [max_pos, {d // 2}, 2] on cuda:{dev}")
+        max_pos, cs_ptr = len(rope_cs), rope_cs.data_ptr()
     if pos is not None:
-        _ints(pos, "pos", (rows,), dev)
+        _ints(pos, "pos", rows, dev)
+        pos_ptr = pos.data_ptr()
     if rows:
-        desc = L.KvAppendDesc(_p(q), k.data_ptr(), v.data_ptr(), _p(q_out), _p(k_out), _p(v_out), cache.data_ptr(),
-                              cu_q.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), _p(pos), _p(rope_cs),
-                              0 if q is None else _row_stride(q), _row_stride(k), _row_stride(v),
-                              0 if q is None else _row_stride(q_out), 0 if k_out is None else _row_stride(k_out),
-                              0 if v_out is None else _row_stride(v_out),
-                              page_table.stride(0) if batch > 1 else page_table.shape[1], batch, rows, hq, hkv, d,
-                              _DT16[k.dtype], bits, page, cache.shape[0], page_table.shape[1], max_pos)
+        desc = L.KvAppendDesc(q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ko_ptr, vo_ptr, cache.data_ptr(),
+                              cu_q.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), pos_ptr, cs_ptr, q_rs, k_rs,
+                              v_rs, qo_rs, ko_rs, vo_rs, table_rs, batch, rows, hq, hkv, d, _DT16[dtype], bits, page,
+                              n_pages, max_pages, max_pos)
         check(lib().svla_kv_append(ctypes.byref(desc), _stream()), "svla_kv_append")
     return (q_out, k_out, v_out) if want_rows else q_out
 
@@ -492,27 +497,26 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     cu_q[b + 1] - 1 of q and cu_k[b] .. of k and v (cu_k None: the same).  Causal: the queries are the last tokens of
     their sequence.  Returns [rows, heads, head_dim]; rows behind the last sequence are left as they are in ``out``
     (undefined without it)."""
-    _packed(q, "q")
-    _packed(k, "k", q)
-    _packed(v, "v", q)
-    if v.shape != k.shape:
+    dtype, dev, d = _packed_first(q, "q")
+    rows, hq, q_rs = _packed(q, "q", dtype, dev, d)
+    k_rows, hkv, k_rs = _packed(k, "k", dtype, dev, d)
+    v_rows, v_heads, v_rs = _packed(v, "v", dtype, dev, d)
+    if v_rows != k_rows or v_heads != hkv:
         raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    dev = q.device
     batch = _batch_of(cu_q, "cu_q", dev)
     if cu_k is None:
         cu_k = cu_q
     else:
-        _ints(cu_k, "cu_k", (batch + 1,), dev)
+        _ints(cu_k, "cu_k", batch + 1, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out, o_rs = q.new_empty(rows, hq, d), hq * d
     else:
-        _packed(out, "out", q)
-        if out.shape != q.shape:
+        o_rows, o_heads, o_rs = _packed(out, "out", dtype, dev, d)
+        if o_rows != rows or o_heads != hq:
             raise ValueError("out must have q's shape")
-    rows, hq, d = q.shape
     desc = L.PackedAttnDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
-                            _row_stride(q), _row_stride(k), _row_stride(v), _row_stride(out), batch, rows, k.shape[0],
-                            hq, k.shape[1], d, _DT16[q.dtype], int(causal), float(scale))
+                            q_rs, k_rs, v_rs, o_rs, batch, rows, k_rows, hq, hkv, d, _DT16[dtype], 1 if causal else 0,
+                            scale)
     check(lib().svla_packed_attention(ctypes.byref(desc), _stream()), "svla_packed_attention")
     return out
 
@@ -524,28 +528,27 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor, kv
     appended) over a paged cache of 16 or 4 bits; kv_len [B] entries, pages in page_table [B, max_pages].  Returns
     [rows, heads, head_dim].  ``workspace``: uint8 of svla_paged_attention_workspace_size bytes, taken from torch's
     allocator when None."""
-    _packed(q, "q")
-    dev = q.device
+    dtype, dev, d = _packed_first(q, "q")
+    rows, hq, q_rs = _packed(q, "q", dtype, dev, d)
     batch = _batch_of(cu_q, "cu_q", dev)
-    rows, hq, d = q.shape
-    hkv = cache.shape[1] if cache.dim() > 1 else 0
-    bits, page = _cache(cache, page_table, kv_len, batch, q, hkv)
+    bits, page, n_pages, hkv, max_pages, table_rs = _cache(cache, page_table, kv_len, batch, dtype, dev, d)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out, o_rs = q.new_empty(rows, hq, d), hq * d
     else:
-        _packed(out, "out", q)
-        if out.shape != q.shape:
+        o_rows, o_heads, o_rs = _packed(out, "out", dtype, dev, d)
+        if o_rows != rows or o_heads != hq:
             raise ValueError("out must have q's shape")
     handle = lib()
     if workspace is None:
-        need = handle.svla_paged_attention_workspace_size(batch, rows, hq, hkv, d)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    elif workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be contiguous uint8 on {dev}")
+        need = handle.svla_paged_attention_workspace_size(batch, rows, hq, hkv, d, max_pages * page)
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise ValueError(f"workspace must be contiguous uint8 on cuda:{dev}")
+    ws_ptr, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
     desc = L.PagedAttnDesc(q.data_ptr(), cache.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(),
-                           page_table.data_ptr(), workspace.data_ptr(), workspace.numel(), _row_stride(q),
-                           _row_stride(out), page_table.stride(0) if batch > 1 else page_table.shape[1], batch, rows, hq,
-                           hkv, d, _DT16[q.dtype], bits, page, cache.shape[0], page_table.shape[1], float(scale))
+                           page_table.data_ptr(), ws_ptr, ws_bytes, q_rs, o_rs, table_rs, batch, rows, hq, hkv, d,
+                           _DT16[dtype], bits, page, n_pages, max_pages, scale)
     check(handle.svla_paged_attention(ctypes.byref(desc), _stream()), "svla_paged_attention")
     return out
 

@@ -572,7 +572,7 @@ def test_paged_attention_repeats_replays_and_other_streams(bits):
 def test_arguments_that_do_not_fit_are_refused():
     q, kv = torch.zeros(4, 6, 64, dtype=BF16, device=DEV), torch.zeros(4, 2, 64, dtype=BF16, device=DEV)
     cu, n, table = ints([0, 4]).to(DEV), ints([4]).to(DEV), ints([[0]]).to(DEV)
-    cache = ops.kv_cache(1, 16, 2, 64)
+    cache, wide = ops.kv_cache(1, 16, 2, 64), torch.zeros(1, 64, dtype=torch.int32, device=DEV)
     calls = [
         lambda: ops.packed_attention(q, kv.half(), kv.half(), cu),
         lambda: ops.packed_attention(q, kv, kv[:2], cu),
@@ -596,7 +596,7 @@ def test_arguments_that_do_not_fit_are_refused():
         lambda: ops.paged_attention(q, cache[:, :, :1], cu, n, table),
         lambda: ops.paged_attention(q, cache, cu, n, table.long()),
         lambda: ops.paged_attention(q, cache, cu, n, table, workspace=torch.zeros(8, device=DEV)),
-        lambda: ops.paged_attention(q, cache, cu, n, table, workspace=torch.zeros(64, dtype=torch.uint8, device=DEV)),
+        lambda: ops.paged_attention(q, cache, cu, n, wide, workspace=torch.zeros(64, dtype=torch.uint8, device=DEV)),
     ]
     for i, call in enumerate(calls):
         with pytest.raises((ValueError, L.SvlaError)):

@@ -46,9 +46,9 @@ def _paged(**kw):
     d = L.PagedAttnDesc()
     d.q, d.cache, d.o, d.cu_q, d.kv_len, d.page_table = 0x100000, 0x200000, 0x300000, 0x400000, 0x500000, 0x600000
     d.workspace, d.workspace_bytes = 0x700000, 1 << 30
-    d.q_rs, d.o_rs, d.page_table_rs = 960, 960, 4
+    d.q_rs, d.o_rs, d.page_table_rs = 960, 960, 64
     d.batch, d.total_q, d.hq, d.hkv, d.head_dim, d.dtype = 1, 1, 15, 5, 64, L.DT_BF16
-    d.bits, d.page_size, d.n_pages, d.max_pages = 4, 16, 8, 4
+    d.bits, d.page_size, d.n_pages, d.max_pages = 4, 16, 80, 64
     for k, v in kw.items():
         setattr(d, k, v)
     return d
@@ -108,8 +108,9 @@ def test_null_descriptors_and_nothing_to_do():
         assert getattr(lib, name)(ctypes.byref(make(batch=0)), None) == 0
     assert lib.svla_rope_table_wide(None, 4, 64, 1e4, None) == 1
     assert lib.svla_rope_table_wide(0x100000, 4, 63, 1e4, None) == 1
-    assert lib.svla_paged_attention_workspace_size(0, 1, 15, 5, 64) == 0
-    assert lib.svla_paged_attention_workspace_size(1, 1, 15, 5, 64) > 0
+    assert lib.svla_paged_attention_workspace_size(0, 1, 15, 5, 64, 4096) == 0
+    assert lib.svla_paged_attention_workspace_size(1, 1, 15, 5, 64, 256) == 0  # short: no second launch, no workspace
+    assert lib.svla_paged_attention_workspace_size(1, 1, 15, 5, 64, 4096) > 0
 
 
 def test_cpu_tensors_are_refused():
