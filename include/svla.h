@@ -350,6 +350,8 @@ typedef struct svla_packed_attn_desc {
   int32_t batch, total_q, total_k;           /* rows of q / o and of k / v */
   int32_t hq, hkv, head_dim, dtype, causal;  /* hq / hkv <= 64 */
   float scale;                               /* 0 = head_dim^-1/2 */
+  int32_t impl;                              /* SVLA_ATTN_AUTO, or force SVLA_ATTN_MMA_SYNC / SVLA_ATTN_TCGEN05 (the
+                                                latter needs total_k > 0) */
 } svla_packed_attn_desc;
 
 int32_t svla_packed_attention(const svla_packed_attn_desc* desc, svla_stream_t stream);

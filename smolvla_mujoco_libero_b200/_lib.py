@@ -126,7 +126,7 @@ class PackedAttnDesc(ctypes.Structure):
         ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("o", c_void_p), ("cu_q", c_void_p), ("cu_k", c_void_p),
         ("q_rs", c_int64), ("k_rs", c_int64), ("v_rs", c_int64), ("o_rs", c_int64), ("batch", c_int32),
         ("total_q", c_int32), ("total_k", c_int32), ("hq", c_int32), ("hkv", c_int32), ("head_dim", c_int32),
-        ("dtype", c_int32), ("causal", c_int32), ("scale", c_float),
+        ("dtype", c_int32), ("causal", c_int32), ("scale", c_float), ("impl", c_int32),
     ]
 
 

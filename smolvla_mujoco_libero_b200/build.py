@@ -35,7 +35,8 @@ FLAGS = [*ARCH, "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC"]
 def units() -> list[tuple[Path, list[Path]]]:
     """(source, the files its object depends on) for every translation unit of the library."""
     shared = [CSRC / "host.cuh", CSRC / "ptx.cuh", HEADER]
-    serving = [CSRC / f"{n}.cuh" for n in ("kv_append", "paged_attention", "packed_attention", "serving_common")]
+    serving = [CSRC / f"{n}.cuh" for n in ("kv_append", "paged_attention", "packed_attention", "packed_attention_tc",
+                                           "serving_common")]
     path = [p for p in sorted(CSRC.glob("*.cuh")) if p not in serving]
     return [(CSRC / "svla.cu", [CSRC / "svla.cu", *path, HEADER]),
             (CSRC / "serving.cu", [CSRC / "serving.cu", *serving, *shared]),

@@ -1,0 +1,466 @@
+// Attention over packed prompts on the 5th-generation tensor cores (tcgen05): the operator of packed_attention.cuh, for
+// prompts long enough to fill 128-row tiles.
+//
+// One CTA per SM takes two query tiles A and B of 128 packed rows (token-major, then the heads of the group; G * QT rows
+// of each are real) of one sequence and kv head, one behind the other, and walks over their keys in tiles of 128 that
+// both use.  320 threads:
+//   warps 0-3, 4-7  softmax of A and of B: thread t owns TMEM lane t = one query row, so maximum and sum need no
+//                   shuffles; the row's 128 scores are held in registers
+//   warp 8          TMA of Q, K and V; it also clears from the last V tiles what must not be multiplied (below)
+//   warp 9          TMEM owner (all 512 columns) and MMA issuer (one elected lane)
+// While one tile's rows are in the softmax, the tensor pipe works for the other.
+//
+// TMEM.  D = 64: S_A, S_B (128 columns each), P_A, P_B (64), O_A, O_B (64): P has columns of its own, so the next scores
+// are computed while the softmax still works on these.  D = 128: P_x over the first half of S_x, O_A, O_B (128): the next
+// scores of a tile follow its P.V (the tensor pipe runs one thread's MMAs in order).
+//
+// Exponentials are the bound at D = 64 (16 per clock and SM: 1024 cycles per 128 x 128 tile against 512 of MMA), both
+// pipes at D = 128.  The running maximum is lazy (O is rescaled only when a row's maximum grows by more than 8 in log2
+// units, by the softmax threads themselves), exponent arguments and sums go through the packed fp32 pipe.
+//
+// What stands behind a sequence's last key belongs to its neighbour: scores there are masked, and the V rows of the tile
+// are set to zero in shared memory before the product (0 * NaN would be NaN).  Under a causal mask the same holds inside
+// the sequence for infinities and NaN in rows that some query of the CTA does not see; the epilogue then adds them to the
+// rows that do.
+#pragma once
+
+#include <type_traits>
+
+#include "packed_attention.cuh"
+
+namespace svla {
+
+struct PackedTcArgs {
+  CUtensorMap tq;      // 3-D (dim, head, token): box 64 x G x QT, 128-byte swizzle
+  CUtensorMap tk, tv;  // 3-D (dim, head, token): box 64 x 1 x 128
+  const void* v;
+  void* o;
+  const int *cu_q, *cu_k;
+  long long v_rs, o_rs;
+  int batch, total_q, total_k, hq, hkv, g, qt;
+  int causal;
+  float scale_log2;
+  int* err;
+};
+
+namespace ptc {
+constexpr int kKeys = 128, kThreads = 320;
+
+template <int D>
+struct Cfg {
+  static constexpr int kSub = D / 64;                 // 64-dimension blocks of a row (one 128-byte swizzle row each)
+  static constexpr int kTile = 128 * D * 2;           // bytes of a Q, K or V tile
+  static constexpr int kStages = D == 64 ? 4 : 2;     // K tiles and V tiles in their rings
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStages * kTile, kBar = kV + kStages * kTile;
+  static constexpr int kSmem = kBar + 512 + 1024;     // + barriers + alignment slack
+  static constexpr bool kOwnP = D == 64;              // P has its own columns
+  static constexpr uint32_t kS = 0;                   // + 128 x
+  static constexpr uint32_t kP = kOwnP ? 256 : 0;     // + 64 x, or over S_x
+  static constexpr uint32_t kPStride = kOwnP ? 64 : 128;
+  static constexpr uint32_t kO = kOwnP ? 384 : 256;   // + D x
+};
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// instruction descriptor of kind::f16 for the type: fp32 accumulators, A and B of one type (fp16 0, bf16 1)
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc(int m, int n) {
+  const uint32_t f = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// bounded wait of a warp: one lane polls
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, err);
+  return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+}
+}  // namespace ptc
+
+template <typename T, int D>
+__global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(const __grid_constant__ PackedTcArgs a) {
+  using namespace ptc;
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kBar);  // [2]
+  uint64_t* k_full = q_full + 2;
+  uint64_t* k_empty = k_full + C::kStages;
+  uint64_t* v_full = k_empty + C::kStages;
+  uint64_t* v_empty = v_full + C::kStages;
+  uint64_t* v_clear = v_empty + C::kStages;  // an edge tile's V has been cleared
+  uint64_t* s_full = v_clear + C::kStages;   // [2] scores are there
+  uint64_t* s_free = s_full + 2;             // [2] (own P) scores are in registers
+  uint64_t* p_full = s_free + 2;             // [2] probabilities are there
+  uint64_t* o_done = p_full + 2;             // [2] the tile's P.V so far is done
+  uint64_t* all_done = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  int* place = reinterpret_cast<int*>(tmem_slot + 1);  // [2] sequence, item
+  int* odd_flag = place + 2;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 8) {
+    if (lane == 0) {
+      for (int s = 0; s < C::kStages; ++s) {
+        mbar_init(&k_full[s], 1);
+        mbar_init(&k_empty[s], 1);
+        mbar_init(&v_full[s], 1);
+        mbar_init(&v_empty[s], 1);
+        mbar_init(&v_clear[s], 1);
+      }
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&q_full[x], 1);
+        mbar_init(&s_full[x], 1);
+        mbar_init(&s_free[x], 4);
+        mbar_init(&p_full[x], 4);
+        mbar_init(&o_done[x], 1);
+      }
+      mbar_init(all_done, 1);
+      fence_mbar_init();
+      *odd_flag = 0;
+    }
+  } else if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  pdl_wait();  // lengths, q, k, v are written by the previous kernel
+  if (warp == 0) {
+    int b = -1, j = 0;
+    const bool ok = packed_detail::find_tile(a.cu_q, a.batch, a.total_q, 2 * a.qt, blockIdx.x / a.hkv, lane, b, j);
+    if (lane == 0) {
+      place[0] = ok ? b : -1;
+      place[1] = j;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_trigger();
+  const uint32_t tmem = *tmem_slot;
+  const int b = place[0], kh = blockIdx.x % a.hkv;
+  if (b >= 0) {
+    const serving::Span sq = serving::span_of(a.cu_q, b, a.total_q), sk = serving::span_of(a.cu_k, b, a.total_k);
+    const int n_q = sq.end - sq.begin, n_k = sk.end - sk.begin, past = n_k - n_q;
+    auto seen = [&](int tok) { return a.causal ? min(max(past + tok + 1, 0), n_k) : n_k; };
+    // tile x: tokens tok[x] .. of the sequence, toks[x] of them, n[x] key tiles
+    int tok[2], toks[2], n[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      tok[x] = (2 * place[1] + x) * a.qt;
+      toks[x] = min(max(n_q - tok[x], 0), a.qt);
+      n[x] = toks[x] > 0 ? (seen(tok[x] + toks[x] - 1) + kKeys - 1) / kKeys : 0;
+    }
+    const int n_all = max(n[0], n[1]);
+    // from this key tile on, V is cleared before it is multiplied: rows behind the sequence, rows that some query of the
+    // CTA does not see
+    const int first_clear = seen(tok[0]) / kKeys;
+
+    if (warp == 8) {
+      // ---------------- producer
+      if (lane == 0) {
+        prefetch_tmap(&a.tq);
+        prefetch_tmap(&a.tk);
+        prefetch_tmap(&a.tv);
+      }
+      auto load_q = [&](int x) {
+        mbar_arrive_expect_tx(&q_full[x], static_cast<uint32_t>(a.g * a.qt * D * 2));
+#pragma unroll
+        for (int c = 0; c < C::kSub; ++c)
+          tma_load_3d(smem + C::kQ + x * C::kTile + c * 16384, &a.tq, &q_full[x], c * 64, kh * a.g, sq.begin + tok[x]);
+      };
+      auto load_kv = [&](const CUtensorMap* map, uint64_t* full, uint8_t* dst, int j) {
+        mbar_arrive_expect_tx(full, C::kTile);
+#pragma unroll
+        for (int c = 0; c < C::kSub; ++c) tma_load_3d(dst + c * 16384, map, full, c * 64, kh, sk.begin + j * kKeys);
+      };
+      // sets what must not be multiplied in V tile j to zero, in shared memory
+      auto clear = [&](int j) -> bool {
+        const int s = j % C::kStages;
+        if (!wait_warp(&v_full[s], (j / C::kStages) & 1, a.err)) return false;
+        uint8_t* vt = smem + C::kV + s * C::kTile;
+        const int behind = min(max(n_k - j * kKeys, 0), kKeys);                  // rows from here on are another's
+        const int hidden = a.causal ? max(seen(tok[0]) - j * kKeys, 0) : kKeys;  // rows from here on some query does not see
+#pragma unroll
+        for (int c = 0; c < C::kSub; ++c) {
+          for (int i = lane + behind * 8; i < 128 * 8; i += 32)
+            *reinterpret_cast<uint4*>(vt + c * 16384 + i * 16) = make_uint4(0, 0, 0, 0);
+          bool odd = false;
+#pragma unroll 4
+          for (int i = lane + hidden * 8; i < behind * 8; i += 32) {
+            const uint4 u = *reinterpret_cast<const uint4*>(vt + c * 16384 + i * 16);
+            odd |= serving::any_nonfinite<T>(u.x) || serving::any_nonfinite<T>(u.y) || serving::any_nonfinite<T>(u.z) ||
+                   serving::any_nonfinite<T>(u.w);
+          }
+          if (odd) {
+            *odd_flag = 1;
+            for (int i = lane + hidden * 8; i < behind * 8; i += 32) {
+              uint32_t* w = reinterpret_cast<uint32_t*>(vt + c * 16384 + i * 16);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if (serving::any_nonfinite<T>(w[e] & 0xFFFFu)) w[e] &= 0xFFFF0000u;
+                if (serving::any_nonfinite<T>(w[e] & 0xFFFF0000u)) w[e] &= 0xFFFFu;
+              }
+            }
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_clear[s]);
+        return true;
+      };
+      bool ok = true;
+      int next_clear = first_clear, issued = 0;
+      for (int j = 0; j < n_all && ok; ++j) {
+        const int s = j % C::kStages;
+        if (j >= C::kStages) {
+          // the tile whose place this one takes has to be cleared before it can be multiplied
+          while (ok && next_clear <= j - C::kStages) ok = clear(next_clear++);
+          ok = ok && wait_warp(&k_empty[s], ((j / C::kStages) - 1) & 1, a.err);
+        }
+        if (ok && lane == 0) {
+          if (j == 0 && n[0] > 0) load_q(0);
+          load_kv(&a.tk, &k_full[s], smem + C::kK + s * C::kTile, j);
+          if (j == 0 && n[1] > 0) load_q(1);
+        }
+        if (j >= C::kStages) ok = ok && wait_warp(&v_empty[s], ((j / C::kStages) - 1) & 1, a.err);
+        if (ok && lane == 0) {
+          load_kv(&a.tv, &v_full[s], smem + C::kV + s * C::kTile, j);
+          issued = j + 1;
+        }
+      }
+      while (ok && next_clear < n_all) ok = clear(next_clear++);
+      if (!ok && lane == 0)  // a wait ran out: no copy may be in flight when the CTA ends
+        for (int j = max(issued - C::kStages, 0); j < issued; ++j) {
+          mbar_wait(&k_full[j % C::kStages], (j / C::kStages) & 1, a.err);
+          mbar_wait(&v_full[j % C::kStages], (j / C::kStages) & 1, a.err);
+        }
+    } else if (warp == 9) {
+      // ---------------- MMA issuer
+      if (elect_one()) {
+        const uint32_t id_qk = idesc<T>(128, kKeys);
+        const uint32_t id_pv = idesc<T>(128, D) | (1u << 16);  // B (V) is MN-major
+        const uint32_t q0 = smem_u32(smem + C::kQ), k0 = smem_u32(smem + C::kK), v0 = smem_u32(smem + C::kV);
+        auto qk = [&](int x, int j) {
+          const uint32_t qa = q0 + x * C::kTile, ka = k0 + (j % C::kStages) * C::kTile;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {  // 16 dimensions (32 bytes) per MMA
+            const uint32_t off = (kk / 4) * 16384 + (kk % 4) * 32;
+            mma_bf16(tmem + C::kS + x * 128, smem_desc_sw128(qa + off), smem_desc_sw128(ka + off), id_qk, kk > 0 ? 1u : 0u);
+          }
+          mma_commit(&s_full[x]);
+        };
+        auto pv = [&](int x, int j) {
+          const uint32_t va = v0 + (j % C::kStages) * C::kTile;
+#pragma unroll
+          for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys per MMA: 8 TMEM columns of P, 16 rows (2048 bytes) of V
+            mma_bf16_tmem_a(tmem + C::kO + x * D, tmem + C::kP + x * C::kPStride + kk * 8,
+                            smem_desc_sw128_lbo(va + kk * 2048, 16384), id_pv, (j > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(&o_done[x]);
+        };
+        auto k_there = [&](int j) { return mbar_wait(&k_full[j % C::kStages], (j / C::kStages) & 1, a.err); };
+        auto v_there = [&](int j) {
+          const int s = j % C::kStages;
+          if (j >= first_clear) return mbar_wait(&v_clear[s], ((j - first_clear) / C::kStages) & 1, a.err);
+          return mbar_wait(&v_full[s], (j / C::kStages) & 1, a.err);
+        };
+        bool ok = n_all > 0;
+        ok = ok && k_there(0);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (ok && n[x] > 0) {
+            ok = mbar_wait(&q_full[x], 0, a.err);
+            tc_fence_after();
+            if (ok) qk(x, 0);
+          }
+        if (ok) mma_commit(&k_empty[0]);
+        for (int j = 0; j < n_all && ok; ++j) {
+          if constexpr (C::kOwnP) {
+            if (j + 1 < n_all) {
+              ok = k_there(j + 1);
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                if (ok && j + 1 < n[x]) {
+                  ok = mbar_wait(&s_free[x], j & 1, a.err);
+                  tc_fence_after();
+                  if (ok) qk(x, j + 1);
+                }
+              if (ok) mma_commit(&k_empty[(j + 1) % C::kStages]);
+            }
+            ok = ok && v_there(j);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              if (ok && j < n[x]) {
+                ok = mbar_wait(&p_full[x], j & 1, a.err);
+                tc_fence_after();
+                if (ok) pv(x, j);
+              }
+            if (ok) mma_commit(&v_empty[j % C::kStages]);
+          } else {
+            ok = v_there(j);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (ok && j < n[x]) {
+                ok = mbar_wait(&p_full[x], j & 1, a.err);
+                tc_fence_after();
+                if (ok) pv(x, j);
+              }
+              if (x == 1 && ok) mma_commit(&v_empty[j % C::kStages]);
+              if (ok && j + 1 < n[x]) {
+                ok = k_there(j + 1);
+                if (ok) qk(x, j + 1);
+              }
+            }
+            if (ok && j + 1 < n_all) mma_commit(&k_empty[(j + 1) % C::kStages]);
+          }
+        }
+        if (n_all > 0) {  // every MMA and every arrival it owes is done before the TMEM and the CTA go
+          mma_commit(all_done);
+          mbar_wait(all_done, 0, a.err);
+        }
+      }
+      __syncwarp();
+    } else {
+      // ---------------- softmax of tile x
+      const int x = warp >> 2, wq = warp & 3;
+      const int row = wq * 32 + lane, t = tok[x] + row / a.g, head = kh * a.g + row % a.g;
+      const bool real = row < toks[x] * a.g;
+      const int sees = real ? seen(t) : 0x7fffffff;  // rows that are not real are not stored, and need no mask
+      const uint32_t lanes = static_cast<uint32_t>(wq * 32) << 16;
+      const uint32_t tS = tmem + lanes + C::kS + x * 128, tP = tmem + lanes + C::kP + x * C::kPStride;
+      const uint32_t tO = tmem + lanes + C::kO + x * D;
+      const float c = a.scale_log2;
+      float m = -INFINITY;
+      float2 l = make_float2(0.f, 0.f);
+      bool ok = true;
+      for (int j = 0; j < n[x] && ok; ++j) {
+        ok = wait_warp(&s_full[x], j & 1, a.err);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t r[kKeys];
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) tmem_ld32(tS + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[ch * 32]));
+        tmem_ld_wait();
+        if constexpr (C::kOwnP) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[x]);
+        }
+        const int left = sees - j * kKeys;  // keys of this tile that the row sees
+        if (__any_sync(0xffffffffu, left < kKeys)) {
+#pragma unroll
+          for (int e = 0; e < kKeys; ++e)
+            if (e >= left) r[e] = 0xFF800000u;  // -infinity
+        }
+        float mp[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mp[u] = fmaxf(__uint_as_float(r[2 * u]), __uint_as_float(r[2 * u + 1]));
+#pragma unroll
+        for (int e = 16; e < kKeys; e += 2)
+          mp[(e >> 1) & 7] = max3(mp[(e >> 1) & 7], __uint_as_float(r[e]), __uint_as_float(r[e + 1]));
+        const float top = fmaxf(max3(mp[0], mp[1], mp[2]), max3(max3(mp[3], mp[4], mp[5]), mp[6], mp[7])) * c;
+        // the tile's P.V before this one: it reads P (own columns) and adds to O, which may be rescaled below
+        const bool grow = top > m + 8.f;
+        if (j > 0 && (C::kOwnP || __any_sync(0xffffffffu, grow))) {
+          ok = wait_warp(&o_done[x], (j - 1) & 1, a.err);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = !grow || m == -INFINITY ? 1.f : ex2_approx(m - top);
+          if (grow) m = top;
+          l = __fmul2_rn(l, make_float2(alpha, alpha));
+          if (j > 0) {
+#pragma unroll
+            for (int ch = 0; ch < D / 16; ++ch) {
+              uint32_t w[16];
+              tmem_ld16(tO + ch * 16, w);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) w[e] = __float_as_uint(__fmul_rn(__uint_as_float(w[e]), alpha));
+              tmem_st16(tO + ch * 16, w);
+            }
+          }
+        }
+        const float use = m == -INFINITY ? 0.f : m;
+        const float2 c2 = make_float2(c, c), nm2 = make_float2(-use, -use);
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const int k = ch * 32 + e;
+            const float2 z = __ffma2_rn(make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), c2, nm2);
+            const float2 p = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+            l = __fadd2_rn(l, p);
+            pk[e / 2] = serving::pack2<T>(p.x, p.y);
+          }
+          tmem_st16(tP + ch * 16, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      // ---------------- epilogue
+      if (ok && n[x] > 0) {
+        ok = wait_warp(&o_done[x], (n[x] - 1) & 1, a.err);
+        tc_fence_after();
+      }
+      if (ok && toks[x] > 0) {
+        const float inv = sees > 0 ? __frcp_rn(l.x + l.y) : 0.f;
+        T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + (real ? t : 0)) * a.o_rs + head * D;
+        const bool odd = *reinterpret_cast<volatile int*>(odd_flag) != 0;
+#pragma unroll
+        for (int ch = 0; ch < D / 32; ++ch) {
+          uint32_t r[32];
+          __syncwarp();
+          if (n[x] > 0) {
+            tmem_ld32(tO + ch * 32, r);
+            tmem_ld_wait();
+          }
+          if (!real) continue;
+          if (odd) {  // rare: the infinities and NaN that left V, for the rows that see them
+            for (int j = first_clear * kKeys; j < sees; ++j) {
+              const T* vr = static_cast<const T*>(a.v) + static_cast<size_t>(sk.begin + j) * a.v_rs + kh * D + ch * 32;
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float2 f = serving::unpack2<T>(*reinterpret_cast<const uint32_t*>(vr + e));
+                if (!isfinite(f.x)) r[e] = __float_as_uint(__uint_as_float(r[e]) + f.x);
+                if (!isfinite(f.y)) r[e + 1] = __float_as_uint(__uint_as_float(r[e + 1]) + f.y);
+              }
+            }
+          }
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            w[e] = sees > 0 ? serving::pack2<T>(__uint_as_float(r[2 * e]) * inv, __uint_as_float(r[2 * e + 1]) * inv) : 0u;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<uint4*>(dst + ch * 32 + u * 8) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace svla

@@ -6,6 +6,7 @@
 #include "host.cuh"
 #include "kv_append.cuh"
 #include "packed_attention.cuh"
+#include "packed_attention_tc.cuh"
 #include "paged_attention.cuh"
 
 namespace svla {
@@ -70,6 +71,51 @@ int32_t launch_packed(const PackedAttnArgs& a, long long items, cudaStream_t st)
   if (int32_t rc = allow_smem(kern, PackedSmem<T, D>::kBytes, configured)) return rc;
   return launch(kern, dim3(static_cast<unsigned>(items)), dim3(packed_detail::kWarps * 32), PackedSmem<T, D>::kBytes, st,
                 "packed_attention_kernel", a);
+}
+
+// a packed tensor as (dim, head, token) with a box of 64 dimensions, 128-byte swizzle
+int32_t make_tmap_packed(CUtensorMap* map, const void* base, int32_t dtype, uint64_t d, uint64_t heads, uint64_t rows,
+                         uint64_t rs, uint32_t box_heads, uint32_t box_rows) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(SVLA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {d, heads, rows};
+  cuuint64_t strides[2] = {d * 2, rs * 2};
+  cuuint32_t box[3] = {64, box_heads, box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, dtype == SVLA_DT_HALF ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                  const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SVLA_ERR_ARG, "cuTensorMapEncodeTiled (packed) failed (%d)", static_cast<int>(r));
+  return SVLA_OK;
+}
+
+template <typename T, int D>
+int32_t launch_packed_tc(const PackedTcArgs& a, long long items, cudaStream_t st) {
+  static bool configured[64] = {false};
+  auto kern = packed_attention_tc_kernel<T, D>;
+  if (int32_t rc = allow_smem(kern, ptc::Cfg<D>::kSmem, configured)) return rc;
+  return launch(kern, dim3(static_cast<unsigned>(items)), dim3(ptc::kThreads), ptc::Cfg<D>::kSmem, st,
+                "packed_attention_tc_kernel", a);
+}
+
+int32_t run_packed_tc(const svla_packed_attn_desc* d, float scale_log2, cudaStream_t st) {
+  const char* who = "svla_packed_attention";
+  PackedTcArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.g = d->hq / d->hkv, a.qt = 128 / a.g;
+  if (int32_t rc = make_tmap_packed(&a.tq, d->q, d->dtype, d->head_dim, d->hq, d->total_q, d->q_rs, a.g, a.qt)) return rc;
+  if (int32_t rc = make_tmap_packed(&a.tk, d->k, d->dtype, d->head_dim, d->hkv, d->total_k, d->k_rs, 1, ptc::kKeys)) return rc;
+  if (int32_t rc = make_tmap_packed(&a.tv, d->v, d->dtype, d->head_dim, d->hkv, d->total_k, d->v_rs, 1, ptc::kKeys)) return rc;
+  a.v = d->v, a.o = d->o, a.cu_q = d->cu_q, a.cu_k = d->cu_k, a.v_rs = d->v_rs, a.o_rs = d->o_rs;
+  a.batch = d->batch, a.total_q = d->total_q, a.total_k = d->total_k, a.hq = d->hq, a.hkv = d->hkv;
+  a.causal = d->causal != 0;
+  a.scale_log2 = scale_log2;
+  a.err = device_error_ptr();
+  const long long items = (static_cast<long long>(d->total_q) / (2 * a.qt) + d->batch) * d->hkv;
+  if (items > 0x7fffffffll) return fail(SVLA_ERR_ARG, "%s: too many query tiles", who);
+  const bool h = d->dtype == SVLA_DT_HALF;
+  if (d->head_dim == 64) return h ? launch_packed_tc<__half, 64>(a, items, st) : launch_packed_tc<__nv_bfloat16, 64>(a, items, st);
+  return h ? launch_packed_tc<__half, 128>(a, items, st) : launch_packed_tc<__nv_bfloat16, 128>(a, items, st);
 }
 
 // ---------------------------------------------------------------- paged
@@ -196,6 +242,9 @@ int32_t svla_packed_attention(const svla_packed_attn_desc* d, svla_stream_t stre
   a.batch = d->batch, a.total_q = d->total_q, a.total_k = d->total_k, a.hq = d->hq, a.hkv = d->hkv, a.g = g;
   a.causal = d->causal != 0;
   a.scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt(static_cast<float>(d->head_dim))) * serving::kLog2e;
+  if (d->impl < SVLA_ATTN_AUTO || d->impl > SVLA_ATTN_TCGEN05) return fail(SVLA_ERR_ARG, "%s: bad impl %d", who, d->impl);
+  if (d->impl == SVLA_ATTN_TCGEN05 && d->total_k == 0) return fail(SVLA_ERR_ARG, "%s: the tcgen05 kernel needs keys", who);
+  if (d->total_k > 0 && d->impl != SVLA_ATTN_MMA_SYNC) return run_packed_tc(d, a.scale_log2, cs(stream));
   a.qt = packed_detail::kRows / g;
   // the lengths are on the device: as many items as the sequences can have (each one's last tile may be short)
   const long long items = (static_cast<long long>(d->total_q) / a.qt + d->batch) * d->hkv;

@@ -491,7 +491,7 @@ def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
                      cu_k: torch.Tensor | None = None, causal: bool = True, scale: float = 0.0,
-                     out: torch.Tensor | None = None) -> torch.Tensor:
+                     out: torch.Tensor | None = None, impl: int = L.ATTN_AUTO) -> torch.Tensor:
     """Attention over prompts of different lengths packed back to back: q [rows, heads, head_dim], k / v
     [rows_k, kv_heads, head_dim] (views of one projection's output are fine), sequence b in rows cu_q[b] ..
     cu_q[b + 1] - 1 of q and cu_k[b] .. of k and v (cu_k None: the same).  Causal: the queries are the last tokens of
@@ -516,7 +516,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
             raise ValueError("out must have q's shape")
     desc = L.PackedAttnDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
                             q_rs, k_rs, v_rs, o_rs, batch, rows, k_rows, hq, hkv, d, _DT16[dtype], 1 if causal else 0,
-                            scale)
+                            scale, impl)
     check(lib().svla_packed_attention(ctypes.byref(desc), _stream()), "svla_packed_attention")
     return out
 

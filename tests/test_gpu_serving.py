@@ -71,14 +71,17 @@ def packed_reference(q, kv, lens_q, lens_k, causal, scale=None):
     return [torch.cat([o[i] for o in outs]) for i in range(3)]
 
 
+KERNELS = [L.ATTN_MMA_SYNC, L.ATTN_TCGEN05]
+
+
 def packed_check(lens_q, lens_k, hq, hkv, d, dtype, causal=True, seed=0, q_scale=1.0):
     q, kv = packed_inputs(lens_q, lens_k, hq, hkv, d, dtype, seed, q_scale)
     o, spread, size = packed_reference(q, kv, lens_q, lens_k, causal)
     kvd = kv.to(DEV)
-    got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints(starts(lens_q)).to(DEV),
-                               ints(starts(lens_k)).to(DEV), causal=causal)
-    within(got, o, S.attention_tolerance(o, spread, size, dtype, d))
-    return got
+    for impl in KERNELS:
+        got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints(starts(lens_q)).to(DEV),
+                                   ints(starts(lens_k)).to(DEV), causal=causal, impl=impl)
+        within(got, o, S.attention_tolerance(o, spread, size, dtype, d), f"impl {impl}")
 
 
 LENGTHS = [
@@ -111,7 +114,8 @@ def test_packed_attention_long_and_many(heads):
     packed_check(lens, lens, *heads, FP16, seed=5)
 
 
-def test_packed_attention_with_sharp_and_growing_scores():
+@pytest.mark.parametrize("impl", KERNELS)
+def test_packed_attention_with_sharp_and_growing_scores(impl):
     """Scores over a range of hundreds, and keys that grow along the sequence, so that the running maximum moves all the
     time."""
     for d, hq, hkv in ((64, 3, 1), (128, 4, 2)):
@@ -122,11 +126,12 @@ def test_packed_attention_with_sharp_and_growing_scores():
         q = q[:1].expand(500, hq, d).contiguous()
         o, spread, size = packed_reference(q, kv, [500], [500], True)
         kvd = kv.to(DEV)
-        got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints([0, 500]).to(DEV))
+        got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints([0, 500]).to(DEV), impl=impl)
         within(got, o, S.attention_tolerance(o, spread, size, BF16, d))
 
 
-def test_packed_attention_scale_and_strided_rows():
+@pytest.mark.parametrize("impl", KERNELS)
+def test_packed_attention_scale_and_strided_rows(impl):
     lens, hq, hkv, d = [70, 3], 6, 2, 64
     q, kv = packed_inputs(lens, lens, hq, hkv, d, BF16, seed=8)
     o, spread, size = packed_reference(q, kv, lens, lens, True, scale=0.3)
@@ -134,7 +139,7 @@ def test_packed_attention_scale_and_strided_rows():
     out = torch.full((73, 9, d), 7.0, dtype=BF16, device=DEV)
     cu = ints(starts(lens)).to(DEV)
     got = ops.packed_attention(fused[:, :hq], fused[:, hq:hq + hkv], fused[:, hq + hkv:hq + 2 * hkv], cu, scale=0.3,
-                               out=out[:, 2:8])
+                               out=out[:, 2:8], impl=impl)
     within(got, o, S.attention_tolerance(o, spread, size, BF16, d))
     assert bool((out[:, :2] == 7).all()) and bool((out[:, 8:] == 7).all())
 
@@ -142,7 +147,8 @@ def test_packed_attention_scale_and_strided_rows():
 @pytest.mark.parametrize("heads", [(15, 5, 64), (8, 2, 128)], ids=str)
 @pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("fill", [float("nan"), float("inf"), -float("inf")])
-def test_packed_attention_keeps_sequences_apart(heads, dtype, fill):
+@pytest.mark.parametrize("impl", KERNELS)
+def test_packed_attention_keeps_sequences_apart(impl, heads, dtype, fill):
     """A sequence full of NaN or infinities between two others, and rows behind the last one: the others' results are
     those without them, and rows behind the last sequence are left as they were."""
     hq, hkv, d = heads
@@ -153,7 +159,7 @@ def test_packed_attention_keeps_sequences_apart(heads, dtype, fill):
     q[211:], kv[211:] = fill, fill
     out = torch.full_like(q, 3.0).to(DEV)
     kvd = kv.to(DEV)
-    ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints(starts(lens)).to(DEV), out=out)
+    ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints(starts(lens)).to(DEV), out=out, impl=impl)
     tol = S.attention_tolerance(o, spread, size, dtype, d)
     for a, b in ((0, 50), (80, 211)):
         within(out[a:b], o[a:b], tol[a:b])
@@ -162,7 +168,8 @@ def test_packed_attention_keeps_sequences_apart(heads, dtype, fill):
 
 @pytest.mark.parametrize("heads", [(15, 5, 64), (8, 2, 128)], ids=str)
 @pytest.mark.parametrize("n,at", [(40, 20), (200, 130), (200, 0), (300, 299), (300, 127), (300, 128)])
-def test_packed_attention_non_finite_value_reaches_only_the_rows_that_see_it(heads, n, at):
+@pytest.mark.parametrize("impl", KERNELS)
+def test_packed_attention_non_finite_value_reaches_only_the_rows_that_see_it(impl, heads, n, at):
     hq, hkv, d = heads
     q, kv = packed_inputs([n], [n], hq, hkv, d, BF16, seed=10)
     o, spread, size = packed_reference(q, kv, [n], [n], True)
@@ -170,11 +177,12 @@ def test_packed_attention_non_finite_value_reaches_only_the_rows_that_see_it(hea
     g = hq // hkv
     o[at:, :g, 3], o[at:, :g, 5], o[at:, g:2 * g, d - 1] = float("nan"), float("inf"), -float("inf")
     kvd = kv.to(DEV)
-    got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints([0, n]).to(DEV))
+    got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints([0, n]).to(DEV), impl=impl)
     within(got, o, S.attention_tolerance(o, spread, size, BF16, d).nan_to_num(1.0))
 
 
-def test_packed_attention_non_finite_queries_and_keys():
+@pytest.mark.parametrize("impl", KERNELS)
+def test_packed_attention_non_finite_queries_and_keys(impl):
     """A NaN in a query row spoils that row alone; one in a key, the rows that see it."""
     hq, hkv, d, n = 6, 2, 64, 150
     q, kv = packed_inputs([n], [n], hq, hkv, d, BF16, seed=11)
@@ -184,26 +192,31 @@ def test_packed_attention_non_finite_queries_and_keys():
     o[10, 1] = float("nan")
     o[100:, 3:] = float("nan")
     kvd = kv.to(DEV)
-    got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints([0, n]).to(DEV))
+    got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints([0, n]).to(DEV), impl=impl)
     within(got, o, S.attention_tolerance(o, spread, size, BF16, d))
 
 
-def test_packed_attention_bounds_its_rows_by_the_tensors():
+@pytest.mark.parametrize("impl", KERNELS)
+def test_packed_attention_bounds_its_rows_by_the_tensors(impl):
     """Starts that point behind the tensors are cut off there; nothing outside is read or written."""
     q, kv = packed_inputs([20], [20], 6, 2, 64, BF16, seed=12)
     kvd = kv.to(DEV)
-    ref = ops.packed_attention(q.to(DEV), kvd[:, :2], kvd[:, 2:], ints([0, 20]).to(DEV))
-    got = ops.packed_attention(q.to(DEV), kvd[:, :2], kvd[:, 2:], ints([0, 1 << 20]).to(DEV))
+    ref = ops.packed_attention(q.to(DEV), kvd[:, :2], kvd[:, 2:], ints([0, 20]).to(DEV), impl=impl)
+    got = ops.packed_attention(q.to(DEV), kvd[:, :2], kvd[:, 2:], ints([0, 1 << 20]).to(DEV), impl=impl)
     assert torch.equal(got, ref)
     none = ops.packed_attention(q.to(DEV), kvd[:0, :2], kvd[:0, 2:], ints([0, 20]).to(DEV), ints([0, 0]).to(DEV))
     assert bool((none == 0).all())
+    if impl == L.ATTN_TCGEN05:
+        with pytest.raises(L.SvlaError, match="needs keys"):
+            ops.packed_attention(q.to(DEV), kvd[:0, :2], kvd[:0, 2:], ints([0, 20]).to(DEV), ints([0, 0]).to(DEV), impl=impl)
 
 
-def test_packed_attention_repeats_replays_and_other_streams():
+@pytest.mark.parametrize("impl", KERNELS)
+def test_packed_attention_repeats_replays_and_other_streams(impl):
     lens = [33, 190, 1]
     q, kv = packed_inputs(lens, lens, 15, 5, 64, BF16, seed=13)
     q, kv, cu = q.to(DEV), kv.to(DEV), ints(starts(lens)).to(DEV)
-    call = lambda: ops.packed_attention(q, kv[:, :5], kv[:, 5:], cu)  # noqa: E731
+    call = lambda: ops.packed_attention(q, kv[:, :5], kv[:, 5:], cu, impl=impl)  # noqa: E731
     ref = call()
     assert all(torch.equal(call(), ref) for _ in range(3))
     side = torch.cuda.Stream()
