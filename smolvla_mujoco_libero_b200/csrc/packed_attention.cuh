@@ -31,41 +31,72 @@ constexpr int kWarps = 4;
 constexpr int kRows = 16 * kWarps;  // query rows per CTA
 constexpr int kKeys = 64;
 
-// The work item `id` of the tiles of all sequences, longest first: tiles are numbered by their place j inside their
-// sequence, from the largest down (a causal tile's keys grow with j), then by sequence.  Sets the sequence and the tile;
-// false: there is no such item.  Called by one whole warp.
-__device__ __forceinline__ bool find_tile(const int* cu_q, int batch, int total, int qt, int id, int lane, int& b, int& j) {
-  auto tiles = [&](int i) { const serving::Span s = serving::span_of(cu_q, i, total); return (s.end - s.begin + qt - 1) / qt; };
-  // number of tiles with place >= x, over all sequences
-  auto at_least = [&](int x) {
-    int n = 0;
-    for (int i = lane; i < batch; i += 32) n += max(tiles(i) - x, 0);
-    return __reduce_add_sync(0xffffffffu, n);
-  };
-  int top = 0;
-  for (int i = lane; i < batch; i += 32) top = max(top, tiles(i));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (id >= at_least(0)) return false;
-  int lo = 0, hi = top;  // at_least(lo) > id >= at_least(hi)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (at_least(mid) > id) lo = mid; else hi = mid;
+// The tiles of `qt` tokens of all sequences, numbered longest first: by their place inside their sequence, from the
+// largest down (a causal tile's keys grow with it), then by sequence.  A warp walks through the numbers upwards; the tile
+// counts of the first 128 sequences stay in registers, those of more are read again (from L1) at every step.
+struct TileWalk {
+  static constexpr int kHeld = 4;
+  const int* cu_q;
+  int batch, total, qt;
+  int held[kHeld];
+  int place;         // tiles with a larger place come before; -1: there are no more
+  long long before;  // number of the first tile with this place
+
+  __device__ __forceinline__ int count(int i) const {
+    const serving::Span s = serving::span_of(cu_q, i, total);
+    return (s.end - s.begin + qt - 1) / qt;
   }
-  j = lo;
-  int rank = id - at_least(lo + 1);  // among the sequences with more than j tiles
-  for (int c = 0; c < batch; c += 32) {
-    const bool has = c + lane < batch && tiles(c + lane) > j;
-    const unsigned m = __ballot_sync(0xffffffffu, has);
-    const int n = __popc(m);
-    if (rank < n) {
-      const bool me = has && __popc(m & ((1u << lane) - 1u)) == rank;
-      b = c + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
-      return true;
+  __device__ __forceinline__ TileWalk(const int* cu_q_, int batch_, int total_, int qt_, int lane)
+      : cu_q(cu_q_), batch(batch_), total(total_), qt(qt_), before(0) {
+    int top = 0;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      held[u] = lane + 32 * u < batch ? count(lane + 32 * u) : 0;
+      top = max(top, held[u]);
     }
-    rank -= n;
+    for (int i = lane + 32 * kHeld; i < batch; i += 32) top = max(top, count(i));
+    place = __reduce_max_sync(0xffffffffu, top) - 1;
   }
-  return false;
-}
+  // sequence and place of tile number id (not below that of the last call); false: there is no such tile
+  __device__ __forceinline__ bool find(long long id, int lane, int& b, int& j) {
+    while (place >= 0) {
+      int rest = static_cast<int>(min(id - before, 0x7fffffffll));
+      int n = 0;
+      b = -1;
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) {
+        const unsigned m = __ballot_sync(0xffffffffu, held[u] > place);
+        pick(m, 32 * u, rest - n, lane, b);
+        n += __popc(m);
+      }
+      for (int c = 32 * kHeld; c < batch; c += 32) {
+        const unsigned m = __ballot_sync(0xffffffffu, c + lane < batch && count(min(c + lane, batch - 1)) > place);
+        pick(m, c, rest - n, lane, b);
+        n += __popc(m);
+      }
+      if (rest < n) {
+        j = place;
+        return true;
+      }
+      // every place down to the next smaller count has as many tiles: pass over those that lie before id
+      int next = 0;
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) next = max(next, held[u] <= place ? held[u] : 0);
+      for (int c = lane + 32 * kHeld; c < batch; c += 32) next = max(next, count(c) <= place ? count(c) : 0);
+      next = __reduce_max_sync(0xffffffffu, next);
+      const int pass = min(rest / n, place - next + 1);
+      before += static_cast<long long>(pass) * n;
+      place -= pass;
+    }
+    return false;
+  }
+  // b = first + the position of set bit number `rank` of m, if there is one
+  __device__ __forceinline__ static void pick(unsigned m, int first, int rank, int lane, int& b) {
+    if (rank < 0 || rank >= __popc(m)) return;
+    const bool me = ((m >> lane) & 1u) && __popc(m & ((1u << lane) - 1u)) == rank;
+    b = first + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
+  }
+};
 }  // namespace packed_detail
 
 template <typename T, int D>
@@ -88,7 +119,8 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
   const int kh = blockIdx.x % a.hkv;
   if (warp == 0) {
     int b = -1, j = 0;
-    const bool ok = find_tile(a.cu_q, a.batch, a.total_q, a.qt, blockIdx.x / a.hkv, lane, b, j);
+    TileWalk walk(a.cu_q, a.batch, a.total_q, a.qt, lane);
+    const bool ok = walk.find(blockIdx.x / a.hkv, lane, b, j);
     if (lane == 0) {
       place[0] = ok ? b : -1;
       place[1] = j;

@@ -3,16 +3,23 @@
 //
 // One CTA per SM takes two query tiles A and B of 128 packed rows (token-major, then the heads of the group; G * QT rows
 // of each are real) of one sequence and kv head, one behind the other, and walks over their keys in tiles of 128 that
-// both use.  320 threads:
+// both use.  384 threads:
 //   warps 0-3, 4-7  softmax of A and of B: thread t owns TMEM lane t = one query row, so maximum and sum need no
-//                   shuffles; the row's 128 scores are held in registers
+//                   shuffles; the row's 128 scores are held in registers (setmaxnreg)
 //   warp 8          TMA of Q, K and V; it also clears from the last V tiles what must not be multiplied (below)
-//   warp 9          TMEM owner (all 512 columns) and MMA issuer (one elected lane)
+//   warps 9, 10     MMA issuers of A and of B (9 owns the 512 columns of TMEM)
 // While one tile's rows are in the softmax, the tensor pipe works for the other.
 //
 // TMEM.  D = 64: S_A, S_B (128 columns each), P_A, P_B (64), O_A, O_B (64): P has columns of its own, so the next scores
 // are computed while the softmax still works on these.  D = 128: P_x over the first half of S_x, O_A, O_B (128): the next
-// scores of a tile follow its P.V (the tensor pipe runs one thread's MMAs in order).
+// scores of a tile follow its P.V (the tensor pipe runs one thread's MMAs in order), and P.V starts with the first half of
+// P (248 us for four prompts of 1024 to 4096 tokens, 257 with the whole).
+//
+// What the issuers wait for decides: a ready barrier asked by try_wait through one lane costs 200 cycles, by test_wait 41,
+// and one issuer for both tiles needed 3100 cycles for an iteration's waits, MMAs and commits.  One 16384-token prompt at
+// D = 64: 860 us; test_wait first: 734; an issuer per tile: 669; one pair of exponentials in eight as polynomials: 650.
+// Measured and left: two CTAs of one tile each per SM (715 us; 61 us for 64 ragged prompts where this takes 65), the same
+// as persistent CTAs that fetch ahead (785 and 63 us), scores read twice from TMEM instead of held (934 us).
 //
 // Exponentials are the bound at D = 64 (16 per clock and SM: 1024 cycles per 128 x 128 tile against 512 of MMA), both
 // pipes at D = 128.  The running maximum is lazy (O is rescaled only when a row's maximum grows by more than 8 in log2
@@ -44,7 +51,10 @@ struct PackedTcArgs {
 };
 
 namespace ptc {
-constexpr int kKeys = 128, kThreads = 320;
+constexpr int kKeys = 128, kThreads = 384;
+// registers: 384 threads x 168 at launch = 64512; the two softmax warpgroups take 208 each, the third keeps 88:
+// 256 * 208 + 128 * 88 = 64512
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 
 template <int D>
 struct Cfg {
@@ -83,11 +93,40 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// bounded wait of a warp: one lane polls
+// 2^z for two z <= 8 or so on the fp32 pipe: z = n + f with n = rint(z) (adding 1.5 * 2^23 leaves n in the low bits), 2^f
+// by its minimax polynomial of degree 4 on [-1/2, 1/2] (relative error 2.6e-6, found by exchanging extrema), n added to the
+// exponent.  z is first raised to at least -126: 2^-126 instead of less.
+__device__ __forceinline__ float2 exp2_poly(float2 z) {
+  z.x = fmaxf(z.x, -126.f);
+  z.y = fmaxf(z.y, -126.f);
+  auto both = [](float c) { return make_float2(c, c); };
+  const float2 t = __fadd2_rn(z, both(12582912.f));
+  const float2 f = __fadd2_rn(z, __ffma2_rn(t, both(-1.f), both(12582912.f)));
+  float2 p = __ffma2_rn(f, both(0.0095701f), both(0.05591786f));
+  p = __ffma2_rn(f, p, both(0.24024745f));
+  p = __ffma2_rn(f, p, both(0.69312181f));
+  p = __ffma2_rn(f, p, both(0.99999926f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
+// Bounded wait of a whole warp.  A phase that is over already, the usual case here, is seen by test_wait in about 40
+// cycles; try_wait takes 100 then, and one lane polling for the others 200.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
-  bool ok = true;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, err);
-  return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  bool ok = done != 0;
+  if (!ok) {
+    for (uint32_t i = 0; i < kSpinLimit && !ok; ++i) ok = mbar_try_wait(bar, parity);
+    if (!ok && (threadIdx.x & 31) == 0) record_error(err, kErrMbarTimeout);
+  }
+  return __all_sync(0xffffffffu, ok);
 }
 }  // namespace ptc
 
@@ -105,31 +144,33 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
   uint64_t* v_clear = v_empty + C::kStages;  // an edge tile's V has been cleared
   uint64_t* s_full = v_clear + C::kStages;   // [2] scores are there
   uint64_t* s_free = s_full + 2;             // [2] (own P) scores are in registers
-  uint64_t* p_full = s_free + 2;             // [2] probabilities are there
+  uint64_t* p_half = s_free + 2;             // [2] the first 64 keys' probabilities are there
+  uint64_t* p_full = p_half + 2;             // [2] all of them
   uint64_t* o_done = p_full + 2;             // [2] the tile's P.V so far is done
-  uint64_t* all_done = o_done + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  uint64_t* all_done = o_done + 2;           // [2] everything the tile's issuer owes
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 2);
   int* place = reinterpret_cast<int*>(tmem_slot + 1);  // [2] sequence, item
   int* odd_flag = place + 2;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (warp == 8) {
     if (lane == 0) {
       for (int s = 0; s < C::kStages; ++s) {
         mbar_init(&k_full[s], 1);
-        mbar_init(&k_empty[s], 1);
+        mbar_init(&k_empty[s], 2);  // both tiles' MMAs
         mbar_init(&v_full[s], 1);
-        mbar_init(&v_empty[s], 1);
+        mbar_init(&v_empty[s], 2);
         mbar_init(&v_clear[s], 1);
       }
       for (int x = 0; x < 2; ++x) {
         mbar_init(&q_full[x], 1);
         mbar_init(&s_full[x], 1);
         mbar_init(&s_free[x], 4);
+        mbar_init(&p_half[x], 4);
         mbar_init(&p_full[x], 4);
         mbar_init(&o_done[x], 1);
+        mbar_init(&all_done[x], 1);
       }
-      mbar_init(all_done, 1);
       fence_mbar_init();
       *odd_flag = 0;
     }
@@ -140,7 +181,8 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
   pdl_wait();  // lengths, q, k, v are written by the previous kernel
   if (warp == 0) {
     int b = -1, j = 0;
-    const bool ok = packed_detail::find_tile(a.cu_q, a.batch, a.total_q, 2 * a.qt, blockIdx.x / a.hkv, lane, b, j);
+    packed_detail::TileWalk walk(a.cu_q, a.batch, a.total_q, 2 * a.qt, lane);
+    const bool ok = walk.find(blockIdx.x / a.hkv, lane, b, j);
     if (lane == 0) {
       place[0] = ok ? b : -1;
       place[1] = j;
@@ -169,6 +211,8 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
     // CTA does not see
     const int first_clear = seen(tok[0]) / kKeys;
 
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
       // ---------------- producer
       if (lane == 0) {
@@ -194,12 +238,12 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
         uint8_t* vt = smem + C::kV + s * C::kTile;
         const int behind = min(max(n_k - j * kKeys, 0), kKeys);                  // rows from here on are another's
         const int hidden = a.causal ? max(seen(tok[0]) - j * kKeys, 0) : kKeys;  // rows from here on some query does not see
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < C::kSub; ++c) {
           for (int i = lane + behind * 8; i < 128 * 8; i += 32)
             *reinterpret_cast<uint4*>(vt + c * 16384 + i * 16) = make_uint4(0, 0, 0, 0);
           bool odd = false;
-#pragma unroll 4
+#pragma unroll 2
           for (int i = lane + hidden * 8; i < behind * 8; i += 32) {
             const uint4 u = *reinterpret_cast<const uint4*>(vt + c * 16384 + i * 16);
             odd |= serving::any_nonfinite<T>(u.x) || serving::any_nonfinite<T>(u.y) || serving::any_nonfinite<T>(u.z) ||
@@ -248,92 +292,94 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
           mbar_wait(&k_full[j % C::kStages], (j / C::kStages) & 1, a.err);
           mbar_wait(&v_full[j % C::kStages], (j / C::kStages) & 1, a.err);
         }
-    } else if (warp == 9) {
-      // ---------------- MMA issuer
-      if (elect_one()) {
-        const uint32_t id_qk = idesc<T>(128, kKeys);
-        const uint32_t id_pv = idesc<T>(128, D) | (1u << 16);  // B (V) is MN-major
-        const uint32_t q0 = smem_u32(smem + C::kQ), k0 = smem_u32(smem + C::kK), v0 = smem_u32(smem + C::kV);
-        auto qk = [&](int x, int j) {
-          const uint32_t qa = q0 + x * C::kTile, ka = k0 + (j % C::kStages) * C::kTile;
+    } else if (warp < 11) {
+      // ---------------- MMA issuer of tile x (warps 9, 10).  The whole warp walks through the loop and one elected lane
+      // issues.  A warp of its own for each tile: waits, issue and commits of one iteration for both tiles took one warp
+      // 3100 cycles, longer than the softmax that they serve.
+      const int x = warp - 9, nx = x ? n[1] : n[0];
+      const uint32_t id_qk = idesc<T>(128, kKeys);
+      const uint32_t id_pv = idesc<T>(128, D) | (1u << 16);  // B (V) is MN-major
+      const uint32_t k0 = smem_u32(smem + C::kK), v0 = smem_u32(smem + C::kV);
+      const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+      // descriptors of a tile's first MMA; the others are constant distances (in 16-byte units) away
+      const uint64_t qd = smem_desc_sw128(smem_u32(smem + C::kQ) + x * C::kTile);
+      auto qk = [&](int j) {  // and the K tile is free again
+        const uint64_t kd = smem_desc_sw128(k0 + (j % C::kStages) * C::kTile);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {  // 16 dimensions (32 bytes) per MMA
-            const uint32_t off = (kk / 4) * 16384 + (kk % 4) * 32;
-            mma_bf16(tmem + C::kS + x * 128, smem_desc_sw128(qa + off), smem_desc_sw128(ka + off), id_qk, kk > 0 ? 1u : 0u);
+            const uint32_t off = ((kk / 4) * 16384 + (kk % 4) * 32) >> 4;
+            mma_bf16(tm + C::kS + x * 128, qd + off, kd + off, id_qk, kk > 0 ? 1u : 0u);
           }
           mma_commit(&s_full[x]);
-        };
-        auto pv = [&](int x, int j) {
-          const uint32_t va = v0 + (j % C::kStages) * C::kTile;
+          mma_commit(&k_empty[j % C::kStages]);
+        }
+        __syncwarp();
+      };
+      // keys 16 first .. 16 last - 1 of the tile; after the last ones the V tile is free again
+      auto pv = [&](int j, auto first, auto last) {
+        const uint64_t vd = smem_desc_sw128_lbo(v0 + (j % C::kStages) * C::kTile, 16384);
+        if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kKeys / 16; ++kk)  // 16 keys per MMA: 8 TMEM columns of P, 16 rows (2048 bytes) of V
-            mma_bf16_tmem_a(tmem + C::kO + x * D, tmem + C::kP + x * C::kPStride + kk * 8,
-                            smem_desc_sw128_lbo(va + kk * 2048, 16384), id_pv, (j > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(&o_done[x]);
-        };
-        auto k_there = [&](int j) { return mbar_wait(&k_full[j % C::kStages], (j / C::kStages) & 1, a.err); };
-        auto v_there = [&](int j) {
-          const int s = j % C::kStages;
-          if (j >= first_clear) return mbar_wait(&v_clear[s], ((j - first_clear) / C::kStages) & 1, a.err);
-          return mbar_wait(&v_full[s], (j / C::kStages) & 1, a.err);
-        };
-        bool ok = n_all > 0;
-        ok = ok && k_there(0);
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (ok && n[x] > 0) {
-            ok = mbar_wait(&q_full[x], 0, a.err);
-            tc_fence_after();
-            if (ok) qk(x, 0);
-          }
-        if (ok) mma_commit(&k_empty[0]);
-        for (int j = 0; j < n_all && ok; ++j) {
-          if constexpr (C::kOwnP) {
-            if (j + 1 < n_all) {
-              ok = k_there(j + 1);
-#pragma unroll
-              for (int x = 0; x < 2; ++x)
-                if (ok && j + 1 < n[x]) {
-                  ok = mbar_wait(&s_free[x], j & 1, a.err);
-                  tc_fence_after();
-                  if (ok) qk(x, j + 1);
-                }
-              if (ok) mma_commit(&k_empty[(j + 1) % C::kStages]);
-            }
-            ok = ok && v_there(j);
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-              if (ok && j < n[x]) {
-                ok = mbar_wait(&p_full[x], j & 1, a.err);
-                tc_fence_after();
-                if (ok) pv(x, j);
-              }
-            if (ok) mma_commit(&v_empty[j % C::kStages]);
-          } else {
-            ok = v_there(j);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              if (ok && j < n[x]) {
-                ok = mbar_wait(&p_full[x], j & 1, a.err);
-                tc_fence_after();
-                if (ok) pv(x, j);
-              }
-              if (x == 1 && ok) mma_commit(&v_empty[j % C::kStages]);
-              if (ok && j + 1 < n[x]) {
-                ok = k_there(j + 1);
-                if (ok) qk(x, j + 1);
-              }
-            }
-            if (ok && j + 1 < n_all) mma_commit(&k_empty[(j + 1) % C::kStages]);
+          for (int kk = first.value; kk < last.value; ++kk)  // 16 keys per MMA: 8 TMEM columns of P, 16 rows (2048 bytes) of V
+            mma_bf16_tmem_a(tm + C::kO + x * D, tm + C::kP + x * C::kPStride + kk * 8, vd + kk * (2048 >> 4), id_pv,
+                            (j > 0 || kk > 0) ? 1u : 0u);
+          if (last.value == 8) {
+            mma_commit(&o_done[x]);
+            mma_commit(&v_empty[j % C::kStages]);
           }
         }
-        if (n_all > 0) {  // every MMA and every arrival it owes is done before the TMEM and the CTA go
-          mma_commit(all_done);
-          mbar_wait(all_done, 0, a.err);
+        __syncwarp();
+      };
+      using std::integral_constant;
+      auto k_there = [&](int j) { return wait_warp(&k_full[j % C::kStages], (j / C::kStages) & 1, a.err); };
+      auto v_there = [&](int j) {
+        const int s = j % C::kStages;
+        if (j >= first_clear) return wait_warp(&v_clear[s], ((j - first_clear) / C::kStages) & 1, a.err);
+        return wait_warp(&v_full[s], (j / C::kStages) & 1, a.err);
+      };
+      bool ok = nx > 0 && wait_warp(&q_full[x], 0, a.err) && k_there(0);
+      if (ok) qk(0);
+      for (int j = 0; j < nx && ok; ++j) {
+        if (C::kOwnP && j + 1 < nx) {  // the next scores as soon as these are in registers
+          ok = k_there(j + 1) && wait_warp(&s_free[x], j & 1, a.err);
+          tc_fence_after();
+          if (ok) qk(j + 1);
+        }
+        ok = ok && v_there(j);
+        if constexpr (C::kOwnP) {
+          ok = ok && wait_warp(&p_full[x], j & 1, a.err);
+          tc_fence_after();
+          if (ok) pv(j, integral_constant<int, 0>{}, integral_constant<int, 8>{});
+        } else {  // both pipes are the bound: start when half of P is there
+          ok = ok && wait_warp(&p_half[x], j & 1, a.err);
+          tc_fence_after();
+          if (ok) pv(j, integral_constant<int, 0>{}, integral_constant<int, 4>{});
+          ok = ok && wait_warp(&p_full[x], j & 1, a.err);
+          tc_fence_after();
+          if (ok) pv(j, integral_constant<int, 4>{}, integral_constant<int, 8>{});
+        }
+        if (!C::kOwnP && j + 1 < nx) {
+          ok = ok && k_there(j + 1);
+          if (ok) qk(j + 1);
         }
       }
-      __syncwarp();
+      // Key tiles that only the other query tile uses: given back once they are there.  Not earlier: an arrival before
+      // would count for the tile that had the place before, and the producer would arm a barrier whose copy is in flight.
+      for (int j = nx; j < n_all && (ok || nx == 0); ++j) {
+        if (!k_there(j)) break;
+        if (lane == 0) mbar_arrive(&k_empty[j % C::kStages]);
+        if (!wait_warp(&v_full[j % C::kStages], (j / C::kStages) & 1, a.err)) break;
+        if (lane == 0) mbar_arrive(&v_empty[j % C::kStages]);
+      }
+      if (nx > 0) {  // every MMA and every arrival it owes is done before the TMEM and the CTA go
+        if (elect_one()) mma_commit(&all_done[x]);
+        __syncwarp();
+        wait_warp(&all_done[x], 0, a.err);
+      }
+    }
     } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
       // ---------------- softmax of tile x
       const int x = warp >> 2, wq = warp & 3;
       const int row = wq * 32 + lane, t = tok[x] + row / a.g, head = kh * a.g + row % a.g;
@@ -350,6 +396,7 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
         ok = wait_warp(&s_full[x], j & 1, a.err);
         if (!ok) break;
         tc_fence_after();
+        const int left = sees - j * kKeys;  // keys of this tile that the row sees
         uint32_t r[kKeys];
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) tmem_ld32(tS + ch * 32, *reinterpret_cast<uint32_t(*)[32]>(&r[ch * 32]));
@@ -359,7 +406,6 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_free[x]);
         }
-        const int left = sees - j * kKeys;  // keys of this tile that the row sees
         if (__any_sync(0xffffffffu, left < kKeys)) {
 #pragma unroll
           for (int e = 0; e < kKeys; ++e)
@@ -384,7 +430,7 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
           if (grow) m = top;
           l = __fmul2_rn(l, make_float2(alpha, alpha));
           if (j > 0) {
-#pragma unroll
+#pragma unroll 1
             for (int ch = 0; ch < D / 16; ++ch) {
               uint32_t w[16];
               tmem_ld16(tO + ch * 16, w);
@@ -404,16 +450,19 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
           for (int e = 0; e < 32; e += 2) {
             const int k = ch * 32 + e;
             const float2 z = __ffma2_rn(make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), c2, nm2);
-            const float2 p = make_float2(ex2_approx(z.x), ex2_approx(z.y));
+            // one pair in eight leaves the exponential unit, where that is the bound (650 us instead of 669; two: 690)
+            const float2 p = (D == 64 && (e / 2) % 8 == 0) ? exp2_poly(z) : make_float2(ex2_approx(z.x), ex2_approx(z.y));
             l = __fadd2_rn(l, p);
             pk[e / 2] = serving::pack2<T>(p.x, p.y);
           }
           tmem_st16(tP + ch * 16, pk);
+          if (ch == 3 || (!C::kOwnP && ch == 1)) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(ch == 1 ? &p_half[x] : &p_full[x]);
+          }
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
       }
       // ---------------- epilogue
       if (ok && n[x] > 0) {

@@ -99,7 +99,6 @@ int32_t launch_packed_tc(const PackedTcArgs& a, long long items, cudaStream_t st
 }
 
 int32_t run_packed_tc(const svla_packed_attn_desc* d, float scale_log2, cudaStream_t st) {
-  const char* who = "svla_packed_attention";
   PackedTcArgs a;
   std::memset(&a, 0, sizeof(a));
   a.g = d->hq / d->hkv, a.qt = 128 / a.g;
@@ -112,10 +111,26 @@ int32_t run_packed_tc(const svla_packed_attn_desc* d, float scale_log2, cudaStre
   a.scale_log2 = scale_log2;
   a.err = device_error_ptr();
   const long long items = (static_cast<long long>(d->total_q) / (2 * a.qt) + d->batch) * d->hkv;
-  if (items > 0x7fffffffll) return fail(SVLA_ERR_ARG, "%s: too many query tiles", who);
   const bool h = d->dtype == SVLA_DT_HALF;
   if (d->head_dim == 64) return h ? launch_packed_tc<__half, 64>(a, items, st) : launch_packed_tc<__nv_bfloat16, 64>(a, items, st);
   return h ? launch_packed_tc<__half, 128>(a, items, st) : launch_packed_tc<__nv_bfloat16, 128>(a, items, st);
+}
+
+// The automatic choice between the two kernels, from what the host knows: the average lengths.  An item of the tcgen05
+// kernel (256 query rows) costs 5 to 6 us beside its key tiles, one of the mma.sync kernel (64 rows, several per SM) 1 or
+// 2; a key costs it less.  One round of items: it wins from 448 keys on (D = 64: 177 keys 8.9 us against 7.8, 512 keys 12.4
+// both, one token after 2000 keys 20.9 against 32.2), at D = 128 from 256 (200 keys and one token 7.9 against 10.5, 177
+// tokens 13.2 against 11.2, 512 tokens 19.0 against 24.4).  Many rounds: it is the keys per item, less what its rows are
+// not filled, that counts (D = 64, 3 heads per group, 64 prompts: 128 tokens 39.1 against 37.3, 256 tokens 78 against 82,
+// 512 tokens 158 against 217, 16 tokens after 500 keys 29.4 against 22.6; D = 128, 4 heads: 48 tokens 40 against 46, one
+// token after 200 keys 32 against 26, after 2000 keys 128 against 153).
+bool packed_prefers_tc(const svla_packed_attn_desc* d, int g) {
+  const long long q = (static_cast<long long>(d->total_q) + d->batch - 1) / d->batch;
+  const long long keys = static_cast<long long>(d->total_k) / d->batch;
+  const long long pair = 2 * (128 / g), items = d->batch * ((q + pair - 1) / pair) * d->hkv;
+  if (items <= sm_count()) return keys >= (d->head_dim == 64 ? 448 : 256);
+  const long long rows = q * g < 256 ? q * g : 256;
+  return keys * rows >= 256 * (d->head_dim == 64 ? 224 : 32);
 }
 
 // ---------------------------------------------------------------- paged
@@ -244,7 +259,8 @@ int32_t svla_packed_attention(const svla_packed_attn_desc* d, svla_stream_t stre
   a.scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt(static_cast<float>(d->head_dim))) * serving::kLog2e;
   if (d->impl < SVLA_ATTN_AUTO || d->impl > SVLA_ATTN_TCGEN05) return fail(SVLA_ERR_ARG, "%s: bad impl %d", who, d->impl);
   if (d->impl == SVLA_ATTN_TCGEN05 && d->total_k == 0) return fail(SVLA_ERR_ARG, "%s: the tcgen05 kernel needs keys", who);
-  if (d->total_k > 0 && d->impl != SVLA_ATTN_MMA_SYNC) return run_packed_tc(d, a.scale_log2, cs(stream));
+  if (d->impl == SVLA_ATTN_TCGEN05 || (d->impl == SVLA_ATTN_AUTO && d->total_k > 0 && packed_prefers_tc(d, g)))
+    return run_packed_tc(d, a.scale_log2, cs(stream));
   a.qt = packed_detail::kRows / g;
   // the lengths are on the device: as many items as the sequences can have (each one's last tile may be short)
   const long long items = (static_cast<long long>(d->total_q) / a.qt + d->batch) * d->hkv;
