@@ -17,8 +17,11 @@ from . import _lib as L
 from ._lib import check, lib
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream builds a Stream object: 3 us a call
+
+
 def _stream() -> int:
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _p(t: torch.Tensor | None) -> int | None:
@@ -356,11 +359,11 @@ _DT16 = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_HALF}
 
 def _packed_first(t: torch.Tensor, name: str) -> tuple[torch.dtype, int, int]:
     """(dtype, device index, head_dim) of the tensor that the call's other tensors have to fit."""
-    if not t.is_cuda:
+    dev = t.get_device()
+    if dev < 0:
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
     if t.dim() != 3 or t.dtype not in _DT16:
         raise ValueError(f"{name} must be bf16 or fp16 [rows, heads, head_dim], got {t.dtype} {tuple(t.shape)}")
-    dev = t.get_device()
     if dev != torch.cuda.current_device():
         raise ValueError(f"{name} is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
     return t.dtype, dev, t.shape[2]
@@ -380,15 +383,14 @@ def _packed(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int, d: int) ->
 
 
 def _ints(t: torch.Tensor, name: str, n: int, dev: int) -> None:
-    if t.dtype is not torch.int32 or t.get_device() != dev or t.dim() != 1 or len(t) != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32 [{n}] on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _batch_of(cu: torch.Tensor, name: str, dev: int) -> int:
-    if cu.dim() != 1 or len(cu) < 1:
-        raise ValueError(f"{name} must be int32 [batch + 1], got {list(cu.shape)}")
-    _ints(cu, name, len(cu), dev)
-    return len(cu) - 1
+    n = cu.numel()
+    _ints(cu, name, n if n else 1, dev)
+    return n - 1
 
 
 def kv_cache(n_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 16,
@@ -418,12 +420,14 @@ def _cache(cache: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, 
     if cache.get_device() != dev or not cache.is_contiguous():
         raise ValueError(f"cache must be contiguous on cuda:{dev}")
     _ints(kv_len, "kv_len", batch, dev)
-    if (page_table.dtype is not torch.int32 or page_table.get_device() != dev or page_table.dim() != 2
-            or len(page_table) != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1)):
-        raise ValueError(f"page_table must be int32 [{batch}, max_pages] on cuda:{dev} with unit column stride, got "
-                         f"{page_table.dtype} {list(page_table.shape)} on {page_table.device}")
-    max_pages = page_table.shape[1]
-    return bits, page, shape[0], shape[1], max_pages, (page_table.stride(0) if batch > 1 else max_pages)
+    table = page_table.shape
+    if page_table.dtype is not torch.int32 or page_table.get_device() != dev or len(table) != 2 or table[0] != batch:
+        raise ValueError(f"page_table must be int32 [{batch}, max_pages] on cuda:{dev}, got {page_table.dtype} "
+                         f"{list(table)} on {page_table.device}")
+    rs, cs = page_table.stride()
+    if cs != 1 and table[1] > 1:
+        raise ValueError(f"page_table must have unit column stride, got strides {page_table.stride()}")
+    return bits, page, shape[0], shape[1], table[1], (rs if batch > 1 else table[1])
 
 
 def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
@@ -473,10 +477,11 @@ def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch
             raise ValueError("v_out must have v's shape")
         vo_ptr = v_out.data_ptr()
     if rope_cs is not None:
-        if (rope_cs.dtype is not torch.float32 or rope_cs.get_device() != dev or rope_cs.dim() != 3
-                or rope_cs.shape[1] != d // 2 or rope_cs.shape[2] != 2 or not rope_cs.is_contiguous()):
+        shape = rope_cs.shape
+        if (rope_cs.dtype is not torch.float32 or rope_cs.get_device() != dev or len(shape) != 3
+                or shape[1] != d // 2 or shape[2] != 2 or not rope_cs.is_contiguous()):
             raise ValueError(f"rope_cs must be contiguous fp32 [max_pos, {d // 2}, 2] on cuda:{dev}")
-        max_pos, cs_ptr = len(rope_cs), rope_cs.data_ptr()
+        max_pos, cs_ptr = shape[0], rope_cs.data_ptr()
     if pos is not None:
         _ints(pos, "pos", rows, dev)
         pos_ptr = pos.data_ptr()
@@ -485,7 +490,7 @@ def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch
                               cu_q.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), pos_ptr, cs_ptr, q_rs, k_rs,
                               v_rs, qo_rs, ko_rs, vo_rs, table_rs, batch, rows, hq, hkv, d, _DT16[dtype], bits, page,
                               n_pages, max_pages, max_pos)
-        check(lib().svla_kv_append(ctypes.byref(desc), _stream()), "svla_kv_append")
+        check(lib().svla_kv_append(ctypes.byref(desc), _raw_stream(dev)), "svla_kv_append")
     return (q_out, k_out, v_out) if want_rows else q_out
 
 
@@ -517,7 +522,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     desc = L.PackedAttnDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
                             q_rs, k_rs, v_rs, o_rs, batch, rows, k_rows, hq, hkv, d, _DT16[dtype], 1 if causal else 0,
                             scale, impl)
-    check(lib().svla_packed_attention(ctypes.byref(desc), _stream()), "svla_packed_attention")
+    check(lib().svla_packed_attention(ctypes.byref(desc), _raw_stream(dev)), "svla_packed_attention")
     return out
 
 
@@ -549,7 +554,7 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor, kv
     desc = L.PagedAttnDesc(q.data_ptr(), cache.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(),
                            page_table.data_ptr(), ws_ptr, ws_bytes, q_rs, o_rs, table_rs, batch, rows, hq, hkv, d,
                            _DT16[dtype], bits, page, n_pages, max_pages, scale)
-    check(handle.svla_paged_attention(ctypes.byref(desc), _stream()), "svla_paged_attention")
+    check(handle.svla_paged_attention(ctypes.byref(desc), _raw_stream(dev)), "svla_paged_attention")
     return out
 
 
