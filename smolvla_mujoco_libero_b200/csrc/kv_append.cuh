@@ -16,11 +16,13 @@
 // exactly between two codes, and a reciprocal's last bit would then decide.  A group with a NaN or an infinity reads
 // back as NaN.
 //
-// Work split: a warp takes one token and, when there are few tokens, a share of its heads; D / 16 lanes hold a head's
-// row (8 dimensions of each half), so a warp's accesses are whole 128- or 256-byte rows, the rotation pairs meet in one
-// lane, the token's (cos, sin) are read once for all heads, and a quantisation group is 4 lanes (two shuffles per
-// extremum).
-// Bound by memory traffic at many tokens, by latency at few.
+// Work split: a warp takes one token and, when there are few tokens, a share of its heads; D / 16 lanes hold a head's row (8
+// dimensions of each half), so a warp's accesses are whole 128- or 256-byte rows, the rotation pairs meet in one lane, the
+// token's (cos, sin) are read once for all heads, and a quantisation group is 4 lanes (two shuffles per extremum).  The
+// first row is on its way while the token's place is looked up, every other one while the one before is worked on.
+// Bound by memory traffic at many tokens (26337 rows of 48 heads into 4 bits, D = 128: 694 MB in 127 us, 5.5 TB/s; with
+// library divisions for the quotients 195 us), by latency at few.  Measured for 15579 rows of 25 heads at D = 64 (104 MB in
+// 26 us) and left: four tokens per warp 34 us, two rows ahead 30 us, whole blocks of tokens staged in shared memory 29 us.
 #pragma once
 
 #include "serving_common.cuh"
@@ -53,6 +55,14 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return r;
 }
 
+// d / s correctly rounded, r = 1 / s correctly rounded: P. Markstein's correction of a quotient (Computation of elementary
+// functions on the IBM RISC System/6000 processor, 1990), q + (d - q s) r with two fused operations.  Checked for all
+// significands of a bf16 s and an fp32 d; steps beyond 2^+-60 take the division itself.
+__device__ __forceinline__ float quotient(float d, float s, float r) {
+  const float q = __fmul_rn(d, r);
+  return __fmaf_rn(__fmaf_rn(-q, s, d), r, q);
+}
+
 // 8 values of a lane, quantised with the 4 lanes of their group; x becomes what the codes stand for
 __device__ __forceinline__ void quantise8(float (&x)[8], uint32_t& codes, uint32_t& pair) {
   float lo = x[0], hi = x[0];
@@ -69,12 +79,24 @@ __device__ __forceinline__ void quantise8(float (&x)[8], uint32_t& codes, uint32
   pair = pack_bf16_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), lo);
   const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xFFFF0000u);
   codes = 0u;
+  constexpr float kC = 12582912.0f;  // 1.5 * 2^23: adding it rounds to an integer (ties to even) in the low bits
+  if (s > 8.6e-19f && s < 1.2e18f) {
+    const float r = __frcp_rn(s);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float c = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[e], m), s)) : 0.f;
-    c = fminf(fmaxf(c, 0.f), 15.f);
-    codes |= static_cast<uint32_t>(c) << (4 * e);
-    x[e] = __fadd_rn(__fmul_rn(c, s), m);
+    for (int e = 0; e < 8; ++e) {
+      const float q = fminf(fmaxf(quotient(__fsub_rn(x[e], m), s, r), 0.f), 15.f);
+      const float t = __fadd_rn(q, kC);
+      codes |= (__float_as_uint(t) & 15u) << (4 * e);
+      x[e] = __fmaf_rn(__fsub_rn(t, kC), s, m);  // the product is exact
+    }
+  } else {  // a step of zero, a tiny or a huge one, or none (NaN)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float c = s > 0.f ? rintf(__fdiv_rn(__fsub_rn(x[e], m), s)) : 0.f;
+      c = fminf(fmaxf(c, 0.f), 15.f);
+      codes |= static_cast<uint32_t>(c) << (4 * e);
+      x[e] = __fadd_rn(__fmul_rn(c, s), m);
+    }
   }
 }
 
@@ -95,8 +117,9 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 }
 }  // namespace append_detail
 
+// 4 bits: at most 64 registers, 32 warps per SM (26337 rows of 48 heads at D = 128: 127 us, 160 with 86 registers)
 template <typename T, int D, int BITS>
-__global__ void __launch_bounds__(append_detail::kWarps * 32) kv_append_kernel(const KvAppendArgs a) {
+__global__ void __launch_bounds__(append_detail::kWarps * 32, BITS == 4 ? 8 : 1) kv_append_kernel(const KvAppendArgs a) {
   using namespace append_detail;
   constexpr int kLanes = D / 16, kSlots = 32 / kLanes;  // lanes of a head's row, rows per warp
   pdl_wait();
@@ -105,6 +128,25 @@ __global__ void __launch_bounds__(append_detail::kWarps * 32) kv_append_kernel(c
   const long long task = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   const int t = static_cast<int>(task / a.parts), part = static_cast<int>(task % a.parts);
   if (t >= a.total) return;
+  const int row = lane / kLanes, c = (lane % kLanes) * 8;  // this lane: dimensions c.. and D / 2 + c..
+  const int nq = a.q ? a.hq : 0, heads = nq + 2 * a.hkv;
+  // input row of head h: query heads, then key heads, then value heads
+  auto source = [&](int h) -> const T* {
+    const size_t row_t = static_cast<size_t>(t);
+    if (h < nq) return static_cast<const T*>(a.q) + row_t * a.q_rs + h * D;
+    h -= nq;
+    if (h < a.hkv) return static_cast<const T*>(a.k) + row_t * a.k_rs + h * D;
+    return static_cast<const T*>(a.v) + row_t * a.v_rs + (h - a.hkv) * D;
+  };
+  const int stride = kSlots * a.parts;
+  int h0 = part * kSlots;
+  // the first row is on its way while the token's place is looked up
+  uint4 w1 = make_uint4(0, 0, 0, 0), w2 = w1;
+  if (h0 + row < heads) {
+    const T* s = source(h0 + row);
+    w1 = *reinterpret_cast<const uint4*>(s + c);
+    w2 = *reinterpret_cast<const uint4*>(s + D / 2 + c);
+  }
   const int b = serving::find_sequence(a.cu_q, a.batch, t, lane);
   if (b < 0) return;  // a row behind the last sequence
   const int first = __ldg(a.cu_q + b), n_new = __ldg(a.cu_q + b + 1) - first;
@@ -119,7 +161,6 @@ __global__ void __launch_bounds__(append_detail::kWarps * 32) kv_append_kernel(c
   const bool kept = page >= 0 && page < a.n_pages;
   if (!kept && lane == 0) record_error(a.err, serving::kErrBadPage);
 
-  const int row = lane / kLanes, c = (lane % kLanes) * 8;  // this lane: dimensions c.. and D / 2 + c..
   float cs_c[8], cs_s[8];
   if (a.cs) {
     int p = a.pos ? __ldg(a.pos + t) : n;
@@ -133,23 +174,6 @@ __global__ void __launch_bounds__(append_detail::kWarps * 32) kv_append_kernel(c
       cs_c[2 * i + 1] = f.z;
       cs_s[2 * i + 1] = f.w;
     }
-  }
-  const int nq = a.q ? a.hq : 0, heads = nq + 2 * a.hkv;
-  // input row of head h: query heads, then key heads, then value heads
-  auto source = [&](int h) -> const T* {
-    const size_t row_t = static_cast<size_t>(t);
-    if (h < nq) return static_cast<const T*>(a.q) + row_t * a.q_rs + h * D;
-    h -= nq;
-    if (h < a.hkv) return static_cast<const T*>(a.k) + row_t * a.k_rs + h * D;
-    return static_cast<const T*>(a.v) + row_t * a.v_rs + (h - a.hkv) * D;
-  };
-  const int stride = kSlots * a.parts;
-  int h0 = part * kSlots;
-  uint4 w1 = make_uint4(0, 0, 0, 0), w2 = w1;
-  if (h0 + row < heads) {
-    const T* s = source(h0 + row);
-    w1 = *reinterpret_cast<const uint4*>(s + c);
-    w2 = *reinterpret_cast<const uint4*>(s + D / 2 + c);
   }
   for (; h0 < heads; h0 += stride) {
     const int h = h0 + row;

@@ -179,19 +179,14 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
   const long long page_bytes = BITS == 16 ? 4ll * a.page * D : static_cast<long long>(a.page) * (D + D / 4);
 
   const int slabs_per_page = a.page / 16;
-  // where a lane finds its words of a slab (4 bits; the swizzles of `issue`)
-  int k_at[kGroups], k_at2[kGroups], v_at[kGroups], v_at2[kGroups];
-  if constexpr (BITS == 4) {
-    auto swz = [](int r) { return D == 64 ? (r >> 2) & 1 : (r >> 1) & 3; };
+  // 4 bits: the row (one group's codes of an entry) whose address this lane gives to an ldmatrix of a slab's groups 2 u and
+  // 2 u + 1: lanes 0-7 entries 0-7 of the first, 8-15 entries 8-15, 16-31 the same of the second (swizzle of `issue`)
+  int code_at[kGroups / 2];
 #pragma unroll
-    for (int gr = 0; gr < kGroups; ++gr) {
-      k_at[gr] = g8 * Tl::kRow + ((gr ^ swz(g8)) * 16) + t4 * 4;
-      k_at2[gr] = (g8 + 8) * Tl::kRow + ((gr ^ swz(g8 + 8)) * 16) + t4 * 4;
-      v_at[gr] = 2 * t4 * Tl::kRow + ((gr ^ swz(2 * t4)) * 16) + (g8 >> 1) * 4;
-      v_at2[gr] = (2 * t4 + 8) * Tl::kRow + ((gr ^ swz(2 * t4 + 8)) * 16) + (g8 >> 1) * 4;
-    }
+  for (int u = 0; u < kGroups / 2; ++u) {
+    const int r = lane & 15, gr = 2 * u + (lane >> 4);
+    code_at[u] = r * Tl::kRow + ((gr ^ (D == 64 ? (r >> 2) & 1 : (r >> 1) & 3)) * 16);
   }
-  const uint32_t v_sel = (g8 & 1) ? 0x7632u : 0x5410u;
   // 4 bits: this lane's chunk of a slab's (step, low) pairs, first the keys', then the values'
   const int pair_is_v = lane / (D / 8), pair_c = lane % (D / 8);
   const int pair_dst = (pair_is_v ? Tl::kVP : Tl::kKP) + pair_c * 16;
@@ -248,8 +243,8 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     unsigned bad, bad_next;
     long long pages = load_pages(0, bad), pages_next = load_pages(kBatch, bad_next);
     // copies tile i of the warp into its ring stage
-    auto issue = [&](int i, long long offs) {
-      uint8_t* st = ring + (i % kStages) * Tl::kBytes;
+    auto issue = [&](int i, int stage, long long offs) {
+      uint8_t* st = ring + stage * Tl::kBytes;
 #pragma unroll
       for (int s = 0; s < kSlabs; ++s) {
         const long long off = __shfl_sync(0xffffffffu, offs, kSlabs * (i % kBatch) + s);
@@ -290,7 +285,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     };
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
-      if (i < mine) issue(i, pages);
+      if (i < mine) issue(i, i, pages);
       serving::copy_commit();
     }
 
@@ -383,14 +378,17 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       for (int u = 0; u < 2; ++u) m[nt][u] = -INFINITY, ref[nt][u] = 0.f, l[nt][u] = 0.f;
     }
 
+    int stage = 0, refill = kStages - 1;  // i % kStages, (i + kStages - 1) % kStages
     for (int i = 0; i < mine; ++i) {
       // refill the stage that tile i - 1 used (every lane has passed the __syncwarp that ends tile i - 1)
       const int ahead = i + kStages - 1;
-      if (ahead < mine) issue(ahead, ahead / kBatch == i / kBatch ? pages : pages_next);
+      if (ahead < mine) issue(ahead, refill, ahead / kBatch == i / kBatch ? pages : pages_next);
       serving::copy_commit();
       serving::copy_wait<kStages - 1>();
       __syncwarp();
-      const uint8_t* st = ring + (i % kStages) * Tl::kBytes;
+      const uint8_t* st = ring + stage * Tl::kBytes;
+      refill = stage;
+      stage = stage + 1 == kStages ? 0 : stage + 1;
       const int key0 = (tile0 + warp + i * kWarps) * kKeys;
       const unsigned gone = (bad >> (kSlabs * (i % kBatch))) & ((1u << kSlabs) - 1u);  // slabs without a page
       if (i % kBatch == kBatch - 1) {
@@ -423,11 +421,17 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             for (int x = 0; x < 4; ++x) s[nt][sl][x] = acc[nt][x] * qf[nt][x & 1];
         } else {
           float acc[NT][kGroups][4];
-          const uint8_t* kt = st + Tl::kK + sl * 16 * Tl::kRow;
+          // word t4 of each group's codes, entries g8 and g8 + 8: an ldmatrix of 32-bit words
+          uint32_t kw[kGroups][2];
+#pragma unroll
+          for (int gr = 0; gr < kGroups; gr += 2) {
+            uint32_t w[4];
+            serving::ldsm_x4(w, st + Tl::kK + sl * 16 * Tl::kRow + code_at[gr / 2]);
+            kw[gr][0] = w[0], kw[gr][1] = w[1], kw[gr + 1][0] = w[2], kw[gr + 1][1] = w[3];
+          }
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr) {
-            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(kt + k_at[gr]);
-            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(kt + k_at2[gr]);
+            const uint32_t w0 = kw[gr][0], w1 = kw[gr][1];
             const uint32_t x0 = w0 >> 8, x1 = w1 >> 8;
             const uint32_t a0[4] = {w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u};
             const uint32_t a1[4] = {x0 & 0x000F000Fu, x1 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x00F000F0u};
@@ -634,15 +638,18 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
                 pb[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(p0 * step, p1 * step));
               }
           }
-          const uint8_t* vt = st + Tl::kV + sl * 16 * Tl::kRow;
+          // the half word g8 of each group's codes (dimensions 4 g8 .. + 3), of entries 2 t4 and 2 t4 + 1 (and + 8) in one
+          // register: a transposed ldmatrix of half words
+          uint32_t vw[kGroups][2];
+#pragma unroll
+          for (int gr = 0; gr < kGroups; gr += 2) {
+            uint32_t w[4];
+            serving::ldsm_x4_trans(w, st + Tl::kV + sl * 16 * Tl::kRow + code_at[gr / 2]);
+            vw[gr][0] = w[0], vw[gr][1] = w[1], vw[gr + 1][0] = w[2], vw[gr + 1][1] = w[3];
+          }
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr) {
-            // this lane's entries 2 t4, 2 t4 + 1 (and + 8): the half word g8 of the group's codes, dimensions 4 g8 .. + 3
-            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vt + v_at[gr]);
-            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(vt + v_at[gr] + Tl::kRow);
-            const uint32_t w2 = *reinterpret_cast<const uint32_t*>(vt + v_at2[gr]);
-            const uint32_t w3 = *reinterpret_cast<const uint32_t*>(vt + v_at2[gr] + Tl::kRow);
-            const uint32_t x0 = __byte_perm(w0, w1, v_sel), x1 = __byte_perm(w2, w3, v_sel);
+            const uint32_t x0 = vw[gr][0], x1 = vw[gr][1];
             const uint32_t y0 = x0 >> 8, y1 = x1 >> 8;
             // rows g8 of the first product: dimension 4 g8, rows g8 + 8: 4 g8 + 1 (16 times); second: 4 g8 + 2, + 3
             const uint32_t a0[4] = {x0 & 0x000F000Fu, x0 & 0x00F000F0u, x1 & 0x000F000Fu, x1 & 0x00F000F0u};
