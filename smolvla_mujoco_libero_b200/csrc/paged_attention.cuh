@@ -80,6 +80,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
+// a / b of two numbers that are not negative; 64 bits only where it has to be (a long division is a long piece of code)
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  if (((a | b) >> 31) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
 // an entry's (step, low) pairs
 __device__ __forceinline__ void load_pairs(uint32_t (&p)[2], const uint8_t* src) {
   const uint2 u = *reinterpret_cast<const uint2*>(src);
@@ -118,8 +124,8 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
   constexpr int kRows = 8 * NT, kGroups = D / 32, kStages = Tl::kStages, kKeys = Tl::kKeys, kSlabs = Tl::kSlabs;
   constexpr int kBatch = 32 / kSlabs;  // tiles whose pages a warp holds
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int place[2];         // first sequence of this CTA's piece, and ...
-  __shared__ long long place64[3]; // its start on the line; the piece
+  __shared__ int place[1];         // first sequence of this CTA's piece, and ...
+  __shared__ long long place64[4]; // its start on the line; the piece; what every piece has
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
   uint8_t* ring = smem + warp * Sm::kPerWarp;
   pdl_wait();
@@ -133,19 +139,24 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     const serving::Span s = serving::span_of(a.cu_q, b, a.total);
     return static_cast<long long>(tiles_of(entries(b))) * query_tiles<NT>(s.end - s.begin, a.g) * a.hkv;
   };
-  // ---- this CTA's piece of the line and the sequence where it starts
+  // ---- this CTA's piece of the line and the sequence where it starts; the weights of the first 128 sequences are held
   if (warp == 0) {
-    long long sum = 0;
-    for (int b = lane; b < a.batch; b += 32) sum += weight(b);
+    constexpr int kHeld = 4;
+    long long held[kHeld], sum = 0;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      held[u] = 32 * u + lane < a.batch ? weight(32 * u + lane) : 0;
+      sum += held[u];
+    }
+    for (int i = 32 * kHeld + lane; i < a.batch; i += 32) sum += weight(i);
 #pragma unroll
     for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    long long share = (sum + gridDim.x - 1) / gridDim.x;
-    if (share < a.min_share) share = a.min_share;
+    const long long share = max(divide(sum + gridDim.x - 1, gridDim.x), static_cast<long long>(a.min_share));
     const long long from = share * blockIdx.x, to = min(from + share, sum);
     int b0 = a.batch;
     long long at = 0, base = 0;
-    for (int c = 0; c < a.batch && from < to; c += 32) {
-      const long long w = c + lane < a.batch ? weight(c + lane) : 0;
+    // sequences 32 i .. + 31, of weight w in this lane: does the piece start there?
+    auto look = [&](int first, long long w) {
       long long upto = w;  // inclusive prefix
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -155,17 +166,24 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       const unsigned past = __ballot_sync(0xffffffffu, base + upto > from);
       if (past) {
         const int l = __ffs(past) - 1;
-        b0 = c + l;
+        b0 = first + l;
         at = base + __shfl_sync(0xffffffffu, upto - w, l);
-        break;
+      } else {
+        base += __shfl_sync(0xffffffffu, upto, 31);
       }
-      base += __shfl_sync(0xffffffffu, upto, 31);
+    };
+    if (from < to) {
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u)
+        if (b0 == a.batch && 32 * u < a.batch) look(32 * u, held[u]);
+      for (int c = 32 * kHeld; c < a.batch && b0 == a.batch; c += 32) look(c, c + lane < a.batch ? weight(c + lane) : 0);
     }
     if (lane == 0) {
       place[0] = b0;
       place64[0] = at;
       place64[1] = from;
       place64[2] = to;
+      place64[3] = share;
       if (a.split) a.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
     }
   }
@@ -173,9 +191,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
   int b = place[0];
   long long at = place64[0];  // start of sequence b on the line
   long long cur = place64[1];
-  const long long from = cur, to = place64[2];
-  const long long share = to - from;
-  const long long full_share = from > 0 ? from / blockIdx.x : share;
+  const long long from = cur, to = place64[2], full_share = place64[3];
   const long long page_bytes = BITS == 16 ? 4ll * a.page * D : static_cast<long long>(a.page) * (D + D / 4);
 
   const int slabs_per_page = a.page / 16;
@@ -204,7 +220,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       continue;
     }
     if (threadIdx.x == 0 && __ldg(a.kv_len + b) > reach) record_error(a.err, serving::kErrBadPage);
-    const int item = static_cast<int>((cur - at) / n_tiles);
+    const int item = static_cast<int>(divide(cur - at, n_tiles));
     const long long item_at = at + static_cast<long long>(item) * n_tiles;
     const int kh = item % a.hkv, qt = item / a.hkv;
     const long long seg_end = min(item_at + n_tiles, to);
@@ -241,7 +257,9 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       return off;
     };
     unsigned bad, bad_next;
-    long long pages = load_pages(0, bad), pages_next = load_pages(kBatch, bad_next);
+    long long pages = load_pages(0, bad), pages_next = -1;
+    bad_next = 0u;
+    if (mine > kBatch) pages_next = load_pages(kBatch, bad_next);
     // copies tile i of the warp into its ring stage
     auto issue = [&](int i, int stage, long long offs) {
       uint8_t* st = ring + stage * Tl::kBytes;
@@ -335,7 +353,8 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
         int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
         ex = (top > 0.f && ex < 128) ? max(ex, -100) : 14;
         const float up = __uint_as_float(static_cast<uint32_t>(14 - ex + 127) << 23);
-        const float f = ldexpf(a.scale_log2, 24 + ex - 14);  // undoes 2^-24 of the codes and `up`
+        // undoes 2^-24 of the codes and `up`
+        const float f = a.scale_log2 * 1024.f * __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
 #pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) {
           // step 0 of the group: (n0, n4 | n1, n5), step 1: (n2, n6 | n3, n7); odd nibbles count 16 times
@@ -394,7 +413,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       if (i % kBatch == kBatch - 1) {
         pages = pages_next;
         bad = bad_next;
-        pages_next = load_pages(i + 1 + kBatch, bad_next);
+        if (i + 1 + kBatch < mine) pages_next = load_pages(i + 1 + kBatch, bad_next);
       }
       // some entry of the tile is hidden from some row (warp-uniform)
       const bool edge = key0 + kKeys > sees_first || gone != 0u;
@@ -511,7 +530,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
           e_new = fmaxf(e, static_cast<float>(static_cast<int>(__float_as_uint(big) >> 23) - 127));
-          big_limit = exp2f(e_new + 1.f);
+          big_limit = ex2_approx(e_new + 1.f);
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -736,7 +755,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     }
     if (!whole && starts_here && threadIdx.x == 0) {
       // the item's last piece: the CTA whose piece holds the item's last tile
-      const long long last = (item_at + n_tiles - 1) / full_share;
+      const long long last = divide(item_at + n_tiles - 1, full_share);
       a.meta[blockIdx.x] = make_int4(b, kh, qt, static_cast<int>(last));
       a.meta[gridDim.x + blockIdx.x].x = slot_id;
     }
