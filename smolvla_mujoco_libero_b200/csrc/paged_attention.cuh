@@ -764,16 +764,20 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
   }
 }
 
-// Joins the partials of the items that the pieces' borders cut; CTA c takes the one that starts in piece c.  The parts'
-// maxima and sums are read by a warp per row, all at once, and turned into factors in shared memory; then a thread per
-// two dimensions of a row adds the parts up in the line's order.
-constexpr int kPagedJoinThreads = 256;
-constexpr int kPagedJoinChunk = 128;  // parts whose factors are held at a time
+// Joins the partials of the items that the pieces' borders cut; CTA c takes the one that starts in piece c.  A warp takes
+// a row and 8 parts at a time, all of whose loads are under way together (a lane D / 32 dimensions, every 8 lanes the
+// parts' maxima and sums); what warps the rows leave over take further parts of the same rows, joined through shared
+// memory.  Always in the line's order.  Short on purpose: it runs once per call, from a cold instruction cache.
+constexpr int kPagedJoinWarps = 16;
+constexpr int kPagedJoinParts = 8;
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kPagedJoinThreads) paged_combine_kernel(const PagedAttnArgs a) {
-  constexpr int kRows = 8 * NT, kSlot = kRows * (D + 2), kPer = kRows * (D / 2) / kPagedJoinThreads;
-  __shared__ float factor[kPagedJoinChunk][kRows], tops[kRows], sums[kRows];
+__global__ void __launch_bounds__(kPagedJoinWarps * 32) paged_combine_kernel(const PagedAttnArgs a) {
+  constexpr int kRows = 8 * NT, kSlot = kRows * (D + 2), kPer = D / 32, kParts = kPagedJoinParts;
+  static_assert(kRows <= kPagedJoinWarps, "a warp per row");
+  struct __align__(4 * kPer) Vec { float x[kPer]; };
+  __shared__ Vec held[kPagedJoinWarps][32];
+  __shared__ float2 held_ml[kPagedJoinWarps];
   pdl_wait();
   pdl_trigger();
   const int4 meta = a.meta[blockIdx.x];
@@ -782,63 +786,72 @@ __global__ void __launch_bounds__(kPagedJoinThreads) paged_combine_kernel(const 
   const int b = meta.x, kh = meta.y, row0 = meta.z * kRows, parts = meta.w - static_cast<int>(blockIdx.x) + 1;
   const serving::Span sq = serving::span_of(a.cu_q, b, a.total);
   const int n_new = sq.end - sq.begin, rows = min(kRows, n_new * a.g - row0);
-  const long long reach = static_cast<long long>(a.max_pages) * a.page;
-  const int len = static_cast<int>(min(static_cast<long long>(max(__ldg(a.kv_len + b), 0)), reach));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto part = [&](int c) { return a.part + static_cast<size_t>(c == 0 ? first_slot : 2 * (static_cast<int>(blockIdx.x) + c)) * kSlot; };
-  for (int r = warp; r < rows; r += kPagedJoinThreads / 32) {
-    float top = -INFINITY;
-    for (int c = lane; c < parts; c += 32) top = fmaxf(top, part(c)[kRows * D + 2 * r]);
+  const int subs = kPagedJoinWarps / rows, used = min(subs, (parts + kParts - 1) / kParts);
+  const int r = warp % rows, sub = warp / rows;
+
+  Vec o;
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float sum = 0.f;
-    for (int c = lane; c < parts; c += 32) {
-      const float2 ml = *reinterpret_cast<const float2*>(part(c) + kRows * D + 2 * r);
-      // a part without anything to see has sum 0; one whose scores are all NaN keeps its NaN
-      sum = fmaf(ml.x == -INFINITY ? 1.f : ex2_approx(ml.x - top), ml.y, sum);
-    }
+  for (int i = 0; i < kPer; ++i) o.x[i] = 0.f;
+  float top = -INFINITY, sum = 0.f;
+  // factors of what is there and of a part with maximum m; nothing to see: sum 0, or NaN where all scores are NaN (kept)
+  auto factor = [](float m, float t) { return m == -INFINITY ? 1.f : ex2_approx(m - t); };
+  if (sub < used) {
+    for (int c0 = sub * kParts; c0 < parts; c0 += used * kParts) {
+      auto part = [&](int c) { return a.part + static_cast<size_t>(c == 0 ? first_slot : 2 * (static_cast<int>(blockIdx.x) + c)) * kSlot; };
+      const int c = c0 + lane % kParts;
+      const float2 ml = c < parts ? *reinterpret_cast<const float2*>(part(c) + kRows * D + 2 * r) : make_float2(-INFINITY, 0.f);
+      Vec x[kParts];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    if (lane == 0) {
-      tops[r] = top;
-      sums[r] = sum;
+      for (int i = 0; i < kParts; ++i) {
+        if (c0 + i < parts) {
+          x[i] = *reinterpret_cast<const Vec*>(part(c0 + i) + r * D + kPer * lane);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kPer; ++j) x[i].x[j] = 0.f;
+        }
+      }
+      float t = fmaxf(top, ml.x);
+#pragma unroll
+      for (int d = 1; d < kParts; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
+      const float old = factor(top, t), f = factor(ml.x, t);
+      float l = f * ml.y;
+#pragma unroll
+      for (int d = 1; d < kParts; d <<= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+      sum = fmaf(sum, old, l);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) o.x[j] *= old;
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        const float fi = __shfl_sync(0xffffffffu, f, i);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) o.x[j] = fmaf(fi, x[i].x[j], o.x[j]);
+      }
+      top = t;
     }
+    held[warp][lane] = o;
+    if (lane == 0) held_ml[warp] = make_float2(top, sum);
   }
   __syncthreads();
-  float2 o[kPer];
+  if (sub > 0) return;
+  for (int i = 1; i < used; ++i) {
+    const float2 ml = held_ml[warp + i * rows];
+    const Vec x = held[warp + i * rows][lane];
+    const float t = fmaxf(top, ml.x), old = factor(top, t), f = factor(ml.x, t);
+    sum = fmaf(sum, old, f * ml.y);
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) o[i] = make_float2(0.f, 0.f);
-  for (int c0 = 0; c0 < parts; c0 += kPagedJoinChunk) {
-    const int n = min(kPagedJoinChunk, parts - c0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < n * rows; i += kPagedJoinThreads) {
-      const int c = i / rows, r = i % rows;
-      const float m = part(c0 + c)[kRows * D + 2 * r];
-      factor[c][r] = m == -INFINITY ? 1.f : ex2_approx(m - tops[r]);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int idx = threadIdx.x + i * kPagedJoinThreads, r = idx / (D / 2), d = (idx % (D / 2)) * 2;
-      if (r >= rows) continue;
-#pragma unroll 8
-      for (int c = 0; c < n; ++c) {
-        const float2 x = *reinterpret_cast<const float2*>(part(c0 + c) + r * D + d);
-        o[i].x = fmaf(factor[c][r], x.x, o[i].x);
-        o[i].y = fmaf(factor[c][r], x.y, o[i].y);
-      }
-    }
+    for (int j = 0; j < kPer; ++j) o.x[j] = fmaf(f, x.x[j], o.x[j] * old);
+    top = t;
   }
+  const long long reach = static_cast<long long>(a.max_pages) * a.page;
+  const int len = static_cast<int>(min(static_cast<long long>(max(__ldg(a.kv_len + b), 0)), reach));
+  const int row = row0 + r;
+  const bool sees_some = len - n_new + row / a.g + 1 > 0 && len > 0;
+  const float inv = sees_some ? __frcp_rn(sum) : 0.f;
+  T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + kPer * lane;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int idx = threadIdx.x + i * kPagedJoinThreads, r = idx / (D / 2), d = (idx % (D / 2)) * 2;
-    if (r >= rows) continue;
-    const int row = row0 + r;
-    const bool sees_some = len - n_new + row / a.g + 1 > 0 && len > 0;
-    const float inv = sees_some ? __frcp_rn(sums[r]) : 0.f;
-    T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + d;
-    *reinterpret_cast<uint32_t*>(dst) = sees_some ? serving::pack2<T>(o[i].x * inv, o[i].y * inv) : 0u;
-  }
+  for (int j = 0; j < kPer; j += 2)
+    *reinterpret_cast<uint32_t*>(dst + j) = sees_some ? serving::pack2<T>(o.x[j] * inv, o.x[j + 1] * inv) : 0u;
 }
 
 }  // namespace svla

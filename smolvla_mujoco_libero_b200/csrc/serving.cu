@@ -166,7 +166,7 @@ int32_t launch_paged_inst(PagedAttnArgs a, cudaStream_t st) {
   if (a.split) a.meta = reinterpret_cast<int4*>(reinterpret_cast<uint8_t*>(a.part) + paged_part_bytes(grid, NT, D));
   int32_t rc = launch(kern, dim3(grid), dim3(paged_detail::kWarps * 32), Sm::kBytes, st, "paged_attention_kernel", a);
   if (rc || !a.split) return rc;
-  return launch(paged_combine_kernel<T, D, NT>, dim3(grid), dim3(kPagedJoinThreads), 0, st, "paged_combine_kernel", a);
+  return launch(paged_combine_kernel<T, D, NT>, dim3(grid), dim3(kPagedJoinWarps * 32), 0, st, "paged_combine_kernel", a);
 }
 
 template <typename T, int D>
