@@ -63,7 +63,8 @@ def attention_tolerance(o, spread, size, dtype, dim, weight_unit=None, floor=0.0
     rounded once (weight_unit spread).  The relative error of an fp32 weight is the error of its score: dim products and
     sums, each off by at most 2^-23 (tensor cores may truncate) of the magnitudes, dim + 8 of them with the scale factors,
     in the weight and again in the sum that divides; plus 2^-22 for each of two exponentials and divisions.  floor:
-    what weights below the second product's normal range lose.  The second order is covered by 2%.
+    what weights below the second product's normal range lose.  The second order is covered by 2%, and so is an exponential
+    by polynomial (2.6e-6 relative, in the weight and in the sum 5.2e-6; 2% of the smallest weight_unit, 2^-11, is 9.7e-6).
     """
     unit = torch.finfo(dtype).eps / 2
     weight_unit = unit if weight_unit is None else weight_unit

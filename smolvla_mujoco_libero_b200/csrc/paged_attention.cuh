@@ -9,7 +9,7 @@
 // rows) += V^T P^T.  A query row is a (token, head) of one kv head, packed token-major, so grouped heads and several
 // tokens share every entry that is read; 8 rows fit one MMA column block, and single tokens of up to 8 grouped heads
 // waste half of what 16 query rows would (that form, without the transposition of P, takes twice the products and
-// registers and measured 60 us where this one takes 50).
+// registers; of two early versions with one choice each it took 60 us, this one 50).
 //
 // 4-bit entries are never expanded to 16-bit values.  A nibble c masked out of a word, as it stands, is the fp16
 // subnormal c 2^-24 (or 16 c 2^-24 for the second nibble of a byte): tensor cores take subnormals exactly, so one AND
@@ -23,17 +23,23 @@
 // seen so far, 2^e <= step < 2^(e + 1), besides that of the running maximum (both cancel in O / l).  Products with low_n
 // stay in fp32.
 //
-// Every warp works alone: its own tiles of 32 entries through its own ring of asynchronous copies, its own running
+// Every warp works alone: its own tiles of 16 to 64 entries through its own ring of asynchronous copies, its own running
 // maximum, sum and O, no barrier in the loop.  The maximum is lazy: it moves (and O is rescaled) only when a score
 // passes it by more than 8 in log2 units (or a step 2^(e + 1)), one vote per tile instead of shuffles.  Instruction issue
 // is what stands beside the memory system: the two query columns of a thread go through packed fp32 operations, a page's
 // address is worked out once by one lane for 16 tiles, and the masks are in a branch that only a sequence's end takes.
 //
 // Work split.  All tiles of all (sequence, kv head, query tile) items form one line, each item 512 entries longer than it
-// is (what its start and its join cost: without that, pieces of many short items came last, 58 us where 44 do); every CTA
-// takes an equal piece of it, whatever the sequences' lengths are, and finds its place from cu_q and kv_len on the device.  An item that lies in
-// one CTA is finished there; one cut by a piece's border leaves partials (maximum, sum, O in fp32) in the workspace,
-// which the combine kernel joins in the line's order, so results do not depend on timing.
+// is (what its start and its join cost: without that, pieces of many short items come last); every CTA takes an equal
+// piece of it, whatever the sequences' lengths are, and finds its place from cu_q and kv_len on the device.  An item that
+// lies in one CTA is finished there; one cut by a piece's border leaves partials (maximum, sum, O in fp32) in the
+// workspace, which the combine kernel joins in the line's order, so results do not depend on timing.
+//
+// Measured, both kernels, 4 bits: 64 single tokens at D = 64 over 255 to 8191 entries (118 MB) 41 us, 2.9 TB/s (2 or 4
+// CTAs per SM instead of 3: 46 and 44; no cost per item: 55; 384 or 1024 entries per item: 44 and 43); two of D = 128
+// over 100000 to 131071 (291 MB) 68 us, 4.3 TB/s.  16 bits, 24 x 5 tokens over 100 to 4000 (65 MB): 23 us, 2.9 TB/s.
+// Of the 41 us about 12 go to the start of a piece and of its items (place, pages, first copies, queries, each from cold
+// code), 3 to the join, the rest to the tiles: 300 cycles per 16 entries and scheduler, of which the products take 75.
 #pragma once
 
 #include "serving_common.cuh"
@@ -112,7 +118,7 @@ struct PagedSmem {
   static constexpr int kBytes = paged_detail::kWarps * kPerWarp;
 };
 
-// single tokens at D = 64: three CTAs per SM (four, at 128 registers, measured 51 us where three take 48)
+// single tokens at D = 64: three CTAs per SM
 template <typename T, int D, int BITS, int NT>
 __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1) ? 3 : 1)
     paged_attention_kernel(const PagedAttnArgs a) {

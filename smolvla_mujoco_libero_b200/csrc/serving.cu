@@ -111,6 +111,7 @@ int32_t run_packed_tc(const svla_packed_attn_desc* d, float scale_log2, cudaStre
   a.scale_log2 = scale_log2;
   a.err = device_error_ptr();
   const long long items = (static_cast<long long>(d->total_q) / (2 * a.qt) + d->batch) * d->hkv;
+  if (items > 0x7fffffffll) return fail(SVLA_ERR_ARG, "svla_packed_attention: too many query tiles");
   const bool h = d->dtype == SVLA_DT_HALF;
   if (d->head_dim == 64) return h ? launch_packed_tc<__half, 64>(a, items, st) : launch_packed_tc<__nv_bfloat16, 64>(a, items, st);
   return h ? launch_packed_tc<__half, 128>(a, items, st) : launch_packed_tc<__nv_bfloat16, 128>(a, items, st);

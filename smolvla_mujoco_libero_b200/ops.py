@@ -605,3 +605,37 @@ def _rope_attention_op(q_raw: torch.Tensor, k_raw: torch.Tensor, v_raw: torch.Te
 def _(q_raw, k_raw, v_raw, pos, mask, q_heads, kv_heads, max_wavelength):
     b, l, w = q_raw.shape
     return q_raw.new_empty(b, q_heads, l, w // q_heads, dtype=torch.float32)
+
+
+@torch.library.custom_op("svla::packed_attention", mutates_args=())
+def _packed_attention_op(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
+                         cu_k: torch.Tensor | None, causal: bool, scale: float) -> torch.Tensor:
+    return packed_attention(q, k, v, cu_q, cu_k, causal, scale)
+
+
+@_packed_attention_op.register_fake
+def _(q, k, v, cu_q, cu_k, causal, scale):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("svla::kv_append", mutates_args=("cache",))
+def _kv_append_op(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+                  page_table: torch.Tensor, q: torch.Tensor, rope_cs: torch.Tensor | None,
+                  pos: torch.Tensor | None) -> torch.Tensor:
+    return kv_append(cache, k, v, cu_q, kv_len, page_table, q, rope_cs, pos)
+
+
+@_kv_append_op.register_fake
+def _(cache, k, v, cu_q, kv_len, page_table, q, rope_cs, pos):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("svla::paged_attention", mutates_args=())
+def _paged_attention_op(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
+                        page_table: torch.Tensor, scale: float) -> torch.Tensor:
+    return paged_attention(q, cache, cu_q, kv_len, page_table, scale)
+
+
+@_paged_attention_op.register_fake
+def _(q, cache, cu_q, kv_len, page_table, scale):
+    return q.new_empty(q.shape)

@@ -451,6 +451,13 @@ def test_paged_attention_split_over_the_gpu(heads, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("heads,new", [((3, 1, 64), 1), ((8, 1, 128), 1), ((5, 1, 128), 3), ((4, 1, 64), 2)], ids=str)
+def test_paged_attention_joins_many_parts(heads, new, bits):
+    """One kv head: all pieces belong to one item, whose parts' maxima lie far apart."""
+    paged_check([new], [13000], heads, bits, 64, BF16, seed=30, q_scale=4.0)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("heads", [(3, 1, 64), (16, 1, 64), (9, 1, 128), (71, 1, 64), (40, 2, 128)], ids=str)
 def test_paged_attention_head_groups_and_drafts(heads, bits):
     paged_check([1, 1], [100, 33], heads, bits, 16, BF16, seed=24)
@@ -624,6 +631,28 @@ def test_no_rows_give_nothing():
     assert ops.packed_attention(q, kv, kv, cu).shape == (0, 6, 64)
     assert ops.paged_attention(q, cache, cu, n, table).shape == (0, 6, 64)
     assert ops.kv_append(cache, kv, kv, cu, n, table, q=q).shape == (0, 6, 64)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_custom_ops_are_the_functions(bits):
+    """torch.ops.svla.*: schema, aliasing and shapes as registered, results as the functions give them."""
+    hq, hkv, d, lens = 6, 2, 64, [20, 600, 1]
+    table, n_pages = make_table(lens, 16, seed=31)
+    x = torch.randn(sum(lens), hq + 2 * hkv, d, generator=gen(32)).to(BF16).to(DEV)
+    q, k, v = (t.contiguous() for t in x.split([hq, hkv, hkv], 1))
+    cu, n, table, cs = ints(starts(lens)).to(DEV), ints(lens).to(DEV), table.to(DEV), ops.rope_table_wide(600, 10000.0, DEV, d)
+    cache, other = ops.kv_cache(n_pages, 16, hkv, d, bits), ops.kv_cache(n_pages, 16, hkv, d, bits)
+    rotated = ops.kv_append(cache, k, v, cu, n, table, q=q, rope_cs=cs)
+    assert torch.equal(torch.ops.svla.kv_append(other, k, v, cu, n, table, q, cs, None), rotated)
+    assert torch.equal(other.view(torch.uint8), cache.view(torch.uint8))
+    last, one = rotated[torch.tensor(lens).cumsum(0) - 1], ints([0, 1, 2, 3]).to(DEV)
+    assert torch.equal(torch.ops.svla.packed_attention(q, k, v, cu, None, True, 0.0), ops.packed_attention(q, k, v, cu))
+    assert torch.equal(torch.ops.svla.paged_attention(last, cache, one, n, table, 0.0),
+                       ops.paged_attention(last, cache, one, n, table))
+    for op, args in [(torch.ops.svla.packed_attention, (q, k, v, cu, None, True, 0.0)),
+                     (torch.ops.svla.kv_append, (other, k, v, cu, n, table, q, cs, None)),
+                     (torch.ops.svla.paged_attention, (last, cache, one, n, table, 0.0))]:
+        torch.library.opcheck(op, args, test_utils=("test_schema", "test_faketensor"))
 
 
 # ----------------------------------------------------------------------------- together
