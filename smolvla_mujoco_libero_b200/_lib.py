@@ -11,6 +11,7 @@ from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_size_t, c_voi
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libsvla.so"
+TORCH_PATH = LIB_PATH.with_name("_torch_serving.so")
 
 KIND_I8, KIND_BF16, KIND_W8A16 = 0, 1, 2
 EPI_BF16, EPI_I32, EPI_ROPE, EPI_RESID, EPI_SILU_MUL, EPI_GELU_QUANT, EPI_EULER, EPI_SILU, EPI_F32 = range(9)
@@ -210,6 +211,7 @@ class SvlaError(RuntimeError):
 
 
 _lib = None
+_serving = None
 
 
 def lib() -> ctypes.CDLL:
@@ -225,6 +227,20 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+def serving():
+    """The torch side of the serving operators (csrc/torch_serving.cpp), bound to the loaded library once."""
+    global _serving
+    if _serving is None:
+        handle = lib()
+        if not TORCH_PATH.exists():
+            raise SvlaError(f"{TORCH_PATH} is missing: build it with `python -m smolvla_mujoco_libero_b200.build`")
+        from . import _torch_serving as module
+        module.bind(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in (
+            "svla_kv_append", "svla_packed_attention", "svla_paged_attention", "svla_paged_attention_workspace_size")))
+        _serving = module
+    return _serving
 
 
 def check(rc: int, what: str = "") -> None:

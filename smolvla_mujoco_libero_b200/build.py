@@ -1,8 +1,9 @@
-"""Build libsvla.so in-tree with nvcc for sm_100a.
+"""Build libsvla.so in-tree with nvcc for sm_100a, and _torch_serving.so, the torch side of the serving operators, with
+the host compiler.
 
     python -m smolvla_mujoco_libero_b200.build [--debug]
 
-The library lands next to this file so that it travels with the source tree.
+Both land next to this file so that they travel with the source tree.
 """
 
 from __future__ import annotations
@@ -12,11 +13,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OUT = PKG / "libsvla.so"
+TORCH_SRC = CSRC / "torch_serving.cpp"
+TORCH_OUT = PKG / "_torch_serving.so"
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -44,7 +48,7 @@ def units() -> list[tuple[Path, list[Path]]]:
 
 
 def sources() -> list[Path]:
-    return sorted({p for _, deps in units() for p in deps})
+    return sorted({p for _, deps in units() for p in deps} | {TORCH_SRC})
 
 
 def _stale(target: Path, deps: list[Path]) -> bool:
@@ -55,7 +59,27 @@ def _stale(target: Path, deps: list[Path]) -> bool:
 
 
 def up_to_date() -> bool:
-    return not _stale(OUT, sources())
+    return not _stale(OUT, [p for p in sources() if p != TORCH_SRC]) and not _stale(TORCH_OUT, [TORCH_SRC, HEADER])
+
+
+def build_torch(force: bool = False) -> Path:
+    """_torch_serving.so: a Python module against this torch's headers (no device code)."""
+    if not force and not _stale(TORCH_OUT, [TORCH_SRC, HEADER]):
+        return TORCH_OUT
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+               sysconfig.get_paths()["include"]]
+    # g++, as nvcc takes it, with the process's own libstdc++ (a compiler named by $CXX may link another one statically,
+    # whose stream facets do not mix with it)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+                    f"-DTORCH_EXTENSION_NAME={TORCH_OUT.stem}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                    *[a for p in include for a in ("-isystem", str(p))], "-o", str(TORCH_OUT), str(TORCH_SRC),
+                    f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"], check=True)
+    return TORCH_OUT
 
 
 def build(force: bool = False, debug: bool = False, verbose: bool = False) -> Path:
@@ -74,6 +98,7 @@ def build(force: bool = False, debug: bool = False, verbose: bool = False) -> Pa
             subprocess.run(cmd, check=True)
         objs.append(str(obj))
     subprocess.run([nvcc(), *ARCH, "-shared", "-o", str(OUT), *objs], check=True)
+    build_torch(force)
     return OUT
 
 

@@ -354,45 +354,6 @@ def rope_table(max_pos: int, max_wavelength: float, device) -> torch.Tensor:
 
 # ----------------------------------------------------------------------------- serving: packed prompts, paged cache
 
-_DT16 = {torch.bfloat16: L.DT_BF16, torch.float16: L.DT_HALF}
-
-
-def _packed_first(t: torch.Tensor, name: str) -> tuple[torch.dtype, int, int]:
-    """(dtype, device index, head_dim) of the tensor that the call's other tensors have to fit."""
-    dev = t.get_device()
-    if dev < 0:
-        raise ValueError(f"{name} must be a CUDA tensor (there is no CPU path)")
-    if t.dim() != 3 or t.dtype not in _DT16:
-        raise ValueError(f"{name} must be bf16 or fp16 [rows, heads, head_dim], got {t.dtype} {tuple(t.shape)}")
-    if dev != torch.cuda.current_device():
-        raise ValueError(f"{name} is on cuda:{dev}, the current device is cuda:{torch.cuda.current_device()}")
-    return t.dtype, dev, t.shape[2]
-
-
-def _packed(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int, d: int) -> tuple[int, int, int]:
-    """(rows, heads, row stride) of t [rows, heads, d], whose heads lie next to each other (any row stride; a single
-    row's does not matter to torch, so it is not taken from it)."""
-    if t.dtype is not dtype or t.get_device() != dev or t.dim() != 3:
-        raise ValueError(f"{name} must be {dtype} [rows, heads, {d}] on cuda:{dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    rows, h, dd = t.shape
-    rs, hs, es = t.stride()
-    if dd != d or (rows and (es != 1 or (hs != d and h > 1))):
-        raise ValueError(f"{name} must be [rows, heads, {d}] with the heads of a row next to each other, got "
-                         f"{tuple(t.shape)} with strides {t.stride()}")
-    return rows, h, (rs if rows > 1 else h * d)
-
-
-def _ints(t: torch.Tensor, name: str, n: int, dev: int) -> None:
-    if t.dtype is not torch.int32 or t.get_device() != dev or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32 [{n}] on cuda:{dev}, got {t.dtype} {list(t.shape)} on {t.device}")
-
-
-def _batch_of(cu: torch.Tensor, name: str, dev: int) -> int:
-    n = cu.numel()
-    _ints(cu, name, n if n else 1, dev)
-    return n - 1
-
-
 def kv_cache(n_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 16,
              dtype: torch.dtype = torch.bfloat16, device="cuda") -> torch.Tensor:
     """An empty paged cache of one layer: ``[n_pages, kv_heads, 2, page_size, head_dim]`` of the dtype, or with
@@ -402,32 +363,9 @@ def kv_cache(n_pages: int, page_size: int, kv_heads: int, head_dim: int, bits: i
                          f"(got {bits}, {page_size}, {head_dim})")
     if bits == 4:
         return torch.zeros(n_pages, kv_heads, page_size, head_dim + head_dim // 4, dtype=torch.uint8, device=device)
-    if dtype not in _DT16:
+    if dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"kv_cache: dtype must be bf16 or fp16, got {dtype}")
     return torch.zeros(n_pages, kv_heads, 2, page_size, head_dim, dtype=dtype, device=device)
-
-
-def _cache(cache: torch.Tensor, page_table: torch.Tensor, kv_len: torch.Tensor, batch: int, dtype: torch.dtype,
-           dev: int, d: int) -> tuple[int, int, int, int, int, int]:
-    """(bits, page_size, n_pages, kv heads, max_pages, page_table's row stride)."""
-    shape = cache.shape
-    if len(shape) == 5 and cache.dtype is dtype and shape[2] == 2 and shape[4] == d:
-        bits, page = 16, shape[3]
-    elif len(shape) == 4 and cache.dtype is torch.uint8 and shape[3] == d + d // 4:
-        bits, page = 4, shape[2]
-    else:
-        raise ValueError(f"cache {cache.dtype} {list(shape)} does not hold entries of {dtype} [{d}] (see kv_cache)")
-    if cache.get_device() != dev or not cache.is_contiguous():
-        raise ValueError(f"cache must be contiguous on cuda:{dev}")
-    _ints(kv_len, "kv_len", batch, dev)
-    table = page_table.shape
-    if page_table.dtype is not torch.int32 or page_table.get_device() != dev or len(table) != 2 or table[0] != batch:
-        raise ValueError(f"page_table must be int32 [{batch}, max_pages] on cuda:{dev}, got {page_table.dtype} "
-                         f"{list(table)} on {page_table.device}")
-    rs, cs = page_table.stride()
-    if cs != 1 and table[1] > 1:
-        raise ValueError(f"page_table must have unit column stride, got strides {page_table.stride()}")
-    return bits, page, shape[0], shape[1], table[1], (rs if batch > 1 else table[1])
 
 
 def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
@@ -439,59 +377,7 @@ def kv_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch
     queries ``q`` are rotated at ``pos`` [rows], or at the entry's index.  Returns the rotated queries (None without q), or
     with ``want_rows`` (q, k, v): the appended rows as the cache holds them, which prompt attention takes.  The outputs may
     be the inputs (in place)."""
-    dtype, dev, d = _packed_first(k, "k")
-    rows, hkv, k_rs = _packed(k, "k", dtype, dev, d)
-    v_rows, v_heads, v_rs = _packed(v, "v", dtype, dev, d)
-    if v_rows != rows or v_heads != hkv:
-        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    batch = _batch_of(cu_q, "cu_q", dev)
-    bits, page, n_pages, cache_heads, max_pages, table_rs = _cache(cache, page_table, kv_len, batch, dtype, dev, d)
-    if cache_heads != hkv:
-        raise ValueError(f"the cache holds {cache_heads} kv heads, k has {hkv}")
-    hq = q_rs = qo_rs = ko_rs = vo_rs = max_pos = 0
-    q_ptr = qo_ptr = ko_ptr = vo_ptr = cs_ptr = pos_ptr = None
-    if q is not None:
-        q_rows, hq, q_rs = _packed(q, "q", dtype, dev, d)
-        if q_rows != rows:
-            raise ValueError(f"q has {q_rows} rows, k {rows}")
-        if q_out is None:
-            q_out, qo_rs = q.new_empty(rows, hq, d), hq * d
-        else:
-            qo_rows, qo_heads, qo_rs = _packed(q_out, "q_out", dtype, dev, d)
-            if qo_rows != rows or qo_heads != hq:
-                raise ValueError("q_out must have q's shape")
-        q_ptr, qo_ptr = q.data_ptr(), q_out.data_ptr()
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    if want_rows:
-        k_out = k.new_empty(rows, hkv, d) if k_out is None else k_out
-        v_out = k.new_empty(rows, hkv, d) if v_out is None else v_out
-    if k_out is not None:
-        o_rows, o_heads, ko_rs = _packed(k_out, "k_out", dtype, dev, d)
-        if o_rows != rows or o_heads != hkv:
-            raise ValueError("k_out must have k's shape")
-        ko_ptr = k_out.data_ptr()
-    if v_out is not None:
-        o_rows, o_heads, vo_rs = _packed(v_out, "v_out", dtype, dev, d)
-        if o_rows != rows or o_heads != hkv:
-            raise ValueError("v_out must have v's shape")
-        vo_ptr = v_out.data_ptr()
-    if rope_cs is not None:
-        shape = rope_cs.shape
-        if (rope_cs.dtype is not torch.float32 or rope_cs.get_device() != dev or len(shape) != 3
-                or shape[1] != d // 2 or shape[2] != 2 or not rope_cs.is_contiguous()):
-            raise ValueError(f"rope_cs must be contiguous fp32 [max_pos, {d // 2}, 2] on cuda:{dev}")
-        max_pos, cs_ptr = shape[0], rope_cs.data_ptr()
-    if pos is not None:
-        _ints(pos, "pos", rows, dev)
-        pos_ptr = pos.data_ptr()
-    if rows:
-        desc = L.KvAppendDesc(q_ptr, k.data_ptr(), v.data_ptr(), qo_ptr, ko_ptr, vo_ptr, cache.data_ptr(),
-                              cu_q.data_ptr(), kv_len.data_ptr(), page_table.data_ptr(), pos_ptr, cs_ptr, q_rs, k_rs,
-                              v_rs, qo_rs, ko_rs, vo_rs, table_rs, batch, rows, hq, hkv, d, _DT16[dtype], bits, page,
-                              n_pages, max_pages, max_pos)
-        check(lib().svla_kv_append(ctypes.byref(desc), _raw_stream(dev)), "svla_kv_append")
-    return (q_out, k_out, v_out) if want_rows else q_out
+    return L.serving().kv_append(cache, k, v, cu_q, kv_len, page_table, q, rope_cs, pos, q_out, want_rows, k_out, v_out)
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor,
@@ -502,28 +388,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     cu_q[b + 1] - 1 of q and cu_k[b] .. of k and v (cu_k None: the same).  Causal: the queries are the last tokens of
     their sequence.  Returns [rows, heads, head_dim]; rows behind the last sequence are left as they are in ``out``
     (undefined without it)."""
-    dtype, dev, d = _packed_first(q, "q")
-    rows, hq, q_rs = _packed(q, "q", dtype, dev, d)
-    k_rows, hkv, k_rs = _packed(k, "k", dtype, dev, d)
-    v_rows, v_heads, v_rs = _packed(v, "v", dtype, dev, d)
-    if v_rows != k_rows or v_heads != hkv:
-        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    batch = _batch_of(cu_q, "cu_q", dev)
-    if cu_k is None:
-        cu_k = cu_q
-    else:
-        _ints(cu_k, "cu_k", batch + 1, dev)
-    if out is None:
-        out, o_rs = q.new_empty(rows, hq, d), hq * d
-    else:
-        o_rows, o_heads, o_rs = _packed(out, "out", dtype, dev, d)
-        if o_rows != rows or o_heads != hq:
-            raise ValueError("out must have q's shape")
-    desc = L.PackedAttnDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(),
-                            q_rs, k_rs, v_rs, o_rs, batch, rows, k_rows, hq, hkv, d, _DT16[dtype], 1 if causal else 0,
-                            scale, impl)
-    check(lib().svla_packed_attention(ctypes.byref(desc), _raw_stream(dev)), "svla_packed_attention")
-    return out
+    return L.serving().packed_attention(q, k, v, cu_q, cu_k, causal, scale, out, impl)
 
 
 def paged_attention(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor, kv_len: torch.Tensor,
@@ -533,29 +398,7 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor, kv
     appended) over a paged cache of 16 or 4 bits; kv_len [B] entries, pages in page_table [B, max_pages].  Returns
     [rows, heads, head_dim].  ``workspace``: uint8 of svla_paged_attention_workspace_size bytes, taken from torch's
     allocator when None."""
-    dtype, dev, d = _packed_first(q, "q")
-    rows, hq, q_rs = _packed(q, "q", dtype, dev, d)
-    batch = _batch_of(cu_q, "cu_q", dev)
-    bits, page, n_pages, hkv, max_pages, table_rs = _cache(cache, page_table, kv_len, batch, dtype, dev, d)
-    if out is None:
-        out, o_rs = q.new_empty(rows, hq, d), hq * d
-    else:
-        o_rows, o_heads, o_rs = _packed(out, "out", dtype, dev, d)
-        if o_rows != rows or o_heads != hq:
-            raise ValueError("out must have q's shape")
-    handle = lib()
-    if workspace is None:
-        need = handle.svla_paged_attention_workspace_size(batch, rows, hq, hkv, d, max_pages * page)
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
-        raise ValueError(f"workspace must be contiguous uint8 on cuda:{dev}")
-    ws_ptr, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
-    desc = L.PagedAttnDesc(q.data_ptr(), cache.data_ptr(), out.data_ptr(), cu_q.data_ptr(), kv_len.data_ptr(),
-                           page_table.data_ptr(), ws_ptr, ws_bytes, q_rs, o_rs, table_rs, batch, rows, hq, hkv, d,
-                           _DT16[dtype], bits, page, n_pages, max_pages, scale)
-    check(handle.svla_paged_attention(ctypes.byref(desc), _raw_stream(dev)), "svla_paged_attention")
-    return out
+    return L.serving().paged_attention(q, cache, cu_q, kv_len, page_table, scale, out, workspace)
 
 
 # ----------------------------------------------------------------------------- torch custom ops
