@@ -53,7 +53,7 @@ struct PagedAttnArgs {
   const int *cu_q, *kv_len, *table;
   float* part;             // workspace: 2 slots per CTA
   int4* meta;              // workspace, per CTA: {b, kv head, query tile, CTA of its last tile} of a cut item that starts
-                           // there, or {-1, ..}; then per CTA that item's first slot
+                           // there, or {-1, ..}; then per CTA that item's {first slot, first row, new tokens, entries}
   long long q_rs, o_rs, table_rs;
   int batch, total, hq, hkv, g, page, n_pages, max_pages;
   unsigned long long page_magic;  // ceil(2^32 / (page / 16)): 16-entry slab -> page
@@ -231,6 +231,12 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     const int kh = item % a.hkv, qt = item / a.hkv;
     const long long seg_end = min(item_at + n_tiles, to);
     const bool whole = cur == item_at && seg_end == item_at + n_tiles;
+    if (!whole && cur == item_at && threadIdx.x == 0) {
+      // the item's last piece: the CTA whose piece holds the item's last tile
+      const long long last = divide(item_at + n_tiles - 1, full_share);
+      a.meta[blockIdx.x] = make_int4(b, kh, qt, static_cast<int>(last));
+      a.meta[gridDim.x + blockIdx.x] = make_int4(2 * blockIdx.x + (cur > from ? 1 : 0), sq.begin, n_new, len);
+    }
     // tiles of the sequence in this segment (an uncut item: all of them)
     const int real_tiles = (len + kKeys - 1) / kKeys;
     const int tile0 = a.split ? max(static_cast<int>(cur - item_at) - a.item_cost, 0) : 0;
@@ -727,7 +733,6 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
         }
       }
     __syncthreads();
-    const bool starts_here = cur == item_at;
     const int slot_id = 2 * blockIdx.x + (cur > from ? 1 : 0);
     for (int idx = threadIdx.x; idx < kRows * (D / 2); idx += kWarps * 32) {
       const int r = idx / (D / 2), d = (idx % (D / 2)) * 2;
@@ -759,12 +764,6 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
         if (d == 0) *reinterpret_cast<float2*>(p + kRows * D + 2 * r) = make_float2(top, sum);
       }
     }
-    if (!whole && starts_here && threadIdx.x == 0) {
-      // the item's last piece: the CTA whose piece holds the item's last tile
-      const long long last = divide(item_at + n_tiles - 1, full_share);
-      a.meta[blockIdx.x] = make_int4(b, kh, qt, static_cast<int>(last));
-      a.meta[gridDim.x + blockIdx.x].x = slot_id;
-    }
     cur = seg_end;
     __syncthreads();  // the join buffers are the next item's ring
   }
@@ -786,12 +785,11 @@ __global__ void __launch_bounds__(kPagedJoinWarps * 32) paged_combine_kernel(con
   __shared__ float2 held_ml[kPagedJoinWarps];
   pdl_wait();
   pdl_trigger();
-  const int4 meta = a.meta[blockIdx.x];
-  const int first_slot = a.meta[gridDim.x + blockIdx.x].x;
+  const int4 meta = a.meta[blockIdx.x], more = a.meta[gridDim.x + blockIdx.x];
   if (meta.x < 0) return;
-  const int b = meta.x, kh = meta.y, row0 = meta.z * kRows, parts = meta.w - static_cast<int>(blockIdx.x) + 1;
-  const serving::Span sq = serving::span_of(a.cu_q, b, a.total);
-  const int n_new = sq.end - sq.begin, rows = min(kRows, n_new * a.g - row0);
+  const int kh = meta.y, row0 = meta.z * kRows, parts = meta.w - static_cast<int>(blockIdx.x) + 1;
+  const int first_slot = more.x, begin = more.y, n_new = more.z, len = more.w;
+  const int rows = min(kRows, n_new * a.g - row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int subs = kPagedJoinWarps / rows, used = min(subs, (parts + kParts - 1) / kParts);
   const int r = warp % rows, sub = warp / rows;
@@ -849,12 +847,10 @@ __global__ void __launch_bounds__(kPagedJoinWarps * 32) paged_combine_kernel(con
     for (int j = 0; j < kPer; ++j) o.x[j] = fmaf(f, x.x[j], o.x[j] * old);
     top = t;
   }
-  const long long reach = static_cast<long long>(a.max_pages) * a.page;
-  const int len = static_cast<int>(min(static_cast<long long>(max(__ldg(a.kv_len + b), 0)), reach));
   const int row = row0 + r;
   const bool sees_some = len - n_new + row / a.g + 1 > 0 && len > 0;
   const float inv = sees_some ? __frcp_rn(sum) : 0.f;
-  T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + kPer * lane;
+  T* dst = static_cast<T*>(a.o) + static_cast<size_t>(begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + kPer * lane;
 #pragma unroll
   for (int j = 0; j < kPer; j += 2)
     *reinterpret_cast<uint32_t*>(dst + j) = sees_some ? serving::pack2<T>(o.x[j] * inv, o.x[j + 1] * inv) : 0u;
