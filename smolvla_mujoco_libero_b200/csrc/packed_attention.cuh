@@ -32,63 +32,65 @@ constexpr int kRows = 16 * kWarps;  // query rows per CTA
 constexpr int kKeys = 64;
 
 // The tiles of `qt` tokens of all sequences, numbered longest first: by their place inside their sequence, from the
-// largest down (a causal tile's keys grow with it), then by sequence.  A warp walks through the numbers upwards; the tile
-// counts of the first 128 sequences stay in registers, those of more are read again (from L1) at every step.
-struct TileWalk {
+// largest down (a causal tile's keys grow with it), then by sequence.  A warp finds a tile's place by bisection over the
+// tiles that lie at a place or behind it, sum_b max(count_b - place, 0); the tile counts of the first 128 sequences stay
+// in registers, those of more are read again (from L1) at every step.
+struct TileOrder {
   static constexpr int kHeld = 4;
   const int* cu_q;
   int batch, total, qt;
   int held[kHeld];
-  int place;         // tiles with a larger place come before; -1: there are no more
-  long long before;  // number of the first tile with this place
+  int top;  // largest count
 
   __device__ __forceinline__ int count(int i) const {
     const serving::Span s = serving::span_of(cu_q, i, total);
     return (s.end - s.begin + qt - 1) / qt;
   }
-  __device__ __forceinline__ TileWalk(const int* cu_q_, int batch_, int total_, int qt_, int lane)
-      : cu_q(cu_q_), batch(batch_), total(total_), qt(qt_), before(0) {
-    int top = 0;
+  __device__ __forceinline__ TileOrder(const int* cu_q_, int batch_, int total_, int qt_, int lane)
+      : cu_q(cu_q_), batch(batch_), total(total_), qt(qt_) {
+    int most = 0;
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) {
       held[u] = lane + 32 * u < batch ? count(lane + 32 * u) : 0;
-      top = max(top, held[u]);
+      most = max(most, held[u]);
     }
-    for (int i = lane + 32 * kHeld; i < batch; i += 32) top = max(top, count(i));
-    place = __reduce_max_sync(0xffffffffu, top) - 1;
+    for (int i = lane + 32 * kHeld; i < batch; i += 32) most = max(most, count(i));
+    top = __reduce_max_sync(0xffffffffu, most);
   }
-  // sequence and place of tile number id (not below that of the last call); false: there is no such tile
-  __device__ __forceinline__ bool find(long long id, int lane, int& b, int& j) {
-    while (place >= 0) {
-      int rest = static_cast<int>(min(id - before, 0x7fffffffll));
-      int n = 0;
-      b = -1;
+  // tiles at `place` or behind it
+  __device__ __forceinline__ int from(int place, int lane) const {
+    int n = 0;
 #pragma unroll
-      for (int u = 0; u < kHeld; ++u) {
-        const unsigned m = __ballot_sync(0xffffffffu, held[u] > place);
-        pick(m, 32 * u, rest - n, lane, b);
-        n += __popc(m);
+    for (int u = 0; u < kHeld; ++u) n += max(held[u] - place, 0);
+    for (int i = lane + 32 * kHeld; i < batch; i += 32) n += max(count(i) - place, 0);
+    return __reduce_add_sync(0xffffffffu, n);
+  }
+  // sequence and place of tile number id; false: there is no such tile
+  __device__ __forceinline__ bool find(int id, int lane, int& b, int& place) const {
+    int behind = top, rank = id;  // from(behind) <= id < from(place), or place = 0 and there may be no such tile
+    place = 0;
+    while (behind - place > 1) {
+      const int mid = (place + behind) >> 1, n = from(mid, lane);
+      if (n > id) {
+        place = mid;
+      } else {
+        behind = mid;
+        rank = id - n;
       }
-      for (int c = 32 * kHeld; c < batch; c += 32) {
-        const unsigned m = __ballot_sync(0xffffffffu, c + lane < batch && count(min(c + lane, batch - 1)) > place);
-        pick(m, c, rest - n, lane, b);
-        n += __popc(m);
-      }
-      if (rest < n) {
-        j = place;
-        return true;
-      }
-      // every place down to the next smaller count has as many tiles: pass over those that lie before id
-      int next = 0;
-#pragma unroll
-      for (int u = 0; u < kHeld; ++u) next = max(next, held[u] <= place ? held[u] : 0);
-      for (int c = lane + 32 * kHeld; c < batch; c += 32) next = max(next, count(c) <= place ? count(c) : 0);
-      next = __reduce_max_sync(0xffffffffu, next);
-      const int pass = min(rest / n, place - next + 1);
-      before += static_cast<long long>(pass) * n;
-      place -= pass;
     }
-    return false;
+    b = -1;
+#pragma unroll
+    for (int u = 0; u < kHeld; ++u) {
+      const unsigned m = __ballot_sync(0xffffffffu, held[u] > place);
+      pick(m, 32 * u, rank, lane, b);
+      rank -= __popc(m);
+    }
+    for (int c = 32 * kHeld; c < batch && rank >= 0; c += 32) {
+      const unsigned m = __ballot_sync(0xffffffffu, c + lane < batch && count(min(c + lane, batch - 1)) > place);
+      pick(m, c, rank, lane, b);
+      rank -= __popc(m);
+    }
+    return b >= 0;
   }
   // b = first + the position of set bit number `rank` of m, if there is one
   __device__ __forceinline__ static void pick(unsigned m, int first, int rank, int lane, int& b) {
@@ -119,8 +121,8 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
   const int kh = blockIdx.x % a.hkv;
   if (warp == 0) {
     int b = -1, j = 0;
-    TileWalk walk(a.cu_q, a.batch, a.total_q, a.qt, lane);
-    const bool ok = walk.find(blockIdx.x / a.hkv, lane, b, j);
+    const TileOrder order(a.cu_q, a.batch, a.total_q, a.qt, lane);
+    const bool ok = order.find(static_cast<int>(blockIdx.x) / a.hkv, lane, b, j);
     if (lane == 0) {
       place[0] = ok ? b : -1;
       place[1] = j;

@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
   pdl_wait();  // lengths, q, k, v are written by the previous kernel
   if (warp == 0) {
     int b = -1, j = 0;
-    packed_detail::TileWalk walk(a.cu_q, a.batch, a.total_q, 2 * a.qt, lane);
-    const bool ok = walk.find(blockIdx.x / a.hkv, lane, b, j);
+    const packed_detail::TileOrder order(a.cu_q, a.batch, a.total_q, 2 * a.qt, lane);
+    const bool ok = order.find(static_cast<int>(blockIdx.x) / a.hkv, lane, b, j);
     if (lane == 0) {
       place[0] = ok ? b : -1;
       place[1] = j;
