@@ -22,6 +22,7 @@ struct PackedAttnArgs {
   const int *cu_q, *cu_k;
   long long q_rs, k_rs, v_rs, o_rs;
   int batch, total_q, total_k, hq, hkv, g, qt;  // qt: tokens of a query tile
+  unsigned g_magic;  // ceil(2^16 / g): row -> token, exact for the 64 rows of a tile and g <= 64
   int causal;
   float scale_log2;
 };
@@ -140,12 +141,14 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
   const int sees_last = seen(tok0 + toks - 1), sees_first = seen(tok0);
   const int n_tiles = (sees_last + kKeys - 1) / kKeys;
 
+  auto token = [&](int r) { return static_cast<int>(static_cast<unsigned>(r) * a.g_magic >> 16); };
   {
     const T* qb = static_cast<const T*>(a.q) + static_cast<size_t>(sq.begin + tok0) * a.q_rs + kh * a.g * D;
-    for (int idx = threadIdx.x; idx < kRows * kChunks; idx += kWarps * 32) {
-      const int r = idx / kChunks, c = idx % kChunks;
+#pragma unroll
+    for (int u = 0; u < kRows * kChunks / (kWarps * 32); ++u) {
+      const int idx = threadIdx.x + u * kWarps * 32, r = idx / kChunks, c = idx % kChunks, tk = token(r);
       const bool in = r < rows;
-      const T* src = qb + (in ? static_cast<size_t>(r / a.g) * a.q_rs + (r % a.g) * D + c * 8 : 0);
+      const T* src = qb + (in ? static_cast<size_t>(tk) * a.q_rs + (r - tk * a.g) * D + c * 8 : 0);
       copy16(smem + Sm::kQ + r * kRow + ((c ^ (r & 7)) * 16), src, in ? 16 : 0);
     }
   }
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
   const int wr = warp * 16;
   int sees[2];  // keys that this thread's rows see
 #pragma unroll
-  for (int hr = 0; hr < 2; ++hr) sees[hr] = seen(tok0 + (wr + g8 + 8 * hr) / a.g);
+  for (int hr = 0; hr < 2; ++hr) sees[hr] = seen(tok0 + token(wr + g8 + 8 * hr));
   uint32_t qa[D / 16][4];
   float o[D / 8][4];
 #pragma unroll
@@ -236,10 +239,10 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
     float use[2];
 #pragma unroll
     for (int hr = 0; hr < 2; ++hr) {
-      float top = m[hr];
+      float top = fmaxf(s[0][2 * hr], s[0][2 * hr + 1]);
 #pragma unroll
-      for (int n = 0; n < kKeys / 8; ++n)
-        top = fmaxf(top, fmaxf(s[n][2 * hr] * a.scale_log2, s[n][2 * hr + 1] * a.scale_log2));
+      for (int n = 1; n < kKeys / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * hr], s[n][2 * hr + 1]));
+      top = fmaxf(m[hr], top * a.scale_log2);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const float alpha = m[hr] == -INFINITY ? 1.f : ex2_approx(m[hr] - top);
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
     l[hr] += __shfl_xor_sync(0xffffffffu, l[hr], 2);
     const int r = wr + g8 + 8 * hr;
     if (r >= rows) continue;
-    const int tok = tok0 + r / a.g, h = kh * a.g + r % a.g;
+    const int tk = token(r), tok = tok0 + tk, h = kh * a.g + r - tk * a.g;
     if (odd_flag) {  // rare: the infinities and NaN that left V, for the rows that see them
       for (int j = sees_first / kKeys * kKeys; j < sees[hr]; ++j) {
         const T* vr = static_cast<const T*>(a.v) + static_cast<size_t>(sk.begin + j) * a.v_rs + kh * D;

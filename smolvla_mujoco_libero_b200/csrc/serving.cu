@@ -263,6 +263,7 @@ int32_t svla_packed_attention(const svla_packed_attn_desc* d, svla_stream_t stre
   if (d->impl == SVLA_ATTN_TCGEN05 || (d->impl == SVLA_ATTN_AUTO && d->total_k > 0 && packed_prefers_tc(d, g)))
     return run_packed_tc(d, a.scale_log2, cs(stream));
   a.qt = packed_detail::kRows / g;
+  a.g_magic = (65535u + g) / g;
   // the lengths are on the device: as many items as the sequences can have (each one's last tile may be short)
   const long long items = (static_cast<long long>(d->total_q) / a.qt + d->batch) * d->hkv;
   if (items > 0x7fffffffll) return fail(SVLA_ERR_ARG, "%s: too many query tiles", who);
