@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
   float o[D / 8][4];
 #pragma unroll
   for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, use[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
 
   for (int tile = 0; tile < n_tiles; ++tile) {
     if (tile + 1 < n_tiles) load(tile + 1);
@@ -236,23 +236,33 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
         for (int e = 0; e < 4; ++e)
           if (key0 + n * 8 + 2 * t4 + (e & 1) >= sees[e >> 1]) s[n][e] = -INFINITY;
     }
-    float use[2];
+    // The running maximum is lazy: it moves, and O is rescaled, only when a score of the warp passes its row's by more than
+    // 8 in log2 units (weights up to 2^8 of the maximum's cancel in O / l; fp16 holds them)
+    float top[2];
+    bool pass = false;
 #pragma unroll
     for (int hr = 0; hr < 2; ++hr) {
-      float top = fmaxf(s[0][2 * hr], s[0][2 * hr + 1]);
+      top[hr] = fmaxf(s[0][2 * hr], s[0][2 * hr + 1]);
 #pragma unroll
-      for (int n = 1; n < kKeys / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * hr], s[n][2 * hr + 1]));
-      top = fmaxf(m[hr], top * a.scale_log2);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float alpha = m[hr] == -INFINITY ? 1.f : ex2_approx(m[hr] - top);
-      m[hr] = top;
-      use[hr] = top == -INFINITY ? 0.f : top;
-      l[hr] *= alpha;
+      for (int n = 1; n < kKeys / 8; ++n) top[hr] = fmaxf(top[hr], fmaxf(s[n][2 * hr], s[n][2 * hr + 1]));
+      top[hr] *= a.scale_log2;
+      pass |= top[hr] > m[hr] + 8.f;
+    }
+    if (__any_sync(0xffffffffu, pass)) {
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        o[n][2 * hr] *= alpha;
-        o[n][2 * hr + 1] *= alpha;
+      for (int hr = 0; hr < 2; ++hr) {
+        float t = fmaxf(m[hr], top[hr]);
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+        t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+        const float alpha = m[hr] == -INFINITY ? 1.f : ex2_approx(m[hr] - t);
+        m[hr] = t;
+        use[hr] = t == -INFINITY ? 0.f : t;
+        l[hr] *= alpha;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][2 * hr] *= alpha;
+          o[n][2 * hr + 1] *= alpha;
+        }
       }
     }
     uint32_t pa[kKeys / 16][4];
