@@ -117,21 +117,23 @@ int32_t run_packed_tc(const svla_packed_attn_desc* d, float scale_log2, cudaStre
   return h ? launch_packed_tc<__half, 128>(a, items, st) : launch_packed_tc<__nv_bfloat16, 128>(a, items, st);
 }
 
-// The automatic choice between the two kernels, from what the host knows: the average lengths.  An item of the tcgen05
-// kernel (256 query rows) costs 5 to 6 us beside its key tiles, one of the mma.sync kernel (64 rows, several per SM) 1 or
-// 2; a key costs it less.  One round of items: it wins from 448 keys on (D = 64: 177 keys 8.9 us against 7.8, 512 keys 12.4
-// both, one token after 2000 keys 20.9 against 32.2), at D = 128 from 256 (200 keys and one token 7.9 against 10.5, 177
-// tokens 13.2 against 11.2, 512 tokens 19.0 against 24.4).  Many rounds: it is the keys per item, less what its rows are
-// not filled, that counts (D = 64, 3 heads per group, 64 prompts: 128 tokens 39.1 against 37.3, 256 tokens 78 against 82,
-// 512 tokens 158 against 217, 16 tokens after 500 keys 29.4 against 22.6; D = 128, 4 heads: 48 tokens 40 against 46, one
-// token after 200 keys 32 against 26, after 2000 keys 128 against 153).
+// The automatic choice between the two kernels, from what the host knows: the average lengths, of which a query sees
+// `seen` keys on the average.  An item of the tcgen05 kernel (256 query rows) costs 5 to 6 us beside its key tiles, one of
+// the mma.sync kernel (64 rows, several per SM) 1 or 2; a key costs it less.  One round of items (mma.sync against tcgen05,
+// us): D = 64, one prompt of 177 tokens 6.8 / 8.9, of 768 15.9 / 15.8, of 1024 23.2 / 18.9, one token after 500 keys
+// 9.8 / 8.9; D = 128, 256 tokens 11.9 / 13.7, 384 16.6 / 16.7, 512 21.9 / 19.0.  Many rounds: it is the keys per item that
+// count, less what its rows are not filled.  D = 64, 3 heads per group, 64 prompts of 256 tokens 72 / 80, of 320 98 / 89, of
+// 384 126 / 112, of 64 after 300 41 / 31, of 16 after 500 21 / 30; D = 128, 4 heads, of 48 38 / 40, of 96 80 / 77, of 192
+// 182 / 145, one token after 200 keys 25 / 32, after 2000 144 / 128.  Lengths that differ move the border: 64 prompts with
+// lengths spread evenly over the logarithm from 1 to 512 after 0 to 300 keys take 52 / 46 and stay with mma.sync.
 bool packed_prefers_tc(const svla_packed_attn_desc* d, int g) {
   const long long q = (static_cast<long long>(d->total_q) + d->batch - 1) / d->batch;
-  const long long keys = static_cast<long long>(d->total_k) / d->batch;
-  const long long pair = 2 * (128 / g), items = d->batch * ((q + pair - 1) / pair) * d->hkv;
-  if (items <= sm_count()) return keys >= (d->head_dim == 64 ? 448 : 256);
-  const long long rows = q * g < 256 ? q * g : 256;
-  return keys * rows >= 256 * (d->head_dim == 64 ? 224 : 32);
+  const long long keys = static_cast<long long>(d->total_k) / d->batch, half = (q < keys ? q : keys) / 2;
+  const long long seen = d->causal ? keys - half : keys;
+  const long long pair = 2 * (128 / g), per_head = (q + pair - 1) / pair;
+  const bool narrow = d->head_dim == 64;
+  if (d->batch * per_head * d->hkv <= sm_count()) return seen >= (narrow ? 400 : 192);
+  return seen * (q * g / per_head) >= 256 * (narrow ? 145 : 28);
 }
 
 // ---------------------------------------------------------------- paged
