@@ -5,6 +5,11 @@
 // One pass over the keys with the running maximum and sum of the softmax, fp32 scores and sums, probabilities rounded
 // to the input type for the second product (as the framework's other attention kernels do).
 //
+// This form is for short prompts: 64 rows per CTA on mma.sync, whose start costs less than a tcgen05 tile's; bound by that
+// start (place, first copies, cold code) and by instruction issue.  One prompt of 177 tokens at 15 / 5 heads of 64 takes
+// 6.8 us (7.8 with divisions from rows to tokens and scaled scores in the maximum, 7.1 with an eager running maximum), 64
+// of 128 tokens 32 us, 64 of 256 72 us.
+//
 // A query row is a (token, head) of one kv head, packed token-major (row r = token r / G, head r % G), so the G heads of
 // a group share every key tile and the causal limit is nearly the same for all rows of a tile.  Whatever stands behind a
 // sequence's last key -- the next sequence, padding, NaN -- is never multiplied in: those rows of V are zeros.  An
@@ -55,6 +60,7 @@ struct TileOrder {
       held[u] = lane + 32 * u < batch ? count(lane + 32 * u) : 0;
       most = max(most, held[u]);
     }
+#pragma unroll 1
     for (int i = lane + 32 * kHeld; i < batch; i += 32) most = max(most, count(i));
     top = __reduce_max_sync(0xffffffffu, most);
   }
@@ -63,6 +69,7 @@ struct TileOrder {
     int n = 0;
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) n += max(held[u] - place, 0);
+#pragma unroll 1
     for (int i = lane + 32 * kHeld; i < batch; i += 32) n += max(count(i) - place, 0);
     return __reduce_add_sync(0xffffffffu, n);
   }
@@ -70,6 +77,7 @@ struct TileOrder {
   __device__ __forceinline__ bool find(int id, int lane, int& b, int& place) const {
     int behind = top, rank = id;  // from(behind) <= id < from(place), or place = 0 and there may be no such tile
     place = 0;
+#pragma unroll 1
     while (behind - place > 1) {
       const int mid = (place + behind) >> 1, n = from(mid, lane);
       if (n > id) {
@@ -86,6 +94,7 @@ struct TileOrder {
       pick(m, 32 * u, rank, lane, b);
       rank -= __popc(m);
     }
+#pragma unroll 1
     for (int c = 32 * kHeld; c < batch && rank >= 0; c += 32) {
       const unsigned m = __ballot_sync(0xffffffffu, c + lane < batch && count(min(c + lane, batch - 1)) > place);
       pick(m, c, rank, lane, b);

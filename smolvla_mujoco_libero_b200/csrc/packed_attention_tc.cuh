@@ -17,8 +17,10 @@
 //
 // What the issuers wait for decides: a ready barrier asked by try_wait through one lane costs 200 cycles, by test_wait 41,
 // and one issuer for both tiles needed 3100 cycles for an iteration's waits, MMAs and commits.  One 16384-token prompt at
-// D = 64: 860 us; test_wait first: 734; an issuer per tile: 669; one pair of exponentials in eight as polynomials: 650.
-// Measured and left: two CTAs of one tile each per SM (715 us; 61 us for 64 ragged prompts where this takes 65), the same
+// D = 64: 860 us; test_wait first: 734; an issuer per tile: 669; one pair of exponentials in eight as polynomials: 650
+// (now 655, 787 TFLOP/s).  64 ragged prompts of 1 to 1024 tokens: 65 us with a CTA's tiles found by a walk through the
+// sequences, 58 by bisection.
+// Measured and left: two CTAs of one tile each per SM (715 us; 61 us for 64 ragged prompts where this took 65), the same
 // as persistent CTAs that fetch ahead (785 and 63 us), scores read twice from TMEM instead of held (934 us).
 //
 // Exponentials are the bound at D = 64 (16 per clock and SM: 1024 cycles per 128 x 128 tile against 512 of MMA), both
