@@ -7,8 +7,8 @@
 //
 // This form is for short prompts: 64 rows per CTA on mma.sync, whose start costs less than a tcgen05 tile's; bound by that
 // start (place, first copies, cold code) and by instruction issue.  One prompt of 177 tokens at 15 / 5 heads of 64 takes
-// 6.8 us (7.8 with divisions from rows to tokens and scaled scores in the maximum, 7.1 with an eager running maximum), 64
-// of 128 tokens 32 us, 64 of 256 72 us.
+// 5.9 us: 7.8 with divisions from rows to tokens, scaled scores in the maximum and a walk to the tile's place, 7.1 with an
+// eager running maximum, 6.4 with the numbering of many sequences.  64 prompts of 128 tokens 30 us, of 256 69 us.
 //
 // A query row is a (token, head) of one kv head, packed token-major (row r = token r / G, head r % G), so the G heads of
 // a group share every key tile and the causal limit is nearly the same for all rows of a tile.  Whatever stands behind a
@@ -37,49 +37,46 @@ constexpr int kWarps = 4;
 constexpr int kRows = 16 * kWarps;  // query rows per CTA
 constexpr int kKeys = 64;
 
-// The tiles of `qt` tokens of all sequences, numbered longest first: by their place inside their sequence, from the
-// largest down (a causal tile's keys grow with it), then by sequence.  A warp finds a tile's place by bisection over the
-// tiles that lie at a place or behind it, sum_b max(count_b - place, 0); the tile counts of the first 128 sequences stay
-// in registers, those of more are read again (from L1) at every step.
+// Tile number id of `qt` tokens of all sequences: its sequence and its place there; false: there is no such tile.  A warp
+// calls it; ids go up to total / qt + batch.
+//
+// 2 to 128 sequences: longest first, by place from the largest down (a causal tile's keys grow with it), then by sequence.
+// The place is found by bisection over the tiles that lie at a place or behind it, sum_b max(count_b - place, 0), with the
+// counts in registers: half a microsecond of a CTA, for which a long sequence at the batch's end does not start last.
+//
+// One sequence, or more than registers hold: sequence b has the numbers from cu_q[b] / qt + b on (enough for its tiles, and
+// a few that there are not), its longest tile first, so a search in cu_q finds them.  Measured, by place / by sequence: one
+// prompt of 177 tokens 6.4 / 5.8 us, of 16384 654 / 641; 64 ragged prompts 57.2 / 57.9; 1024 prompts of 64 tokens, counts
+// read again at every step, 527 / 217.
 struct TileOrder {
   static constexpr int kHeld = 4;
   const int* cu_q;
   int batch, total, qt;
-  int held[kHeld];
-  int top;  // largest count
 
   __device__ __forceinline__ int count(int i) const {
     const serving::Span s = serving::span_of(cu_q, i, total);
     return (s.end - s.begin + qt - 1) / qt;
   }
-  __device__ __forceinline__ TileOrder(const int* cu_q_, int batch_, int total_, int qt_, int lane)
-      : cu_q(cu_q_), batch(batch_), total(total_), qt(qt_) {
-    int most = 0;
+  __device__ __forceinline__ bool find(int id, int lane, int& b, int& place) const {
+    return batch > 1 && batch <= 32 * kHeld ? by_place(id, lane, b, place) : by_sequence(id, lane, b, place);
+  }
+  __device__ __forceinline__ bool by_place(int id, int lane, int& b, int& place) const {
+    int held[kHeld], top = 0;
 #pragma unroll
     for (int u = 0; u < kHeld; ++u) {
       held[u] = lane + 32 * u < batch ? count(lane + 32 * u) : 0;
-      most = max(most, held[u]);
+      top = max(top, held[u]);
     }
-#pragma unroll 1
-    for (int i = lane + 32 * kHeld; i < batch; i += 32) most = max(most, count(i));
-    top = __reduce_max_sync(0xffffffffu, most);
-  }
-  // tiles at `place` or behind it
-  __device__ __forceinline__ int from(int place, int lane) const {
-    int n = 0;
-#pragma unroll
-    for (int u = 0; u < kHeld; ++u) n += max(held[u] - place, 0);
-#pragma unroll 1
-    for (int i = lane + 32 * kHeld; i < batch; i += 32) n += max(count(i) - place, 0);
-    return __reduce_add_sync(0xffffffffu, n);
-  }
-  // sequence and place of tile number id; false: there is no such tile
-  __device__ __forceinline__ bool find(int id, int lane, int& b, int& place) const {
-    int behind = top, rank = id;  // from(behind) <= id < from(place), or place = 0 and there may be no such tile
-    place = 0;
+    // from(place): tiles at `place` or behind it
+    int behind = __reduce_max_sync(0xffffffffu, top), rank = id;  // from(behind) <= id < from(place), or place = 0 and
+    place = 0;                                                    // there may be no such tile
 #pragma unroll 1
     while (behind - place > 1) {
-      const int mid = (place + behind) >> 1, n = from(mid, lane);
+      const int mid = (place + behind) >> 1;
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < kHeld; ++u) n += max(held[u] - mid, 0);
+      n = __reduce_add_sync(0xffffffffu, n);
       if (n > id) {
         place = mid;
       } else {
@@ -89,24 +86,31 @@ struct TileOrder {
     }
     b = -1;
 #pragma unroll
-    for (int u = 0; u < kHeld; ++u) {
+    for (int u = 0; u < kHeld; ++u) {  // set bit number `rank` of the sequences that have this place
       const unsigned m = __ballot_sync(0xffffffffu, held[u] > place);
-      pick(m, 32 * u, rank, lane, b);
-      rank -= __popc(m);
-    }
-#pragma unroll 1
-    for (int c = 32 * kHeld; c < batch && rank >= 0; c += 32) {
-      const unsigned m = __ballot_sync(0xffffffffu, c + lane < batch && count(min(c + lane, batch - 1)) > place);
-      pick(m, c, rank, lane, b);
+      if (rank >= 0 && rank < __popc(m)) {
+        const bool me = ((m >> lane) & 1u) && __popc(m & ((1u << lane) - 1u)) == rank;
+        b = 32 * u + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
+      }
       rank -= __popc(m);
     }
     return b >= 0;
   }
-  // b = first + the position of set bit number `rank` of m, if there is one
-  __device__ __forceinline__ static void pick(unsigned m, int first, int rank, int lane, int& b) {
-    if (rank < 0 || rank >= __popc(m)) return;
-    const bool me = ((m >> lane) & 1u) && __popc(m & ((1u << lane) - 1u)) == rank;
-    b = first + __ffs(__ballot_sync(0xffffffffu, me)) - 1;
+  __device__ __forceinline__ bool by_sequence(int id, int lane, int& b, int& place) const {
+    auto start = [&](int i) { return min(max(__ldg(cu_q + i), 0), total) / qt + i; };
+    int lo = 0, hi = batch;  // start(lo) <= id < start(hi)
+#pragma unroll 1
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32;
+      const int at = lo + (lane + 1) * step;
+      const bool below = at < hi && start(at) <= id;
+      lo += __popc(__ballot_sync(0xffffffffu, below)) * step;
+      hi = min(lo + step, hi);
+    }
+    b = lo;
+    const int n = count(lo), j = id - start(lo);
+    place = n - 1 - j;
+    return j >= 0 && j < n;
   }
 };
 }  // namespace packed_detail
@@ -131,7 +135,7 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
   const int kh = blockIdx.x % a.hkv;
   if (warp == 0) {
     int b = -1, j = 0;
-    const TileOrder order(a.cu_q, a.batch, a.total_q, a.qt, lane);
+    const TileOrder order{a.cu_q, a.batch, a.total_q, a.qt};
     const bool ok = order.find(static_cast<int>(blockIdx.x) / a.hkv, lane, b, j);
     if (lane == 0) {
       place[0] = ok ? b : -1;

@@ -18,8 +18,8 @@
 // What the issuers wait for decides: a ready barrier asked by try_wait through one lane costs 200 cycles, by test_wait 41,
 // and one issuer for both tiles needed 3100 cycles for an iteration's waits, MMAs and commits.  One 16384-token prompt at
 // D = 64: 860 us; test_wait first: 734; an issuer per tile: 669; one pair of exponentials in eight as polynomials: 650
-// (now 655, 787 TFLOP/s).  64 ragged prompts of 1 to 1024 tokens: 65 us with a CTA's tiles found by a walk through the
-// sequences, 58 by bisection.
+// (now 645, 799 TFLOP/s).  64 ragged prompts of 1 to 1024 tokens: 65 us with a CTA's tiles found by a walk through the
+// sequences, 57 by bisection.
 // Measured and left: two CTAs of one tile each per SM (715 us; 61 us for 64 ragged prompts where this took 65), the same
 // as persistent CTAs that fetch ahead (785 and 63 us), scores read twice from TMEM instead of held (934 us).
 //
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
   pdl_wait();  // lengths, q, k, v are written by the previous kernel
   if (warp == 0) {
     int b = -1, j = 0;
-    const packed_detail::TileOrder order(a.cu_q, a.batch, a.total_q, 2 * a.qt, lane);
+    const packed_detail::TileOrder order{a.cu_q, a.batch, a.total_q, 2 * a.qt};
     const bool ok = order.find(static_cast<int>(blockIdx.x) / a.hkv, lane, b, j);
     if (lane == 0) {
       place[0] = ok ? b : -1;

@@ -120,12 +120,12 @@ int32_t run_packed_tc(const svla_packed_attn_desc* d, float scale_log2, cudaStre
 // The automatic choice between the two kernels, from what the host knows: the average lengths, of which a query sees
 // `seen` keys on the average.  An item of the tcgen05 kernel (256 query rows) costs 5 to 6 us beside its key tiles, one of
 // the mma.sync kernel (64 rows, several per SM) 1 or 2; a key costs it less.  One round of items (mma.sync against tcgen05,
-// us): D = 64, one prompt of 177 tokens 6.8 / 8.9, of 768 15.9 / 15.8, of 1024 23.2 / 18.9, one token after 500 keys
-// 9.8 / 8.9; D = 128, 256 tokens 11.9 / 13.7, 384 16.6 / 16.7, 512 21.9 / 19.0.  Many rounds: it is the keys per item that
-// count, less what its rows are not filled.  D = 64, 3 heads per group, 64 prompts of 256 tokens 72 / 80, of 320 98 / 89, of
-// 384 126 / 112, of 64 after 300 41 / 31, of 16 after 500 21 / 30; D = 128, 4 heads, of 48 38 / 40, of 96 80 / 77, of 192
-// 182 / 145, one token after 200 keys 25 / 32, after 2000 144 / 128.  Lengths that differ move the border: 64 prompts with
-// lengths spread evenly over the logarithm from 1 to 512 after 0 to 300 keys take 52 / 46 and stay with mma.sync.
+// us): D = 64, one prompt of 177 tokens 5.9 / 8.4, of 768 14.5 / 14.8, of 1024 21.2 / 18.0, one token after 500 keys
+// 8.9 / 8.2; D = 128, 256 tokens 11.1 / 13.2, 384 16.1 / 16.1, 512 21.5 / 18.5.  Many rounds: it is the keys per item that
+// count, less what its rows are not filled.  D = 64, 3 heads per group, 64 prompts of 256 tokens 69 / 77, of 320 94 / 87, of
+// 384 121 / 109, of 64 after 300 39 / 30, of 16 after 500 20 / 30; D = 128, 4 heads, of 48 37 / 40, of 96 79 / 77, of 192
+// 180 / 143, one token after 200 keys 25 / 32, after 2000 144 / 128.  Lengths that differ move the border: 64 prompts with
+// lengths spread evenly over the logarithm from 1 to 512 after 0 to 300 keys take 50 / 45 and stay with mma.sync.
 bool packed_prefers_tc(const svla_packed_attn_desc* d, int g) {
   const long long q = (static_cast<long long>(d->total_q) + d->batch - 1) / d->batch;
   const long long keys = static_cast<long long>(d->total_k) / d->batch, half = (q < keys ? q : keys) / 2;

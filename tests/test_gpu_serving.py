@@ -114,6 +114,13 @@ def test_packed_attention_long_and_many(heads):
     packed_check(lens, lens, *heads, FP16, seed=5)
 
 
+@pytest.mark.parametrize("n", [127, 128, 129, 1000])
+def test_packed_attention_finds_every_tile_of_many_sequences(n):
+    """Lengths of nothing, of less than a tile, of whole tiles (21 and 42 tokens at 3 heads) and of several."""
+    lens = [(0, 1, 21, 42, 43, 7, 130)[(i * i + i // 9) % 7] for i in range(n)]
+    packed_check(lens, lens, 3, 1, 64, BF16, seed=33)
+
+
 @pytest.mark.parametrize("impl", KERNELS)
 def test_packed_attention_with_sharp_and_growing_scores(impl):
     """Scores over a range of hundreds, and keys that grow along the sequence, so that the running maximum moves all the
