@@ -18,7 +18,7 @@
 // What the issuers wait for decides: a ready barrier asked by try_wait through one lane costs 200 cycles, by test_wait 41,
 // and one issuer for both tiles needed 3100 cycles for an iteration's waits, MMAs and commits.  One 16384-token prompt at
 // D = 64: 860 us; test_wait first: 734; an issuer per tile: 669; one pair of exponentials in eight as polynomials: 650
-// (now 645, 799 TFLOP/s).  64 ragged prompts of 1 to 1024 tokens: 65 us with a CTA's tiles found by a walk through the
+// (now 638, 807 TFLOP/s).  64 ragged prompts of 1 to 1024 tokens: 65 us with a CTA's tiles found by a walk through the
 // sequences, 57 by bisection.
 // Measured and left: two CTAs of one tile each per SM (715 us; 61 us for 64 ragged prompts where this took 65), the same
 // as persistent CTAs that fetch ahead (785 and 63 us), scores read twice from TMEM instead of held (934 us).
@@ -96,11 +96,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // 2^z for two z <= 8 or so on the fp32 pipe: z = n + f with n = rint(z) (adding 1.5 * 2^23 leaves n in the low bits), 2^f
-// by its minimax polynomial of degree 4 on [-1/2, 1/2] (relative error 2.6e-6, found by exchanging extrema), n added to the
-// exponent.  z is first raised to at least -126: 2^-126 instead of less.
+// by its minimax polynomial of degree 4 on [-1/2, 1/2] (relative error 2.6e-6, found by exchanging extrema), times 2^n.  z is
+// first raised to at least -126: 2^-126 instead of less.  A NaN stays one: the maximum keeps it, and so does the product
+// (n added to the exponent's bits would not).
 __device__ __forceinline__ float2 exp2_poly(float2 z) {
-  z.x = fmaxf(z.x, -126.f);
-  z.y = fmaxf(z.y, -126.f);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.y) : "f"(-126.f));
   auto both = [](float c) { return make_float2(c, c); };
   const float2 t = __fadd2_rn(z, both(12582912.f));
   const float2 f = __fadd2_rn(z, __ffma2_rn(t, both(-1.f), both(12582912.f)));
@@ -108,8 +109,8 @@ __device__ __forceinline__ float2 exp2_poly(float2 z) {
   p = __ffma2_rn(f, p, both(0.24024745f));
   p = __ffma2_rn(f, p, both(0.69312181f));
   p = __ffma2_rn(f, p, both(0.99999926f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  auto power = [](float n) { return __uint_as_float((__float_as_uint(n) << 23) + 0x3F800000u); };  // of n's low bits
+  return __fmul2_rn(p, make_float2(power(t.x), power(t.y)));
 }
 
 // Bounded wait of a whole warp.  A phase that is over already, the usual case here, is seen by test_wait in about 40

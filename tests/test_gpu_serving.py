@@ -204,6 +204,24 @@ def test_packed_attention_non_finite_queries_and_keys(impl):
 
 
 @pytest.mark.parametrize("impl", KERNELS)
+@pytest.mark.parametrize("heads", [(3, 1, 64), (4, 2, 128)], ids=str)
+def test_packed_attention_nan_score_at_any_place_spoils_its_rows(impl, heads):
+    """One sequence per place of the NaN key: whichever way its exponential is computed, the rows that see it are NaN."""
+    hq, hkv, d, n = *heads, 145
+    places = list(range(0, 20)) + [32, 33, 63, 64, 80, 113, 127, 128, 129, 144]
+    lens = [n] * len(places)
+    q, kv = packed_inputs(lens, lens, hq, hkv, d, BF16, seed=34)
+    for i, j in enumerate(places):
+        kv[i * n + j, :hkv, 3] = float("nan")
+    cu = ints(starts(lens)).to(DEV)
+    kvd = kv.to(DEV)
+    got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], cu, impl=impl).isnan().flatten(1).cpu()
+    for i, j in enumerate(places):
+        rows = got[i * n:(i + 1) * n]
+        assert not rows[:j].any() and rows[j:].all(), f"place {j}"
+
+
+@pytest.mark.parametrize("impl", KERNELS)
 def test_packed_attention_bounds_its_rows_by_the_tensors(impl):
     """Starts that point behind the tensors are cut off there; nothing outside is read or written."""
     q, kv = packed_inputs([20], [20], 6, 2, 64, BF16, seed=12)
