@@ -16,7 +16,6 @@ namespace serving {
 constexpr int kErrBadPage = 104;
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kGroup = 32;  // dimensions that share one (step, low) pair in a 4-bit cache
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -39,17 +38,6 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<__half2*>(&w));
-}
-
-template <typename T>
-__device__ __forceinline__ T from_float(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
-  return __float2bfloat16_rn(x);
-}
-template <>
-__device__ __forceinline__ __half from_float<__half>(float x) {
-  return __float2half_rn(x);
 }
 
 // bits that are all ones in an infinity or a NaN of the type, for two packed values
