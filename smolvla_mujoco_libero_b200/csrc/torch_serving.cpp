@@ -9,6 +9,7 @@
 #include <cstdint>
 #include <limits>
 #include <optional>
+#include <string>
 
 #include "../../include/svla.h"
 
@@ -32,9 +33,21 @@ void bind(uintptr_t append, uintptr_t packed, uintptr_t paged, uintptr_t paged_w
   calls.paged_workspace = reinterpret_cast<decltype(calls.paged_workspace)>(paged_workspace);
 }
 
+// a message's pieces; no streams, whose state belongs to the C++ library that a process loaded
+std::string text(const char* s) { return s; }
+std::string text(int64_t x) { return std::to_string(x); }
+std::string text(int x) { return std::to_string(x); }
+std::string text(at::ScalarType t) { return c10::toString(t); }
+std::string text(c10::Device d) { return d.str(); }
+std::string text(at::IntArrayRef a) {
+  std::string s = "[";
+  for (size_t i = 0; i < a.size(); ++i) s += (i ? ", " : "") + std::to_string(a[i]);
+  return s + "]";
+}
+
 template <typename... A>
 [[noreturn]] void refuse(const A&... a) {
-  throw py::value_error(c10::str(a...));
+  throw py::value_error((text(a) + ...));
 }
 
 // the library's own refusals and CUDA errors, as SvlaError with its message
