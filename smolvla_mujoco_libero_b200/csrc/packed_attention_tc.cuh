@@ -95,13 +95,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^z for two z <= 8 or so on the fp32 pipe: z = n + f with n = rint(z) (adding 1.5 * 2^23 leaves n in the low bits), 2^f
-// by its minimax polynomial of degree 4 on [-1/2, 1/2] (relative error 2.6e-6, found by exchanging extrema), times 2^n.  z is
-// first raised to at least -126: 2^-126 instead of less.  A NaN stays one: the maximum keeps it, and so does the product
-// (n added to the exponent's bits would not).
+// 2^z for two z <= 8 or so on the fp32 pipe, by Cody and Waite's reduction (Software manual for the elementary functions,
+// 1980): z = n + f with n = rint(z) (adding 1.5 * 2^23 leaves n in the low bits), 2^f by its minimax polynomial of degree 4
+// on [-1/2, 1/2] (relative error 2.6e-6, found by exchanging extrema), times 2^n.  z is first raised to at least -127, whose
+// power's exponent field is 0: a masked score's weight (z = -infinity), and every weight below 2^-126.5, is exactly 0, so
+// no hidden value enters whatever its size.  A NaN stays one: the maximum keeps it, and so does the product (n added to the
+// exponent's bits would not).
 __device__ __forceinline__ float2 exp2_poly(float2 z) {
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.y) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.x) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(z.y) : "f"(-127.f));
   auto both = [](float c) { return make_float2(c, c); };
   const float2 t = __fadd2_rn(z, both(12582912.f));
   const float2 f = __fadd2_rn(z, __ffma2_rn(t, both(-1.f), both(12582912.f)));
