@@ -303,7 +303,8 @@ int32_t svla_fused_rope_attention_f32_mask_implicit_pos(const float* q_raw, cons
  * Packed tensors are [rows, heads * head_dim] with a row stride (elements, a multiple of 8, rows 16-byte aligned):
  * sequence b owns rows cu[b] .. cu[b + 1] - 1 of a non-decreasing int32 [batch + 1]; rows behind cu[batch] are neither
  * read nor written.  head_dim 64 or 128; dtype SVLA_DT_BF16 or SVLA_DT_HALF; query head h reads kv head
- * h / (hq / hkv).  A query with no key to see gives zeros.
+ * h / (hq / hkv).  A query whose keys weigh nothing (none to see, none whose page is there, or all scores -infinity) gives
+ * zeros.
  *
  * Cache pages (page_size a multiple of 16, 16 to 256): entry n of sequence b is slot n % page_size of page
  * page_table[b, n / page_size].  bits 16: [n_pages, hkv, 2, page_size, head_dim] of the dtype (keys, values).  bits 4:

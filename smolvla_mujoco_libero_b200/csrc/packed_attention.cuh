@@ -1,6 +1,7 @@
 // Attention over packed prompts: sequence b has queries cu_q[b] .. cu_q[b + 1] and keys cu_k[b] .. cu_k[b + 1] (n_q and
 // n_k of them) of one packed tensor each; query i sees key j iff not causal, or j <= n_k - n_q + i (the queries are the
-// last tokens);  o_i = sum_j softmax_j(scale q_i . k_j) v_j, zeros where there is no key to see.
+// last tokens);  o_i = sum_j softmax_j(scale q_i . k_j) v_j, zeros where no key weighs anything: where there is none to see,
+// or every score is -infinity.
 //
 // One pass over the keys with the running maximum and sum of the softmax, fp32 scores and sums, probabilities rounded
 // to the input type for the second product (as the framework's other attention kernels do).
@@ -325,12 +326,13 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
         }
       }
     }
-    const float inv = sees[hr] > 0 ? __frcp_rn(l[hr]) : 0.f;
+    const bool some = l[hr] != 0.f;  // 0: no key to see, or none whose score is above -infinity; a NaN stays one
+    const float inv = some ? __frcp_rn(l[hr]) : 0.f;
     T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + tok) * a.o_rs + h * D + 2 * t4;
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
       *reinterpret_cast<uint32_t*>(dst + n * 8) =
-          sees[hr] > 0 ? serving::pack2<T>(o[n][2 * hr] * inv, o[n][2 * hr + 1] * inv) : 0u;
+          some ? serving::pack2<T>(o[n][2 * hr] * inv, o[n][2 * hr + 1] * inv) : 0u;
   }
 }
 

@@ -475,7 +475,9 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
         tc_fence_after();
       }
       if (ok && toks[x] > 0) {
-        const float inv = sees > 0 ? __frcp_rn(l.x + l.y) : 0.f;
+        const float sum = l.x + l.y;
+        const bool some = sum != 0.f;  // 0: no key to see, or none whose score is above -infinity; a NaN stays one
+        const float inv = some ? __frcp_rn(sum) : 0.f;
         T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + (real ? t : 0)) * a.o_rs + head * D;
         const bool odd = *reinterpret_cast<volatile int*>(odd_flag) != 0;
 #pragma unroll
@@ -501,7 +503,7 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e)
-            w[e] = sees > 0 ? serving::pack2<T>(__uint_as_float(r[2 * e]) * inv, __uint_as_float(r[2 * e + 1]) * inv) : 0u;
+            w[e] = some ? serving::pack2<T>(__uint_as_float(r[2 * e]) * inv, __uint_as_float(r[2 * e + 1]) * inv) : 0u;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
             *reinterpret_cast<uint4*>(dst + ch * 32 + u * 8) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);

@@ -1,6 +1,7 @@
 // Attention over a paged key / value cache (layouts in kv_append.cuh), 16-bit or 4-bit entries, for a few new tokens
 // per sequence: query i of sequence b (of n_b) sees the cache entries n <= kv_len[b] - n_b + i,
-//   o_i = sum_n softmax_n(scale q_i . k_n) v_n          (no entry to see: zeros).
+//   o_i = sum_n softmax_n(scale q_i . k_n) v_n      (zeros where no entry weighs anything: none to see, none whose page
+// is there, or every score -infinity).
 //
 // Bound by the bytes of the live cache; the work around them has to stay below what an SM issues in the time they
 // take (4 bits, D = 64: 1280 bytes, 55 cycles, per 16 entries of one head).
@@ -53,7 +54,7 @@ struct PagedAttnArgs {
   const int *cu_q, *kv_len, *table;
   float* part;             // workspace: 2 slots per CTA
   int4* meta;              // workspace, per CTA: {b, kv head, query tile, CTA of its last tile} of a cut item that starts
-                           // there, or {-1, ..}; then per CTA that item's {first slot, first row, new tokens, entries}
+                           // there, or {-1, ..}; then per CTA that item's {first slot, first row, new tokens, -}
   long long q_rs, o_rs, table_rs;
   int batch, total, hq, hkv, g, page, n_pages, max_pages;
   unsigned long long page_magic;  // ceil(2^32 / (page / 16)): 16-entry slab -> page
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       // the item's last piece: the CTA whose piece holds the item's last tile
       const long long last = divide(item_at + n_tiles - 1, full_share);
       a.meta[blockIdx.x] = make_int4(b, kh, qt, static_cast<int>(last));
-      a.meta[gridDim.x + blockIdx.x] = make_int4(2 * blockIdx.x + (cur > from ? 1 : 0), sq.begin, n_new, len);
+      a.meta[gridDim.x + blockIdx.x] = make_int4(2 * blockIdx.x + (cur > from ? 1 : 0), sq.begin, n_new, 0);
     }
     // tiles of the sequence in this segment (an uncut item: all of them)
     const int real_tiles = (len + kKeys - 1) / kKeys;
@@ -754,10 +755,10 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       }
       if (whole) {
         const int row = row0 + r;
-        const bool sees_some = len - n_new + row / a.g + 1 > 0 && len > 0;
-        const float inv = sees_some ? __frcp_rn(sum) : 0.f;
+        const bool some = sum != 0.f;  // a NaN stays one
+        const float inv = some ? __frcp_rn(sum) : 0.f;
         T* dst = static_cast<T*>(a.o) + static_cast<size_t>(sq.begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + d;
-        *reinterpret_cast<uint32_t*>(dst) = sees_some ? serving::pack2<T>(o0 * inv, o1 * inv) : 0u;
+        *reinterpret_cast<uint32_t*>(dst) = some ? serving::pack2<T>(o0 * inv, o1 * inv) : 0u;
       } else {
         float* p = a.part + static_cast<size_t>(slot_id) * kRows * (D + 2);
         *reinterpret_cast<float2*>(p + r * D + d) = make_float2(o0, o1);
@@ -788,7 +789,7 @@ __global__ void __launch_bounds__(kPagedJoinWarps * 32) paged_combine_kernel(con
   const int4 meta = a.meta[blockIdx.x], more = a.meta[gridDim.x + blockIdx.x];
   if (meta.x < 0) return;
   const int kh = meta.y, row0 = meta.z * kRows, parts = meta.w - static_cast<int>(blockIdx.x) + 1;
-  const int first_slot = more.x, begin = more.y, n_new = more.z, len = more.w;
+  const int first_slot = more.x, begin = more.y, n_new = more.z;
   const int rows = min(kRows, n_new * a.g - row0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int subs = kPagedJoinWarps / rows, used = min(subs, (parts + kParts - 1) / kParts);
@@ -848,12 +849,12 @@ __global__ void __launch_bounds__(kPagedJoinWarps * 32) paged_combine_kernel(con
     top = t;
   }
   const int row = row0 + r;
-  const bool sees_some = len - n_new + row / a.g + 1 > 0 && len > 0;
-  const float inv = sees_some ? __frcp_rn(sum) : 0.f;
+  const bool some = sum != 0.f;  // a NaN stays one
+  const float inv = some ? __frcp_rn(sum) : 0.f;
   T* dst = static_cast<T*>(a.o) + static_cast<size_t>(begin + row / a.g) * a.o_rs + (kh * a.g + row % a.g) * D + kPer * lane;
 #pragma unroll
   for (int j = 0; j < kPer; j += 2)
-    *reinterpret_cast<uint32_t*>(dst + j) = sees_some ? serving::pack2<T>(o.x[j] * inv, o.x[j + 1] * inv) : 0u;
+    *reinterpret_cast<uint32_t*>(dst + j) = some ? serving::pack2<T>(o.x[j] * inv, o.x[j + 1] * inv) : 0u;
 }
 
 }  // namespace svla
