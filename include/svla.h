@@ -358,9 +358,10 @@ typedef struct svla_packed_attn_desc {
 int32_t svla_packed_attention(const svla_packed_attn_desc* desc, svla_stream_t stream);
 
 /* Attention of a few new tokens per sequence (one, or several drafted ones) over a paged cache: query i of the n_b new
- * ones sees entries n <= kv_len[b] - n_b + i, so the tokens themselves are appended first (svla_kv_append).  The
- * workspace (256-byte aligned, at least svla_paged_attention_workspace_size bytes, max_entries = max_pages * page_size;
- * 0 bytes: none is needed) needs no initialisation; calls that overlap on the GPU must not share one. */
+ * ones sees entries n <= kv_len[b] - n_b + i, so the tokens themselves are appended first (svla_kv_append); of those, the
+ * ones that can be read (inside the table, page inside the cache).  The workspace (256-byte aligned, at least
+ * svla_paged_attention_workspace_size bytes, max_entries = max_pages * page_size; 0 bytes: none is needed) needs no
+ * initialisation; calls that overlap on the GPU must not share one. */
 size_t svla_paged_attention_workspace_size(int32_t batch, int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim,
                                            int64_t max_entries);
 

@@ -219,6 +219,9 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     // ---- the item at `cur`
     const serving::Span sq = serving::span_of(a.cu_q, b, a.total);
     const int n_new = sq.end - sq.begin, len = entries(b), n_tiles = tiles_of(len);
+    // entries that token i sees; the causal limit counts from kv_len itself, also where the table ends before it
+    const int past = min(max(__ldg(a.kv_len + b), 0) - n_new, len);
+    auto seen = [&](int i) { return min(max(past + i + 1, 0), len); };
     const int qt_n = query_tiles<NT>(n_new, a.g);
     const long long w = static_cast<long long>(n_tiles) * qt_n * a.hkv;
     if (cur >= at + w) {
@@ -244,8 +247,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     int tile1 = a.split ? min(static_cast<int>(seg_end - item_at) - a.item_cost, real_tiles) : real_tiles;
     const int row0 = qt * kRows, rows = min(kRows, n_new * a.g - row0);
     // entries the last / first row of this query tile sees
-    const int sees_last = min(max(len - n_new + (row0 + rows - 1) / a.g + 1, 0), len);
-    const int sees_first = min(max(len - n_new + row0 / a.g + 1, 0), len);
+    const int sees_last = seen((row0 + rows - 1) / a.g), sees_first = seen(row0 / a.g);
     tile1 = min(tile1, (sees_last + kKeys - 1) / kKeys);
 
     // ---- this warp's tiles: tile0 + warp, + 4, ...
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int r = row0 + nt * 8 + 2 * t4 + u;
-        sees[nt][u] = min(max(len - n_new + r / a.g + 1, 0), len);
+        sees[nt][u] = seen(r / a.g);
       }
 
     float o[NT][D / 16][4];     // O^T: see the P.V product for which dimensions a thread holds

@@ -10,9 +10,10 @@ import pytest
 import torch
 
 from oracle import serving as S
+from smolvla_mujoco_libero_b200 import _lib as L
 from smolvla_mujoco_libero_b200 import ops
 from tests.test_gpu_serving import (BF16, DEV, FP16, KERNELS, _no_device_error, filled_cache, gen, ints,  # noqa: F401
-                                    packed_inputs, packed_reference, starts, within)
+                                    packed_inputs, packed_reference, paged_tolerance, starts, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +78,43 @@ def test_paged_attention_scores_of_minus_infinity(heads, gone, total, width):
     none = [i for i in range(new) if total - new + i < gone]
     assert bool((got[none] == 0).all())
     within(got, o, S.attention_tolerance(o, spread, size, BF16, d))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("width", [None, 64], ids=["one piece", "pieces"])
+def test_paged_attention_rows_whose_pages_are_missing(bits, width):
+    """What is readable counts, and where nothing is, zeros: a page outside the cache in the middle, all pages outside, a
+    sequence longer than its table (three drafted tokens, all of which see all that the table reaches)."""
+    hq, hkv, d, page = 6, 2, 64, 16
+    heads, lens, new = (hq, hkv, d), [40, 20, 48, 40], [2, 1, 3, 1]
+    cache, table = filled_cache(lens, heads, bits, page, BF16, seed=57, width=width)
+    q = torch.randn(sum(new), hq, d, generator=gen(58)).to(BF16)
+    broken, at = table.clone(), starts(new)
+    broken[0, 1], broken[1, :2] = 1 << 20, -1
+    total = [40, 20, 500, 40]
+    if width is not None:
+        broken = broken.clone()
+        total[2] = 48 + 2  # the table is wide: two entries that it does not name
+        broken[2, 3] = -1
+    got = ops.paged_attention(q.to(DEV), cache.to(DEV), ints(at).to(DEV), ints(total).to(DEV), broken.to(DEV))
+    assert L.device_error(reset=True) == L.ERR_BAD_PAGE
+    assert bool((got[at[1]:at[2]] == 0).all())
+    for b, keep, seen in ((0, [n for n in range(40) if n // page != 1], [23, 24]),
+                          (2, list(range(48)), [48] * 3), (3, list(range(40)), [40])):
+        k, v, ks, vs = S.rows(cache, page, d, table[b], lens[b])
+        o, spread, size = S.attend_dense(q[at[b]:at[b + 1]].double(), k[keep], v[keep], seen, d ** -0.5, ks[keep], vs[keep])
+        within(got[at[b]:at[b + 1]], o, paged_tolerance(o, spread, size, BF16, d, bits, [lens[b]], 1.0), f"sequence {b}")
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_paged_attention_limit_counts_entries_past_the_table(bits):
+    """Three drafted tokens of a sequence that is two entries longer than its table: the first sees all the table holds, as
+    do the others."""
+    heads, page = (6, 2, 64), 16
+    cache, table = filled_cache([48], heads, bits, page, BF16, seed=59)
+    q = torch.randn(1, 6, 64, generator=gen(60)).to(BF16).expand(3, 6, 64).contiguous()
+    got = ops.paged_attention(q.to(DEV), cache.to(DEV), ints([0, 3]).to(DEV), ints([50]).to(DEV), table.to(DEV))
+    assert L.device_error(reset=True) == L.ERR_BAD_PAGE
+    k, v, ks, vs = S.rows(cache, page, 64, table[0], 48)
+    o, spread, size = S.attend_dense(q.double(), k, v, [48] * 3, 0.125, ks, vs)
+    within(got, o, paged_tolerance(o, spread, size, BF16, 64, bits, [48], 1.0))
