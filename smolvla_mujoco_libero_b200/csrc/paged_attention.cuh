@@ -494,21 +494,24 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
           }
         }
       }
-      // 4 bits: largest step of the tile's values, a lane's share of the pairs at a time
+      // 4 bits: largest step of the tile's values, a lane's share of the pairs at a time; one that is no number does not count
       float big = 0.f;
       if constexpr (BITS == 4) {
         constexpr int kWords = kKeys * kGroups / 32;  // 4
         static_assert(kWords == 4, "a lane takes 16 bytes of the pairs");
         const uint4 v = *reinterpret_cast<const uint4*>(st + Tl::kVP + lane * 16);
-        big = max3(max3(big, __uint_as_float(v.x << 16), __uint_as_float(v.y << 16)), __uint_as_float(v.z << 16),
-                   __uint_as_float(v.w << 16));
+        auto step = [](uint32_t w) {
+          const float x = __uint_as_float(w << 16);
+          return x < INFINITY ? x : 0.f;
+        };
+        big = max3(max3(big, step(v.x), step(v.y)), step(v.z), step(v.w));
         if (edge) {  // whatever stands in entries that nobody sees does not count
           const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
           big = 0.f;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const int n = (lane * 4 + w) / kGroups;
-            if (key0 + n < sees_last && !((gone >> (n / 16)) & 1u)) big = fmaxf(big, __uint_as_float(vv[w] << 16));
+            if (key0 + n < sees_last && !((gone >> (n / 16)) & 1u)) big = fmaxf(big, step(vv[w]));
           }
         }
       }
@@ -539,9 +542,8 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       if (__any_sync(0xffffffffu, pass)) {
         float e_new = e;
         if constexpr (BITS == 4) {
-          // steps that are no number do not count; below 2^-60 the factor would push p beyond fp32's range, and what
-          // fp16 loses there is nothing beside any other entry
-          big = big < 1.7e38f ? big : 0.f;
+          // below 2^-60 the factor would push p beyond fp32's range, and what fp16 loses there is nothing beside any other
+          // entry
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
           e_new = fmaxf(e, static_cast<float>(static_cast<int>(__float_as_uint(big) >> 23) - 127));

@@ -13,7 +13,7 @@ from oracle import serving as S
 from smolvla_mujoco_libero_b200 import _lib as L
 from smolvla_mujoco_libero_b200 import ops
 from tests.test_gpu_serving import (BF16, DEV, FP16, KERNELS, _no_device_error, filled_cache, gen, ints,  # noqa: F401
-                                    packed_inputs, packed_reference, paged_tolerance, starts, within)
+                                    make_table, packed_inputs, packed_reference, paged_reference, paged_tolerance, starts, within)
 
 pytestmark = pytest.mark.gpu
 
@@ -59,6 +59,59 @@ def test_packed_attention_scores_of_minus_infinity(impl, heads, dtype, gone):
     got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints([0, n]).to(DEV), impl=impl)
     assert bool((got[:gone] == 0).all())
     within(got[some.to(DEV)], o[some], S.attention_tolerance(o, spread, size, dtype, d)[some])
+
+
+# ----------------------------------------------------------------------------- paged attention
+
+def step_floor(q, cache, page, table, new, total):
+    """4 bits: what rounding the weights p step to fp16 can lose below its normal range, [rows, heads, D].
+
+    A warp keeps the weights of every group of 32 dimensions at a power of two of their own, such that the largest it has
+    met is 2^2 or more; a smaller one is off by half a subnormal step, 2^-25, that is by 2^-27 of the largest, times a code
+    of at most 15, for each entry."""
+    d, at, out = q.shape[2], starts(new), []
+    g = q.shape[1] // cache.shape[1]
+    for b in range(len(new)):
+        k = S.rows(cache, page, d, table[b], total[b])[0]
+        pairs = [S.split4(cache[int(table[b, n // page])], page, d)[1][1][:, n % page, :, 0] for n in range(total[b])]
+        step = torch.stack(pairs).double().abs()  # [entries, hkv, d / 32]
+        for i, n in enumerate(S.causal_seen(new[b], total[b])):
+            row = torch.zeros(q.shape[1], d, dtype=torch.float64)
+            for h in range(q.shape[1] if n else 0):
+                p = torch.softmax(k[:n, h // g] @ q[at[b] + i, h].double() * d ** -0.5, 0)
+                row[h] = (p[:, None] * step[:n, h // g]).amax(0).repeat_interleave(32)
+            out.append(row * n * 15 * 2.0 ** -27)
+    return torch.stack(out)
+
+
+def check_groups(q, cache, page, table, new, total, what):
+    d = q.shape[2]
+    o, spread, size = paged_reference(q, cache, page, table, new, total)
+    got = ops.paged_attention(q.to(DEV), cache.to(DEV), ints(starts(new)).to(DEV), ints(total).to(DEV), table.to(DEV))
+    tol = S.attention_tolerance(o, spread, size, q.dtype, d, weight_unit=2.0 ** -11)
+    within(got, o, tol + step_floor(q, cache, page, table, new, total), what)
+
+
+def cache_of(k, v, page, width=None, seed=50):
+    table, n_pages = make_table([k.shape[0]], page, seed, width=width)
+    cache = ops.kv_cache(n_pages, page, k.shape[1], k.shape[2], 4, k.dtype, device="cpu")
+    S.append(cache, page, k, v, [0, k.shape[0]], [k.shape[0]], table)
+    return cache, table
+
+
+@pytest.mark.parametrize("heads", [(3, 1, 64), (8, 2, 128)], ids=str)
+@pytest.mark.parametrize("n", [1, 2, 33, 65, 130])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_paged_attention_non_finite_group_leaves_the_others(heads, n, bad):
+    """4 bits, an infinity or a NaN in the last entry's values: its group of 32 dimensions is NaN, the others are right."""
+    hq, hkv, d = heads
+    g = gen(54)
+    k, v = (torch.randn(n, hkv, d, generator=g) for _ in range(2))
+    q = torch.randn(1, hq, d, generator=g).to(BF16)
+    v[n - 1, :, 40] = bad
+    for width in (None, 64):
+        cache, table = cache_of(k.to(BF16), v.to(BF16), 16, width)
+        check_groups(q, cache, 16, table, [1], [n], f"{n} entries")
 
 
 @pytest.mark.parametrize("heads", [(3, 1, 64), (8, 2, 128)], ids=str)
