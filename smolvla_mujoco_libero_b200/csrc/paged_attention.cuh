@@ -19,14 +19,16 @@
 // needs one accumulator per group and two FMAs per score, and
 //   sum_n p_n v_n = sum_n (p_n step_n) c_n + sum_n p_n low_n
 // takes p_n step_n as the other operand.  Query rows are scaled by a power of two to the top of fp16's range (exact but
-// for components below 2^-25 of the row's largest), so bf16 queries lose nothing.  p_n step_n is rounded to fp16
-// (2^-11 relative); to keep it in fp16's range whatever the steps are, p_n carries the factor 2^-e of the largest step
-// seen so far, 2^e <= step < 2^(e + 1), besides that of the running maximum (both cancel in O / l).  Products with low_n
-// stay in fp32.
+// for components below 2^-25 of the row's largest), so bf16 queries lose nothing.  p_n step_n is rounded to fp16, 2^-11
+// relative.  Every query column and group has a power of two of its own that brings the largest p_n step_n so far to 2^2,
+// so that groups of different size, and large entries of little weight, leave the others their bits; what is smaller than
+// 2^-16 of the largest is off by 2^-27 of it (half a subnormal step).  These factors move with the maximum, or when a step
+// reaches a limit below which nothing can leave fp16's range; what a tile costs for them otherwise is a comparison and one
+// product per weight.  Products with low_n stay in fp32.
 //
 // Every warp works alone: its own tiles of 16 to 64 entries through its own ring of asynchronous copies, its own running
 // maximum, sum and O, no barrier in the loop.  The maximum is lazy: it moves (and O is rescaled) only when a score
-// passes it by more than 8 in log2 units (or a step 2^(e + 1)), one vote per tile instead of shuffles.  Instruction issue
+// passes it by more than 8 in log2 units (or a step the limit), one vote per tile instead of shuffles.  Instruction issue
 // is what stands beside the memory system: the two query columns of a thread go through packed fp32 operations, a page's
 // address is worked out once by one lane for 16 tiles, and the masks are in a branch that only a sequence's end takes.
 //
@@ -80,6 +82,16 @@ struct Tile {
   static constexpr int kK = 0, kV = kKeys * kRow, kKP = 2 * kKeys * kRow, kVP = kKP + kKeys * kPairs;
   static constexpr int kBytes = 2 * kKeys * (kRow + kPairs);
 };
+
+// 4 bits, weights p step of the second product in fp16: a factor brings a column's largest weight in a group to 2^2 (below
+// 2^3); p grows by 2^8 at most before the maximum moves, so steps below 2^7 / factor keep them below 2^15.  Factors are
+// powers of two from 2^-126 to 2^100; a limit is kept as the bits of a step without its sign, times 2.
+constexpr int kWeightTop = 2;
+constexpr float kWeightFactorTop = 0x1p100f;
+__device__ __forceinline__ float power_inverse(float f) { return __uint_as_float(0x7F000000u - __float_as_uint(f)); }
+__device__ __forceinline__ uint32_t step_limit(float factor) {
+  return 2u * min(0x7F000000u - __float_as_uint(factor) + (7u << 23), 0x7F800000u);
+}
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
@@ -327,7 +339,10 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     uint32_t qb[NT][kQRegs];
     float qf[NT][2];            // factors of this thread's two score columns (queries 2 t4, 2 t4 + 1)
     float qs[NT][kGroups][2];   // 4 bits: sums of their components, per group, times scale
-    float big_limit = 0.f;      // 4 bits: a step from here on moves the exponent e
+    // 4 bits: powers of two that bring the weights p step of a column and group into fp16's range; a step of the group from
+    // limit on may leave it
+    float2 f[NT][kGroups];
+    uint32_t limit[kGroups];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = row0 + nt * 8 + g8;
@@ -369,7 +384,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
         ex = (top > 0.f && ex < 128) ? max(ex, -100) : 14;
         const float up = __uint_as_float(static_cast<uint32_t>(14 - ex + 127) << 23);
         // undoes 2^-24 of the codes and `up`
-        const float f = a.scale_log2 * 1024.f * __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
+        const float down = a.scale_log2 * 1024.f * __uint_as_float(static_cast<uint32_t>(ex + 127) << 23);
 #pragma unroll
         for (int gr = 0; gr < kGroups; ++gr) {
           // step 0 of the group: (n0, n4 | n1, n5), step 1: (n2, n6 | n3, n7); odd nibbles count 16 times
@@ -381,7 +396,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
         // the score columns of this thread are queries 2 t4 and 2 t4 + 1: take their factors from lanes 8 t4, 8 t4 + 4
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          qf[nt][u] = __shfl_sync(0xffffffffu, f, 8 * t4 + 4 * u);
+          qf[nt][u] = __shfl_sync(0xffffffffu, down, 8 * t4 + 4 * u);
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr)
             qs[nt][gr][u] = __shfl_sync(0xffffffffu, sum[gr] * a.scale_log2, 8 * t4 + 4 * u);
@@ -401,13 +416,17 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
     float o[NT][D / 16][4];     // O^T: see the P.V product for which dimensions a thread holds
     float om[NT][kGroups][2];   // 4 bits: sums of p low
     float m[NT][2], ref[NT][2], l[NT][2];
-    float e = -60.f;            // 4 bits: exponent of the largest step so far (not below 2^-60: see below)
+#pragma unroll
+    for (int gr = 0; gr < kGroups; ++gr) limit[gr] = step_limit(kWeightFactorTop);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
 #pragma unroll
-      for (int gr = 0; gr < kGroups; ++gr) om[nt][gr][0] = om[nt][gr][1] = 0.f;
+      for (int gr = 0; gr < kGroups; ++gr) {
+        om[nt][gr][0] = om[nt][gr][1] = 0.f;
+        f[nt][gr] = make_float2(kWeightFactorTop, kWeightFactorTop);
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) m[nt][u] = -INFINITY, ref[nt][u] = 0.f, l[nt][u] = 0.f;
     }
@@ -494,24 +513,21 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
           }
         }
       }
-      // 4 bits: largest step of the tile's values, a lane's share of the pairs at a time; one that is no number does not count
-      float big = 0.f;
+      // 4 bits: does a step of the tile's values, a lane's share of the pairs at a time, reach its group's limit?
+      bool large = false;
       if constexpr (BITS == 4) {
         constexpr int kWords = kKeys * kGroups / 32;  // 4
         static_assert(kWords == 4, "a lane takes 16 bytes of the pairs");
         const uint4 v = *reinterpret_cast<const uint4*>(st + Tl::kVP + lane * 16);
-        auto step = [](uint32_t w) {
-          const float x = __uint_as_float(w << 16);
-          return x < INFINITY ? x : 0.f;
-        };
-        big = max3(max3(big, step(v.x), step(v.y)), step(v.z), step(v.w));
+        const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+        auto reaches = [&](int w) { return vv[w] << 17 >= limit[w % kGroups]; };  // (or is no number)
+        large = reaches(0) || reaches(1) || reaches(2) || reaches(3);
         if (edge) {  // whatever stands in entries that nobody sees does not count
-          const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
-          big = 0.f;
+          large = false;
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const int n = (lane * 4 + w) / kGroups;
-            if (key0 + n < sees_last && !((gone >> (n / 16)) & 1u)) big = fmaxf(big, step(vv[w]));
+            if (key0 + n < sees_last && !((gone >> (n / 16)) & 1u)) large |= reaches(w);
           }
         }
       }
@@ -528,7 +544,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       }
       // ---- lazy running maximum
       float top[NT][2];
-      bool pass = BITS == 4 && big >= big_limit;
+      bool pass = large;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -539,16 +555,8 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
           top[nt][u] = t;
           pass |= t > m[nt][u] + 8.f;
         }
-      if (__any_sync(0xffffffffu, pass)) {
-        float e_new = e;
-        if constexpr (BITS == 4) {
-          // below 2^-60 the factor would push p beyond fp32's range, and what fp16 loses there is nothing beside any other
-          // entry
-#pragma unroll
-          for (int d = 1; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-          e_new = fmaxf(e, static_cast<float>(static_cast<int>(__float_as_uint(big) >> 23) - 127));
-          big_limit = ex2_approx(e_new + 1.f);
-        }
+      const bool moves = __any_sync(0xffffffffu, pass);
+      if (moves) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -556,22 +564,28 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             float t = fmaxf(top[nt][u], m[nt][u]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
-            // nothing seen so far: O and the sums are zeros, any factor will do
-            const float alpha = m[nt][u] == -INFINITY ? 1.f : ex2_approx((m[nt][u] - t) + (e - e_new));
-            m[nt][u] = t;
-            ref[nt][u] = t == -INFINITY ? 0.f : t + (BITS == 4 ? e_new : 0.f);
-            l[nt][u] *= alpha;
-#pragma unroll
-            for (int i2 = 0; i2 < D / 16; ++i2) {
-              o[nt][i2][u] *= alpha;
-              o[nt][i2][2 + u] *= alpha;
+            float alpha;
+            if constexpr (BITS == 4) {  // a power of two, 0 from 2^-127 on and where nothing has been seen
+              t = ceilf(t);
+              alpha = __uint_as_float(static_cast<uint32_t>(127 - static_cast<int>(fminf(t - m[nt][u], 127.f))) << 23);
+            } else {  // nothing seen so far: O and the sums are zeros, any factor will do
+              alpha = m[nt][u] == -INFINITY ? 1.f : ex2_approx(m[nt][u] - t);
             }
+            m[nt][u] = t;
+            ref[nt][u] = t == -INFINITY ? 0.f : t;
+            l[nt][u] *= alpha;
             if constexpr (BITS == 4) {
+              top[nt][u] = alpha;  // O follows below, with its factors
 #pragma unroll
               for (int gr = 0; gr < kGroups; ++gr) om[nt][gr][u] *= alpha;
+            } else {
+#pragma unroll
+              for (int i2 = 0; i2 < D / 16; ++i2) {
+                o[nt][i2][u] *= alpha;
+                o[nt][i2][2 + u] *= alpha;
+              }
             }
           }
-        e = e_new;
       }
       // ---- probabilities
 #pragma unroll
@@ -583,6 +597,63 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             s[nt][sl][x] = ex2_approx(s[nt][sl][x] - ref[nt][x & 1]);
             l[nt][x & 1] += s[nt][sl][x];
           }
+      // ---- 4 bits: the weights' factors
+      if constexpr (BITS == 4) {
+        if (moves) {
+          float2 w[NT][kGroups];  // largest weights, times 2^-10 (p goes up to 2^8)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int gr = 0; gr < kGroups; ++gr) w[nt][gr] = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int sl = 0; sl < kSlabs; ++sl)
+#pragma unroll
+            for (int hr = 0; hr < 2; ++hr) {
+              uint32_t vp[kGroups];
+              load_pairs(vp, st + Tl::kVP + (sl * 16 + g8 + 8 * hr) * Tl::kPairs);
+#pragma unroll
+              for (int gr = 0; gr < kGroups; ++gr) {
+                float step = fabsf(__uint_as_float(vp[gr] << 16)) * 0x1p-10f;
+                if (!(step < INFINITY)) step = 0.f;  // no number: does not count
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  w[nt][gr].x = fmaxf(w[nt][gr].x, s[nt][sl][2 * hr] * step);
+                  w[nt][gr].y = fmaxf(w[nt][gr].y, s[nt][sl][2 * hr + 1] * step);
+                }
+              }
+            }
+#pragma unroll
+          for (int gr = 0; gr < kGroups; ++gr) {
+            float most = 0.f;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              // both columns' upper halves in one word
+              uint32_t both = __byte_perm(__float_as_uint(w[nt][gr].x), __float_as_uint(w[nt][gr].y), 0x7632);
+#pragma unroll
+              for (int d = 4; d < 32; d <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xffffffffu, both, d));
+              // 2^(kWeightTop - exponent of the weight), from the exponent field of weight 2^-10; O's factor grows with the
+              // maximum, up to kWeightFactorTop, and O stays
+              auto next = [&](uint32_t field, float was, float alpha) {
+                const float room = __uint_as_float(min(max(kWeightTop + 244 - static_cast<int>(field & 255u), 1), 227) << 23);
+                return fminf(was * power_inverse(alpha), room);
+              };
+              const float2 a2 = make_float2(top[nt][0], top[nt][1]), was = f[nt][gr];
+              const float2 now = make_float2(next(both >> 7, was.x, a2.x), next(both >> 23, was.y, a2.y));
+              f[nt][gr] = now;
+              most = fmaxf(most, fmaxf(now.x, now.y));
+              const float2 r = __fmul2_rn(__fmul2_rn(now, a2), make_float2(power_inverse(was.x), power_inverse(was.y)));
+#pragma unroll
+              for (int i2 = 2 * gr; i2 < 2 * gr + 2; ++i2) {
+                o[nt][i2][0] *= r.x, o[nt][i2][1] *= r.y;
+                o[nt][i2][2] *= r.x, o[nt][i2][3] *= r.y;
+              }
+            }
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            limit[gr] = step_limit(most);
+          }
+        }
+      }
       // ---- O^T += V^T P^T
       if constexpr (BITS == 16) {
         // an infinity or a NaN in the value of an entry that some row does not see would reach that row as 0 * inf
@@ -668,10 +739,11 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
 #pragma unroll
               for (int gr = 0; gr < kGroups; ++gr) {
                 const float step = __uint_as_float(vp[gr] << 16), low = __uint_as_float(vp[gr] & 0xFFFF0000u);
-                const float p0 = s[nt][sl][2 * hr], p1 = s[nt][sl][2 * hr + 1];
-                om[nt][gr][0] = fmaf(p0, low, om[nt][gr][0]);
-                om[nt][gr][1] = fmaf(p1, low, om[nt][gr][1]);
-                pb[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(p0 * step, p1 * step));
+                const float2 p = make_float2(s[nt][sl][2 * hr], s[nt][sl][2 * hr + 1]);
+                const float2 y = __fmul2_rn(p, __fmul2_rn(make_float2(step, step), f[nt][gr]));
+                om[nt][gr][0] = fmaf(p.x, low, om[nt][gr][0]);
+                om[nt][gr][1] = fmaf(p.y, low, om[nt][gr][1]);
+                pb[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(y.x, y.y));
               }
           }
           // the half word g8 of each group's codes (dimensions 4 g8 .. + 3), of entries 2 t4 and 2 t4 + 1 (and + 8) in one
@@ -732,8 +804,9 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
           } else {
             // 2^24 undoes the codes' subnormals, odd dimensions counted 16 times
             const int d = (mt >> 1) * 32 + 4 * g8 + 2 * (mt & 1);
-            js[r * (D + 1) + d] = fmaf(o[nt][mt][u], 16777216.f, om[nt][mt >> 1][u]);
-            js[r * (D + 1) + d + 1] = fmaf(o[nt][mt][2 + u], 1048576.f, om[nt][mt >> 1][u]);
+            const float back = power_inverse(u ? f[nt][mt >> 1].y : f[nt][mt >> 1].x);
+            js[r * (D + 1) + d] = fmaf(o[nt][mt][u] * 16777216.f, back, om[nt][mt >> 1][u]);
+            js[r * (D + 1) + d + 1] = fmaf(o[nt][mt][2 + u] * 1048576.f, back, om[nt][mt >> 1][u]);
           }
         }
       }

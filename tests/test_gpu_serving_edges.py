@@ -99,6 +99,54 @@ def cache_of(k, v, page, width=None, seed=50):
     return cache, table
 
 
+@pytest.mark.parametrize("heads", [(3, 1, 64), (15, 5, 64), (8, 2, 128), (16, 1, 128)], ids=str)
+@pytest.mark.parametrize("new,n,width", [(1, 200, None), (5, 333, None), (1, 1500, 100), (3, 1500, 100)])
+@pytest.mark.parametrize("factor", [1e4, 1e6, 1e-6])
+def test_paged_attention_groups_of_very_different_size(heads, new, n, width, factor):
+    """One group of dimensions `factor` times the others: each is as precise as if it were alone."""
+    hq, hkv, d = heads
+    g = gen(51)
+    k, v = (torch.randn(n, hkv, d, generator=g) for _ in range(2))
+    v[..., 32:64] *= factor
+    cache, table = cache_of(k.to(BF16), v.to(BF16), 16, width)
+    q = torch.randn(new, hq, d, generator=g).to(BF16)
+    check_groups(q, cache, 16, table, [new], [n], f"factor {factor}")
+
+
+@pytest.mark.parametrize("heads", [(3, 1, 64), (8, 2, 128)], ids=str)
+@pytest.mark.parametrize("new,n,width", [(1, 200, None), (5, 333, None), (3, 1500, 100)])
+@pytest.mark.parametrize("factor,score,at", [(1e4, -30.0, 0), (1e6, -40.0, 77), (1e6, -40.0, 190), (1e9, -60.0, 3)])
+def test_paged_attention_large_value_at_a_low_score(heads, new, n, width, factor, score, at):
+    """One entry's values are `factor` times the others' and its weight next to nothing: the others keep their precision."""
+    hq, hkv, d = heads
+    g = gen(52)
+    k, v = (torch.randn(n, hkv, d, generator=g) for _ in range(2))
+    q = torch.randn(new, hq, d, generator=g)
+    q[..., 0], k[..., 0] = 4.0, 0.0
+    k[at, :, 0] = score * d ** 0.5 / 4.0
+    v[at] *= factor
+    cache, table = cache_of(k.to(BF16), v.to(BF16), 16, width)
+    check_groups(q.to(BF16), cache, 16, table, [new], [n], f"entry {at}")
+
+
+@pytest.mark.parametrize("heads", [(3, 1, 64), (8, 2, 128)], ids=str)
+def test_paged_attention_growing_and_shrinking_steps_and_scores(heads):
+    """Scores that rise along the sequence while the values' steps fall, and the other way round: maxima and exponents
+    move all the time."""
+    hq, hkv, d, n = *heads, 1500
+    for way, rise in ((1, 60.0), (-1, 60.0), (1, 400.0)):
+        g = gen(53)
+        k, v = (torch.randn(n, hkv, d, generator=g) for _ in range(2))
+        q = torch.randn(2, hq, d, generator=g)
+        q[..., 0] = 4.0
+        k[..., 0] = (torch.linspace(0, rise, n) * d ** 0.5 / 4.0)[:, None]
+        v *= torch.logspace(-12 * way, 12 * way, n).flip(0)[:, None, None]
+        v[..., 32:64] *= torch.logspace(6, -6, n)[:, None, None]
+        for width in (None, 120):
+            cache, table = cache_of(k.to(BF16), v.to(BF16), 16, width)
+            check_groups(q.to(BF16), cache, 16, table, [2], [n], f"way {way} rise {rise}")
+
+
 @pytest.mark.parametrize("heads", [(3, 1, 64), (8, 2, 128)], ids=str)
 @pytest.mark.parametrize("n", [1, 2, 33, 65, 130])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
