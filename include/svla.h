@@ -350,7 +350,7 @@ typedef struct svla_packed_attn_desc {
   int64_t q_rs, k_rs, v_rs, o_rs;
   int32_t batch, total_q, total_k;           /* rows of q / o and of k / v */
   int32_t hq, hkv, head_dim, dtype, causal;  /* hq / hkv <= 64 */
-  float scale;                               /* 0 = head_dim^-1/2 */
+  float scale;                               /* positive; 0 = head_dim^-1/2 */
   int32_t impl;                              /* SVLA_ATTN_AUTO, or force SVLA_ATTN_MMA_SYNC / SVLA_ATTN_TCGEN05 (the
                                                 latter needs total_k > 0) */
 } svla_packed_attn_desc;
@@ -373,7 +373,7 @@ typedef struct svla_paged_attn_desc {
   int64_t q_rs, o_rs, page_table_rs;
   int32_t batch, total_q, hq, hkv, head_dim, dtype;
   int32_t bits, page_size, n_pages, max_pages;
-  float scale;                               /* 0 = head_dim^-1/2 */
+  float scale;                               /* positive; 0 = head_dim^-1/2 */
 } svla_paged_attn_desc;
 
 int32_t svla_paged_attention(const svla_paged_attn_desc* desc, svla_stream_t stream);

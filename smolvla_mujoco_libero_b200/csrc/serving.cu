@@ -42,6 +42,15 @@ int32_t check_cache(const char* who, const void* cache, int32_t bits, int32_t pa
   return SVLA_OK;
 }
 
+// the scores' factor in log2 units; 0 stands for head_dim^-1/2.  Not negative: the kernels take the maximum of unscaled
+// scores
+int32_t score_scale(const char* who, float scale, int32_t head_dim, float* log2_scale) {
+  if (!(scale >= 0.f) || std::isinf(scale))
+    return fail(SVLA_ERR_ARG, "%s: scale must be positive and finite, or 0 for head_dim^-1/2 (got %g)", who, scale);
+  *log2_scale = (scale > 0.f ? scale : 1.f / std::sqrt(static_cast<float>(head_dim))) * serving::kLog2e;
+  return SVLA_OK;
+}
+
 template <typename Kern>
 int32_t allow_smem(Kern kern, int bytes, bool (&configured)[64]) {
   int dev = 0;
@@ -244,6 +253,8 @@ int32_t svla_packed_attention(const svla_packed_attn_desc* d, svla_stream_t stre
   const int g = d->hq / d->hkv;
   if (g > packed_detail::kRows) return fail(SVLA_ERR_ARG, "%s: at most %d query heads per kv head (got %d)", who, packed_detail::kRows, g);
   if (!d->cu_q || !d->cu_k) return fail(SVLA_ERR_ARG, "%s: cu_q or cu_k is null", who);
+  float scale_log2 = 0.f;
+  if (int32_t rc = score_scale(who, d->scale, d->head_dim, &scale_log2)) return rc;
   if (d->batch == 0 || d->total_q == 0) return SVLA_OK;
   const int64_t qw = static_cast<int64_t>(d->hq) * d->head_dim, kw = static_cast<int64_t>(d->hkv) * d->head_dim;
   if (int32_t rc = check_rows(who, "q", d->q, d->q_rs, qw)) return rc;
@@ -259,7 +270,7 @@ int32_t svla_packed_attention(const svla_packed_attn_desc* d, svla_stream_t stre
   a.q_rs = d->q_rs, a.k_rs = d->k_rs, a.v_rs = d->v_rs, a.o_rs = d->o_rs;
   a.batch = d->batch, a.total_q = d->total_q, a.total_k = d->total_k, a.hq = d->hq, a.hkv = d->hkv, a.g = g;
   a.causal = d->causal != 0;
-  a.scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt(static_cast<float>(d->head_dim))) * serving::kLog2e;
+  a.scale_log2 = scale_log2;
   if (d->impl < SVLA_ATTN_AUTO || d->impl > SVLA_ATTN_TCGEN05) return fail(SVLA_ERR_ARG, "%s: bad impl %d", who, d->impl);
   if (d->impl == SVLA_ATTN_TCGEN05 && d->total_k == 0) return fail(SVLA_ERR_ARG, "%s: the tcgen05 kernel needs keys", who);
   if (d->impl == SVLA_ATTN_TCGEN05 || (d->impl == SVLA_ATTN_AUTO && d->total_k > 0 && packed_prefers_tc(d, g)))
@@ -288,6 +299,8 @@ int32_t svla_paged_attention(const svla_paged_attn_desc* d, svla_stream_t stream
   if (int32_t rc = check_heads(who, d->hq, d->hkv, d->head_dim, d->dtype)) return rc;
   if (int32_t rc = check_cache(who, d->cache, d->bits, d->page_size, d->n_pages, d->page_table, d->page_table_rs, d->max_pages, d->kv_len)) return rc;
   if (!d->cu_q) return fail(SVLA_ERR_ARG, "%s: cu_q is null", who);
+  float scale_log2 = 0.f;
+  if (int32_t rc = score_scale(who, d->scale, d->head_dim, &scale_log2)) return rc;
   if (d->batch == 0 || d->total_q == 0) return SVLA_OK;
   const int64_t qw = static_cast<int64_t>(d->hq) * d->head_dim;
   if (int32_t rc = check_rows(who, "q", d->q, d->q_rs, qw)) return rc;
@@ -305,7 +318,7 @@ int32_t svla_paged_attention(const svla_paged_attn_desc* d, svla_stream_t stream
   a.batch = d->batch, a.total = d->total_q, a.hq = d->hq, a.hkv = d->hkv, a.g = d->hq / d->hkv;
   a.page = d->page_size, a.n_pages = d->n_pages, a.max_pages = d->max_pages;
   a.page_magic = ((1ull << 32) + a.page / 16 - 1) / (a.page / 16);
-  a.scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt(static_cast<float>(d->head_dim))) * serving::kLog2e;
+  a.scale_log2 = scale_log2;
   a.err = device_error_ptr();
   a.split = paged_split(max_entries);
   const int nt = paged_nt(d->batch, d->total_q, a.g);

@@ -60,6 +60,13 @@ int32_t i32(int64_t x, const char* what) {
   return static_cast<int32_t>(x);
 }
 
+// a number that is not 0 must not become the 0 that stands for head_dim^-1/2
+float f32_scale(double x) {
+  const float f = static_cast<float>(x);
+  if (f == 0.f && x != 0.0) refuse("scale is too small for fp32");
+  return f;
+}
+
 // what the call's tensors share, taken from its first one
 struct Call {
   at::ScalarType dtype;
@@ -200,7 +207,7 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   d.total_q = i32(rq.rows, "the number of rows"), d.total_k = i32(rk.rows, "the number of rows");
   d.hq = i32(rq.heads, "query heads"), d.hkv = i32(rk.heads, "kv heads");
   d.head_dim = i32(c.d, "head_dim"), d.dtype = c.code(), d.causal = causal;
-  d.scale = static_cast<float>(scale), d.impl = impl;
+  d.scale = f32_scale(scale), d.impl = impl;
   check(calls.packed(&d, c.stream()), "svla_packed_attention");
   return *out;
 }
@@ -228,7 +235,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& cache, const Tensor& cu_q,
   d.q = q.const_data_ptr(), d.cache = cache.const_data_ptr(), d.o = out->data_ptr();
   d.cu_q = static_cast<const int32_t*>(cu_q.const_data_ptr());
   d.page_table = static_cast<const int32_t*>(page_table.const_data_ptr()), d.page_table_rs = ca.table_rs;
-  d.q_rs = rq.rs, d.scale = static_cast<float>(scale);
+  d.q_rs = rq.rs, d.scale = f32_scale(scale);
   check(calls.paged(&d, c.stream()), "svla_paged_attention");
   return *out;
 }

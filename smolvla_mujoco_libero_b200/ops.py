@@ -386,8 +386,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: to
     """Attention over prompts of different lengths packed back to back: q [rows, heads, head_dim], k / v
     [rows_k, kv_heads, head_dim] (views of one projection's output are fine), sequence b in rows cu_q[b] ..
     cu_q[b + 1] - 1 of q and cu_k[b] .. of k and v (cu_k None: the same).  Causal: the queries are the last tokens of
-    their sequence.  Returns [rows, heads, head_dim]; rows behind the last sequence are left as they are in ``out``
-    (undefined without it)."""
+    their sequence.  ``scale`` of the scores: positive, 0 for head_dim ** -0.5.  Returns [rows, heads, head_dim]; rows
+    behind the last sequence are left as they are in ``out`` (undefined without it)."""
     return L.serving().packed_attention(q, k, v, cu_q, cu_k, causal, scale, out, impl)
 
 
@@ -395,9 +395,9 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor, kv
                     page_table: torch.Tensor, scale: float = 0.0, out: torch.Tensor | None = None,
                     workspace: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the newest tokens (q [rows, heads, head_dim], sequence b's in rows cu_q[b] .. cu_q[b + 1] - 1, already
-    appended) over a paged cache of 16 or 4 bits; kv_len [B] entries, pages in page_table [B, max_pages].  Returns
-    [rows, heads, head_dim].  ``workspace``: uint8 of svla_paged_attention_workspace_size bytes, taken from torch's
-    allocator when None."""
+    appended) over a paged cache of 16 or 4 bits; kv_len [B] entries, pages in page_table [B, max_pages].  ``scale`` as in
+    ``packed_attention``.  Returns [rows, heads, head_dim].  ``workspace``: uint8 of svla_paged_attention_workspace_size
+    bytes, taken from torch's allocator when None."""
     return L.serving().paged_attention(q, cache, cu_q, kv_len, page_table, scale, out, workspace)
 
 

@@ -219,3 +219,16 @@ def test_paged_attention_limit_counts_entries_past_the_table(bits):
     k, v, ks, vs = S.rows(cache, page, 64, table[0], 48)
     o, spread, size = S.attend_dense(q.double(), k, v, [48] * 3, 0.125, ks, vs)
     within(got, o, paged_tolerance(o, spread, size, BF16, 64, bits, [48], 1.0))
+
+
+# ----------------------------------------------------------------------------- arguments
+
+def test_scales_that_do_not_fit_are_refused():
+    q, kv = torch.zeros(4, 6, 64, dtype=BF16, device=DEV), torch.zeros(4, 2, 64, dtype=BF16, device=DEV)
+    cu, n, table = ints([0, 4]).to(DEV), ints([4]).to(DEV), ints([[0]]).to(DEV)
+    cache = ops.kv_cache(1, 16, 2, 64)
+    for scale in (-0.125, math.inf, -math.inf, math.nan, 1e-60, 1e60):
+        for call in (lambda: ops.packed_attention(q, kv, kv, cu, scale=scale),
+                     lambda: ops.paged_attention(q, cache, cu, n, table, scale=scale)):
+            with pytest.raises((ValueError, L.SvlaError), match="scale"):
+                call()
