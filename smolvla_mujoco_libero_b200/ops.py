@@ -342,12 +342,16 @@ def rope_table_wide(max_pos: int, max_wavelength: float, device, head_dim: int =
     """(cos, sin) [max_pos, head_dim / 2, 2] from angles in 64 bits: the table of ``kv_append`` (``rope_table`` keeps the
     reference's fp32 angles and its width of 64)."""
     cs = torch.empty(max_pos, head_dim // 2, 2, dtype=torch.float32, device=device)
+    _need(cs, torch.float32, "the rotation table")
+    if cs.get_device() != torch.cuda.current_device():
+        raise ValueError(f"rope_table_wide: {cs.device} is not the current device, cuda:{torch.cuda.current_device()}")
     check(lib().svla_rope_table_wide(_p(cs), max_pos, head_dim, float(max_wavelength), _stream()), "rope_table_wide")
     return cs
 
 
 def rope_table(max_pos: int, max_wavelength: float, device) -> torch.Tensor:
     cs = torch.empty(max_pos, 32, 2, dtype=torch.float32, device=device)
+    _need(cs, torch.float32, "the rotation table")
     check(lib().svla_rope_table(_p(cs), max_pos, float(max_wavelength), _stream()), "rope_table")
     return cs
 
