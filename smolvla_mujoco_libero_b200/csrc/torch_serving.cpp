@@ -176,6 +176,7 @@ py::object kv_append(const Tensor& cache, const Tensor& k, const Tensor& v, cons
     const Tensor& t = *rope_cs;
     if (t.scalar_type() != at::kFloat || !c.here(t) || t.dim() != 3 || t.size(1) != c.d / 2 || t.size(2) != 2 || !t.is_contiguous())
       refuse("rope_cs must be contiguous fp32 [max_pos, ", c.d / 2, ", 2] on cuda:", c.dev);
+    if (t.size(0) == 0) refuse("rope_cs holds no positions");  // (its null pointer would stand for no rotation)
     d.max_pos = i32(t.size(0), "max_pos"), d.rope_cs = static_cast<const float*>(t.const_data_ptr());
   }
   if (pos) d.pos = ints(c, *pos, "pos", rk.rows);

@@ -232,3 +232,10 @@ def test_scales_that_do_not_fit_are_refused():
                      lambda: ops.paged_attention(q, cache, cu, n, table, scale=scale)):
             with pytest.raises((ValueError, L.SvlaError), match="scale"):
                 call()
+
+
+def test_rotation_table_without_positions_is_refused():
+    kv = torch.zeros(4, 2, 64, dtype=BF16, device=DEV)
+    with pytest.raises((ValueError, L.SvlaError), match="rope_cs"):
+        ops.kv_append(ops.kv_cache(1, 16, 2, 64), kv, kv, ints([0, 4]).to(DEV), ints([4]).to(DEV), ints([[0]]).to(DEV),
+                      rope_cs=torch.zeros(0, 32, 2, device=DEV))
