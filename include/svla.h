@@ -361,7 +361,7 @@ int32_t svla_packed_attention(const svla_packed_attn_desc* desc, svla_stream_t s
  * ones sees entries n <= kv_len[b] - n_b + i, so the tokens themselves are appended first (svla_kv_append); of those, the
  * ones that can be read (inside the table, page inside the cache).  The workspace (256-byte aligned, at least
  * svla_paged_attention_workspace_size bytes, max_entries = max_pages * page_size; 0 bytes: none is needed) needs no
- * initialisation; calls that overlap on the GPU must not share one. */
+ * initialisation; calls that overlap on the GPU must not share one.  max_pages * page_size stays below 2^31 - 63. */
 size_t svla_paged_attention_workspace_size(int32_t batch, int32_t total_q, int32_t hq, int32_t hkv, int32_t head_dim,
                                            int64_t max_entries);
 

@@ -306,6 +306,8 @@ int32_t svla_paged_attention(const svla_paged_attn_desc* d, svla_stream_t stream
   if (int32_t rc = check_rows(who, "q", d->q, d->q_rs, qw)) return rc;
   if (int32_t rc = check_rows(who, "o", d->o, d->o_rs, qw)) return rc;
   const long long max_entries = static_cast<long long>(d->max_pages) * d->page_size;
+  if (max_entries > 0x7fffffffll - 63)  // entries, up to the end of a sequence's last tile, are numbered in 32 bits
+    return fail(SVLA_ERR_ARG, "%s: max_pages * page_size must stay below 2^31 - 63 (got %lld)", who, max_entries);
   const size_t need = svla_paged_attention_workspace_size(d->batch, d->total_q, d->hq, d->hkv, d->head_dim, max_entries);
   if (need && (!d->workspace || !aligned(d->workspace, 256) || d->workspace_bytes < need))
     return fail(SVLA_ERR_ARG, "%s: workspace must be 256-byte aligned with at least %zu bytes (got %zu)", who, need, d->workspace_bytes);

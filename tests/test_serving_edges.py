@@ -23,3 +23,12 @@ def test_scales_that_do_not_fit_are_refused(name, make, scale):
 def test_rotation_tables_are_made_on_a_gpu_only(table):
     with pytest.raises(ValueError, match="CUDA"):
         table(16, 10000.0, "cpu")
+
+
+def test_tables_that_reach_past_31_bits_are_refused():
+    """Entries are numbered in 32 bits, and a tile's last one may lie up to 63 behind the sequence's."""
+    lib = L.lib()
+    for pages, page in ((1 << 23, 256), (1 << 27, 16), ((1 << 31) - 1, 256)):
+        d = _paged(max_pages=pages, page_size=page, page_table_rs=1 << 31)
+        assert lib.svla_paged_attention(ctypes.byref(d), None) == 1
+        assert "max_pages" in lib.svla_last_error().decode()
