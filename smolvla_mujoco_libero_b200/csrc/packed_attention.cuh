@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
           if (key0 + n * 8 + 2 * t4 + (e & 1) >= sees[e >> 1]) s[n][e] = -INFINITY;
     }
     // The running maximum is lazy: it moves, and O is rescaled, only when a score of the warp passes its row's by more than
-    // 8 in log2 units (weights up to 2^8 of the maximum's cancel in O / l; fp16 holds them)
+    // 8 in log2 units (weights up to 2^8 of the maximum's cancel in O / l)
     float top[2];
     bool pass = false;
 #pragma unroll
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(packed_detail::kWarps * 32) packed_attention_k
         t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
         const float alpha = m[hr] == -INFINITY ? 1.f : ex2_approx(m[hr] - t);
         m[hr] = t;
-        use[hr] = t == -INFINITY ? 0.f : t;
+        use[hr] = t == -INFINITY ? 0.f : t - serving::kWeightLift<T>;
         l[hr] *= alpha;
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) {

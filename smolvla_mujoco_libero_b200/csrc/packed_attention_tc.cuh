@@ -95,7 +95,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// 2^z for two z <= 8 or so on the fp32 pipe, by Cody and Waite's reduction (Software manual for the elementary functions,
+// 2^z for two z <= 15 or so on the fp32 pipe, by Cody and Waite's reduction (Software manual for the elementary functions,
 // 1980): z = n + f with n = rint(z) (adding 1.5 * 2^23 leaves n in the low bits), 2^f by its minimax polynomial of degree 4
 // on [-1/2, 1/2] (relative error 2.6e-6, found by exchanging extrema), times 2^n.  z is first raised to at least -127, whose
 // power's exponent field is 0: a masked score's weight (z = -infinity), and every weight below 2^-126.5, is exactly 0, so
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(ptc::kThreads, 1) packed_attention_tc_kernel(c
             }
           }
         }
-        const float use = m == -INFINITY ? 0.f : m;
+        const float use = m == -INFINITY ? 0.f : m - serving::kWeightLift<T>;
         const float2 c2 = make_float2(c, c), nm2 = make_float2(-use, -use);
 #pragma unroll
         for (int ch = 0; ch < 4; ++ch) {

@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
               alpha = m[nt][u] == -INFINITY ? 1.f : ex2_approx(m[nt][u] - t);
             }
             m[nt][u] = t;
-            ref[nt][u] = t == -INFINITY ? 0.f : t;
+            ref[nt][u] = t == -INFINITY ? 0.f : t - (BITS == 16 ? serving::kWeightLift<T> : 0.f);
             l[nt][u] *= alpha;
             if constexpr (BITS == 4) {
               top[nt][u] = alpha;  // O follows below, with its factors

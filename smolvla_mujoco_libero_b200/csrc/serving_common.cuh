@@ -40,6 +40,15 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<__half2*>(&w));
 }
 
+// Softmax weights, rounded to the type for the second product, are 2^(score - maximum + lift); the lift cancels in O / l.
+// A lazy maximum lets them grow by 2^8, so fp16, which ends at 2^16, has room for 2^7: weights are rounded by 2^-11 of
+// themselves down to 2^-21 of the largest, and below by 2^-32 of the largest (half a subnormal step, 2^-25).  bf16 has
+// fp32's range.
+template <typename T>
+constexpr float kWeightLift = 0.f;
+template <>
+constexpr float kWeightLift<__half> = 7.f;
+
 // bits that are all ones in an infinity or a NaN of the type, for two packed values
 template <typename T>
 __device__ __forceinline__ bool any_nonfinite(uint32_t w);

@@ -61,6 +61,28 @@ def test_packed_attention_scores_of_minus_infinity(impl, heads, dtype, gone):
     within(got[some.to(DEV)], o[some], S.attention_tolerance(o, spread, size, dtype, d)[some])
 
 
+@pytest.mark.parametrize("impl", KERNELS)
+@pytest.mark.parametrize("heads", [(3, 1, 64), (4, 2, 128)], ids=str)
+def test_packed_attention_small_weights_beside_a_large_one(impl, heads):
+    """fp16: a first key with values of zero takes all but 2^-23.5 per key of the weight, and the rest of the weights make
+    the result.  Their rounding is the type's down to 2^-21 of the largest (oracle tolerance); below, half a subnormal step,
+    2^-25, of weights whose largest is 2^7 or more: 2^-32 of the largest for each key, times the largest value."""
+    hq, hkv, d, n = *heads, 900
+    q, kv = packed_inputs([n], [n], hq, hkv, d, FP16, seed=42)
+    q[:] = 0
+    q[..., 0] = 8.0
+    kv[:, :hkv, 0] = 0
+    kv[0, :hkv, 0] = 23.5 * math.log(2.0) * d ** 0.5 / 8.0
+    kv[:, hkv:] = 1 + kv[:, hkv:].abs()
+    kv[0, hkv:] = 0
+    o, spread, size = packed_reference(q, kv, [n], [n], True)
+    kvd = kv.to(DEV)
+    got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints([0, n]).to(DEV), impl=impl)
+    floor = n * 2.0 ** -32 * float(kv[:, hkv:].max())
+    # results of 1e-7 to 1e-3: the output's own half step is 2^-25 where it is subnormal
+    within(got, o, S.attention_tolerance(o, spread, size, FP16, d, floor=floor + 2.0 ** -25))
+
+
 # ----------------------------------------------------------------------------- paged attention
 
 def step_floor(q, cache, page, table, new, total):
@@ -160,6 +182,26 @@ def test_paged_attention_non_finite_group_leaves_the_others(heads, n, bad):
     for width in (None, 64):
         cache, table = cache_of(k.to(BF16), v.to(BF16), 16, width)
         check_groups(q, cache, 16, table, [1], [n], f"{n} entries")
+
+
+@pytest.mark.parametrize("heads", [(3, 1, 64), (8, 2, 128)], ids=str)
+@pytest.mark.parametrize("new", [1, 3])
+def test_paged_attention_small_weights_beside_a_large_one(heads, new):
+    """16 bits, fp16, as for packed prompts above: the floor is 2^-32 of the largest weight for each entry."""
+    hq, hkv, d, n, page = *heads, 900, 16
+    g = gen(61)
+    k, v = (torch.randn(n, hkv, d, generator=g) for _ in range(2))
+    k[..., 0], k[0, :, 0] = 0, 23.5 * math.log(2.0) * d ** 0.5 / 8.0
+    v = 1 + v.abs()
+    v[0] = 0
+    q = torch.zeros(new, hq, d, dtype=FP16)
+    q[..., 0] = 8.0
+    table, n_pages = make_table([n], page, 62)
+    cache = ops.kv_cache(n_pages, page, hkv, d, 16, FP16, device="cpu")
+    S.append(cache, page, k.half(), v.half(), [0, n], [n], table)
+    o, spread, size = paged_reference(q, cache, page, table, [new], [n])
+    got = ops.paged_attention(q.to(DEV), cache.to(DEV), ints([0, new]).to(DEV), ints([n]).to(DEV), table.to(DEV))
+    within(got, o, S.attention_tolerance(o, spread, size, FP16, d, floor=n * 2.0 ** -32 * float(v.max()) + 2.0 ** -25))
 
 
 @pytest.mark.parametrize("heads", [(3, 1, 64), (8, 2, 128)], ids=str)
