@@ -322,9 +322,10 @@ int32_t svla_rope_table_wide(float* cs, int32_t max_pos, int32_t head_dim, doubl
  * sequence b becomes entry kv_len[b] - n_b + i (kv_len counts them).  With rope_cs ([max_pos][head_dim / 2] (cos, sin),
  * svla_rope_table_wide) keys and, if given, queries are rotated (rotate-half, fp32) at position pos[t], or the entry's
  * index without pos; positions are clamped to 0 .. max_pos - 1.  4 bits, per 32 dimensions: low = bf16(min), step =
- * bf16((max - min) / 15), code = round((x - low) / step) clamped to 0 .. 15; a group with an infinity or a NaN reads
- * back as NaN.  k_out / v_out (or NULL): the appended rows as the cache holds them, rounded to the dtype, packed like
- * k / v.  q_out, k_out, v_out may alias q, k, v.  Two tokens must not share an entry. */
+ * bf16((max - min) / 15), code = round((x - low) / step) clamped to 0 .. 15; a value is off by at most
+ * step / 2 + |low| 2^-8 + 15 step 2^-8, and a group with an infinity, a NaN or a range beyond fp32's reads back as NaN.
+ * k_out / v_out (or NULL): the appended rows as the cache holds them, rounded to the dtype, packed like k / v.  q_out,
+ * k_out, v_out may alias q, k, v.  Two tokens must not share an entry. */
 typedef struct svla_kv_append_desc {
   const void* q; const void* k; const void* v;   /* packed; q may be NULL */
   void* q_out; void* k_out; void* v_out;

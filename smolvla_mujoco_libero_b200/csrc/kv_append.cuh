@@ -11,10 +11,12 @@
 // pairs [page][D / 32].  Per group of 32 dimensions
 //   low = bf16(min),  step = bf16((max - min) / 15),  code = clamp(rint((x - low) / step), 0, 15)   (0 for step 0)
 // and the entry stands for low + step * code.  A linear code with its own offset spends all 16 codes on the group's
-// range; the codes are computed against the rounded pair that the reader sees, so rounding the pair to bf16 (2^-9 of
-// its size) costs no more than a few hundredths of a step.  Both quotients are true divisions: bf16 inputs often lie
-// exactly between two codes, and a reciprocal's last bit would then decide.  A group with a NaN or an infinity reads
-// back as NaN.
+// range, and the codes are computed against the rounded pair that the reader sees.  An entry is off by half a step where
+// its code is not clamped; rounding the pair to bf16 moves the ends of the range by 2^-8 |low| at the lower and by 2^-8 |low|
+// + 15 steps 2^-8 at the upper, and what lies beyond them is clamped.  So a group whose offset is large beside its range
+// loses more: 100.2 to 101.2 has step 0.067 and low 100, and its largest value reads back as 101, three steps off.  Both
+// quotients are true divisions: bf16 inputs often lie exactly between two codes, and a reciprocal's last bit would then
+// decide.  A group with a NaN, an infinity or a range beyond fp32's largest number reads back as NaN.
 //
 // Work split: a warp takes one token and, when there are few tokens, a share of its heads; D / 16 lanes hold a head's row (8
 // dimensions of each half), so a warp's accesses are whole 128- or 256-byte rows, the rotation pairs meet in one lane, the

@@ -263,6 +263,28 @@ def test_paged_attention_limit_counts_entries_past_the_table(bits):
     within(got, o, paged_tolerance(o, spread, size, BF16, 64, bits, [48], 1.0))
 
 
+# ----------------------------------------------------------------------------- appending
+
+@pytest.mark.parametrize("heads", [(2, 64), (2, 128)], ids=str)
+def test_kv_append_of_groups_with_an_offset_or_a_huge_range(heads):
+    """4 bits: bytes and rows as the same fp32 operations give them, with an offset beside the range and a range beyond
+    fp32's largest number."""
+    hkv, d, n, page = *heads, 40, 16
+    k = torch.rand(n, hkv, d, generator=gen(63)) + torch.tensor([100.0, -100.0, 1000.0, 0.0]).repeat(n // 4)[:, None, None]
+    k, v = k.to(BF16), (k.flip(0) * 3).to(BF16)
+    v[7, 0, 0], v[7, 0, 1] = -3e38, 3e38
+    table, n_pages = make_table([n], page, 64)
+    cache = ops.kv_cache(n_pages, page, hkv, d, 4, device=DEV)
+    want = cache.cpu().clone()
+    _, rk, rv = S.append(want, page, k, v, [0, n], [n], table)
+    _, gk, gv = ops.kv_append(cache, k.to(DEV), v.to(DEV), ints([0, n]).to(DEV), ints([n]).to(DEV), table.to(DEV), want_rows=True)
+    assert torch.equal(cache.cpu(), want)
+    assert torch.equal(gk.cpu(), rk)
+    nan = torch.isnan(rv)
+    assert bool(nan[7, 0, :32].all()) and int(nan.sum()) == 32
+    assert torch.equal(torch.isnan(gv).cpu(), nan) and torch.equal(gv.cpu()[~nan], rv[~nan])
+
+
 # ----------------------------------------------------------------------------- arguments
 
 def test_scales_that_do_not_fit_are_refused():

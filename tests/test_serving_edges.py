@@ -5,7 +5,9 @@ import ctypes
 import math
 
 import pytest
+import torch
 
+from oracle import serving as S
 from smolvla_mujoco_libero_b200 import _lib as L
 from smolvla_mujoco_libero_b200 import ops
 from tests.test_serving import _packed, _paged
@@ -32,3 +34,24 @@ def test_tables_that_reach_past_31_bits_are_refused():
         d = _paged(max_pages=pages, page_size=page, page_table_rs=1 << 31)
         assert lib.svla_paged_attention(ctypes.byref(d), None) == 1
         assert "max_pages" in lib.svla_last_error().decode()
+
+
+@pytest.mark.parametrize("offset,spread", [(100.0, 1.0), (-100.0, 1.0), (1000.0, 0.5), (0.0, 1.0)])
+def test_plain_quantisation_of_groups_with_an_offset(offset, spread):
+    """step / 2 + |low| 2^-8 + 15 step 2^-8, as the header states it.  Both pairs enter rounded: by at most 2^-8 of
+    themselves, which 1 / (1 - 2^-8) covers; 1e-6 of the size for fp32's own roundings."""
+    x = offset + spread * torch.rand(200, 128, generator=torch.Generator().manual_seed(6))
+    codes, step, low = S.quantise(x)
+    err = (S.held(codes, step, low) - x).abs().unflatten(-1, (-1, 32))
+    s, m = step.float().unsqueeze(-1), low.float().abs().unsqueeze(-1)
+    bound = s / 2 + (m + 15 * s) * 2.0 ** -8 / (1 - 2.0 ** -8) + 1e-6 * (m + 15 * s)
+    assert bool((err <= bound).all())
+    if offset:  # the offset costs whole steps
+        assert float((err / s).max()) > 2
+
+
+def test_plain_quantisation_of_a_range_beyond_fp32():
+    x = torch.zeros(1, 64)
+    x[0, 0], x[0, 1] = -3e38, 3e38
+    held = S.held(*S.quantise(x))
+    assert bool(torch.isnan(held[0, :32]).all()) and bool((held[0, 32:] == 0).all())
