@@ -233,9 +233,13 @@ def serving():
     """The torch side of the serving operators (csrc/torch_serving.cpp), bound to the loaded library once."""
     global _serving
     if _serving is None:
+        from . import build
         handle = lib()
         if not TORCH_PATH.exists():
             raise SvlaError(f"{TORCH_PATH} is missing: build it with `python -m smolvla_mujoco_libero_b200.build`")
+        if not build.torch_module_fits():
+            raise SvlaError(f"{TORCH_PATH} was built for another torch or Python (not {build.torch_tag()}): rebuild it with "
+                            "`python -m smolvla_mujoco_libero_b200.build`")
         from . import _torch_serving as module
         module.bind(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in (
             "svla_kv_append", "svla_packed_attention", "svla_paged_attention", "svla_paged_attention_workspace_size")))

@@ -58,13 +58,28 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(p.stat().st_mtime > t for p in deps)
 
 
+def torch_tag() -> str:
+    """What _torch_serving.so is bound to; the module holds it as a string."""
+    import torch
+    return f"built for torch {torch.__version__}, {sys.implementation.cache_tag}"
+
+
+def torch_module_fits() -> bool:
+    """Whether _torch_serving.so is one of this torch and Python; it is read, not loaded."""
+    return TORCH_OUT.exists() and torch_tag().encode() + b"\0" in TORCH_OUT.read_bytes()
+
+
+def _torch_current() -> bool:
+    return not _stale(TORCH_OUT, [TORCH_SRC, HEADER]) and torch_module_fits()
+
+
 def up_to_date() -> bool:
-    return not _stale(OUT, [p for p in sources() if p != TORCH_SRC]) and not _stale(TORCH_OUT, [TORCH_SRC, HEADER])
+    return not _stale(OUT, [p for p in sources() if p != TORCH_SRC]) and _torch_current()
 
 
 def build_torch(force: bool = False) -> Path:
     """_torch_serving.so: a Python module against this torch's headers (no device code)."""
-    if not force and not _stale(TORCH_OUT, [TORCH_SRC, HEADER]):
+    if not force and _torch_current():
         return TORCH_OUT
     import torch
 
@@ -76,6 +91,7 @@ def build_torch(force: bool = False) -> Path:
     # whose stream facets do not mix with it)
     subprocess.run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared",
                     f"-DTORCH_EXTENSION_NAME={TORCH_OUT.stem}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                    f'-DSVLA_TORCH_TAG="{torch_tag()}"',
                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                     *[a for p in include for a in ("-isystem", str(p))], "-o", str(TORCH_OUT), str(TORCH_SRC),
                     f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"], check=True)

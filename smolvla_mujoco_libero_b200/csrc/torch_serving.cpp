@@ -244,6 +244,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& cache, const Tensor& cu_q,
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.attr("__doc__") = SVLA_TORCH_TAG;  // build.py looks for it in the file
   m.def("bind", &bind);
   m.def("kv_append", &kv_append);
   m.def("packed_attention", &packed_attention);

@@ -9,7 +9,7 @@ import torch
 
 from oracle import serving as S
 from smolvla_mujoco_libero_b200 import _lib as L
-from smolvla_mujoco_libero_b200 import ops
+from smolvla_mujoco_libero_b200 import build, ops
 from tests.test_serving import _packed, _paged
 
 
@@ -55,3 +55,14 @@ def test_plain_quantisation_of_a_range_beyond_fp32():
     x[0, 0], x[0, 1] = -3e38, 3e38
     held = S.held(*S.quantise(x))
     assert bool(torch.isnan(held[0, :32]).all()) and bool((held[0, 32:] == 0).all())
+
+
+def test_module_of_another_torch_is_noticed(monkeypatch):
+    """The torch side is bound to the torch and the Python it was built with: another one's is rebuilt by the build, and
+    refused, not loaded, at the first call."""
+    assert build.torch_module_fits()
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + "1")
+    assert not build.torch_module_fits() and not build.up_to_date()
+    monkeypatch.setattr(L, "_serving", None)
+    with pytest.raises(L.SvlaError, match="another torch"):
+        L.serving()
