@@ -83,6 +83,18 @@ def test_packed_attention_small_weights_beside_a_large_one(impl, heads):
     within(got, o, S.attention_tolerance(o, spread, size, FP16, d, floor=floor + 2.0 ** -25))
 
 
+@pytest.mark.parametrize("impl", KERNELS)
+@pytest.mark.parametrize("heads", [(15, 5, 64), (8, 2, 128)], ids=str)
+def test_packed_attention_one_long_prompt_among_many_short_ones(impl, heads):
+    hq, hkv, d = heads
+    lens = [5] * 60 + [1500] + [5] * 67
+    q, kv = packed_inputs(lens, lens, hq, hkv, d, BF16, seed=43)
+    o, spread, size = packed_reference(q, kv, lens, lens, True)
+    kvd = kv.to(DEV)
+    got = ops.packed_attention(q.to(DEV), kvd[:, :hkv], kvd[:, hkv:], ints(starts(lens)).to(DEV), impl=impl)
+    within(got, o, S.attention_tolerance(o, spread, size, BF16, d))
+
+
 # ----------------------------------------------------------------------------- paged attention
 
 def step_floor(q, cache, page, table, new, total):
