@@ -17,14 +17,16 @@
 // makes two MMA operands.  With k = low + step c per group of 32 dimensions
 //   q . k = sum_g step_g (sum_{d in g} q_d c_d) + low_g (sum_{d in g} q_d)
 // needs one accumulator per group and two FMAs per score, and
-//   sum_n p_n v_n = sum_n (p_n step_n) c_n + sum_n p_n low_n
-// takes p_n step_n as the other operand.  Query rows are scaled by a power of two to the top of fp16's range (exact but
+//   sum_n p_n v_n = sum_n (p_n step_n) (c_n - 8) + sum_n p_n (low_n + 8 step_n)
+// takes p_n step_n as the other operand, the 8 through a product with a constant row: what rounding p_n step_n to fp16 costs
+// is multiplied by a distance from the middle of the group's range, not by one from its end (fp16 results 3.0e-4 off
+// instead of 5.3e-4, relative; their own rounding is 2.1e-4).  Query rows are scaled by a power of two to the top of fp16's range (exact but
 // for components below 2^-25 of the row's largest), so bf16 queries lose nothing.  p_n step_n is rounded to fp16, 2^-11
 // relative.  Every query column and group has a power of two of its own that brings the largest p_n step_n so far to 2^2,
 // so that groups of different size, and large entries of little weight, leave the others their bits; what is smaller than
 // 2^-16 of the largest is off by 2^-27 of it (half a subnormal step).  These factors move with the maximum, or when a step
 // reaches a limit below which nothing can leave fp16's range; what a tile costs for them otherwise is a comparison and one
-// product per weight.  Products with low_n stay in fp32.
+// product per weight.  The second sum stays in fp32.
 //
 // Every warp works alone: its own tiles of 16 to 64 entries through its own ring of asynchronous copies, its own running
 // maximum, sum and O, no barrier in the loop.  The maximum is lazy: it moves (and O is rescaled) only when a score
@@ -414,7 +416,8 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       }
 
     float o[NT][D / 16][4];     // O^T: see the P.V product for which dimensions a thread holds
-    float om[NT][kGroups][2];   // 4 bits: sums of p low
+    float om[NT][kGroups][2];   // 4 bits: sums of p (low + 8 step)
+    float z[NT][kGroups / 2][4];  // 4 bits: sums of the rounded weights, times 8, of an even and of the next group
     float m[NT][2], ref[NT][2], l[NT][2];
 #pragma unroll
     for (int gr = 0; gr < kGroups; ++gr) limit[gr] = step_limit(kWeightFactorTop);
@@ -426,6 +429,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       for (int gr = 0; gr < kGroups; ++gr) {
         om[nt][gr][0] = om[nt][gr][1] = 0.f;
         f[nt][gr] = make_float2(kWeightFactorTop, kWeightFactorTop);
+        z[nt][gr / 2][2 * (gr & 1)] = z[nt][gr / 2][2 * (gr & 1) + 1] = 0.f;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) m[nt][u] = -INFINITY, ref[nt][u] = 0.f, l[nt][u] = 0.f;
@@ -499,17 +503,17 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             uint32_t kp[kGroups];
             load_pairs(kp, st + Tl::kKP + (sl * 16 + g8 + 8 * hr) * Tl::kPairs);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
+              float2 dot = make_float2(0.f, 0.f), add = dot;
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                float dot = 0.f, add = 0.f;
-#pragma unroll
-                for (int gr = 0; gr < kGroups; ++gr) {
-                  dot = fmaf(__uint_as_float(kp[gr] << 16), acc[nt][gr][2 * hr + u], dot);
-                  add = fmaf(__uint_as_float(kp[gr] & 0xFFFF0000u), qs[nt][gr][u], add);
-                }
-                s[nt][sl][2 * hr + u] = fmaf(dot, qf[nt][u], add);
+              for (int gr = 0; gr < kGroups; ++gr) {
+                const float step = __uint_as_float(kp[gr] << 16), low = __uint_as_float(kp[gr] & 0xFFFF0000u);
+                dot = __ffma2_rn(make_float2(step, step), make_float2(acc[nt][gr][2 * hr], acc[nt][gr][2 * hr + 1]), dot);
+                add = __ffma2_rn(make_float2(low, low), make_float2(qs[nt][gr][0], qs[nt][gr][1]), add);
               }
+              const float2 x = __ffma2_rn(dot, make_float2(qf[nt][0], qf[nt][1]), add);
+              s[nt][sl][2 * hr] = x.x, s[nt][sl][2 * hr + 1] = x.y;
+            }
           }
         }
       }
@@ -589,14 +593,20 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       }
       // ---- probabilities
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        const float2 shift = make_float2(-ref[nt][0], -ref[nt][1]);
+        float2 sum = make_float2(l[nt][0], l[nt][1]);
 #pragma unroll
         for (int sl = 0; sl < kSlabs; ++sl)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            s[nt][sl][x] = ex2_approx(s[nt][sl][x] - ref[nt][x & 1]);
-            l[nt][x & 1] += s[nt][sl][x];
+          for (int hr = 0; hr < 2; ++hr) {
+            const float2 x = __fadd2_rn(make_float2(s[nt][sl][2 * hr], s[nt][sl][2 * hr + 1]), shift);
+            const float2 p = make_float2(ex2_approx(x.x), ex2_approx(x.y));
+            sum = __fadd2_rn(sum, p);
+            s[nt][sl][2 * hr] = p.x, s[nt][sl][2 * hr + 1] = p.y;
           }
+        l[nt][0] = sum.x, l[nt][1] = sum.y;
+      }
       // ---- 4 bits: the weights' factors
       if constexpr (BITS == 4) {
         if (moves) {
@@ -647,6 +657,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
                 o[nt][i2][0] *= r.x, o[nt][i2][1] *= r.y;
                 o[nt][i2][2] *= r.x, o[nt][i2][3] *= r.y;
               }
+              z[nt][gr / 2][2 * (gr & 1)] *= r.x, z[nt][gr / 2][2 * (gr & 1) + 1] *= r.y;
             }
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
@@ -720,7 +731,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
 #pragma unroll
               for (int gr = 0; gr < kGroups; ++gr) {
                 // whatever stands in an entry that nobody sees counts nothing; a pair that is no number, of an entry
-                // that some rows see: those get their NaN through the sum of p low (p = 0 would not keep it from the
+                // that some rows see: those get their NaN through the sum in fp32 (p = 0 would not keep it from the
                 // others), and the codes count nothing
                 const bool none = n >= sees_last || ((gone >> sl) & 1u);
                 const bool fine = isfinite(__uint_as_float(vp[gr] << 16)) && isfinite(__uint_as_float(vp[gr] & 0xFFFF0000u));
@@ -741,8 +752,9 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
                 const float step = __uint_as_float(vp[gr] << 16), low = __uint_as_float(vp[gr] & 0xFFFF0000u);
                 const float2 p = make_float2(s[nt][sl][2 * hr], s[nt][sl][2 * hr + 1]);
                 const float2 y = __fmul2_rn(p, __fmul2_rn(make_float2(step, step), f[nt][gr]));
-                om[nt][gr][0] = fmaf(p.x, low, om[nt][gr][0]);
-                om[nt][gr][1] = fmaf(p.y, low, om[nt][gr][1]);
+                const float middle = fmaf(8.f, step, low);
+                const float2 sum = __ffma2_rn(p, make_float2(middle, middle), make_float2(om[nt][gr][0], om[nt][gr][1]));
+                om[nt][gr][0] = sum.x, om[nt][gr][1] = sum.y;
                 pb[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(y.x, y.y));
               }
           }
@@ -764,8 +776,12 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             const uint32_t a1[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
+              // rows g8 of the constant operand: 8 for an even group, rows g8 + 8: for an odd one
+              constexpr uint32_t k8 = 0x00080008u;
+              const uint32_t az[4] = {gr & 1 ? 0u : k8, gr & 1 ? k8 : 0u, gr & 1 ? 0u : k8, gr & 1 ? k8 : 0u};
               mma16816<__half>(o[nt][2 * gr], a0, pb[nt][gr][0], pb[nt][gr][1]);
               mma16816<__half>(o[nt][2 * gr + 1], a1, pb[nt][gr][0], pb[nt][gr][1]);
+              mma16816<__half>(z[nt][gr / 2], az, pb[nt][gr][0], pb[nt][gr][1]);
             }
           }
         }
@@ -805,8 +821,9 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             // 2^24 undoes the codes' subnormals, odd dimensions counted 16 times
             const int d = (mt >> 1) * 32 + 4 * g8 + 2 * (mt & 1);
             const float back = power_inverse(u ? f[nt][mt >> 1].y : f[nt][mt >> 1].x);
-            js[r * (D + 1) + d] = fmaf(o[nt][mt][u] * 16777216.f, back, om[nt][mt >> 1][u]);
-            js[r * (D + 1) + d + 1] = fmaf(o[nt][mt][2 + u] * 1048576.f, back, om[nt][mt >> 1][u]);
+            const float mid = z[nt][mt >> 2][2 * ((mt >> 1) & 1) + u];
+            js[r * (D + 1) + d] = fmaf((o[nt][mt][u] - mid) * 16777216.f, back, om[nt][mt >> 1][u]);
+            js[r * (D + 1) + d + 1] = fmaf(fmaf(o[nt][mt][2 + u], 0.0625f, -mid) * 16777216.f, back, om[nt][mt >> 1][u]);
           }
         }
       }
