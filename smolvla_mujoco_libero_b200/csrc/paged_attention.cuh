@@ -20,13 +20,16 @@
 //   sum_n p_n v_n = sum_n (p_n step_n) (c_n - 8) + sum_n p_n (low_n + 8 step_n)
 // takes p_n step_n as the other operand, the 8 through a product with a constant row: what rounding p_n step_n to fp16 costs
 // is multiplied by a distance from the middle of the group's range, not by one from its end (fp16 results 3.0e-4 off
-// instead of 5.3e-4, relative; their own rounding is 2.1e-4).  Query rows are scaled by a power of two to the top of fp16's range (exact but
-// for components below 2^-25 of the row's largest), so bf16 queries lose nothing.  p_n step_n is rounded to fp16, 2^-11
-// relative.  Every query column and group has a power of two of its own that brings the largest p_n step_n so far to 2^2,
-// so that groups of different size, and large entries of little weight, leave the others their bits; what is smaller than
-// 2^-16 of the largest is off by 2^-27 of it (half a subnormal step).  These factors move with the maximum, or when a step
-// reaches a limit below which nothing can leave fp16's range; what a tile costs for them otherwise is a comparison and one
-// product per weight.  The second sum stays in fp32.
+// instead of 5.3e-4, relative; their own rounding is 2.1e-4).  Query rows are scaled by a power of two to the top of
+// fp16's range (exact but for components below 2^-25 of the row's largest), so bf16 queries lose nothing.
+//
+// p_n step_n is rounded to fp16, 2^-11 relative.  Every query column and group has a power of two of its own that brings
+// the largest p_n step_n so far to 2^2, so that groups of different size, and large entries of little weight, leave the
+// others their bits; what is smaller than 2^-16 of the largest is off by 2^-27 of it (half a subnormal step).  These
+// factors move with the maximum, or when a step reaches a limit below which nothing can leave fp16's range; what a tile
+// costs for them otherwise is a comparison and one product per weight.  Steps that vary by a factor of 4.5 (a standard
+// deviation) from entry to entry reach it all the time: 48 and 92 us instead of 44 and 71 for the shapes below.  The second
+// sum stays in fp32.
 //
 // Every warp works alone: its own tiles of 16 to 64 entries through its own ring of asynchronous copies, its own running
 // maximum, sum and O, no barrier in the loop.  The maximum is lazy: it moves (and O is rescaled) only when a score
@@ -634,7 +637,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             }
 #pragma unroll
           for (int gr = 0; gr < kGroups; ++gr) {
-            float most = 0.f;
+            float most = 0.f;  // of the columns that see something: the others' weights are zeros
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               // both columns' upper halves in one word
@@ -650,7 +653,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
               const float2 a2 = make_float2(top[nt][0], top[nt][1]), was = f[nt][gr];
               const float2 now = make_float2(next(both >> 7, was.x, a2.x), next(both >> 23, was.y, a2.y));
               f[nt][gr] = now;
-              most = fmaxf(most, fmaxf(now.x, now.y));
+              most = fmaxf(most, fmaxf(m[nt][0] == -INFINITY ? 0.f : now.x, m[nt][1] == -INFINITY ? 0.f : now.y));
               const float2 r = __fmul2_rn(__fmul2_rn(now, a2), make_float2(power_inverse(was.x), power_inverse(was.y)));
 #pragma unroll
               for (int i2 = 2 * gr; i2 < 2 * gr + 2; ++i2) {
