@@ -3,7 +3,7 @@
 //   o_i = sum_n softmax_n(scale q_i . k_n) v_n      (zeros where no entry weighs anything: none to see, none whose page
 // is there, or every score -infinity).
 //
-// Bound by the bytes of the live cache; the work around them has to stay below what an SM issues in the time they
+// The floor is the bytes of the live cache; the work around them has to stay below what an SM issues in the time they
 // take (4 bits, D = 64: 1280 bytes, 55 cycles, per 16 entries of one head).
 //
 // Shape of the products.  Entries are the M side: S^T (16 entries x 8 query rows) = K Q^T, O^T (16 dimensions x 8 query
@@ -17,19 +17,19 @@
 // makes two MMA operands.  With k = low + step c per group of 32 dimensions
 //   q . k = sum_g step_g (sum_{d in g} q_d c_d) + low_g (sum_{d in g} q_d)
 // needs one accumulator per group and two FMAs per score, and
-//   sum_n p_n v_n = sum_n (p_n step_n) (c_n - 8) + sum_n p_n (low_n + 8 step_n)
-// takes p_n step_n as the other operand, the 8 through a product with a constant row: what rounding p_n step_n to fp16 costs
-// is multiplied by a distance from the middle of the group's range, not by one from its end (fp16 results 3.0e-4 off
-// instead of 5.3e-4, relative; their own rounding is 2.1e-4).  Query rows are scaled by a power of two to the top of
-// fp16's range (exact but for components below 2^-25 of the row's largest), so bf16 queries lose nothing.
+//   sum_n p_n v_n = sum_n (p_n step_n) c_n + sum_n p_n low_n
+// takes p_n step_n as the other operand.  Query rows are scaled by a power of two to the top of fp16's range (exact but
+// for components below 2^-25 of the row's largest), so bf16 queries lose nothing.
 //
-// p_n step_n is rounded to fp16, 2^-11 relative.  Every query column and group has a power of two of its own that brings
-// the largest p_n step_n so far to 2^2, so that groups of different size, and large entries of little weight, leave the
-// others their bits; what is smaller than 2^-16 of the largest is off by 2^-27 of it (half a subnormal step).  These
-// factors move with the maximum, or when a step reaches a limit below which nothing can leave fp16's range; what a tile
-// costs for them otherwise is a comparison and one product per weight.  Steps that vary by a factor of 4.5 (a standard
-// deviation) from entry to entry reach it all the time: 48 and 92 us instead of 44 and 71 for the shapes below.  The second
-// sum stays in fp32.
+// p_n step_n is rounded to fp16, 2^-11 relative, less than a bf16 result's own rounding (1.75e-3 off instead of 1.67e-3 with
+// exact weights).  For fp16 results, which it would move from 2.1e-4 to 5.3e-4, what the rounding left is a second operand of
+// the same products: 46.0 and 77.3 us instead of 42.3 and 67.0 for the shapes below.  Every query column and group has a
+// power of two of its own that brings the largest p_n step_n so far to 2^2, so that groups of different size, and large
+// entries of little weight, leave the others their bits; what is smaller than 2^-16 of the largest is off by 2^-27 of it
+// (half a subnormal step).  These factors move with the maximum, or when a step reaches a limit below which nothing can
+// leave fp16's range; what a tile costs for them otherwise is a comparison and one product per weight.  Steps that vary by a
+// factor of 4.5 (a standard deviation) from entry to entry reach it all the time: 46 and 86 us.  The products with low_n
+// stay in fp32.
 //
 // Every warp works alone: its own tiles of 16 to 64 entries through its own ring of asynchronous copies, its own running
 // maximum, sum and O, no barrier in the loop.  The maximum is lazy: it moves (and O is rescaled) only when a score
@@ -43,12 +43,17 @@
 // lies in one CTA is finished there; one cut by a piece's border leaves partials (maximum, sum, O in fp32) in the
 // workspace, which the combine kernel joins in the line's order, so results do not depend on timing.
 //
-// Measured, both kernels, 4 bits: 64 single tokens at D = 64 over 255 to 8191 entries (118 MB) 41 us, 2.9 TB/s (2 or 4
-// CTAs per SM instead of 3: 46 and 44; no cost per item: 55; 384 or 1024 entries per item: 44 and 43); two of D = 128
-// over 100000 to 131071 (291 MB) 68 us, 4.3 TB/s.  16 bits, 24 x 5 tokens over 100 to 4000 (65 MB): 23 us, 2.9 TB/s.
-// Of the 41 us about 12 go to the start of a piece and of its items (place, pages, first copies, queries, each from cold
-// code), 3 to the join, the rest to the tiles: 300 cycles per 16 entries and scheduler, of which the products take 75.
+// Measured, both kernels, bf16, 4 bits: 64 single tokens at D = 64 over 255 to 8191 entries (118 MB) 42.3 us, 2.8 TB/s; two
+// of D = 128 over 100000 to 131071 (291 MB) 67.0 us, 4.3 TB/s.  16 bits: 24 x 5 tokens over 100 to 4000 (65 MB) 21.5 us,
+// 3.0 TB/s; single tokens as above 65 us (376 MB, 5.8 TB/s) and 145 us (930 MB, 6.4 TB/s: what the memory gives).  The first
+// shape with 2 or 4 CTAs per SM instead of 3: 46 and 44 us; no cost per item: 55; 384 or 1024 entries per item: 44 and 43.
+// What bounds 4 bits is the latency of dependent instructions with two or three warps per scheduler (issue slots 53% busy,
+// DRAM 35 and 50%); time stamps gave about 12 us of the first shape to the start of a piece and of its items (place, pages,
+// first copies, queries, each from cold code), 3 to the join, the rest to the tiles: 300 cycles per 16 entries and
+// scheduler, of which the products take 75.
 #pragma once
+
+#include <type_traits>
 
 #include "serving_common.cuh"
 
@@ -419,8 +424,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       }
 
     float o[NT][D / 16][4];     // O^T: see the P.V product for which dimensions a thread holds
-    float om[NT][kGroups][2];   // 4 bits: sums of p (low + 8 step)
-    float z[NT][kGroups / 2][4];  // 4 bits: sums of the rounded weights, times 8, of an even and of the next group
+    float om[NT][kGroups][2];   // 4 bits: sums of p low
     float m[NT][2], ref[NT][2], l[NT][2];
 #pragma unroll
     for (int gr = 0; gr < kGroups; ++gr) limit[gr] = step_limit(kWeightFactorTop);
@@ -432,7 +436,6 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       for (int gr = 0; gr < kGroups; ++gr) {
         om[nt][gr][0] = om[nt][gr][1] = 0.f;
         f[nt][gr] = make_float2(kWeightFactorTop, kWeightFactorTop);
-        z[nt][gr / 2][2 * (gr & 1)] = z[nt][gr / 2][2 * (gr & 1) + 1] = 0.f;
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) m[nt][u] = -INFINITY, ref[nt][u] = 0.f, l[nt][u] = 0.f;
@@ -660,7 +663,6 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
                 o[nt][i2][0] *= r.x, o[nt][i2][1] *= r.y;
                 o[nt][i2][2] *= r.x, o[nt][i2][3] *= r.y;
               }
-              z[nt][gr / 2][2 * (gr & 1)] *= r.x, z[nt][gr / 2][2 * (gr & 1) + 1] *= r.y;
             }
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
             most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
@@ -724,7 +726,9 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
       } else {
 #pragma unroll
         for (int sl = 0; sl < kSlabs; ++sl) {
-          uint32_t pb[NT][kGroups][2];
+          // fp16 callers: what the rounding of the weights to fp16 left goes through the products as well
+          constexpr bool kRest = std::is_same<T, __half>::value;
+          uint32_t pb[NT][kGroups][2], pr[NT][kRest ? kGroups : 1][2];
 #pragma unroll
           for (int hr = 0; hr < 2; ++hr) {
             uint32_t vp[kGroups];
@@ -734,7 +738,7 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
 #pragma unroll
               for (int gr = 0; gr < kGroups; ++gr) {
                 // whatever stands in an entry that nobody sees counts nothing; a pair that is no number, of an entry
-                // that some rows see: those get their NaN through the sum in fp32 (p = 0 would not keep it from the
+                // that some rows see: those get their NaN through the sum of p low (p = 0 would not keep it from the
                 // others), and the codes count nothing
                 const bool none = n >= sees_last || ((gone >> sl) & 1u);
                 const bool fine = isfinite(__uint_as_float(vp[gr] << 16)) && isfinite(__uint_as_float(vp[gr] & 0xFFFF0000u));
@@ -755,10 +759,14 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
                 const float step = __uint_as_float(vp[gr] << 16), low = __uint_as_float(vp[gr] & 0xFFFF0000u);
                 const float2 p = make_float2(s[nt][sl][2 * hr], s[nt][sl][2 * hr + 1]);
                 const float2 y = __fmul2_rn(p, __fmul2_rn(make_float2(step, step), f[nt][gr]));
-                const float middle = fmaf(8.f, step, low);
-                const float2 sum = __ffma2_rn(p, make_float2(middle, middle), make_float2(om[nt][gr][0], om[nt][gr][1]));
+                const float2 sum = __ffma2_rn(p, make_float2(low, low), make_float2(om[nt][gr][0], om[nt][gr][1]));
                 om[nt][gr][0] = sum.x, om[nt][gr][1] = sum.y;
-                pb[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(y.x, y.y));
+                const uint32_t yh = serving::pack2<__half>(y.x, y.y);
+                pb[nt][gr][hr] = serving::movmatrix_trans(yh);
+                if constexpr (kRest) {
+                  const float2 f2 = serving::unpack2<__half>(yh), rest = __fadd2_rn(y, make_float2(-f2.x, -f2.y));
+                  pr[nt][gr][hr] = serving::movmatrix_trans(serving::pack2<__half>(rest.x, rest.y));
+                }
               }
           }
           // the half word g8 of each group's codes (dimensions 4 g8 .. + 3), of entries 2 t4 and 2 t4 + 1 (and + 8) in one
@@ -779,12 +787,12 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             const uint32_t a1[4] = {y0 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x000F000Fu, y1 & 0x00F000F0u};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              // rows g8 of the constant operand: 8 for an even group, rows g8 + 8: for an odd one
-              constexpr uint32_t k8 = 0x00080008u;
-              const uint32_t az[4] = {gr & 1 ? 0u : k8, gr & 1 ? k8 : 0u, gr & 1 ? 0u : k8, gr & 1 ? k8 : 0u};
               mma16816<__half>(o[nt][2 * gr], a0, pb[nt][gr][0], pb[nt][gr][1]);
               mma16816<__half>(o[nt][2 * gr + 1], a1, pb[nt][gr][0], pb[nt][gr][1]);
-              mma16816<__half>(z[nt][gr / 2], az, pb[nt][gr][0], pb[nt][gr][1]);
+              if constexpr (kRest) {
+                mma16816<__half>(o[nt][2 * gr], a0, pr[nt][gr][0], pr[nt][gr][1]);
+                mma16816<__half>(o[nt][2 * gr + 1], a1, pr[nt][gr][0], pr[nt][gr][1]);
+              }
             }
           }
         }
@@ -824,9 +832,8 @@ __global__ void __launch_bounds__(paged_detail::kWarps * 32, (D == 64 && NT == 1
             // 2^24 undoes the codes' subnormals, odd dimensions counted 16 times
             const int d = (mt >> 1) * 32 + 4 * g8 + 2 * (mt & 1);
             const float back = power_inverse(u ? f[nt][mt >> 1].y : f[nt][mt >> 1].x);
-            const float mid = z[nt][mt >> 2][2 * ((mt >> 1) & 1) + u];
-            js[r * (D + 1) + d] = fmaf((o[nt][mt][u] - mid) * 16777216.f, back, om[nt][mt >> 1][u]);
-            js[r * (D + 1) + d + 1] = fmaf(fmaf(o[nt][mt][2 + u], 0.0625f, -mid) * 16777216.f, back, om[nt][mt >> 1][u]);
+            js[r * (D + 1) + d] = fmaf(o[nt][mt][u] * 16777216.f, back, om[nt][mt >> 1][u]);
+            js[r * (D + 1) + d + 1] = fmaf(o[nt][mt][2 + u] * 1048576.f, back, om[nt][mt >> 1][u]);
           }
         }
       }

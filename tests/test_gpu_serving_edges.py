@@ -183,28 +183,17 @@ def test_paged_attention_growing_and_shrinking_steps_and_scores(heads):
 
 @pytest.mark.parametrize("heads", [(15, 5, 64), (32, 8, 128)], ids=str)
 @pytest.mark.parametrize("new,n", [(1, 1), (1, 2), (1, 7), (3, 40), (1, 300)])
-def test_paged_attention_weights_round_around_the_middle_of_a_group(heads, new, n):
-    """4 bits, fp16: the weights p step, rounded by 2^-11 of themselves, multiply code - 8, and p times low + 8 step is added
-    in fp32.  The bar is oracle.serving.attention_tolerance's with these two in the place of |low| + step code."""
+def test_paged_attention_fp16_weights_keep_the_rest_of_their_rounding(heads, new, n):
+    """4 bits, fp16: a weight p step is two fp16 numbers, off by 2^-22 of itself.  The bar is attention_tolerance with that,
+    and the output's own rounding."""
     hq, hkv, d = heads
     g = gen(65)
     k, v = (torch.randn(n, hkv, d, generator=g) for _ in range(2))
     cache, table = cache_of(k.half(), v.half(), 16)
     q = torch.randn(new, hq, d, generator=g).half()
-    o, _, size = paged_reference(q, cache, 16, table, [new], [n])
-    rows_k, rows_v, _, _ = S.rows(cache, 16, d, table[0], n)
-    split = [S.split4(cache[int(table[0, i // 16])], 16, d) for i in range(n)]
-    codes = torch.stack([S.unpack4(c[1][:, i % 16]) for i, (c, _) in enumerate(split)]).double()
-    step, low = (torch.stack([p[1][:, i % 16, :, j] for i, (_, p) in enumerate(split)]).double().repeat_interleave(32, -1)
-                 for j in (0, 1))
-    away, middle = step * (codes - 8).abs(), (low + 8 * step).abs()
-    assert torch.allclose(rows_v, low + step * codes, rtol=1e-6)
-    seen = S.causal_seen(new, n)
-    around = S.attend_dense(q.double(), rows_k, rows_v, seen, d ** -0.5, None, away)[1]
-    all_of = S.attend_dense(q.double(), rows_k, rows_v, seen, d ** -0.5, None, away + middle)[1]
-    score = 2 * (d + 8) * 2.0 ** -23 * size[..., None] + 8 * 2.0 ** -22
-    tol = 1.02 * (2.0 ** -11 * o.abs() + 2.0 ** -11 * around + 2 * score * all_of)
+    o, spread, size = paged_reference(q, cache, 16, table, [new], [n])
     got = ops.paged_attention(q.to(DEV), cache.to(DEV), ints([0, new]).to(DEV), ints([n]).to(DEV), table.to(DEV))
+    tol = S.attention_tolerance(o, spread, size, FP16, d, weight_unit=2.0 ** -22)
     within(got, o, tol + step_floor(q, cache, 16, table, [new], [n]))
 
 
