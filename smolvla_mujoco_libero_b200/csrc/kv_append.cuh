@@ -22,9 +22,10 @@
 // dimensions of each half), so a warp's accesses are whole 128- or 256-byte rows, the rotation pairs meet in one lane, the
 // token's (cos, sin) are read once for all heads, and a quantisation group is 4 lanes (two shuffles per extremum).  The
 // first row is on its way while the token's place is looked up, every other one while the one before is worked on.
-// Bound by memory traffic at many tokens (26337 rows of 48 heads into 4 bits, D = 128: 694 MB in 127 us, 5.5 TB/s; with
-// library divisions for the quotients 195 us), by latency at few.  Measured for 15579 rows of 25 heads at D = 64 (104 MB in
-// 26 us) and left: four tokens per warp 34 us, two rows ahead 30 us, whole blocks of tokens staged in shared memory 29 us.
+// Bound by memory traffic at many tokens (26337 rows of 48 heads into 4 bits, D = 128: 694 MB in 127 us, 5.5 TB/s, in a
+// graph, 136 where calls follow each other; with library divisions for the quotients 195 us), by latency at few.  Measured
+// for 15579 rows of 25 heads at D = 64 (104 MB in 26 us) and left: four tokens per warp 34 us, two rows ahead 30 us, whole
+// blocks of tokens staged in shared memory 29 us.
 #pragma once
 
 #include "serving_common.cuh"

@@ -18,14 +18,15 @@
 // What the issuers wait for decides: a ready barrier asked by try_wait through one lane costs 200 cycles, by test_wait 41,
 // and one issuer for both tiles needed 3100 cycles for an iteration's waits, MMAs and commits.  One 16384-token prompt at
 // D = 64: 860 us; test_wait first: 734; an issuer per tile: 669; one pair of exponentials in eight as polynomials: 650
-// (now 638, 807 TFLOP/s).  64 ragged prompts of 1 to 1024 tokens: 65 us with a CTA's tiles found by a walk through the
-// sequences, 57 by bisection.
+// (now 640, 800 TFLOP/s, in a graph; 695 where calls follow each other under the power cap).  64 ragged prompts of 1 to 1024
+// tokens: 65 us with a CTA's tiles found by a walk through the sequences, 57 by bisection.
 // Measured and left: two CTAs of one tile each per SM (715 us; 61 us for 64 ragged prompts where this took 65), the same
 // as persistent CTAs that fetch ahead (785 and 63 us), scores read twice from TMEM instead of held (934 us).
 //
-// Exponentials are the bound at D = 64 (16 per clock and SM: 1024 cycles per 128 x 128 tile against 512 of MMA), both
-// pipes at D = 128.  The running maximum is lazy (O is rescaled only when a row's maximum grows by more than 8 in log2
-// units, by the softmax threads themselves), exponent arguments and sums go through the packed fp32 pipe.
+// Exponentials are the bound at D = 64 (16 per clock and SM: 1024 cycles per 128 x 128 tile against 512 of MMA; the unit is
+// 67% busy).  At D = 128 both pipes need 1024 cycles per tile and overlap little: 1800, and an item takes 6.5 us beside its
+// tiles.  The running maximum is lazy (O is rescaled only when a row's maximum grows by more than 8 in log2 units, by the
+// softmax threads themselves), exponent arguments and sums go through the packed fp32 pipe.
 //
 // What stands behind a sequence's last key belongs to its neighbour: scores there are masked, and the V rows of the tile
 // are set to zero in shared memory before the product (0 * NaN would be NaN).  Under a causal mask the same holds inside

@@ -1,7 +1,7 @@
 // The torch side of the serving operators (kv_append, packed_attention, paged_attention of ops.py): the tensors' checks,
 // the outputs and the call of the C ABI.  In C++ because a single token's operators take less time on the GPU than an
-// interpreter needs to look at a dozen tensors: host time of an append of one token 6.2 us, 11.6 with the checks in Python
-// and the call through ctypes (prompt attention 9.9 and paged attention 10.5 then, 5.3 the latter now).
+// interpreter needs to look at a dozen tensors: an append of one token, called again and again, takes 5.9 us, 12.5 with the
+// checks in Python and the call through ctypes (attention of one token 6.0 and 11.0).
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
