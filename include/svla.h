@@ -301,8 +301,8 @@ int32_t svla_fused_rope_attention_f32_mask_implicit_pos(const float* q_raw, cons
  * (deploy/trt_sample_actions_core_deploy.py:108-237).
  *
  * Packed tensors are [rows, heads * head_dim] with a row stride (elements, a multiple of 8, rows 16-byte aligned):
- * sequence b owns rows cu[b] .. cu[b + 1] - 1 of a non-decreasing int32 [batch + 1]; rows behind cu[batch] are neither
- * read nor written.  head_dim 64 or 128; dtype SVLA_DT_BF16 or SVLA_DT_HALF; query head h reads kv head
+ * sequence b owns rows cu[b] .. cu[b + 1] - 1 of a non-decreasing int32 [batch + 1]; rows behind cu[batch] count for
+ * nothing and are not written.  head_dim 64 or 128; dtype SVLA_DT_BF16 or SVLA_DT_HALF; query head h reads kv head
  * h / (hq / hkv).  A query whose keys weigh nothing (none to see, none whose page is there, or all scores -infinity) gives
  * zeros.
  *

@@ -200,15 +200,16 @@ def test_paged_attention_fp16_weights_keep_the_rest_of_their_rounding(heads, new
 @pytest.mark.parametrize("heads", [(3, 1, 64), (8, 2, 128)], ids=str)
 @pytest.mark.parametrize("n", [1, 2, 33, 65, 130])
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
-def test_paged_attention_non_finite_group_leaves_the_others(heads, n, bad):
+@pytest.mark.parametrize("dtype", [BF16, FP16], ids=["bf16", "fp16"])
+def test_paged_attention_non_finite_group_leaves_the_others(heads, n, bad, dtype):
     """4 bits, an infinity or a NaN in the last entry's values: its group of 32 dimensions is NaN, the others are right."""
     hq, hkv, d = heads
     g = gen(54)
     k, v = (torch.randn(n, hkv, d, generator=g) for _ in range(2))
-    q = torch.randn(1, hq, d, generator=g).to(BF16)
+    q = torch.randn(1, hq, d, generator=g).to(dtype)
     v[n - 1, :, 40] = bad
     for width in (None, 64):
-        cache, table = cache_of(k.to(BF16), v.to(BF16), 16, width)
+        cache, table = cache_of(k.to(dtype), v.to(dtype), 16, width)
         check_groups(q, cache, 16, table, [1], [n], f"{n} entries")
 
 
