@@ -95,6 +95,28 @@ def test_packed_attention_one_long_prompt_among_many_short_ones(impl, heads):
     within(got, o, S.attention_tolerance(o, spread, size, BF16, d))
 
 
+@pytest.mark.parametrize("impl", KERNELS)
+def test_packed_attention_and_append_rows_beyond_32_bits(impl):
+    """Rows 2^26 elements apart: the last ones lie behind 2^31 elements."""
+    hq, hkv, d, n, page = 6, 2, 64, 40, 16
+    q, kv = packed_inputs([n], [n], hq, hkv, d, BF16, seed=44)
+    o, spread, size = packed_reference(q, kv, [n], [n], True)
+    far = torch.empty(n, 1 << 20, d, dtype=BF16, device=DEV)
+    x, out = far[:, :hq + 2 * hkv], far[:, 20:20 + hq]
+    x.copy_(torch.cat([q, kv], 1))
+    qd, kd, vd = x.split([hq, hkv, hkv], 1)
+    got = ops.packed_attention(qd, kd, vd, ints([0, n]).to(DEV), out=out, impl=impl)
+    within(got, o, S.attention_tolerance(o, spread, size, BF16, d))
+    table, n_pages = make_table([n], page)
+    cache = ops.kv_cache(n_pages, page, hkv, d, 4, device=DEV)
+    want = cache.cpu().clone()
+    cs = ops.rope_table_wide(n, 10000.0, DEV, d)
+    rq, rk, rv = S.append(want, page, kv[:, :hkv], kv[:, hkv:], [0, n], [n], table, cs.cpu(), None, q)
+    ops.kv_append(cache, kd, vd, ints([0, n]).to(DEV), ints([n]).to(DEV), table.to(DEV), q=qd, rope_cs=cs, q_out=qd, k_out=kd,
+                  v_out=vd)
+    assert torch.equal(cache.cpu(), want) and torch.equal(x.cpu(), torch.cat([rq, rk, rv], 1))
+
+
 # ----------------------------------------------------------------------------- paged attention
 
 def step_floor(q, cache, page, table, new, total):
@@ -250,6 +272,21 @@ def test_paged_attention_scores_of_minus_infinity(heads, gone, total, width):
     none = [i for i in range(new) if total - new + i < gone]
     assert bool((got[none] == 0).all())
     within(got, o, S.attention_tolerance(o, spread, size, BF16, d))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("batch", [127, 128, 129, 300])
+@pytest.mark.parametrize("width", [None, 100], ids=["one piece", "pieces"])
+def test_paged_attention_finds_every_item_of_many_sequences(bits, batch, width):
+    """Sequences without tokens, with one and with several, with nothing cached before and with up to 70 entries."""
+    hq, hkv, d, page = 3, 1, 64, 16
+    new = [(1, 0, 1, 2, 1, 9)[(i * i + i // 7) % 6] for i in range(batch)]
+    total = [n + (i * 31) % 70 for i, n in enumerate(new)]
+    cache, table = filled_cache(total, (hq, hkv, d), bits, page, BF16, seed=66, width=width)
+    q = torch.randn(sum(new), hq, d, generator=gen(67)).to(BF16)
+    o, spread, size = paged_reference(q, cache, page, table, new, total)
+    got = ops.paged_attention(q.to(DEV), cache.to(DEV), ints(starts(new)).to(DEV), ints(total).to(DEV), table.to(DEV))
+    within(got, o, paged_tolerance(o, spread, size, BF16, d, bits, total, 1.0))
 
 
 @pytest.mark.parametrize("bits", [16, 4])
