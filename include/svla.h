@@ -380,6 +380,80 @@ typedef struct svla_paged_attn_desc {
 int32_t svla_paged_attention(const svla_paged_attn_desc* desc, svla_stream_t stream);
 
 /* -------------------------------------------------------------------------------------------------
+ * Answering with the text model in 8-bit integers: rows quantised with a scale each (no calibration: the
+ * reference's dynamic activation scales, deploy/linear_only_quant.py, taken per token), products of such
+ * rows with the int8 weights of svla_pack_weight_i8, and the choice of a token from the logits.
+ * ------------------------------------------------------------------------------------------------*/
+
+/* h = x + residual;  y = h, or its RMSNorm (weight), or its LayerNorm (weight and bias), divided by smooth;
+ * scale[m] = max |y| / 127;  codes = round(y / scale) (ties to even);  sum = h;  values = codes * scale.
+ * Statistics in fp32 of the unrounded h.  A row of zeros gets scale 0 and codes 0; one whose largest |y| is
+ * not finite gets scale NaN and codes 0 (and its products are NaN).  sum and values may be x or residual
+ * itself (in place, same row stride).  Rows, and weight, bias and smooth, of any alignment; 16-byte aligned
+ * ones of k a multiple of 8 are read 16 bytes at a time.  1 <= k <= 32768. */
+typedef struct svla_quant_rows_desc {
+  const void* x;         /* [m, k] BF16 or HALF (dtype, as every void* here) */
+  const void* residual;  /* [m, k] or NULL */
+  const void* weight;    /* [k] or NULL: no norm */
+  const void* bias;      /* [k] or NULL: RMSNorm */
+  const float* smooth;   /* [k] or NULL */
+  int8_t* codes;         /* [m, k] out */
+  float* scale;          /* [m] out */
+  void* sum;             /* [m, k] out, or NULL */
+  void* values;          /* [m, k] out, or NULL */
+  int64_t x_rs, residual_rs, codes_rs, sum_rs, values_rs; /* row strides in elements */
+  int32_t m, k, dtype;
+  float eps;
+} svla_quant_rows_desc;
+int32_t svla_quant_rows(const svla_quant_rows_desc* desc, svla_stream_t stream);
+
+/* out[m, n] = xscale[m] * wscale[n] * sum_k x[m, k] w[n, k] + bias[n] + residual[m, n], the sum exact, the rest in
+ * fp32, rounded once.  gated: w and wscale hold 2 n rows, the gate's n first, and out = silu(gate) * up.
+ * x and w 16-byte aligned with row strides that are multiples of 16 bytes (k itself may be any number below
+ * 2^17: what stands behind a row's k is not read).  out may be residual (in place, same row stride). */
+#define SVLA_LINEAR_AUTO 0
+#define SVLA_LINEAR_FEW 1  /* the kernel for few rows, at any m */
+#define SVLA_LINEAR_MANY 2 /* the kernel for many rows, at any m */
+typedef struct svla_linear_i8_desc {
+  const int8_t* x;       /* [m, k] */
+  const float* xscale;   /* [m] */
+  const int8_t* w;       /* [n, k], gated [2 n, k] */
+  const float* wscale;   /* [n], gated [2 n] */
+  const float* bias;     /* [n] or NULL (gated: NULL) */
+  const void* residual;  /* [m, n] of the output's type or NULL (gated: NULL) */
+  void* out;             /* [m, n] BF16, HALF or FLOAT (dtype) */
+  int64_t x_rs, w_rs, residual_rs, out_rs; /* row strides in elements */
+  int32_t m, n, k, dtype, gated, impl;     /* impl: SVLA_LINEAR_* */
+} svla_linear_i8_desc;
+int32_t svla_linear_i8(const svla_linear_i8_desc* desc, svla_stream_t stream);
+
+/* One token per row of logits l, drawn with the row's u in [0, 1].  With w_i = round(2^44 exp((l_i - max l) /
+ * temperature)), kept are the top_k largest logits (top_k <= 0: all) with w_i >= min_p 2^44, of these, the most
+ * likely first, each one before which the w of the kept do not reach ceil(top_p sum w) (top_p >= 1: all); equal
+ * logits rank by index; the most likely one is always kept.  The token is the first, by index, up to which the
+ * kept w add up to more than floor(u sum w); logprob = ln(w / sum w) among the kept.  temperature 0: the largest
+ * logit (the lowest index of equal ones), logprob 0.  Logits may be -infinity.  A row whose largest logit is not
+ * finite or that holds a NaN, and settings that are none (temperature negative or not finite, top_p or min_p
+ * negative or NaN, u outside [0, 1]), give token -1 and logprob NaN.  Settings are per row (device arrays) or,
+ * where the array is NULL, the value for all rows.  1 <= vocab <= 2^18. */
+typedef struct svla_sample_desc {
+  const void* logits;        /* [batch, vocab] BF16, HALF or FLOAT (dtype) */
+  const float* u;            /* [batch] */
+  const float* temperature;  /* [batch] or NULL */
+  const int32_t* top_k;      /* [batch] or NULL */
+  const float* top_p;        /* [batch] or NULL */
+  const float* min_p;        /* [batch] or NULL */
+  int32_t* tokens;           /* [batch] out */
+  float* logprob;            /* [batch] out, or NULL */
+  int64_t logits_rs;         /* row stride in elements */
+  int32_t batch, vocab, dtype;
+  float temperature_value;
+  int32_t top_k_value;
+  float top_p_value, min_p_value;
+} svla_sample_desc;
+int32_t svla_sample_tokens(const svla_sample_desc* desc, svla_stream_t stream);
+
+/* -------------------------------------------------------------------------------------------------
  * sample_actions glue
  * ------------------------------------------------------------------------------------------------*/
 /* Policy-side processing around sample_actions (lerobot SmolVLA prepare_images / prepare_state and the

@@ -141,6 +141,36 @@ class PagedAttnDesc(ctypes.Structure):
     ]
 
 
+class QuantRowsDesc(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p), ("residual", c_void_p), ("weight", c_void_p), ("bias", c_void_p), ("smooth", c_void_p),
+        ("codes", c_void_p), ("scale", c_void_p), ("sum", c_void_p), ("values", c_void_p), ("x_rs", c_int64),
+        ("residual_rs", c_int64), ("codes_rs", c_int64), ("sum_rs", c_int64), ("values_rs", c_int64), ("m", c_int32),
+        ("k", c_int32), ("dtype", c_int32), ("eps", c_float),
+    ]
+
+
+LINEAR_AUTO, LINEAR_FEW, LINEAR_MANY = range(3)  # SVLA_LINEAR_*
+
+
+class LinearI8Desc(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p), ("xscale", c_void_p), ("w", c_void_p), ("wscale", c_void_p), ("bias", c_void_p),
+        ("residual", c_void_p), ("out", c_void_p), ("x_rs", c_int64), ("w_rs", c_int64), ("residual_rs", c_int64),
+        ("out_rs", c_int64), ("m", c_int32), ("n", c_int32), ("k", c_int32), ("dtype", c_int32), ("gated", c_int32),
+        ("impl", c_int32),
+    ]
+
+
+class SampleDesc(ctypes.Structure):
+    _fields_ = [
+        ("logits", c_void_p), ("u", c_void_p), ("temperature", c_void_p), ("top_k", c_void_p), ("top_p", c_void_p),
+        ("min_p", c_void_p), ("tokens", c_void_p), ("logprob", c_void_p), ("logits_rs", c_int64), ("batch", c_int32),
+        ("vocab", c_int32), ("dtype", c_int32), ("temperature_value", c_float), ("top_k_value", c_int32),
+        ("top_p_value", c_float), ("min_p_value", c_float),
+    ]
+
+
 class RopeParams(ctypes.Structure):
     _fields_ = [("q_heads", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("max_wavelength", c_float)]
 
@@ -186,6 +216,9 @@ SIGNATURES = {
     "svla_packed_attention": (c_int32, [POINTER(PackedAttnDesc), c_void_p]),
     "svla_paged_attention_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int64]),
     "svla_paged_attention": (c_int32, [POINTER(PagedAttnDesc), c_void_p]),
+    "svla_quant_rows": (c_int32, [POINTER(QuantRowsDesc), c_void_p]),
+    "svla_linear_i8": (c_int32, [POINTER(LinearI8Desc), c_void_p]),
+    "svla_sample_tokens": (c_int32, [POINTER(SampleDesc), c_void_p]),
     "svla_build_masks": (c_int32, [c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_void_p,
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "svla_embed_tokens": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_int32, c_int32, c_float, c_void_p,
@@ -242,7 +275,8 @@ def serving():
                             "`python -m smolvla_mujoco_libero_b200.build`")
         from . import _torch_serving as module
         module.bind(*(ctypes.cast(getattr(handle, name), c_void_p).value for name in (
-            "svla_kv_append", "svla_packed_attention", "svla_paged_attention", "svla_paged_attention_workspace_size")))
+            "svla_kv_append", "svla_packed_attention", "svla_paged_attention", "svla_paged_attention_workspace_size",
+            "svla_quant_rows", "svla_linear_i8", "svla_sample_tokens")))
         _serving = module
     return _serving
 

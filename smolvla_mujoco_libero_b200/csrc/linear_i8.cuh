@@ -1,0 +1,427 @@
+// Products of int8 rows that carry a scale each with int8 weights that carry one per output channel:
+//   y[m, n] = xscale[m] wscale[n] sum_k x[m, k] w[n, k] + bias[n] + residual[m, n],      gated: silu(gate) up
+// where a gated product has 2 N weight rows, the gate's first.  The sums are exact (int32: K below 2^17); they are scaled in
+// fp32 and rounded once to the output's type.
+//
+// Two kernels on tcgen05 (kind::i8, int32 accumulators in tensor memory), operands brought by TMA in 128-byte slices of K.
+//
+// Few rows (linear_i8_few_kernel).  The floor is the weights' bytes, so the weights are the M side of the MMA (128 of them per
+// tile) and up to MT tokens its N side: no tensor time goes into empty rows, a lane of tensor memory is an output channel, and
+// a token's outputs leave in whole lines.  Where the tiles are fewer than the SMs, a cluster of up to 8 CTAs shares a tile's K
+// and adds its parts through distributed shared memory; whole numbers, so the order does not matter.
+//
+// Many rows (linear_i8_many_kernel).  Bound by the tensor pipe: CTA pairs compute 256 tokens x 256 weights (cta_group::2), which
+// halves the weights' way into each SM: an MMA of 128 x 256 x 32 per SM takes 128 cycles and 8 KB of shared memory, its operands
+// arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 8 epilogue warps.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+#include "serving_common.cuh"
+
+namespace svla {
+
+struct LinearI8Args {
+  CUtensorMap tx, tw;  // 2-D (k, row), 128-byte swizzle
+  const float *xscale, *wscale, *bias;
+  const void* residual;
+  void* out;
+  long long residual_rs, out_rs;
+  int m, n, k;
+  int tiles_m, tiles_n;
+  int splits;  // few rows: CTAs of a cluster that share a tile's K
+  int wide;    // many rows: output (and residual) rows can be written 16 bytes at a time
+  int* err;
+};
+
+namespace li8 {
+constexpr int kSlice = 128;  // bytes of K per stage
+
+template <typename T>
+__device__ __forceinline__ void put(T* p, float v);
+template <>
+__device__ __forceinline__ void put<float>(float* p, float v) { *p = v; }
+template <>
+__device__ __forceinline__ void put<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ void put<__half>(__half* p, float v) { *p = __float2half_rn(v); }
+
+// x sigmoid(x) with the hardware's 2^x and reciprocal (2^-22 relative each; a sigmoid below 2^-126, x < -87, is 0)
+__device__ __forceinline__ float silu(float x) { return __fmul_rn(x, rcp_approx(__fadd_rn(1.f, ex2_approx(__fmul_rn(x, -serving::kLog2e))))); }
+
+__device__ __forceinline__ float scaled(uint32_t acc, float a, float b) {
+  return __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(acc)), a), b);
+}
+
+template <int MT, bool GATED>
+struct Few {
+  static constexpr int kP = GATED ? 2 : 1;
+  static constexpr int kW = 128 * kSlice, kX = MT * kSlice;
+  static constexpr int kStage = kP * kW + kX;
+  // two CTAs per SM (a tile's start and end beside the other's stream) where three stages fit twice, else one
+  static constexpr int kStages = kStage <= 32768 ? 98304 / kStage : 196608 / kStage;
+  static constexpr int kBar = kStages * kStage;
+  static constexpr int kBytes = kBar + 256 + 1024;  // + alignment slack
+  static constexpr int kCols = kP * MT < 32 ? 32 : kP * MT;
+  static_assert(kStages * kStage >= kP * MT * 512, "a tile's parts lie where its operands were");
+  static_assert(kCols <= 512 && kBytes <= 232448);
+};
+constexpr int kFewThreads = 128;
+}  // namespace li8
+
+// One tile of 128 output channels x MT tokens per CTA, or per cluster of `splits` CTAs
+template <typename T, int MT, bool GATED>
+__global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const __grid_constant__ LinearI8Args a) {
+  using namespace li8;
+  using C = Few<MT, GATED>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBar);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* done = empty + C::kStages;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+  const int warp = threadIdx.x >> 5;
+  const int split = blockIdx.x % a.splits, tile = blockIdx.x / a.splits;
+  const int m0 = (tile / a.tiles_n) * MT, n0 = (tile % a.tiles_n) * 128;
+  const int slices = (a.k + kSlice - 1) / kSlice;
+  const int per = (slices + a.splits - 1) / a.splits;
+  const int kb = min(split * per, slices), ke = min(kb + per, slices);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(slot, C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  pdl_wait();
+  pdl_trigger();
+
+  bool ok = true;
+  if (warp == 0) {
+    for (int i = 0; i < ke - kb && ok; ++i) {
+      const int s = i % C::kStages;
+      ok = serving::wait_warp(&empty[s], ((i / C::kStages) & 1) ^ 1, a.err);
+      if (ok && serving::elect_one()) {
+        uint8_t* st = smem + s * C::kStage;
+        mbar_arrive_expect_tx(&full[s], C::kStage);
+#pragma unroll
+        for (int p = 0; p < C::kP; ++p) tma_load_2d(st + p * C::kW, &a.tw, &full[s], (kb + i) * kSlice, p * a.n + n0);
+        tma_load_2d(st + C::kP * C::kW, &a.tx, &full[s], (kb + i) * kSlice, m0);
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1) {
+    for (int i = 0; i < ke - kb && ok; ++i) {
+      const int s = i % C::kStages;
+      ok = serving::wait_warp(&full[s], (i / C::kStages) & 1, a.err);
+      tc_fence_after();
+      if (ok && serving::elect_one()) {
+        const uint32_t st = smem_u32(smem + s * C::kStage);
+        const uint64_t x = smem_desc_sw128(st + C::kP * C::kW);
+#pragma unroll
+        for (int p = 0; p < C::kP; ++p) {
+          const uint64_t w = smem_desc_sw128(st + p * C::kW);
+#pragma unroll
+          for (int kk = 0; kk < kSlice / 32; ++kk)  // 32 bytes are 2 units of a descriptor's address
+            mma_i8(tmem + p * MT, w + 2 * kk, x + 2 * kk, idesc_i8(128, MT), i > 0 || kk > 0);
+        }
+        mma_commit(&empty[s]);
+        if (i + 1 == ke - kb) mma_commit(done);
+      }
+      __syncwarp();
+    }
+  }
+  // (a producer or issuer that gave up leaves `done` alone, and this wait gives up too)
+  ok = ke > kb ? serving::wait_warp(done, 0, a.err) : true;
+  __syncwarp();
+  tc_fence_after();
+
+  const int lane_n = threadIdx.x, n = n0 + lane_n;
+  const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+  const int cols = min(MT, a.m - m0);
+  const bool in = n < a.n;
+  const float ws = in ? __ldg(a.wscale + n) : 0.f, wu = GATED && in ? __ldg(a.wscale + a.n + n) : 0.f;
+  const float bias = a.bias && in ? __ldg(a.bias + n) : -0.f;
+  T* out = static_cast<T*>(a.out) + n;
+  const T* res = static_cast<const T*>(a.residual) + n;
+  auto finish = [&](uint32_t acc, uint32_t acc2, float xs, int m) {
+    float v = scaled(acc, xs, ws);
+    if constexpr (GATED) v = __fmul_rn(silu(v), scaled(acc2, xs, wu));
+    v = __fadd_rn(v, bias);
+    if (a.residual) v = __fadd_rn(v, static_cast<float>(res[m * a.residual_rs]));
+    put<T>(out + m * a.out_rs, v);
+  };
+  if (a.splits == 1) {
+    for (int c = 0; c < cols; c += 16) {
+      uint32_t r[16], r2[GATED ? 16 : 1];
+      if (ok) {
+        tmem_ld16(t_row + c, r);
+        if constexpr (GATED) tmem_ld16(t_row + MT + c, reinterpret_cast<uint32_t(&)[16]>(r2));
+        tmem_ld_wait();
+      }
+      if (ok && in) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (c + j < cols) finish(r[j], r2[GATED ? j : 0], __ldg(a.xscale + m0 + c + j), m0 + c + j);
+      }
+      __syncwarp();
+    }
+  } else {
+    uint32_t* part = reinterpret_cast<uint32_t*>(smem);  // [P][MT][128]; every operand has been read
+    for (int c = 0; c < cols; c += 16) {
+      uint32_t r[16], r2[GATED ? 16 : 1];
+      if (ok && ke > kb) {
+        tmem_ld16(t_row + c, r);
+        if constexpr (GATED) tmem_ld16(t_row + MT + c, reinterpret_cast<uint32_t(&)[16]>(r2));
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = 0u, r2[GATED ? j : 0] = 0u;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (c + j < cols) {
+          part[(c + j) * 128 + lane_n] = r[j];
+          if constexpr (GATED) part[(MT + c + j) * 128 + lane_n] = r2[j];
+        }
+    }
+    __syncwarp();
+    cluster_sync();
+    if (ok && in) {
+      const uint32_t base = smem_u32(part) + lane_n * 4;
+      for (int c = split; c < cols; c += a.splits) {
+        uint32_t sum = 0u, sum2 = 0u;
+#pragma unroll 8
+        for (int s = 0; s < a.splits; ++s) {
+          const uint32_t from = mapa_shared(base + c * 512, s);
+          uint32_t v;
+          asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(from));
+          sum += v;
+          if constexpr (GATED) {
+            asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(from + MT * 512));
+            sum2 += v;
+          }
+        }
+        finish(sum, sum2, __ldg(a.xscale + m0 + c), m0 + c);
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // no CTA leaves while its parts are read
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+}
+
+namespace li8 {
+struct Many {
+  static constexpr int kStages = 6, kTile = 128 * kSlice, kStage = 2 * kTile;  // a CTA's rows of x and its half of w
+  static constexpr int kBar = kStages * kStage;
+  static constexpr int kConst = kBar + 256;                // 8 warps x 2 x 128 column constants
+  static constexpr int kBytes = kConst + 8 * 256 * 4 + 1024;  // + alignment slack
+  static_assert(kBytes <= 232448);
+};
+constexpr int kManyThreads = 320;
+}  // namespace li8
+
+// Tiles of 256 tokens x 256 weights (gated: 128 gates and their 128 ups) per CTA pair
+template <typename T, bool GATED>
+__global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(const __grid_constant__ LinearI8Args a) {
+  using namespace li8;
+  using C = Many;
+  constexpr int kOutCols = GATED ? 128 : 256;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBar);  // the leader's: both CTAs' operands are there
+  uint64_t* empty = full + C::kStages;                           // each CTA's own: its operands have been read
+  uint64_t* tfull = empty + C::kStages;                          // [2] each CTA's own: an accumulator is complete
+  uint64_t* tempty = tfull + 2;                                  // [2] the leader's: both CTAs' epilogues have read it
+  uint32_t* slot = reinterpret_cast<uint32_t*>(tempty + 2);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+  const int slices = (a.k + kSlice - 1) / kSlice, tiles = a.tiles_m * a.tiles_n;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 16);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(slot, 512);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are initialised before either uses the other's
+  tc_fence_after();
+  const uint32_t tmem = *slot;
+  pdl_wait();
+  pdl_trigger();
+
+  if (warp == 0) {
+    uint32_t s = 0, ph = 1;
+    bool ok = true;
+    for (int t = pair; t < tiles && ok; t += pairs) {
+      const int m0 = (t / a.tiles_n) * 256 + static_cast<int>(rank) * 128;
+      const int n0 = (t % a.tiles_n) * kOutCols + static_cast<int>(rank) * (GATED ? a.n : 128);
+      for (int i = 0; i < slices && ok; ++i) {
+        ok = serving::wait_warp(&empty[s], ph, a.err);
+        if (ok && serving::elect_one()) {
+          uint8_t* st = smem + s * C::kStage;
+          const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * C::kStage);
+          tma_load_2d_pair(st, &a.tx, bar, i * kSlice, m0);
+          tma_load_2d_pair(st + C::kTile, &a.tw, bar, i * kSlice, n0);
+        }
+        __syncwarp();
+        if (++s == C::kStages) s = 0, ph ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      uint32_t s = 0, ph = 0, lt = 0;
+      bool ok = true;
+      auto commit = [&](uint64_t* bar) {
+        mma_commit_pair(mapa_shared(smem_u32(bar), 0));
+        mma_commit_pair(mapa_shared(smem_u32(bar), 1));
+      };
+      for (int t = pair; t < tiles && ok; t += pairs, ++lt) {
+        const uint32_t ab = lt & 1;
+        ok = serving::wait_warp(&tempty[ab], ((lt >> 1) & 1) ^ 1, a.err);
+        tc_fence_after();
+        for (int i = 0; i < slices && ok; ++i) {
+          ok = serving::wait_warp(&full[s], ph, a.err);
+          tc_fence_after();
+          if (ok && serving::elect_one()) {
+            const uint32_t st = smem_u32(smem + s * C::kStage);
+            const uint64_t x = smem_desc_sw128(st), w = smem_desc_sw128(st + C::kTile);
+#pragma unroll
+            for (int kk = 0; kk < kSlice / 32; ++kk)
+              mma_i8_pair(tmem + ab * 256, x + 2 * kk, w + 2 * kk, idesc_i8(256, 256), i > 0 || kk > 0);
+            commit(&empty[s]);
+            if (i + 1 == slices) commit(&tfull[ab]);
+          }
+          __syncwarp();
+          if (++s == C::kStages) s = 0, ph ^= 1;
+        }
+      }
+    }
+  } else {
+    const int q = warp & 3, part = (warp - 2) / 4;
+    float* consts = reinterpret_cast<float*>(smem + C::kConst) + (warp - 2) * 256;  // scales, then biases or ups' scales
+    const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty[0]), 0), mapa_shared(smem_u32(&tempty[1]), 0)};
+    constexpr int kCols = kOutCols / 2;  // of this warp
+    bool ok = true;
+    uint32_t lt = 0;
+    for (int t = pair; t < tiles; t += pairs, ++lt) {
+      const uint32_t ab = lt & 1;
+      const int m = (t / a.tiles_n) * 256 + static_cast<int>(rank) * 128 + q * 32 + lane;
+      const int n0 = (t % a.tiles_n) * kOutCols + part * kCols;
+      const int cols = min(kCols, a.n - n0);
+      for (int c = lane; c < kCols; c += 32) {
+        const bool in = c < cols;
+        consts[c] = in ? __ldg(a.wscale + n0 + c) : 0.f;
+        consts[128 + c] = GATED ? (in ? __ldg(a.wscale + a.n + n0 + c) : 0.f) : (a.bias && in ? __ldg(a.bias + n0 + c) : -0.f);
+      }
+      const bool row = m < a.m;
+      const float xs = row ? __ldg(a.xscale + m) : 0.f;
+      T* out = static_cast<T*>(a.out) + m * a.out_rs + n0;
+      const T* res = static_cast<const T*>(a.residual) + m * a.residual_rs + n0;
+      __syncwarp();
+      ok = ok && serving::wait_warp(&tfull[ab], (lt >> 1) & 1, a.err);
+      tc_fence_after();
+      const uint32_t t_row = tmem + ab * 256 + (static_cast<uint32_t>(q * 32) << 16) + part * kCols;
+#pragma unroll 1
+      for (int c = 0; c < kCols && c < cols; c += 32) {
+        uint32_t r[32], r2[GATED ? 32 : 1];
+        if (ok) {
+          tmem_ld32(t_row + c, r);
+          if constexpr (GATED) tmem_ld32(t_row + 128 + c, reinterpret_cast<uint32_t(&)[32]>(r2));
+          tmem_ld_wait();
+        }
+        if (ok && row) {
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 w4 = *reinterpret_cast<const float4*>(consts + c + j);
+            const float4 b4 = *reinterpret_cast<const float4*>(consts + 128 + c + j);
+            const float w[4] = {w4.x, w4.y, w4.z, w4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float y = scaled(r[j + e], xs, w[e]);
+              if constexpr (GATED) y = __fmul_rn(silu(y), scaled(r2[GATED ? j + e : 0], xs, b[e]));
+              else y = __fadd_rn(y, b[e]);
+              v[j + e] = y;
+            }
+          }
+          if (a.wide && c + 32 <= cols) {
+            constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+            for (int j = 0; j < 32; j += kPer) {
+              if (a.residual) {
+                const uint4 w = *reinterpret_cast<const uint4*>(res + c + j);
+                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if constexpr (sizeof(T) == 4) {
+                    v[j + e] = __fadd_rn(v[j + e], __uint_as_float(u[e]));
+                  } else {
+                    const float2 f = serving::unpack2<T>(u[e]);
+                    v[j + 2 * e] = __fadd_rn(v[j + 2 * e], f.x);
+                    v[j + 2 * e + 1] = __fadd_rn(v[j + 2 * e + 1], f.y);
+                  }
+                }
+              }
+              uint32_t p[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(T) == 4) p[e] = __float_as_uint(v[j + e]);
+                else p[e] = serving::pack2<T>(v[j + 2 * e], v[j + 2 * e + 1]);
+              }
+              *reinterpret_cast<uint4*>(out + c + j) = make_uint4(p[0], p[1], p[2], p[3]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (c + j < cols) put<T>(out + c + j, a.residual ? __fadd_rn(v[j], static_cast<float>(res[c + j])) : v[j]);
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty_leader[ab]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA leaves while the other may still arrive on its barriers
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+}  // namespace svla

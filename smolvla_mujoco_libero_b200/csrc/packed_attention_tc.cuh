@@ -73,15 +73,8 @@ struct Cfg {
   static constexpr uint32_t kO = kOwnP ? 384 : 256;   // + D x
 };
 
-__device__ __forceinline__ bool elect_one() {
-  uint32_t p;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(p));
-  return p != 0;
-}
+using serving::elect_one;
+using serving::wait_warp;
 
 // instruction descriptor of kind::f16 for the type: fp32 accumulators, A and B of one type (fp16 0, bf16 1)
 template <typename T>
@@ -114,25 +107,6 @@ __device__ __forceinline__ float2 exp2_poly(float2 z) {
   p = __ffma2_rn(f, p, both(0.99999926f));
   auto power = [](float n) { return __uint_as_float((__float_as_uint(n) << 23) + 0x3F800000u); };  // of n's low bits
   return __fmul2_rn(p, make_float2(power(t.x), power(t.y)));
-}
-
-// Bounded wait of a whole warp.  A phase that is over already, the usual case here, is seen by test_wait in about 40
-// cycles; try_wait takes 100 then, and one lane polling for the others 200.
-__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  bool ok = done != 0;
-  if (!ok) {
-    for (uint32_t i = 0; i < kSpinLimit && !ok; ++i) ok = mbar_try_wait(bar, parity);
-    if (!ok && (threadIdx.x & 31) == 0) record_error(err, kErrMbarTimeout);
-  }
-  return __all_sync(0xffffffffu, ok);
 }
 }  // namespace ptc
 

@@ -121,6 +121,36 @@ __device__ __forceinline__ void copy_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// one lane of a converged warp; the compiler knows that it is one, which `lane == 0` does not tell it
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+
+// Bounded wait of a whole warp.  A phase that is over already, the usual case here, is seen by test_wait in about 40
+// cycles; try_wait takes 100 then, and one lane polling for the others 200.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, int* err) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  bool ok = done != 0;
+  if (!ok) {
+    for (uint32_t i = 0; i < kSpinLimit && !ok; ++i) ok = mbar_try_wait(bar, parity);
+    if (!ok && (threadIdx.x & 31) == 0) record_error(err, kErrMbarTimeout);
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
 // The sequence of packed row t: the b with starts[b] <= t < starts[b + 1], or -1.  Every lane of the warp calls it and
 // gets the answer; each round reads 32 entries at once and narrows the range 32 times, so 1024 sequences take two
 // dependent reads.

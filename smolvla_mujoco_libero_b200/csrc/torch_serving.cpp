@@ -1,5 +1,5 @@
-// The torch side of the serving operators (kv_append, packed_attention, paged_attention of ops.py): the tensors' checks,
-// the outputs and the call of the C ABI.  In C++ because a single token's operators take less time on the GPU than an
+// The torch side of the serving operators (kv_append, packed_attention, paged_attention, quantize_rows, linear_i8_rows,
+// sample_tokens of ops.py): the tensors' checks, the outputs and the call of the C ABI.  In C++ because a single token's operators take less time on the GPU than an
 // interpreter needs to look at a dozen tensors: an append of one token, called again and again, takes 5.9 us, 12.5 with the
 // checks in Python and the call through ctypes (attention of one token 6.0 and 11.0).
 #include <c10/cuda/CUDAFunctions.h>
@@ -24,13 +24,20 @@ struct {
   decltype(&svla_packed_attention) packed = nullptr;
   decltype(&svla_paged_attention) paged = nullptr;
   decltype(&svla_paged_attention_workspace_size) paged_workspace = nullptr;
+  decltype(&svla_quant_rows) quant_rows = nullptr;
+  decltype(&svla_linear_i8) linear = nullptr;
+  decltype(&svla_sample_tokens) sample = nullptr;
 } calls;
 
-void bind(uintptr_t append, uintptr_t packed, uintptr_t paged, uintptr_t paged_workspace) {
+void bind(uintptr_t append, uintptr_t packed, uintptr_t paged, uintptr_t paged_workspace, uintptr_t quant_rows, uintptr_t linear,
+          uintptr_t sample) {
   calls.append = reinterpret_cast<decltype(calls.append)>(append);
   calls.packed = reinterpret_cast<decltype(calls.packed)>(packed);
   calls.paged = reinterpret_cast<decltype(calls.paged)>(paged);
   calls.paged_workspace = reinterpret_cast<decltype(calls.paged_workspace)>(paged_workspace);
+  calls.quant_rows = reinterpret_cast<decltype(calls.quant_rows)>(quant_rows);
+  calls.linear = reinterpret_cast<decltype(calls.linear)>(linear);
+  calls.sample = reinterpret_cast<decltype(calls.sample)>(sample);
 }
 
 // a message's pieces; no streams, whose state belongs to the C++ library that a process loaded
@@ -241,6 +248,132 @@ Tensor paged_attention(const Tensor& q, const Tensor& cache, const Tensor& cu_q,
   return *out;
 }
 
+// ---------------------------------------------------------------- rows and products in 8 bits, tokens
+
+// the device that a call's tensors share: the first one's, which has to be the current one
+struct Where {
+  int dev;
+
+  Where(const Tensor& t, const char* name) : dev(-1) {
+    if (!t.is_cuda()) refuse(name, " must be a CUDA tensor (there is no CPU path)");
+    dev = t.get_device();
+    const int now = c10::cuda::current_device();
+    if (dev != now) refuse(name, " is on cuda:", dev, ", the current device is cuda:", now);
+  }
+  bool here(const Tensor& t) const { return t.is_cuda() && t.get_device() == dev; }
+  svla_stream_t stream() const { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream(); }
+
+  // a matrix [rows, cols] whose rows are contiguous; -> row stride (a single row's does not matter to torch: `one` then)
+  int64_t matrix(const Tensor& t, const char* name, at::ScalarType dtype, int64_t rows, int64_t cols, int64_t one) const {
+    if (t.scalar_type() != dtype || !here(t) || t.dim() != 2 || t.size(0) != rows || t.size(1) != cols || (cols > 1 && rows && t.stride(1) != 1))
+      refuse(name, " must be ", dtype, " [", rows, ", ", cols, "] with contiguous rows on cuda:", dev, ", got ", t.scalar_type(), " ",
+             t.sizes(), " with strides ", t.strides(), " on ", t.device());
+    if (rows > 1 && t.stride(0) < cols) refuse(name, " has overlapping rows: strides ", t.strides());
+    return rows > 1 ? t.stride(0) : one;
+  }
+  const void* vector(const Tensor& t, const char* name, at::ScalarType dtype, int64_t n) const {
+    if (t.scalar_type() != dtype || !here(t) || t.dim() != 1 || t.size(0) != n || !t.is_contiguous())
+      refuse(name, " must be contiguous ", dtype, " [", n, "] on cuda:", dev, ", got ", t.scalar_type(), " ", t.sizes(), " on ", t.device());
+    return t.const_data_ptr();
+  }
+};
+
+int32_t dtype_code(at::ScalarType t) {
+  return t == at::kHalf ? SVLA_DT_HALF : t == at::kBFloat16 ? SVLA_DT_BF16 : t == at::kFloat ? SVLA_DT_FLOAT : -1;
+}
+
+py::tuple quantize_rows(const Tensor& x, const Opt& weight, const Opt& bias, double eps, const Opt& residual, const Opt& smooth,
+                        bool want_values, Opt codes, Opt scale, Opt sum, Opt values) {
+  const Where w(x, "x");
+  const at::ScalarType t = x.scalar_type();
+  if ((t != at::kBFloat16 && t != at::kHalf) || x.dim() != 2) refuse("x must be bf16 or fp16 [rows, k], got ", t, " ", x.sizes());
+  const int64_t m = x.size(0), k = x.size(1);
+  svla_quant_rows_desc d = {};
+  d.x_rs = w.matrix(x, "x", t, m, k, k);
+  if (residual) d.residual_rs = w.matrix(*residual, "residual", t, m, k, k), d.residual = residual->const_data_ptr();
+  if (weight) d.weight = w.vector(*weight, "weight", t, k);
+  if (bias) d.bias = w.vector(*bias, "bias", t, k);
+  if (smooth) d.smooth = static_cast<const float*>(w.vector(*smooth, "smooth", at::kFloat, k));
+  if (codes) {
+    d.codes_rs = w.matrix(*codes, "codes", at::kChar, m, k, k);
+  } else {  // rows 16 bytes apart, as the product takes them
+    d.codes_rs = (k + 15) / 16 * 16;
+    codes = x.new_empty({m, d.codes_rs}, x.options().dtype(at::kChar));
+    if (d.codes_rs != k) codes = codes->narrow(1, 0, k);
+  }
+  if (scale) w.vector(*scale, "scale", at::kFloat, m);
+  else scale = x.new_empty({m}, x.options().dtype(at::kFloat));
+  if (sum) d.sum_rs = w.matrix(*sum, "sum", t, m, k, k);
+  else if (residual) sum = x.new_empty({m, k}), d.sum_rs = k;
+  if (values) d.values_rs = w.matrix(*values, "values", t, m, k, k);
+  else if (want_values) values = x.new_empty({m, k}), d.values_rs = k;
+  d.x = x.const_data_ptr(), d.codes = static_cast<int8_t*>(codes->data_ptr()), d.scale = static_cast<float*>(scale->data_ptr());
+  if (sum) d.sum = sum->data_ptr();
+  if (values) d.values = values->data_ptr();
+  d.m = i32(m, "the number of rows"), d.k = i32(k, "k"), d.dtype = dtype_code(t), d.eps = static_cast<float>(eps);
+  check(calls.quant_rows(&d, w.stream()), "svla_quant_rows");
+  return py::make_tuple(*codes, *scale, sum, values);
+}
+
+Tensor linear_i8_rows(const Tensor& x, const Tensor& xscale, const Tensor& weight, const Tensor& wscale, const Opt& bias,
+                      const Opt& residual, bool gated, at::ScalarType dtype, Opt out, int impl) {
+  const Where w(x, "x");
+  if (x.dim() != 2 || weight.dim() != 2) refuse("x and weight must be matrices, got ", x.sizes(), " and ", weight.sizes());
+  const int64_t m = x.size(0), k = x.size(1), rows = weight.size(0), padded = (k + 15) / 16 * 16;
+  if (gated && rows % 2) refuse("a gated product's weight holds gate and up rows, got ", rows, " rows");
+  const int64_t n = gated ? rows / 2 : rows;
+  if (out) dtype = out->scalar_type();
+  if (dtype_code(dtype) < 0) refuse("dtype must be bf16, fp16 or fp32, got ", dtype);
+  svla_linear_i8_desc d = {};
+  d.x_rs = w.matrix(x, "x", at::kChar, m, k, padded);
+  d.w_rs = w.matrix(weight, "weight", at::kChar, rows, k, padded);
+  d.xscale = static_cast<const float*>(w.vector(xscale, "x_scale", at::kFloat, m));
+  d.wscale = static_cast<const float*>(w.vector(wscale, "wscale", at::kFloat, rows));
+  if (bias) d.bias = static_cast<const float*>(w.vector(*bias, "bias", at::kFloat, n));
+  if (residual) d.residual_rs = w.matrix(*residual, "residual", dtype, m, n, n), d.residual = residual->const_data_ptr();
+  if (out) d.out_rs = w.matrix(*out, "out", dtype, m, n, n);
+  else out = x.new_empty({m, n}, x.options().dtype(dtype)), d.out_rs = n;
+  d.x = static_cast<const int8_t*>(x.const_data_ptr()), d.w = static_cast<const int8_t*>(weight.const_data_ptr());
+  d.out = out->data_ptr();
+  d.m = i32(m, "the number of rows"), d.n = i32(n, "n"), d.k = i32(k, "k");
+  d.dtype = dtype_code(dtype), d.gated = gated, d.impl = impl;
+  check(calls.linear(&d, w.stream()), "svla_linear_i8");
+  return *out;
+}
+
+// a setting of sample_tokens: a tensor with a value per row, a number for all rows, or None
+template <typename V>
+void setting(const Where& w, const py::object& o, const char* name, at::ScalarType dtype, int64_t batch, const V** rows, V* value) {
+  if (o.is_none()) return;
+  if (THPVariable_Check(o.ptr())) *rows = static_cast<const V*>(w.vector(THPVariable_Unpack(o.ptr()), name, dtype, batch));
+  else *value = o.cast<V>();
+}
+
+py::tuple sample_tokens(const Tensor& logits, const Tensor& u, const py::object& temperature, const py::object& top_k,
+                        const py::object& top_p, const py::object& min_p, Opt tokens, Opt logprob) {
+  const Where w(logits, "logits");
+  const at::ScalarType t = logits.scalar_type();
+  if (dtype_code(t) < 0 || logits.dim() != 2) refuse("logits must be bf16, fp16 or fp32 [batch, vocab], got ", t, " ", logits.sizes());
+  const int64_t batch = logits.size(0), vocab = logits.size(1);
+  svla_sample_desc d = {};
+  d.logits_rs = w.matrix(logits, "logits", t, batch, vocab, vocab);
+  d.u = static_cast<const float*>(w.vector(u, "u", at::kFloat, batch));
+  d.temperature_value = 1.f, d.top_p_value = 1.f;
+  setting(w, temperature, "temperature", at::kFloat, batch, &d.temperature, &d.temperature_value);
+  setting(w, top_k, "top_k", at::kInt, batch, &d.top_k, &d.top_k_value);
+  setting(w, top_p, "top_p", at::kFloat, batch, &d.top_p, &d.top_p_value);
+  setting(w, min_p, "min_p", at::kFloat, batch, &d.min_p, &d.min_p_value);
+  if (tokens) w.vector(*tokens, "tokens", at::kInt, batch);
+  else tokens = logits.new_empty({batch}, logits.options().dtype(at::kInt));
+  if (logprob) w.vector(*logprob, "logprob", at::kFloat, batch);
+  else logprob = logits.new_empty({batch}, logits.options().dtype(at::kFloat));
+  d.logits = logits.const_data_ptr();
+  d.tokens = static_cast<int32_t*>(tokens->data_ptr()), d.logprob = static_cast<float*>(logprob->data_ptr());
+  d.batch = i32(batch, "the number of rows"), d.vocab = i32(vocab, "vocab"), d.dtype = dtype_code(t);
+  check(calls.sample(&d, w.stream()), "svla_sample_tokens");
+  return py::make_tuple(*tokens, *logprob);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -249,4 +382,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kv_append", &kv_append);
   m.def("packed_attention", &packed_attention);
   m.def("paged_attention", &paged_attention);
+  m.def("quantize_rows", &quantize_rows);
+  m.def("linear_i8_rows", &linear_i8_rows);
+  m.def("sample_tokens", &sample_tokens);
 }

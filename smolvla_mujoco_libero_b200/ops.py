@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -403,6 +404,48 @@ def paged_attention(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor, kv
     ``packed_attention``.  Returns [rows, heads, head_dim].  ``workspace``: uint8 of svla_paged_attention_workspace_size
     bytes, taken from torch's allocator when None."""
     return L.serving().paged_attention(q, cache, cu_q, kv_len, page_table, scale, out, workspace)
+
+
+# ----------------------------------------------------------------------------- serving: rows and products in int8, tokens
+
+class QuantizedRows(NamedTuple):
+    codes: torch.Tensor          # int8 [rows, k], rows 16 bytes apart
+    scale: torch.Tensor          # fp32 [rows]
+    sum: torch.Tensor | None     # x + residual, in x's type
+    values: torch.Tensor | None  # codes * scale, in x's type
+
+
+def quantize_rows(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5,
+                  residual: torch.Tensor | None = None, smooth: torch.Tensor | None = None, want_values: bool = False,
+                  codes: torch.Tensor | None = None, scale: torch.Tensor | None = None, sum: torch.Tensor | None = None,
+                  values: torch.Tensor | None = None) -> QuantizedRows:
+    """Rows of bf16 or fp16 x [rows, k] (any row stride) in int8 with a scale each: h = x + residual, its RMSNorm (``weight``) or
+    LayerNorm (``weight`` and ``bias``), divided by ``smooth`` (fp32 [k]); scale = max |y| / 127, codes = round(y / scale).
+    ``sum`` is h (there with a residual; it may be x or the residual itself), ``values`` what the codes stand for
+    (``want_values``: the activations that a fake-quantised linear multiplies, deploy/linear_only_quant.py:140-162).  A row
+    that is not finite gets scale NaN and codes 0.  The outputs may be given."""
+    return QuantizedRows(*L.serving().quantize_rows(x, weight, bias, eps, residual, smooth, want_values, codes, scale, sum, values))
+
+
+def linear_i8_rows(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wscale: torch.Tensor,
+                   bias: torch.Tensor | None = None, residual: torch.Tensor | None = None, gated: bool = False,
+                   dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None, impl: int = L.LINEAR_AUTO) -> torch.Tensor:
+    """x_scale[m] wscale[n] sum_k x[m, k] weight[n, k] + bias[n] + residual[m, n] from int8 rows with a scale each
+    (``quantize_rows``) and int8 weights with one per output channel (``pack_weight_i8``); bf16, fp16 or fp32.  ``gated``: weight
+    and wscale hold gate and up rows, one behind the other, and the result is silu(gate) * up.  Rows of x and weight 16-byte
+    aligned and a multiple of 16 bytes apart, whatever k is.  ``out`` may be the residual."""
+    return L.serving().linear_i8_rows(x, x_scale, weight, wscale, bias, residual, gated, dtype, out, impl)
+
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | float | None = None,
+                  top_k: torch.Tensor | int | None = None, top_p: torch.Tensor | float | None = None,
+                  min_p: torch.Tensor | float | None = None, tokens: torch.Tensor | None = None,
+                  logprob: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """One token per row of logits [batch, vocab] (bf16, fp16 or fp32, any row stride), drawn with u [batch] (fp32 in [0, 1]), and
+    its log-probability among the tokens that the settings keep: (int32 [batch], fp32 [batch]).  Settings are fp32 (``top_k``:
+    int32) tensors [batch], numbers for all rows, or None; temperature 0 takes the largest logit.  svla.h has the definition.  Rows
+    without a finite largest logit, and settings that are none, give token -1 and NaN."""
+    return L.serving().sample_tokens(logits, u, temperature, top_k, top_p, min_p, tokens, logprob)
 
 
 # ----------------------------------------------------------------------------- torch custom ops
