@@ -41,11 +41,11 @@ def units() -> list[tuple[Path, list[Path]]]:
     shared = [CSRC / "host.cuh", CSRC / "ptx.cuh", HEADER]
     serving = [CSRC / f"{n}.cuh" for n in ("kv_append", "paged_attention", "packed_attention", "packed_attention_tc",
                                            "serving_common")]
-    answer = [CSRC / f"{n}.cuh" for n in ("linear_i8", "quant_rows", "sample")]
+    answer = [CSRC / f"{n}.cuh" for n in ("answer_host", "linear_i8", "quant_rows", "sample")]
     path = [p for p in sorted(CSRC.glob("*.cuh")) if p not in serving + answer]
     return [(CSRC / "svla.cu", [CSRC / "svla.cu", *path, HEADER]),
             (CSRC / "serving.cu", [CSRC / "serving.cu", *serving, *shared]),
-            (CSRC / "answer.cu", [CSRC / "answer.cu", *answer, CSRC / "serving_common.cuh", *shared]),
+            *[(CSRC / n, [CSRC / n, *answer, CSRC / "serving_common.cuh", *shared]) for n in ("answer.cu", "sample.cu")],
             (CSRC / "engine.cpp", [CSRC / "engine.cpp", HEADER])]
 
 

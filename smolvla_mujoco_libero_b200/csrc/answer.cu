@@ -1,46 +1,19 @@
 // C-ABI entry points of the operators that answer with the text model in 8-bit integers (include/svla.h): rows normalised
-// and quantised with a scale each, products of such rows, the choice of a token.  Argument checks, dispatch and launches;
-// nothing allocates memory.
+// and quantised with a scale each, and products of such rows.  Argument checks, dispatch and launches; nothing allocates memory.
 #include <cmath>
 #include <cstring>
 
-#include "host.cuh"
+#include "answer_host.cuh"
 #include "linear_i8.cuh"
 #include "quant_rows.cuh"
-#include "sample.cuh"
 
 namespace svla {
 namespace {
-
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 int32_t check_dtype16(const char* who, int32_t dtype) {
   if (dtype != SVLA_DT_BF16 && dtype != SVLA_DT_HALF) return fail(SVLA_ERR_ARG, "%s: dtype must be BF16 or HALF (got %d)", who, dtype);
   return SVLA_OK;
 }
-
-// rows of `width` elements of `size` bytes, `rs` apart
-int32_t check_rows(const char* who, const char* name, const void* p, int64_t rs, int64_t width, int size) {
-  if (!p) return fail(SVLA_ERR_ARG, "%s: %s is null", who, name);
-  if (!aligned(p, size)) return fail(SVLA_ERR_ARG, "%s: %s must be aligned to its elements", who, name);
-  if (rs < width) return fail(SVLA_ERR_ARG, "%s: %s has a row stride below %lld", who, name, static_cast<long long>(width));
-  return SVLA_OK;
-}
-
-template <typename Kern>
-int32_t allow_smem(Kern kern, int bytes, bool (&configured)[64]) {
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return fail(SVLA_ERR_ARG, "device index %d out of range", dev);
-  if (!configured[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return fail(SVLA_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
-    configured[dev] = true;
-  }
-  return SVLA_OK;
-}
-
-constexpr int kSampleVocab = 1 << 18;
 
 // ---------------------------------------------------------------- quantised rows
 template <typename T, bool VEC, int W, int CH>
@@ -137,22 +110,6 @@ int32_t launch_linear_t(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStrea
   return d->gated ? launch_linear<T, true>(a, d, st) : launch_linear<T, false>(a, d, st);
 }
 
-// ---------------------------------------------------------------- tokens
-template <typename T>
-int32_t launch_sample(SampleArgs& a, cudaStream_t st) {
-  static bool configured[64] = {false};
-  auto kern = sample_kernel<T>;
-  constexpr int kMost = 129;  // tokens of a thread: 8 CTAs of 256 threads hold 2^18
-  auto bytes = [](int each) { return static_cast<int>(sizeof(sample::Shared)) + each * sample::kThreads * 4; };
-  static_assert(8 * sample::kThreads * kMost >= kSampleVocab);
-  if (int32_t rc = allow_smem(kern, bytes(kMost), configured)) return rc;
-  int ctas = 1;
-  while (ctas < sample::kMaxCtas && a.vocab > 1024 * ctas) ctas *= 2;
-  a.each = ((a.vocab + ctas * sample::kThreads - 1) / (ctas * sample::kThreads)) | 1;
-  return launch_cluster(kern, dim3(static_cast<unsigned>(a.batch) * ctas), dim3(sample::kThreads), bytes(a.each), st, "sample_kernel",
-                        static_cast<unsigned>(ctas), a);
-}
-
 }  // namespace
 }  // namespace svla
 
@@ -220,34 +177,6 @@ int32_t svla_linear_i8(const svla_linear_i8_desc* d, svla_stream_t stream) {
   if (d->dtype == SVLA_DT_FLOAT) return launch_linear_t<float>(a, d, cs(stream));
   if (d->dtype == SVLA_DT_HALF) return launch_linear_t<__half>(a, d, cs(stream));
   return launch_linear_t<__nv_bfloat16>(a, d, cs(stream));
-}
-
-int32_t svla_sample_tokens(const svla_sample_desc* d, svla_stream_t stream) {
-  const char* who = "svla_sample_tokens";
-  if (!d) return fail(SVLA_ERR_ARG, "%s: null descriptor", who);
-  if (d->dtype != SVLA_DT_BF16 && d->dtype != SVLA_DT_HALF && d->dtype != SVLA_DT_FLOAT)
-    return fail(SVLA_ERR_ARG, "%s: dtype must be BF16, HALF or FLOAT (got %d)", who, d->dtype);
-  if (d->vocab < 1 || d->vocab > kSampleVocab) return fail(SVLA_ERR_ARG, "%s: vocab must be 1 to %d (got %d)", who, kSampleVocab, d->vocab);
-  if (d->batch < 0 || d->batch > (1 << 27)) return fail(SVLA_ERR_ARG, "%s: batch must be 0 to 2^27 (got %d)", who, d->batch);
-  if (!d->temperature && !(d->temperature_value >= 0.f && !std::isinf(d->temperature_value)))
-    return fail(SVLA_ERR_ARG, "%s: temperature must be finite and not negative (got %g)", who, d->temperature_value);
-  if (!d->top_p && !(d->top_p_value >= 0.f)) return fail(SVLA_ERR_ARG, "%s: top_p must not be negative (got %g)", who, d->top_p_value);
-  if (!d->min_p && !(d->min_p_value >= 0.f)) return fail(SVLA_ERR_ARG, "%s: min_p must not be negative (got %g)", who, d->min_p_value);
-  if (d->batch == 0) return SVLA_OK;
-  if (int32_t rc = check_rows(who, "logits", d->logits, d->logits_rs, d->vocab, d->dtype == SVLA_DT_FLOAT ? 4 : 2)) return rc;
-  if (!d->u || !d->tokens) return fail(SVLA_ERR_ARG, "%s: u or tokens is null", who);
-  const void* words[] = {d->u, d->temperature, d->top_k, d->top_p, d->min_p, d->tokens, d->logprob};
-  for (const void* p : words)
-    if (!aligned(p, 4)) return fail(SVLA_ERR_ARG, "%s: an argument is not aligned to its elements", who);
-  SampleArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.logits = d->logits, a.logits_rs = d->logits_rs, a.u = d->u;
-  a.temperature = d->temperature, a.top_k = d->top_k, a.top_p = d->top_p, a.min_p = d->min_p;
-  a.temperature_value = d->temperature_value, a.top_k_value = d->top_k_value, a.top_p_value = d->top_p_value, a.min_p_value = d->min_p_value;
-  a.tokens = d->tokens, a.logprob = d->logprob, a.batch = d->batch, a.vocab = d->vocab;
-  if (d->dtype == SVLA_DT_FLOAT) return launch_sample<float>(a, cs(stream));
-  if (d->dtype == SVLA_DT_HALF) return launch_sample<__half>(a, cs(stream));
-  return launch_sample<__nv_bfloat16>(a, cs(stream));
 }
 
 }  // extern "C"
