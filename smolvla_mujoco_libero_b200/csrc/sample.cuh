@@ -9,8 +9,8 @@
 // A cluster of up to 8 CTAs holds a row in shared memory, read once from DRAM; every later pass is over shared memory, a
 // thread's tokens next to each other (an odd number of words: no bank conflicts), so thread order is index order.  Without
 // filters there is one pass of exponentials and a scan.  Filters need the place where a running count (top_k) or a running weight
-// (top_p), in falling order of the logits, reaches a limit: a histogram over 2048 bins of (max - l) / temperature, whose bins
-// the CTAs add up by shares through distributed shared memory, gives the bin.  Up to 512 tokens are then ranked by one CTA: all
+// (top_p), in falling order of the logits, reaches a limit: a histogram over 1024 bins of (max - l) / temperature, whose bins
+// the CTAs add up by shares through distributed shared memory, gives the bin.  Up to 256 tokens are then ranked by one CTA: all
 // that top_k leaves, and the token is found among them at once, or those of the bin.  A bin of more is divided again, by the bits
 // of its logits; one of equal logits is cut by index.
 //
@@ -43,7 +43,7 @@ struct SampleArgs {
 
 namespace sample {
 using u64 = unsigned long long;
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBins = 2048, kList = 512, kMaxCtas = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBinBits = 10, kBins = 1 << kBinBits, kFine = 4 * kBins, kList = 256, kMaxCtas = 8;
 constexpr double kUnit = 17592186044416.0;  // 2^44
 
 __device__ const double kPowers[64] = {  // 2^(j / 64)
@@ -65,11 +65,11 @@ __device__ const double kPowers[64] = {  // 2^(j / 64)
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
 
 struct alignas(16) Shared {
-  unsigned hist[4][kBins];  // tokens, and the weights' bits 0-14, 15-29 and 30-44 (sums of 2^16 of them stay in 32 bits)
+  unsigned hist[4][kBins];  // at first kFine bins of tokens; later tokens, and the weights' bits 0-14, 15-29 and 30-44 (sums of 2^16 of them stay in 32 bits)
   u64 list[kList], list_w[kList];
   u64 own[kList];           // of this CTA, on their way to the list of CTA 0
   double powers[64];
-  u64 exch[2][2];           // what the CTAs tell one another, in turn
+  u64 exch[2][3];           // what the CTAs tell one another, in turn
   u64 warp_sum[2][kWarps];
   u64 found[4];             // a crossing or a cut, written by the CTA that has it
   unsigned listed[2], own_n, own_at;
@@ -88,7 +88,9 @@ struct Weigh {
   double factor, top;  // 64 log2(e) / temperature, the largest logit
   const double* powers;
   // the weight of a logit less than 33 temperatures below the largest
-  __device__ __forceinline__ u64 operator()(float l) const {
+  __device__ __forceinline__ u64 operator()(float l) const { return bits(l) & 0xFFFFFFFFFFFFFull; }
+  // the same in the low bits of 2^52 + weight
+  __device__ __forceinline__ u64 bits(float l) const {
     const double d = static_cast<double>(l) - top;
     constexpr double kMagic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer in the low bits
     const double t = fma(d, factor, kMagic);
@@ -101,7 +103,7 @@ struct Weigh {
     p *= powers[n & 63];
     // times 2^(44 + n / 64), then rounded to an integer by adding 2^52
     p = __hiloint2double(__double2hiint(p) + ((44 + (n >> 6)) << 20), __double2loint(p)) + 4503599627370496.0;
-    return static_cast<u64>(__double_as_longlong(p)) & 0xFFFFFFFFFFFFFull;
+    return static_cast<u64>(__double_as_longlong(p));
   }
 };
 
@@ -113,6 +115,14 @@ __device__ __forceinline__ u64 remote_ld(const u64* p, unsigned rank) {
 __device__ __forceinline__ unsigned remote_ld(const unsigned* p, unsigned rank) {
   unsigned v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_u32(p), rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 remote_ld4(const unsigned* p, unsigned rank) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(mapa_shared(smem_u32(p), rank))
+               : "memory");
   return v;
 }
 __device__ __forceinline__ void remote_st(u64* p, unsigned rank, u64 v) {
@@ -146,13 +156,24 @@ struct Block {
   const int tid, lane, warp;
   unsigned turn, scan_turn;
 
-  // all CTAs' (a, b), of which thread 0's count; lane r of every warp gets CTA r's, other lanes zeros
-  __device__ __forceinline__ void exchange(u64& a, u64& b) {
-    if (tid == 0) s.exch[turn][0] = a, s.exch[turn][1] = b;
+  // all CTAs' (a, b, c), of which thread 0's count; lane r of every warp gets CTA r's, other lanes zeros
+  __device__ __forceinline__ void exchange(u64& a, u64& b, u64& c) {
+    if (tid == 0) s.exch[turn][0] = a, s.exch[turn][1] = b, s.exch[turn][2] = c;
     csync();
-    a = b = 0ull;
-    if (lane < static_cast<int>(ctas)) a = remote_ld(&s.exch[turn][0], lane), b = remote_ld(&s.exch[turn][1], lane);
+    a = b = c = 0ull;
+    if (lane < static_cast<int>(ctas)) {
+      a = remote_ld(&s.exch[turn][0], lane);
+      b = remote_ld(&s.exch[turn][1], lane);
+      c = remote_ld(&s.exch[turn][2], lane);
+    }
     turn ^= 1u;  // the other place is free: every CTA has read it before it came to the barrier above
+    __syncwarp();
+  }
+  __device__ __forceinline__ void exchange(u64& a) {
+    if (tid == 0) s.exch[turn][0] = a;
+    csync();
+    a = lane < static_cast<int>(ctas) ? remote_ld(&s.exch[turn][0], lane) : 0ull;
+    turn ^= 1u;
     __syncwarp();
   }
   // a value of every warp to all threads, joined by f
@@ -206,6 +227,14 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// the low bits that are 0 in every logit of the type, as fp32
+template <typename T>
+constexpr int kZeroBits = 0;
+template <>
+constexpr int kZeroBits<__nv_bfloat16> = 16;
+template <>
+constexpr int kZeroBits<__half> = 13;
+
 // the logits of a word, one or two of them
 template <typename T>
 __device__ __forceinline__ float2 logits_of(unsigned w) {
@@ -215,7 +244,7 @@ __device__ __forceinline__ float2 logits_of(unsigned w) {
 }  // namespace sample
 
 template <typename T>
-__global__ void __launch_bounds__(sample::kThreads) sample_kernel(const SampleArgs a) {
+__global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const SampleArgs a) {
   using namespace sample;
   constexpr int kIn = 4 / sizeof(T);  // logits of a word
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -230,6 +259,11 @@ __global__ void __launch_bounds__(sample::kThreads) sample_kernel(const SampleAr
   if (tid < 2) s.listed[tid] = 0u;
   pdl_wait();
   pdl_trigger();
+
+  const float temperature = a.temperature ? __ldg(a.temperature + row) : a.temperature_value;
+  const float top_p = a.top_p ? __ldg(a.top_p + row) : a.top_p_value, min_p = a.min_p ? __ldg(a.min_p + row) : a.min_p_value;
+  const int top_k = a.top_k ? __ldg(a.top_k + row) : a.top_k_value;
+  const float u = __ldg(a.u + row);
 
   // ---------------- this CTA's share of the row, -infinity behind its end, and the largest logit
   const int slice = a.words * kThreads * kIn, first = static_cast<int>(k.rank) * slice;
@@ -266,26 +300,30 @@ __global__ void __launch_bounds__(sample::kThreads) sample_kernel(const SampleAr
   auto larger = [](u64 x, u64 y) { return x > y ? x : y; };
   auto smaller = [](u64 x, u64 y) { return x < y ? x : y; };
   {
-    u64 p = k.over_warps(top != top ? ~0ull : key_of(top), larger), none = 0ull;
-    k.exchange(p, none);
+    u64 p = k.over_warps(top != top ? ~0ull : key_of(top), larger);
+    k.exchange(p);
 #pragma unroll
     for (int d = 4; d > 0; d >>= 1) p = larger(p, __shfl_xor_sync(0xffffffffu, p, d));
     p = __shfl_sync(0xffffffffu, p, 0);
     top = p == ~0ull ? INFINITY : of_key(static_cast<unsigned>(p));
   }
 
-  const float temperature = a.temperature ? __ldg(a.temperature + row) : a.temperature_value;
-  const float top_p = a.top_p ? __ldg(a.top_p + row) : a.top_p_value, min_p = a.min_p ? __ldg(a.min_p + row) : a.min_p_value;
-  const int top_k = a.top_k ? __ldg(a.top_k + row) : a.top_k_value;
-  const float u = __ldg(a.u + row);
   const unsigned* mine = row_words + tid * a.words;
   const int mine_first = first + tid * a.words * kIn;
-  auto for_mine = [&](auto f) {  // f(logit, index) of this thread's tokens
-#pragma unroll 4
-    for (int j = 0; j < a.words; ++j) {
-      const float2 l = logits_of<T>(mine[j]);
-      f(l.x, mine_first + j * kIn);
-      if constexpr (kIn == 2) f(l.y, mine_first + j * kIn + 1);
+  // f(four logits, index of the first) over this thread's tokens; -infinity behind the last
+  auto for_mine = [&](auto f) {
+    constexpr int kGroup = 4 / kIn;
+#pragma unroll 1
+    for (int j = 0; j < a.words; j += kGroup) {
+      float l[4];
+#pragma unroll
+      for (int e = 0; e < kGroup; ++e) {
+        const bool in = e == 0 || j + e < a.words;
+        const float2 v = logits_of<T>(in ? mine[j + e] : 0u);
+        l[e * kIn] = in ? v.x : -INFINITY;
+        if constexpr (kIn == 2) l[e * kIn + 1] = in ? v.y : -INFINITY;
+      }
+      f(l, mine_first + j * kIn);
     }
   };
   // a row without a finite largest logit or with a NaN, and settings that are none
@@ -300,12 +338,14 @@ __global__ void __launch_bounds__(sample::kThreads) sample_kernel(const SampleAr
   }
   if (temperature == 0.f || top_k == 1 || top_p == 0.f || min_p > 1.f) {  // the most likely token alone is kept
     unsigned at = 0xFFFFFFFFu;
-    for_mine([&](float l, int i) {
-      if (l == top) at = min(at, static_cast<unsigned>(i));
+    for_mine([&](const float (&l)[4], int i) {
+#pragma unroll
+      for (int e = 3; e >= 0; --e)
+        if (l[e] == top) at = min(at, static_cast<unsigned>(i + e));
     });
     at = __reduce_min_sync(0xffffffffu, at);
-    u64 p = k.over_warps(at, smaller), none = 0ull;
-    k.exchange(p, none);
+    u64 p = k.over_warps(at, smaller);
+    k.exchange(p);
     if (lane >= static_cast<int>(ctas)) p = ~0ull;
     at = __reduce_min_sync(0xffffffffu, static_cast<unsigned>(p));
     if (k.rank == 0 && tid == 0) {
@@ -318,113 +358,145 @@ __global__ void __launch_bounds__(sample::kThreads) sample_kernel(const SampleAr
   const Weigh weigh{92.33248261689366 / static_cast<double>(temperature), static_cast<double>(top), s.powers};
   // Kept are logits above cut_l, and of those that equal it the ones up to index cut_i.  At first what weighs something: less
   // than 45 octaves, 31.2 temperatures below the largest (rounded so that nothing is lost)
-  float cut_l = __fsub_rd(top, __fmul_ru(33.f, temperature));
-  int cut_i = -1;
-  bool filtered = false;
-  auto keeps = [&](float l, int i) { return l > cut_l || (l == cut_l && i <= cut_i); };
-
-  if (min_p > 0.f) {
-    // the smallest key whose weight reaches the bound, between one that does not and one that does: 33-fold search
-    const double bound = static_cast<double>(min_p) * kUnit;
-    unsigned lo = max(key_of(cut_l), 0x007FFFFFu), hi = key_of(top);
-    while (hi - lo > 1u) {
-      const unsigned step = (hi - lo + 32u) / 33u, at = lo + step * (lane + 1u);
-      const bool yes = at >= hi || static_cast<double>(weigh(of_key(at))) >= bound;
-      const int f = __ffs(__ballot_sync(0xffffffffu, yes));  // 1 + the first lane that does; 0: none
+  float cut_l = fmaxf(__fsub_rd(top, __fmul_ru(33.f, temperature)), -3.4028234663852886e38f);
+  if (static_cast<double>(top) - static_cast<double>(cut_l) > 34.0 * static_cast<double>(temperature))
+    cut_l = of_key(key_of(cut_l) + 1u);  // one step of the logits is more than that
+  int cut_i = 0x7FFFFFFF;
+  auto keeps = [&](float l, int i) { return l >= cut_l && !(l == cut_l && i > cut_i); };
+  // the smallest key from lo to hi for which `yes`, which holds for hi and all above the smallest: 33-fold search
+  auto smallest = [&](unsigned lo, unsigned hi, auto yes) {
+    while (lo < hi) {
+      const unsigned step = (hi - lo + 32u) / 33u, at = lo + step * lane + (step - 1u);  // (the last of each piece)
+      const int f = __ffs(__ballot_sync(0xffffffffu, at >= hi || yes(of_key(at))));       // 1 + the first that does; 0: none
       if (f == 0) {
         lo += 32u * step;
       } else {
-        hi = min(hi, lo + static_cast<unsigned>(f) * step);
-        lo += static_cast<unsigned>(f - 1) * step;
+        const unsigned before = lo + static_cast<unsigned>(f - 1) * step;
+        hi = min(hi, before + step - 1u);
+        lo = before;
       }
     }
-    cut_l = of_key(hi), cut_i = 0x7FFFFFFF, filtered = true;
+    return hi;
+  };
+
+  // the sum of all weights, 2^52 in front of each taken off at the end; what is raised to cut_l weighs nothing
+  auto weight_of_all = [&](auto more) {
+    u64 all = 0ull;
+    for_mine([&](const float (&l)[4], int) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const u64 w = weigh.bits(fmaxf(l[e], cut_l));
+        all += w;
+        more(l[e], w & 0xFFFFFFFFFFFFFull);
+      }
+    });
+    return all - static_cast<u64>((a.words * kIn + 3) / 4 * 4) * 0x4330000000000000ull;
+  };
+
+  if (min_p > 0.f) {
+    const double bound = static_cast<double>(min_p) * kUnit;
+    auto reaches = [&](float l) { return static_cast<double>(weigh(l)) >= bound; };
+    const unsigned lo = key_of(cut_l), hi = key_of(top);
+    // the border is at top + temperature ln(min_p): nearly always within 16 steps of that in fp32
+    const unsigned guess = key_of(fminf(fmaxf(top + temperature * __logf(min_p), cut_l), top)), from = guess - min(guess - lo, 16u);
+    const unsigned yes = __ballot_sync(0xffffffffu, from + lane >= hi || reaches(of_key(from + lane)));
+    cut_l = of_key((yes & 1u) || yes == 0u ? smallest(lo, hi, reaches) : from + __ffs(yes) - 1u);
   }
 
-  const bool by_count = top_k > 0 && top_k < a.vocab;
-  const bool by_weight = top_p < 1.f;
+  const bool by_count = top_k > 0 && top_k < a.vocab, by_weight = top_p < 1.f;
+  // (cut_l weighs something where -3.4e38 does)
+  const bool dense = !by_count && min_p == 0.f && weigh(cut_l) == 0ull;
+  u64 sum = 0ull;  // of this thread's kept tokens
   if (by_count || by_weight) {
-    filtered = true;
-    const float to_bin = 64.f / temperature;
-    auto linear_bin = [&](float l) {  // (0 * infinity, the largest logit's, is bin 0 too)
-      return min(__float2int_rz(__fmul_rn(__fsub_rn(top, l), to_bin)), kBins - 1);
+    // at first bins of 1 / 120 of the temperature: what is kept lies less than 33 (or one step of the logits) below the largest
+    const float to_bin = fminf(120.f / temperature, 3.4028234663852886e38f);
+    auto fine_bin = [&](float l) { return __float2int_rn(fminf(__fmul_rn(__fsub_rn(top, l), to_bin), static_cast<float>(kFine - 1))); };
+    unsigned* fine = &s.hist[0][0];
+    int my_bin = 0, my_bins = 0;  // this thread's of this CTA's share of the bins
+    auto share = [&](int bins) {
+      const int per = bins / static_cast<int>(ctas), per_thread = max(4, per / kThreads);
+      my_bin = static_cast<int>(k.rank) * per + tid * per_thread, my_bins = tid * per_thread < per ? per_thread : 0;
     };
-    const int per = kBins / static_cast<int>(ctas), per_thread = per > kThreads ? per / kThreads : 1;  // bins of a CTA, of a thread
-    const int my_bin = static_cast<int>(k.rank) * per + tid * per_thread, my_bins = tid * per_thread < per ? per_thread : 0;
-    bool counting = false, weighing = false;  // what the histogram holds
     auto clear = [&]() {
       for (int i = tid; i < kBins; i += kThreads) reinterpret_cast<uint4*>(&s.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
       __syncthreads();
     };
-    auto count_in = [&](int bin, float l) {
-      if (counting) atomicAdd(&s.hist[0][bin], 1u);
-      if (weighing) {
-        const u64 w = weigh(l);
-        atomicAdd(&s.hist[1][bin], static_cast<unsigned>(w) & 0x7FFFu);
-        atomicAdd(&s.hist[2][bin], static_cast<unsigned>(w >> 15) & 0x7FFFu);
-        atomicAdd(&s.hist[3][bin], static_cast<unsigned>(w >> 30));
-      }
-    };
-    u64 c_before = 0ull, w_before = 0ull, c_total = 0ull, w_total = 0ull;  // before this thread's bins, over all bins
     // the CTAs' histograms added up: each CTA's share of the bins lies in its own hist[0] (tokens) and hist[1], hist[2] (weight)
-    auto merge = [&]() {
+    u64 c_before = 0ull, w_before = 0ull, c_total = 0ull;  // tokens and weight before this thread's bins, tokens of all bins
+    auto merge = [&](bool weights) {
       csync();
       u64 c = 0ull, w = 0ull;
-      for (int j = 0; j < my_bins; ++j) {
-        const int bin = my_bin + j;
-        unsigned n = 0u;
-        u64 weight = 0ull;
+      for (int bin = my_bin; bin < my_bin + my_bins; bin += 4) {  // four bins of every CTA at once
+        uint4 n = make_uint4(0u, 0u, 0u, 0u);
+        u64 weight[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
         for (unsigned r = 0; r < kMaxCtas; ++r) {
           if (r >= ctas) break;
-          if (counting) n += remote_ld(&s.hist[0][bin], r);
-          if (weighing)
-            weight += remote_ld(&s.hist[1][bin], r) + (static_cast<u64>(remote_ld(&s.hist[2][bin], r)) << 15) +
-                      (static_cast<u64>(remote_ld(&s.hist[3][bin], r)) << 30);
-        }
-        // (no other CTA reads this CTA's share)
-        s.hist[0][bin] = n, s.hist[1][bin] = static_cast<unsigned>(weight), s.hist[2][bin] = static_cast<unsigned>(weight >> 32);
-        c += n, w += weight;
-      }
-      u64 tc = 0ull, tw = 0ull, below;
-      if (counting) c_before = k.scan(c, tc);
-      if (weighing) w_before = k.scan(w, tw);
-      k.exchange(tc, tw);
-      c_total = k.over_ctas(tc, below), c_before += below;
-      w_total = k.over_ctas(tw, below), w_before += below;
-    };
-    // the bin in which the running count (or weight) reaches `limit`, 1 <= limit <= its total
-    int bin = 0;
-    u64 bin_n = 0ull, bin_c = 0ull, bin_w = 0ull;  // its tokens; before the bin: tokens, weight
-    auto cross = [&](bool count, u64 limit) {
-      u64 c = c_before, w = w_before;
-      for (int b = my_bin; b < my_bin + my_bins; ++b) {
-        const u64 n = s.hist[0][b], weight = (static_cast<u64>(s.hist[2][b]) << 32) | s.hist[1][b];
-        const u64 at = count ? c : w, size = count ? n : weight;
-        if (at < limit && limit <= at + size)
-          for (unsigned r = 0; r < ctas; ++r) {
-            remote_st(&s.found[0], r, static_cast<u64>(b));
-            remote_st(&s.found[1], r, n);
-            remote_st(&s.found[2], r, c);
-            remote_st(&s.found[3], r, w);
+          const uint4 v = remote_ld4(&fine[bin], r);
+          n.x += v.x, n.y += v.y, n.z += v.z, n.w += v.w;
+          if (weights) {
+            const uint4 w0 = remote_ld4(&s.hist[1][bin], r), w1 = remote_ld4(&s.hist[2][bin], r), w2 = remote_ld4(&s.hist[3][bin], r);
+            weight[0] += w0.x + (static_cast<u64>(w1.x) << 15) + (static_cast<u64>(w2.x) << 30);
+            weight[1] += w0.y + (static_cast<u64>(w1.y) << 15) + (static_cast<u64>(w2.y) << 30);
+            weight[2] += w0.z + (static_cast<u64>(w1.z) << 15) + (static_cast<u64>(w2.z) << 30);
+            weight[3] += w0.w + (static_cast<u64>(w1.w) << 15) + (static_cast<u64>(w2.w) << 30);
           }
-        c += n, w += weight;
+        }
+        *reinterpret_cast<uint4*>(&fine[bin]) = n;  // (no other CTA reads this CTA's share)
+        c += static_cast<u64>(n.x) + n.y + n.z + n.w;
+        if (weights)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s.hist[1][bin + e] = static_cast<unsigned>(weight[e]), s.hist[2][bin + e] = static_cast<unsigned>(weight[e] >> 32);
+            w += weight[e];
+          }
+      }
+      u64 tc = 0ull, tw = 0ull, none = 0ull, below;
+      c_before = k.scan(c, tc);
+      if (weights) w_before = k.scan(w, tw);
+      k.exchange(tc, tw, none);
+      c_total = k.over_ctas(tc, below), c_before += below;
+      if (weights) k.over_ctas(tw, below), w_before += below;
+    };
+    auto count_of = [&](int b) { return static_cast<u64>(fine[b]); };
+    auto weight_of = [&](int b) { return (static_cast<u64>(s.hist[2][b]) << 32) | s.hist[1][b]; };
+    auto tell = [&](int slot, u64 v) {
+      for (unsigned r = 0; r < ctas; ++r) remote_st(&s.found[slot], r, v);
+    };
+    // the bin in which a running size, `before` in front of this thread's bins, reaches `limit` (from 1 to the sum of sizes)
+    int bin = 0;
+    u64 bin_n = 0ull, bin_before = 0ull;  // its tokens, the size before it
+    auto cross = [&](u64 limit, u64 before, auto size_of) {
+      for (int b = my_bin; b < my_bin + my_bins; ++b) {
+        const u64 size = size_of(b);
+        if (before < limit && limit <= before + size) tell(0, b), tell(1, fine[b]), tell(2, before);
+        before += size;
       }
       csync();
-      bin = static_cast<int>(s.found[0]), bin_n = s.found[1], bin_c = s.found[2], bin_w = s.found[3];
+      bin = static_cast<int>(s.found[0]), bin_n = s.found[1], bin_before = s.found[2];
     };
-    // the tokens that `member` says, to the list of CTA 0 as far as it takes them; -> how many there are
+    auto some = [](const float (&l)[4], float from, float to) {  // any of the four between the two
+      bool in = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) in |= l[e] >= from && l[e] <= to;
+      return in;
+    };
+    // the tokens from one logit to another, as far as they are kept, to the list of CTA 0; -> how many there are, at most kList
     unsigned gather_turn = 0u;
-    auto gather = [&](auto member) -> unsigned {
+    auto gather = [&](float from, float to) -> int {
       if (tid == 0) s.own_n = 0u;
       __syncthreads();
-      for_mine([&](float l, int i) {
-        if (!member(l, i)) return;
-        const unsigned at = atomicAdd(&s.own_n, 1u);
-        if (at < kList) s.own[at] = place_of(l, i);
+      for_mine([&](const float (&l)[4], int i) {
+        if (!some(l, from, to)) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (l[e] >= from && l[e] <= to && keeps(l[e], i + e)) {
+            const unsigned at = atomicAdd(&s.own_n, 1u);
+            if (at < kList) s.own[at] = place_of(l[e], i + e);
+          }
       });
       __syncthreads();
-      const unsigned n = s.own_n;
+      const unsigned n = min(s.own_n, static_cast<unsigned>(kList));
       if (tid == 0 && n) s.own_at = remote_add(&s.listed[gather_turn], 0, n);
       __syncthreads();
       if (n) {
@@ -432,10 +504,10 @@ __global__ void __launch_bounds__(sample::kThreads) sample_kernel(const SampleAr
         for (unsigned i = tid; i < n && at + i < kList; i += kThreads) remote_st(&s.list[at + i], 0, s.own[i]);
       }
       csync();
-      const unsigned all = remote_ld(&s.listed[gather_turn], 0);
+      const unsigned all = min(remote_ld(&s.listed[gather_turn], 0), static_cast<unsigned>(kList));
       gather_turn ^= 1u;
       if (k.rank == 0 && tid == 0) s.listed[gather_turn] = 0u;  // (every CTA has read it before it came to the barrier above)
-      return all;
+      return static_cast<int>(all);
     };
     // CTA 0: for token i of the list, how many of the m come before it and what they weigh
     auto rank_of = [&](int i, int m, unsigned& rank, u64& weight) {
@@ -445,197 +517,248 @@ __global__ void __launch_bounds__(sample::kThreads) sample_kernel(const SampleAr
       for (int j = 0; j < m; ++j) {
         const bool before = s.list[j] > own;
         rank += before;
-        if (before) weight += s.list_w[j];
+        weight += before ? s.list_w[j] : 0ull;
       }
     };
     auto weigh_list = [&](int m) {
       for (int i = tid; i < m; i += kThreads) s.list_w[i] = weigh(of_key(static_cast<unsigned>(s.list[i] >> 32)));
       __syncthreads();
     };
-    bool divided = false;  // the histogram is one of a bin's
-    // the cut inside a bin: after `need` tokens of it, or after the token with which their weight reaches `need`.
-    // -> the weight of what is kept of it
-    auto resolve = [&](bool count, u64 need) -> u64 {
-      bool ranged = false;  // members: of the linear bin, or with keys from lo to hi
-      unsigned lo = 0u, hi = 0u;
-      const int in_bin = bin;
-      auto member = [&](float l, int i) {
-        if (!keeps(l, i)) return false;
-        const unsigned key = key_of(l);
-        return ranged ? key >= lo && key <= hi : linear_bin(l) == in_bin;
-      };
-      u64 kept_w = 0ull;
-      // (a division takes 11 of the keys' 32 bits, so the fourth round at the latest has few or equal ones)
-      for (int round = 0; round < 4; ++round) {
-        if (!count || bin_n <= kList) {
-          const int m = static_cast<int>(gather(member));
-          if (m <= kList) {
-            if (k.rank == 0) {
-              weigh_list(m);
-              u64 last = ~0ull, sum = 0ull;  // of the kept: the least likely place, the weight
-              for (int i = tid; i < m; i += kThreads) {
-                unsigned rank;
-                u64 before;
-                rank_of(i, m, rank, before);
-                if ((count ? rank : before) < need) last = smaller(last, s.list[i]), sum += s.list_w[i];
-              }
-#pragma unroll
-              for (int d = 16; d > 0; d >>= 1) last = smaller(last, __shfl_xor_sync(0xffffffffu, last, d));
-              last = k.over_warps(last, smaller);
-              u64 total;
-              k.scan(sum, total);
-              if (tid < static_cast<int>(ctas)) remote_st(&s.found[0], tid, last), remote_st(&s.found[1], tid, total);
+    // the cut inside a range of logits with at most n kept tokens: after `need` of them, or after the one with which their
+    // weight reaches `need`
+    auto resolve = [&](bool count, u64 need, float from, float to, u64 n) {
+      constexpr unsigned kZeros = (1u << kZeroBits<T>) - 1u;
+      // (a division takes kBinBits of the keys' 32 bits, so the last round has few or equal ones)
+      for (int round = 0; round <= (31 + kBinBits) / kBinBits; ++round) {
+        if (n <= kList) {
+          const int m = gather(from, to);
+          if (k.rank == 0) {
+            weigh_list(m);
+            u64 last = ~0ull;  // of the kept: the least likely place
+            for (int i = tid; i < m; i += kThreads) {
+              unsigned rank;
+              u64 before;
+              rank_of(i, m, rank, before);
+              if ((count ? rank : before) < need) last = smaller(last, s.list[i]);
             }
-            csync();
-            cut_l = of_key(static_cast<unsigned>(s.found[0] >> 32)), cut_i = static_cast<int>(~static_cast<unsigned>(s.found[0]));
-            return kept_w + s.found[1];
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) last = smaller(last, __shfl_xor_sync(0xffffffffu, last, d));
+            last = k.over_warps(last, smaller);
+            if (tid < static_cast<int>(ctas)) remote_st(&s.found[0], tid, last);
           }
+          csync();
+          cut_l = of_key(static_cast<unsigned>(s.found[0] >> 32)), cut_i = static_cast<int>(~static_cast<unsigned>(s.found[0]));
+          return;
         }
-        // too many: the range of their keys
-        unsigned least = 0xFFFFFFFFu, most = 0u;
-        for_mine([&](float l, int i) {
-          if (member(l, i)) least = min(least, key_of(l)), most = max(most, key_of(l));
-        });
-        least = __reduce_min_sync(0xffffffffu, least), most = __reduce_max_sync(0xffffffffu, most);
-        u64 range = (static_cast<u64>(~least) << 32) | most, none = 0ull;  // (both as maxima)
-        auto both = [](u64 x, u64 y) {
-          const unsigned h = max(static_cast<unsigned>(x >> 32), static_cast<unsigned>(y >> 32)), l = max(static_cast<unsigned>(x), static_cast<unsigned>(y));
-          return (static_cast<u64>(h) << 32) | l;
-        };
-        range = k.over_warps(range, both);
-        k.exchange(range, none);
-        least = ~__reduce_max_sync(0xffffffffu, static_cast<unsigned>(range >> 32)), most = __reduce_max_sync(0xffffffffu, static_cast<unsigned>(range));
-        if (least == most) {  // equal logits: the first ones by index
-          const float l0 = of_key(most);
-          const u64 w = weigh(l0), r = count ? need : (need + w - 1ull) / w;
+        // (the keys of both signs end in the type's zero bits, negative ones inverted: all ones)
+        unsigned lo = key_of(fmaxf(from, cut_l)), hi = key_of(to);
+        lo = (lo & 0x80000000u) ? (lo + kZeros) & ~kZeros : lo | kZeros;
+        hi = (hi & 0x80000000u) ? hi & ~kZeros : (hi & kZeros) == kZeros ? hi : (hi | kZeros) - (kZeros + 1u);
+        if (lo >= hi) {  // equal logits: the first ones by index
+          const float l0 = of_key(hi);
+          const u64 r = count ? need : (need + weigh(l0) - 1ull) / weigh(l0);
           u64 here = 0ull, total, below;
-          for_mine([&](float l, int i) { here += l == l0; });
+          for_mine([&](const float (&l)[4], int i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) here += l[e] == l0;
+          });
           u64 before = k.scan(here, total);
-          k.exchange(total, none);
+          k.exchange(total);
           k.over_ctas(total, below);
           before += below;
           if (before < r && r <= before + here) {
             u64 at = before;
-            for_mine([&](float l, int i) {
-              if (l == l0 && ++at == r)
-                for (unsigned q = 0; q < ctas; ++q) remote_st(&s.found[0], q, static_cast<u64>(i));
-            });
+            const T* tokens = reinterpret_cast<const T*>(mine);
+            for (int j = 0; j < a.words * kIn; ++j)
+              if (static_cast<float>(tokens[j]) == l0 && ++at == r)
+                tell(0, mine_first + j);
           }
           csync();
           cut_l = l0, cut_i = static_cast<int>(s.found[0]);
-          return kept_w + r * w;
+          return;
         }
-        const int bits = 32 - __clz(most - least), shift = bits > 11 ? bits - 11 : 0;
+        const int bits = 32 - __clz(hi - lo), shift = bits > kBinBits ? bits - kBinBits : 0;
         clear();
-        for_mine([&](float l, int i) {
-          if (member(l, i)) count_in(static_cast<int>((most - key_of(l)) >> shift), l);
+        share(kBins);
+        for_mine([&](const float (&l)[4], int i) {
+          if (!__any_sync(0xffffffffu, some(l, from, to))) return;
+          u64 w[4] = {0ull, 0ull, 0ull, 0ull};
+          if (!count)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = weigh(l[e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (!(l[e] >= from && l[e] <= to && keeps(l[e], i + e))) continue;
+            const int b = static_cast<int>((hi - key_of(l[e])) >> shift);
+            atomicAdd(&s.hist[0][b], 1u);
+            if (count) continue;
+            atomicAdd(&s.hist[1][b], static_cast<unsigned>(w[e]) & 0x7FFFu);
+            atomicAdd(&s.hist[2][b], static_cast<unsigned>(w[e] >> 15) & 0x7FFFu);
+            atomicAdd(&s.hist[3][b], static_cast<unsigned>(w[e] >> 30));
+          }
         });
-        merge();
-        cross(count, need);
-        need -= count ? bin_c : bin_w;
-        kept_w += bin_w;
-        hi = most - (static_cast<unsigned>(bin) << shift);
-        lo = max(least, hi - ((1u << shift) - 1u));
-        ranged = divided = true;
+        merge(!count);
+        if (count) cross(need, c_before, count_of);
+        else cross(need, w_before, weight_of);
+        need -= bin_before, n = bin_n;
+        hi -= static_cast<unsigned>(bin) << shift;
+        lo = max(lo, hi - ((1u << shift) - 1u));
+        from = of_key(lo), to = of_key(hi);
       }
-      return kept_w;
     };
-    auto count_all = [&]() {
-      clear();
-      for_mine([&](float l, int i) {
-        if (keeps(l, i)) count_in(linear_bin(l), l);
-      });
-      merge();
-    };
+    // the logits whose bins are at most b, and at least b
+    auto lowest_of = [&](int b) { return b >= kFine - 1 ? cut_l : of_key(smallest(key_of(cut_l), key_of(top), [&](float l) { return fine_bin(l) <= b; })); };
+    auto highest_of = [&](int b) { return b <= 0 ? top : of_key(smallest(key_of(cut_l), key_of(top), [&](float l) { return fine_bin(l) < b; }) - 1u); };
 
-    u64 kept_w = 0ull;
-    if (by_count) {
-      counting = true;
-      count_all();
-      const bool all = c_total <= static_cast<u64>(top_k);  // (what weighs nothing is not counted)
-      u64 most = c_total;
-      if (!all) {
-        cross(true, static_cast<u64>(top_k));
-        most = bin_c + bin_n;
-      }
-      if (most <= kList) {
-        // all that can be kept is few: CTA 0 ranks it and finds the token
-        const int last_bin = bin;
-        const int m = static_cast<int>(gather([&](float l, int i) { return keeps(l, i) && (all || linear_bin(l) <= last_bin); }));
-        if (k.rank == 0) {
-          constexpr int kEach = kList / kThreads;
-          weigh_list(m);
-          unsigned rank[kEach];
-          u64 weight[kEach], w[kEach], sum = 0ull, total;
+    // tokens per bin
+    clear();
+    share(kFine);
+    for_mine([&](const float (&l)[4], int) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (l[e] >= cut_l) atomicAdd(&fine[fine_bin(l[e])], 1u);
+    });
+    merge(false);
+    const bool cuts = by_count && static_cast<u64>(top_k) < c_total;  // (what weighs nothing is not counted)
+    u64 candidates = c_total;
+    int last_bin = kFine - 1;
+    if (cuts) {
+      cross(static_cast<u64>(top_k), c_before, count_of);
+      candidates = bin_before + bin_n, last_bin = bin;
+    }
+    const float last_l = lowest_of(last_bin);
+    if (candidates <= kList) {
+      // all that can be kept is few: CTA 0 ranks it and finds the token
+      const int m = gather(last_l, top);
+      if (k.rank == 0) {
+        constexpr int kEach = (kList + kThreads - 1) / kThreads;
+        const unsigned most = by_count ? static_cast<unsigned>(top_k) : kList;
+        weigh_list(m);
+        unsigned rank[kEach];
+        u64 weight[kEach], w[kEach], total;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const int i = tid + e * kThreads;
+          w[e] = 0ull, rank[e] = 0u, weight[e] = 0ull;
+          if (i >= m) continue;
+          rank_of(i, m, rank[e], weight[e]);
+          if (rank[e] < most) w[e] = s.list_w[i];
+          sum += w[e];
+        }
+        k.scan(sum, total);
+        if (by_weight) {
+          const u64 limit = larger(1ull, static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(total))));
+          sum = 0ull;
 #pragma unroll
           for (int e = 0; e < kEach; ++e) {
-            const int i = tid + e * kThreads;
-            w[e] = 0ull, rank[e] = 0u, weight[e] = 0ull;
-            if (i >= m) continue;
-            rank_of(i, m, rank[e], weight[e]);
-            if (rank[e] < static_cast<unsigned>(top_k)) w[e] = s.list_w[i];
+            if (weight[e] >= limit) w[e] = 0ull;
             sum += w[e];
           }
           k.scan(sum, total);
-          if (by_weight) {
-            const u64 limit = larger(1ull, static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(total))));
-            sum = 0ull;
+        }
+        __syncthreads();
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) {
-              if (weight[e] >= limit) w[e] = 0ull;
-              sum += w[e];
-            }
-            k.scan(sum, total);
-          }
-          __syncthreads();
+        for (int e = 0; e < kEach; ++e)
+          if (tid + e * kThreads < m) s.list_w[tid + e * kThreads] = w[e];
+        __syncthreads();
+        const u64 target = smaller(static_cast<u64>(static_cast<double>(u) * static_cast<double>(total)), total - 1ull);
 #pragma unroll
-          for (int e = 0; e < kEach; ++e)
-            if (tid + e * kThreads < m) s.list_w[tid + e * kThreads] = w[e];
-          __syncthreads();
-          const u64 target = smaller(static_cast<u64>(static_cast<double>(u) * static_cast<double>(total)), total - 1ull);
-#pragma unroll
-          for (int e = 0; e < kEach; ++e) {
-            if (w[e] == 0ull) continue;
-            const unsigned own = static_cast<unsigned>(s.list[tid + e * kThreads]);
-            u64 before = 0ull;
+        for (int e = 0; e < kEach; ++e) {
+          if (w[e] == 0ull) continue;
+          const unsigned own = static_cast<unsigned>(s.list[tid + e * kThreads]);
+          u64 before = 0ull;
 #pragma unroll 4
-            for (int j = 0; j < m; ++j)
-              if (static_cast<unsigned>(s.list[j]) > own) before += s.list_w[j];  // (of a lower index)
-            if (before <= target && target < before + w[e]) {
-              a.tokens[row] = static_cast<int>(~own);
-              if (a.logprob) a.logprob[row] = static_cast<float>(log(static_cast<double>(w[e]) / static_cast<double>(total)));
-            }
+          for (int j = 0; j < m; ++j) before += static_cast<unsigned>(s.list[j]) > own ? s.list_w[j] : 0ull;  // (of a lower index)
+          if (before <= target && target < before + w[e]) {
+            a.tokens[row] = static_cast<int>(~own);
+            if (a.logprob) a.logprob[row] = static_cast<float>(log(static_cast<double>(w[e]) / static_cast<double>(total)));
           }
         }
-        csync();
-        return;
       }
-      if (!all) resolve(true, static_cast<u64>(top_k) - bin_c);
+      csync();
+      return;
     }
+    float from = cut_l, to = top;  // between which top_p cuts
+    u64 window = 0ull;             // tokens there
     if (by_weight) {
-      counting = false, weighing = true;
-      count_all();
-      kept_w = w_total;
-      const u64 limit = larger(1ull, static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(kept_w))));
-      cross(false, limit);
-      resolve(false, limit - bin_w);
+      // A bin's tokens times the weight at its middle is right to 1 / 240 in the exponent, sums of it and the limit that they
+      // are compared with too: the cut lies between the bins where 0.991 and 1.009 of the limit are reached
+      auto about = [&](int b) {
+        u64 n = fine[b];
+        if (cuts && b >= last_bin) n = b == last_bin ? static_cast<u64>(top_k) - bin_before : 0ull;
+        return n * static_cast<u64>(ex2_approx(static_cast<float>(b) * (-1.4426950408889634f / 120.f)) * 1099511627776.f);
+      };
+      u64 size = 0ull, total, below, c = c_before;
+      for (int b = my_bin; b < my_bin + my_bins; ++b) size += about(b);
+      u64 before = k.scan(size, total);
+      k.exchange(total);
+      const u64 all = k.over_ctas(total, below);
+      before += below;
+      const double limit = static_cast<double>(top_p) * static_cast<double>(all);
+      const u64 least = larger(1ull, static_cast<u64>(0.991 * limit)), most = smaller(all, static_cast<u64>(1.009 * limit) + 1ull);
+      for (int b = my_bin; b < my_bin + my_bins; ++b) {
+        const u64 after = before + about(b);
+        if (before < least && least <= after) tell(0, b), tell(1, c);
+        c += fine[b];
+        if (before < most && most <= after) tell(2, b), tell(3, c);
+        before = after;
+      }
+      csync();
+      const int b0 = static_cast<int>(s.found[0]), b1 = static_cast<int>(s.found[2]);
+      from = most == all ? cut_l : lowest_of(b1), to = highest_of(b0);  // (tokens of weight 0 here stand behind the last bin)
+      window = (most == all ? c_total : s.found[3]) - s.found[1];
+      csync();  // every CTA has read what it was told
+    }
+    if (cuts) resolve(true, static_cast<u64>(top_k) - bin_before, last_l, highest_of(last_bin), bin_n);
+    if (by_weight) {
+      // exact sums: of all that is kept, and of what lies above the window
+      u64 all = 0ull, t_all, t_above, below, none = 0ull;
+      if (dense) {
+        all = weight_of_all([&](float l, u64 w) { sum += l > to ? w : 0ull; });
+      } else for_mine([&](const float (&l)[4], int i) {
+        if (!__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= cut_l)) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u64 w = weigh(l[e]);
+          all += keeps(l[e], i + e) ? w : 0ull;
+          if (l[e] > to) sum += w;
+        }
+      });
+      k.scan(all, t_all), k.scan(sum, t_above);
+      k.exchange(t_all, t_above, none);
+      all = k.over_ctas(t_all, below);
+      const u64 limit = larger(1ull, static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(all))));
+      resolve(false, limit - k.over_ctas(t_above, below), from, to, window);
+      for_mine([&](const float (&l)[4], int i) {
+        if (!__any_sync(0xffffffffu, some(l, from, to))) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u64 w = weigh(l[e]);
+          sum += l[e] >= from && l[e] <= to && keeps(l[e], i + e) ? w : 0ull;
+        }
+      });
+    }
+  }
+  if (!by_weight) {
+    if (dense) {
+      sum = weight_of_all([](float, u64) {});
+    } else {
+      for_mine([&](const float (&l)[4], int i) {
+        // (a warp without any skips the exponentials)
+        if (!__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= cut_l)) return;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const u64 w = weigh(l[e]);
+          sum += keeps(l[e], i + e) ? w : 0ull;
+        }
+      });
     }
   }
 
   // ---------------- the token
-  u64 sum = 0ull, total, none = 0ull, below;
-  if (filtered) {
-    for_mine([&](float l, int i) {  // few of them: a warp without one skips the exponential
-      if (keeps(l, i)) sum += weigh(l);
-    });
-  } else {
-    for_mine([&](float l, int) {
-      const u64 w = weigh(l);
-      sum += l > cut_l ? w : 0ull;
-    });
-  }
+  u64 total, below;
   u64 before = k.scan(sum, total);
-  k.exchange(total, none);
+  k.exchange(total);
   cluster_arrive();  // this CTA has read what the others told
   const u64 all = k.over_ctas(total, below);
   before += below;
