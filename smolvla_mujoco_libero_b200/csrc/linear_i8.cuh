@@ -12,7 +12,7 @@
 //
 // Many rows (linear_i8_many_kernel).  Bound by the tensor pipe: CTA pairs compute 256 tokens x 256 weights (cta_group::2), which
 // halves the weights' way into each SM: an MMA of 128 x 256 x 32 per SM takes 128 cycles and 8 KB of shared memory, its operands
-// arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 8 epilogue warps.
+// arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 16 epilogue warps.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -60,15 +60,23 @@ struct Few {
   static constexpr int kP = GATED ? 2 : 1;
   static constexpr int kW = 128 * kSlice, kX = MT * kSlice;
   static constexpr int kStage = kP * kW + kX;
-  // two CTAs per SM (a tile's start and end beside the other's stream) where three stages fit twice, else one
-  static constexpr int kStages = kStage <= 32768 ? 98304 / kStage : 196608 / kStage;
+  // three CTAs per SM (a tile's start and end beside the others' streams) where three stages of each fit, or two, or one
+  static constexpr int kStages = (kStage <= 24576 ? 73728 : kStage <= 32768 ? 98304 : 196608) / kStage;
   static constexpr int kBar = kStages * kStage;
-  static constexpr int kBytes = kBar + 256 + 1024;  // + alignment slack
+  static constexpr int kScales = kBar + 256;              // of the tokens
+  static constexpr int kBytes = kScales + MT * 4 + 1024;  // + alignment slack
   static constexpr int kCols = kP * MT < 32 ? 32 : kP * MT;
   static_assert(kStages * kStage >= kP * MT * 512, "a tile's parts lie where its operands were");
   static_assert(kCols <= 512 && kBytes <= 232448);
 };
-constexpr int kFewThreads = 128;
+constexpr int kFewThreads = 256;
+
+// 32 lanes x 32 bit, 8 consecutive columns -> 8 registers per thread
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
 }  // namespace li8
 
 // One tile of 128 output channels x MT tokens per CTA, or per cluster of `splits` CTAs
@@ -109,6 +117,9 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
   pdl_trigger();
 
   bool ok = true;
+  float* scales = reinterpret_cast<float*>(smem + C::kScales);
+  if (warp >= 2)
+    for (int c = threadIdx.x - 64; c < MT; c += kFewThreads - 64) scales[c] = m0 + c < a.m ? __ldg(a.xscale + m0 + c) : 0.f;
   if (warp == 0) {
     for (int i = 0; i < ke - kb && ok; ++i) {
       const int s = i % C::kStages;
@@ -143,65 +154,73 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
       __syncwarp();
     }
   }
+  __syncthreads();  // the tokens' scales are there
   // (a producer or issuer that gave up leaves `done` alone, and this wait gives up too)
   ok = ke > kb ? serving::wait_warp(done, 0, a.err) : true;
   __syncwarp();
   tc_fence_after();
 
-  const int lane_n = threadIdx.x, n = n0 + lane_n;
-  const uint32_t t_row = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+  // warps w and w + 4 share the lanes 32 (w % 4) .. and take every other 8 tokens
+  const int lane_n = threadIdx.x & 127, part = threadIdx.x >> 7, n = n0 + lane_n;
+  const uint32_t t_row = tmem + (static_cast<uint32_t>(warp & 3) << 21);
   const int cols = min(MT, a.m - m0);
   const bool in = n < a.n;
   const float ws = in ? __ldg(a.wscale + n) : 0.f, wu = GATED && in ? __ldg(a.wscale + a.n + n) : 0.f;
   const float bias = a.bias && in ? __ldg(a.bias + n) : -0.f;
-  T* out = static_cast<T*>(a.out) + n;
-  const T* res = static_cast<const T*>(a.residual) + n;
-  auto finish = [&](uint32_t acc, uint32_t acc2, float xs, int m) {
+  auto value = [&](uint32_t acc, uint32_t acc2, float xs) {
     float v = scaled(acc, xs, ws);
     if constexpr (GATED) v = __fmul_rn(silu(v), scaled(acc2, xs, wu));
-    v = __fadd_rn(v, bias);
-    if (a.residual) v = __fadd_rn(v, static_cast<float>(res[m * a.residual_rs]));
-    put<T>(out + m * a.out_rs, v);
+    return __fadd_rn(v, bias);
   };
   if (a.splits == 1) {
-    for (int c = 0; c < cols; c += 16) {
-      uint32_t r[16], r2[GATED ? 16 : 1];
+    for (int c = part * 8; c < cols; c += 16) {
+      uint32_t r[8], r2[GATED ? 8 : 1];
       if (ok) {
-        tmem_ld16(t_row + c, r);
-        if constexpr (GATED) tmem_ld16(t_row + MT + c, reinterpret_cast<uint32_t(&)[16]>(r2));
+        tmem_ld8(t_row + c, r);
+        if constexpr (GATED) tmem_ld8(t_row + MT + c, reinterpret_cast<uint32_t(&)[8]>(r2));
         tmem_ld_wait();
       }
       if (ok && in) {
+        float v[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c + j < cols) finish(r[j], r2[GATED ? j : 0], __ldg(a.xscale + m0 + c + j), m0 + c + j);
+        for (int j = 0; j < 8; ++j) v[j] = value(r[j], r2[GATED ? j : 0], scales[c + j]);
+        const int some = min(8, cols - c);
+        if (a.residual) {
+          const T* res = static_cast<const T*>(a.residual) + (m0 + c) * a.residual_rs + n;
+#pragma unroll
+          for (int j = 0; j < 8; ++j, res += a.residual_rs)
+            if (j < some) v[j] = __fadd_rn(v[j], static_cast<float>(*res));
+        }
+        T* out = static_cast<T*>(a.out) + (m0 + c) * a.out_rs + n;
+#pragma unroll
+        for (int j = 0; j < 8; ++j, out += a.out_rs)
+          if (j < some) put<T>(out, v[j]);
       }
       __syncwarp();
     }
   } else {
-    uint32_t* part = reinterpret_cast<uint32_t*>(smem);  // [P][MT][128]; every operand has been read
-    for (int c = 0; c < cols; c += 16) {
-      uint32_t r[16], r2[GATED ? 16 : 1];
+    uint32_t* parts = reinterpret_cast<uint32_t*>(smem);  // [P][MT][128]; every operand has been read
+    for (int c = part * 8; c < cols; c += 16) {
+      uint32_t r[8], r2[GATED ? 8 : 1];
       if (ok && ke > kb) {
-        tmem_ld16(t_row + c, r);
-        if constexpr (GATED) tmem_ld16(t_row + MT + c, reinterpret_cast<uint32_t(&)[16]>(r2));
+        tmem_ld8(t_row + c, r);
+        if constexpr (GATED) tmem_ld8(t_row + MT + c, reinterpret_cast<uint32_t(&)[8]>(r2));
         tmem_ld_wait();
       } else {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = 0u, r2[GATED ? j : 0] = 0u;
+        for (int j = 0; j < 8; ++j) r[j] = 0u, r2[GATED ? j : 0] = 0u;
       }
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (c + j < cols) {
-          part[(c + j) * 128 + lane_n] = r[j];
-          if constexpr (GATED) part[(MT + c + j) * 128 + lane_n] = r2[j];
-        }
+      for (int j = 0; j < 8; ++j) {
+        parts[(c + j) * 128 + lane_n] = r[j];
+        if constexpr (GATED) parts[(MT + c + j) * 128 + lane_n] = r2[j];
+      }
     }
     __syncwarp();
     cluster_sync();
     if (ok && in) {
-      const uint32_t base = smem_u32(part) + lane_n * 4;
-      for (int c = split; c < cols; c += a.splits) {
+      const uint32_t base = smem_u32(parts) + lane_n * 4;
+      for (int c = split + part * a.splits; c < cols; c += 2 * a.splits) {
         uint32_t sum = 0u, sum2 = 0u;
 #pragma unroll 8
         for (int s = 0; s < a.splits; ++s) {
@@ -214,7 +233,9 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
             sum2 += v;
           }
         }
-        finish(sum, sum2, __ldg(a.xscale + m0 + c), m0 + c);
+        float v = value(sum, sum2, scales[c]);
+        if (a.residual) v = __fadd_rn(v, static_cast<float>(static_cast<const T*>(a.residual)[(m0 + c) * a.residual_rs + n]));
+        put<T>(static_cast<T*>(a.out) + (m0 + c) * a.out_rs + n, v);
       }
     }
     __syncwarp();
@@ -232,11 +253,11 @@ namespace li8 {
 struct Many {
   static constexpr int kStages = 6, kTile = 128 * kSlice, kStage = 2 * kTile;  // a CTA's rows of x and its half of w
   static constexpr int kBar = kStages * kStage;
-  static constexpr int kConst = kBar + 256;                // 8 warps x 2 x 128 column constants
-  static constexpr int kBytes = kConst + 8 * 256 * 4 + 1024;  // + alignment slack
+  static constexpr int kConst = kBar + 256;                    // 16 warps x 2 x 64 column constants
+  static constexpr int kBytes = kConst + 16 * 128 * 4 + 1024;  // + alignment slack
   static_assert(kBytes <= 232448);
 };
-constexpr int kManyThreads = 320;
+constexpr int kManyThreads = 576;  // TMA, MMA, 16 warps of epilogue
 }  // namespace li8
 
 // Tiles of 256 tokens x 256 weights (gated: 128 gates and their 128 ups) per CTA pair
@@ -264,7 +285,7 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 16);
+      mbar_init(&tempty[b], 32);
     }
     fence_mbar_init();
   }
@@ -330,9 +351,9 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
     }
   } else {
     const int q = warp & 3, part = (warp - 2) / 4;
-    float* consts = reinterpret_cast<float*>(smem + C::kConst) + (warp - 2) * 256;  // scales, then biases or ups' scales
+    float* consts = reinterpret_cast<float*>(smem + C::kConst) + (warp - 2) * 128;  // scales, then biases or ups' scales
     const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty[0]), 0), mapa_shared(smem_u32(&tempty[1]), 0)};
-    constexpr int kCols = kOutCols / 2;  // of this warp
+    constexpr int kCols = kOutCols / 4;  // of this warp
     bool ok = true;
     uint32_t lt = 0;
     for (int t = pair; t < tiles; t += pairs, ++lt) {
@@ -343,7 +364,7 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
       for (int c = lane; c < kCols; c += 32) {
         const bool in = c < cols;
         consts[c] = in ? __ldg(a.wscale + n0 + c) : 0.f;
-        consts[128 + c] = GATED ? (in ? __ldg(a.wscale + a.n + n0 + c) : 0.f) : (a.bias && in ? __ldg(a.bias + n0 + c) : -0.f);
+        consts[64 + c] = GATED ? (in ? __ldg(a.wscale + a.n + n0 + c) : 0.f) : (a.bias && in ? __ldg(a.bias + n0 + c) : -0.f);
       }
       const bool row = m < a.m;
       const float xs = row ? __ldg(a.xscale + m) : 0.f;
@@ -366,7 +387,7 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 w4 = *reinterpret_cast<const float4*>(consts + c + j);
-            const float4 b4 = *reinterpret_cast<const float4*>(consts + 128 + c + j);
+            const float4 b4 = *reinterpret_cast<const float4*>(consts + 64 + c + j);
             const float w[4] = {w4.x, w4.y, w4.z, w4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
