@@ -12,7 +12,9 @@
 //
 // Many rows (linear_i8_many_kernel).  Bound by the tensor pipe: CTA pairs compute 256 tokens x 256 weights (cta_group::2), which
 // halves the weights' way into each SM: an MMA of 128 x 256 x 32 per SM takes 128 cycles and 8 KB of shared memory, its operands
-// arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 16 epilogue warps.
+// arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 16 epilogue warps.  Outputs leave through
+// shared memory and TMA stores: written by the threads that own a row each, every warp's store touches 32 lines, and the stores'
+// way through L1 took 8000 cycles per tile.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -25,6 +27,7 @@ namespace svla {
 
 struct LinearI8Args {
   CUtensorMap tx, tw;  // 2-D (k, row), 128-byte swizzle
+  CUtensorMap to;      // many rows, staged: 2-D (n, row) of the output, a warp's box
   const float *xscale, *wscale, *bias;
   const void* residual;
   void* out;
@@ -32,7 +35,7 @@ struct LinearI8Args {
   int m, n, k;
   int tiles_m, tiles_n;
   int splits;  // few rows: CTAs of a cluster that share a tile's K
-  int wide;    // many rows: output (and residual) rows can be written 16 bytes at a time
+  int staged;  // many rows: outputs leave by TMA, which writes whole 16 bytes (and residual rows come 16 bytes at a time)
   int* err;
 };
 
@@ -251,13 +254,17 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
 
 namespace li8 {
 struct Many {
-  static constexpr int kStages = 6, kTile = 128 * kSlice, kStage = 2 * kTile;  // a CTA's rows of x and its half of w
-  static constexpr int kBar = kStages * kStage;
+  static constexpr int kStages = 4, kTile = 128 * kSlice, kStage = 2 * kTile;  // a CTA's rows of x and its half of w
+  static constexpr int kOut = kStages * kStage, kOutBox = 32 * 128;  // 16 warps' boxes of outputs, 32 rows of up to 128 bytes
+  static constexpr int kBar = kOut + 16 * kOutBox;
   static constexpr int kConst = kBar + 256;                    // 16 warps x 2 x 64 column constants
   static constexpr int kBytes = kConst + 16 * 128 * 4 + 1024;  // + alignment slack
   static_assert(kBytes <= 232448);
 };
 constexpr int kManyThreads = 576;  // TMA, MMA, 16 warps of epilogue
+// columns of a warp's box of outputs: 32 of a gated product or of fp32, 64 otherwise
+template <typename T, bool GATED>
+constexpr int kBoxCols = GATED || sizeof(T) == 4 ? 32 : 64;
 }  // namespace li8
 
 // Tiles of 256 tokens x 256 weights (gated: 128 gates and their 128 ups) per CTA pair
@@ -352,89 +359,154 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
   } else {
     const int q = warp & 3, part = (warp - 2) / 4;
     float* consts = reinterpret_cast<float*>(smem + C::kConst) + (warp - 2) * 128;  // scales, then biases or ups' scales
+    uint8_t* box = smem + C::kOut + (warp - 2) * C::kOutBox;
     const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty[0]), 0), mapa_shared(smem_u32(&tempty[1]), 0)};
     constexpr int kCols = kOutCols / 4;  // of this warp
+    // a tile's constants: fetched one tile ahead
+    float next[2 * kCols / 32], next_xs;
+    auto row_of = [&](int t) { return (t / a.tiles_n) * 256 + static_cast<int>(rank) * 128 + q * 32 + lane; };
+    auto fetch = [&](int t) {
+      if (t >= tiles) return;
+      const int n = (t % a.tiles_n) * kOutCols + part * kCols + lane, m = row_of(t);
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) {
+        const bool in = n + i * 32 < a.n;
+        next[2 * i] = in ? __ldg(a.wscale + n + i * 32) : 0.f;
+        next[2 * i + 1] = GATED ? (in ? __ldg(a.wscale + a.n + n + i * 32) : 0.f) : (a.bias && in ? __ldg(a.bias + n + i * 32) : -0.f);
+      }
+      next_xs = m < a.m ? __ldg(a.xscale + m) : 0.f;
+    };
+    fetch(pair);
     bool ok = true;
     uint32_t lt = 0;
     for (int t = pair; t < tiles; t += pairs, ++lt) {
       const uint32_t ab = lt & 1;
-      const int m = (t / a.tiles_n) * 256 + static_cast<int>(rank) * 128 + q * 32 + lane;
-      const int n0 = (t % a.tiles_n) * kOutCols + part * kCols;
-      const int cols = min(kCols, a.n - n0);
-      for (int c = lane; c < kCols; c += 32) {
-        const bool in = c < cols;
-        consts[c] = in ? __ldg(a.wscale + n0 + c) : 0.f;
-        consts[64 + c] = GATED ? (in ? __ldg(a.wscale + a.n + n0 + c) : 0.f) : (a.bias && in ? __ldg(a.bias + n0 + c) : -0.f);
-      }
-      const bool row = m < a.m;
-      const float xs = row ? __ldg(a.xscale + m) : 0.f;
-      T* out = static_cast<T*>(a.out) + m * a.out_rs + n0;
-      const T* res = static_cast<const T*>(a.residual) + m * a.residual_rs + n0;
+      const int m = row_of(t), n0 = (t % a.tiles_n) * kOutCols + part * kCols;
+      const int cols = max(0, min(kCols, a.n - n0));
+#pragma unroll
+      for (int i = 0; i < kCols / 32; ++i) consts[i * 32 + lane] = next[2 * i], consts[64 + i * 32 + lane] = next[2 * i + 1];
+      const float xs = next_xs;
+      fetch(t + pairs);
+      constexpr int kBox = kBoxCols<T, GATED>, kRowBytes = kBox * static_cast<int>(sizeof(T)), kChunks = kRowBytes / 16;
+      // place of a row's 16-byte chunk in the box, as the TMA's swizzle of 128- or 64-byte rows has it
+      auto at = [&](int r, int j) { return box + r * kRowBytes + ((kChunks == 8 ? j ^ (r & 7) : j ^ ((r >> 1) & 3)) << 4); };
+      const bool some = cols > 0 && m - lane < a.m;
+      // the box is free once its last store has read it; then the residual is brought there, whole lines at a time
+      auto residual_box = [&](int c) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+        if (!a.residual) return;
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) {
+          const int r = i * (32 / kChunks) + lane / kChunks, j = lane % kChunks, from = c + j * (16 / static_cast<int>(sizeof(T)));
+          const int bytes = m - lane + r < a.m ? max(0, min(16, (cols - from) * static_cast<int>(sizeof(T)))) : 0;
+          const T* res = static_cast<const T*>(a.residual);
+          serving::copy16(at(r, j), bytes ? res + (m - lane + r) * a.residual_rs + n0 + from : res, bytes);
+        }
+        serving::copy_commit();
+      };
+      if (a.staged && some) residual_box(0);
       __syncwarp();
       ok = ok && serving::wait_warp(&tfull[ab], (lt >> 1) & 1, a.err);
       tc_fence_after();
       const uint32_t t_row = tmem + ab * 256 + (static_cast<uint32_t>(q * 32) << 16) + part * kCols;
+      // the accumulator is free once its last columns are in registers; the arrival releases nothing beyond that (a release at
+      // cluster scope would wait for the stores)
+      auto give_back = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(tempty_leader[ab]) : "memory");
+      };
+      if (cols == 0) give_back();
 #pragma unroll 1
-      for (int c = 0; c < kCols && c < cols; c += 32) {
+      for (int c = 0; c < cols; c += 32) {
         uint32_t r[32], r2[GATED ? 32 : 1];
         if (ok) {
           tmem_ld32(t_row + c, r);
           if constexpr (GATED) tmem_ld32(t_row + 128 + c, reinterpret_cast<uint32_t(&)[32]>(r2));
           tmem_ld_wait();
         }
-        if (ok && row) {
-          float v[32];
+        if (c + 32 >= cols) give_back();
+        float v[32];
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 w4 = *reinterpret_cast<const float4*>(consts + c + j);
-            const float4 b4 = *reinterpret_cast<const float4*>(consts + 64 + c + j);
-            const float w[4] = {w4.x, w4.y, w4.z, w4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+        for (int j = 0; j < 32; j += 4) {
+          const float4 w4 = *reinterpret_cast<const float4*>(consts + c + j);
+          const float4 b4 = *reinterpret_cast<const float4*>(consts + 64 + c + j);
+          const float w[4] = {w4.x, w4.y, w4.z, w4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float y = scaled(r[j + e], xs, w[e]);
-              if constexpr (GATED) y = __fmul_rn(silu(y), scaled(r2[GATED ? j + e : 0], xs, b[e]));
-              else y = __fadd_rn(y, b[e]);
-              v[j + e] = y;
-            }
+          for (int e = 0; e < 4; ++e) {
+            float y = scaled(r[j + e], xs, w[e]);
+            if constexpr (GATED) y = __fmul_rn(silu(y), scaled(r2[GATED ? j + e : 0], xs, b[e]));
+            else y = __fadd_rn(y, b[e]);
+            v[j + e] = y;
           }
-          if (a.wide && c + 32 <= cols) {
-            constexpr int kPer = 16 / sizeof(T);
+        }
+        if (!some) continue;
+        if (a.staged) {
+          constexpr int kIn = 4 / static_cast<int>(sizeof(T)), kPer = 4 * kIn;  // outputs of a word, of 16 bytes
+          const int first = c % kBox;
+          if (a.residual && first == 0) {
+            serving::copy_wait<0>();
+            __syncwarp();
+          }
 #pragma unroll
-            for (int j = 0; j < 32; j += kPer) {
-              if (a.residual) {
-                const uint4 w = *reinterpret_cast<const uint4*>(res + c + j);
-                const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  if constexpr (sizeof(T) == 4) {
-                    v[j + e] = __fadd_rn(v[j + e], __uint_as_float(u[e]));
-                  } else {
-                    const float2 f = serving::unpack2<T>(u[e]);
-                    v[j + 2 * e] = __fadd_rn(v[j + 2 * e], f.x);
-                    v[j + 2 * e + 1] = __fadd_rn(v[j + 2 * e + 1], f.y);
-                  }
-                }
-              }
-              uint32_t p[4];
+          for (int j = 0; j < 32; j += kPer) {
+            uint4* place = reinterpret_cast<uint4*>(at(lane, (first + j) / kPer));
+            if (a.residual) {
+              const uint4 w = *place;
+              const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                if constexpr (sizeof(T) == 4) p[e] = __float_as_uint(v[j + e]);
-                else p[e] = serving::pack2<T>(v[j + 2 * e], v[j + 2 * e + 1]);
+                if constexpr (sizeof(T) == 4) {
+                  v[j + e] = __fadd_rn(v[j + e], __uint_as_float(u[e]));
+                } else {
+                  const float2 f = serving::unpack2<T>(u[e]);
+                  v[j + 2 * e] = __fadd_rn(v[j + 2 * e], f.x);
+                  v[j + 2 * e + 1] = __fadd_rn(v[j + 2 * e + 1], f.y);
+                }
               }
-              *reinterpret_cast<uint4*>(out + c + j) = make_uint4(p[0], p[1], p[2], p[3]);
             }
-          } else {
+            uint32_t p[4];
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c + j < cols) put<T>(out + c + j, a.residual ? __fadd_rn(v[j], static_cast<float>(res[c + j])) : v[j]);
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (sizeof(T) == 4) p[e] = __float_as_uint(v[j + e]);
+              else p[e] = serving::pack2<T>(v[j + 2 * e], v[j + 2 * e + 1]);
+            }
+            *place = make_uint4(p[0], p[1], p[2], p[3]);
+          }
+          if (first + 32 == kBox || c + 32 >= cols) {  // the box is complete (what is behind the last column TMA leaves out)
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && ok)
+              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;" ::"l"(
+                               reinterpret_cast<uint64_t>(&a.to)),
+                           "r"(n0 + c - first), "r"(m), "r"(smem_u32(box))
+                           : "memory");
+            __syncwarp();
+            if (c + 32 < cols) residual_box(c + 32);
+          }
+        } else {  // through the box as well, 32 columns in fp32, and on from there a row of them at a time
+#pragma unroll
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(box + lane * 128 + (((j / 4) ^ (lane & 7)) << 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          __syncwarp();
+          if (ok && c + lane < cols) {
+            const int rows = min(32, a.m - (m - lane));
+            T* out = static_cast<T*>(a.out) + (m - lane) * a.out_rs + n0 + c + lane;
+            const T* res = static_cast<const T*>(a.residual) + (m - lane) * a.residual_rs + n0 + c + lane;
+#pragma unroll 8
+            for (int i = 0; i < rows; ++i) {
+              float y = *reinterpret_cast<const float*>(box + i * 128 + (((lane / 4) ^ (i & 7)) << 4) + (lane % 4) * 4);
+              if (a.residual) y = __fadd_rn(y, static_cast<float>(res[i * a.residual_rs]));
+              put<T>(out + i * a.out_rs, y);
+            }
           }
         }
         __syncwarp();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty_leader[ab]);
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the box is read before the CTA ends
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();

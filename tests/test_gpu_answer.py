@@ -154,17 +154,26 @@ def product_check(m, n, k, dtype, gated=False, bias=False, residual=False, seed=
     y, size = A.product(x, xs, w, ws, b, r, gated)
     pad = lambda t: torch.nn.functional.pad(t, (0, -t.shape[1] % 16), value=111).to(DEV)[:, :t.shape[1]]  # noqa: E731
     out = torch.full((m, n + 5), 9.0, dtype=dtype, device=DEV)
-    for o in (None, out[:, :n]):
-        got = ops.linear_i8_rows(pad(x), dev(xs), pad(w), dev(ws), dev(b), dev(r), gated, dtype, o, impl)
+    # rows a multiple of 16 bytes apart, whatever n is; the residual likewise
+    wide = torch.full((m + 1, -(-n // 16) * 16 + 16), 9.0, dtype=dtype, device=DEV)
+    res = None if r is None else torch.full_like(wide, 5.0)
+    if r is not None:
+        res[:m, :n] = dev(r)
+    for o in (None, out[:, :n], wide[:m, :n]):
+        given = res[:m, :n] if r is not None and o is not None and o.stride(0) == wide.stride(0) else dev(r)
+        got = ops.linear_i8_rows(pad(x), dev(xs), pad(w), dev(ws), dev(b), given, gated, dtype, o, impl)
         assert got.dtype == dtype and got.shape == (m, n)
         off = (got.double().cpu() - y).abs() / A.product_tolerance(y, size, dtype)
         assert float(off.max()) <= 1, float(off.max())
-    assert bool((out[:, n:] == 9).all())
+    assert bool((out[:, n:] == 9).all()) and bool((wide[:m, n:] == 9).all()) and bool((wide[m:] == 9).all())
+    if r is not None:  # in place
+        got = ops.linear_i8_rows(pad(x), dev(xs), pad(w), dev(ws), dev(b), res[:m, :n], gated, dtype, res[:m, :n], impl)
+        assert torch.equal(got, wide[:m, :n]) and bool((res[:m, n:] == 5).all()) and bool((res[m:] == 5).all())
 
 
 FEW = [(1, 1600, 960), (1, 1, 1), (1, 7, 3), (2, 130, 77), (16, 128, 128), (17, 960, 2560), (33, 100, 16), (64, 4096, 960), (65, 129, 129),
        (128, 320, 4096), (129, 257, 640), (200, 960, 960), (256, 1000, 144)]
-MANY = [(1, 1, 1), (257, 256, 128), (300, 1000, 960), (512, 129, 77), (1000, 2560, 960), (11, 500, 2000), (2500, 8, 16)]
+MANY = [(1, 1, 1), (257, 256, 128), (300, 1000, 960), (700, 328, 200), (512, 129, 77), (1000, 2560, 960), (11, 500, 2000), (2500, 8, 16)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
