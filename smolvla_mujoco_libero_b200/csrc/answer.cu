@@ -58,16 +58,16 @@ int32_t make_tmap_i8(CUtensorMap* map, const void* base, uint64_t k, uint64_t ro
   return SVLA_OK;
 }
 
-// the output as (column, row) with a warp's box of 32 rows, of 64 or 128 bytes each
-int32_t make_tmap_out(CUtensorMap* map, const svla_linear_i8_desc* d, uint32_t cols, int size) {
+// the output as (column, row) with a warp's box of 32 rows of 64 bytes
+int32_t make_tmap_out(CUtensorMap* map, const svla_linear_i8_desc* d, int size) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return fail(SVLA_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
   cuuint64_t dims[2] = {static_cast<cuuint64_t>(d->n), static_cast<cuuint64_t>(d->m)};
   cuuint64_t strides[1] = {static_cast<cuuint64_t>(d->out_rs) * size};
-  cuuint32_t box[2] = {cols, 32};
+  cuuint32_t box[2] = {64u / size, 32};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, d->out, dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(SVLA_ERR_ARG, "cuTensorMapEncodeTiled (output) failed (%d)", static_cast<int>(r));
   return SVLA_OK;
@@ -104,7 +104,7 @@ int32_t launch_many(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStream_t 
   const int size = static_cast<int>(sizeof(T));
   auto by_16 = [&](const void* p, int64_t rs) { return aligned(p, 16) && rs * size % 16 == 0; };
   a.staged = d->n * size % 16 == 0 && by_16(a.out, a.out_rs) && (!a.residual || by_16(a.residual, a.residual_rs));
-  if (a.staged) if (int32_t rc = make_tmap_out(&a.to, d, li8::kBoxCols<T, GATED>, size)) return rc;
+  if (a.staged) if (int32_t rc = make_tmap_out(&a.to, d, size)) return rc;
   const long long pairs = sm_count() / 2;
   return launch_cluster(kern, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(li8::kManyThreads),
                         li8::Many::kBytes, st, "linear_i8_many_kernel", 2, a);

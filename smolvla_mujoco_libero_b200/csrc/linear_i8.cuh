@@ -12,7 +12,7 @@
 //
 // Many rows (linear_i8_many_kernel).  Bound by the tensor pipe: CTA pairs compute 256 tokens x 256 weights (cta_group::2), which
 // halves the weights' way into each SM: an MMA of 128 x 256 x 32 per SM takes 128 cycles and 8 KB of shared memory, its operands
-// arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 16 epilogue warps.  Outputs leave through
+// arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 8 epilogue warps for each.  Outputs leave through
 // shared memory and TMA stores: written by the threads that own a row each, every warp's store touches 32 lines, and the stores'
 // way through L1 took 8000 cycles per tile.
 #pragma once
@@ -255,16 +255,20 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
 namespace li8 {
 struct Many {
   static constexpr int kStages = 4, kTile = 128 * kSlice, kStage = 2 * kTile;  // a CTA's rows of x and its half of w
-  static constexpr int kOut = kStages * kStage, kOutBox = 32 * 128;  // 16 warps' boxes of outputs, 32 rows of up to 128 bytes
-  static constexpr int kBar = kOut + 16 * kOutBox;
-  static constexpr int kConst = kBar + 256;                    // 16 warps x 2 x 64 column constants
-  static constexpr int kBytes = kConst + 16 * 128 * 4 + 1024;  // + alignment slack
+  static constexpr int kOut = kStages * kStage, kBoxes = 4096;  // each epilogue warp's two boxes of 32 rows x 64 bytes
+  static constexpr int kBar = kOut + 16 * kBoxes;
+  static constexpr int kConst = kBar + 256;                    // each epilogue warp's 2 x 128 column constants
+  static constexpr int kBytes = kConst + 16 * 256 * 4 + 1024;  // + alignment slack
   static_assert(kBytes <= 232448);
 };
-constexpr int kManyThreads = 576;  // TMA, MMA, 16 warps of epilogue
-// columns of a warp's box of outputs: 32 of a gated product or of fp32, 64 otherwise
-template <typename T, bool GATED>
-constexpr int kBoxCols = GATED || sizeof(T) == 4 ? 32 : 64;
+constexpr int kManyThreads = 576;  // TMA, MMA, 2 x 8 warps of epilogue
+template <typename T>
+constexpr int kBoxCols = 64 / static_cast<int>(sizeof(T));
+// 16-byte chunk j of row r where rows of 64 or 128 bytes lie behind each other, spread over the banks as TMA's swizzles do
+template <int kRow>
+__device__ __forceinline__ uint8_t* spread(uint8_t* base, int r, int j) {
+  return base + r * kRow + ((kRow == 128 ? j ^ (r & 7) : j ^ ((r >> 1) & 3)) << 4);
+}
 }  // namespace li8
 
 // Tiles of 256 tokens x 256 weights (gated: 128 gates and their 128 ups) per CTA pair
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 32);
+      mbar_init(&tempty[b], 16);
     }
     fence_mbar_init();
   }
@@ -357,17 +361,19 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
       }
     }
   } else {
-    const int q = warp & 3, part = (warp - 2) / 4;
-    float* consts = reinterpret_cast<float*>(smem + C::kConst) + (warp - 2) * 128;  // scales, then biases or ups' scales
-    uint8_t* box = smem + C::kOut + (warp - 2) * C::kOutBox;
-    const uint32_t tempty_leader[2] = {mapa_shared(smem_u32(&tempty[0]), 0), mapa_shared(smem_u32(&tempty[1]), 0)};
-    constexpr int kCols = kOutCols / 4;  // of this warp
+    // Warps 2-9 take the even tiles and 10-17 the odd ones, so that one half's exponentials run beside the other's stores; of a
+    // tile, two warps per lane quarter have half of the columns each
+    const int q = warp & 3, part = ((warp - 2) / 4) & 1, half = (warp - 2) / 8;
+    constexpr int kCols = kOutCols / 2, kChunk = GATED ? 16 : 32, kBox = kBoxCols<T>, kPer = 16 / static_cast<int>(sizeof(T));
+    float* consts = reinterpret_cast<float*>(smem + C::kConst) + (warp - 2) * 256;  // scales, then biases or ups' scales
+    uint8_t* boxes = smem + C::kOut + (warp - 2) * C::kBoxes;
+    const uint32_t tempty_leader = mapa_shared(smem_u32(&tempty[half]), 0);
     // a tile's constants: fetched one tile ahead
     float next[2 * kCols / 32], next_xs;
-    auto row_of = [&](int t) { return (t / a.tiles_n) * 256 + static_cast<int>(rank) * 128 + q * 32 + lane; };
+    auto row0_of = [&](int t) { return (t / a.tiles_n) * 256 + static_cast<int>(rank) * 128 + q * 32; };
     auto fetch = [&](int t) {
       if (t >= tiles) return;
-      const int n = (t % a.tiles_n) * kOutCols + part * kCols + lane, m = row_of(t);
+      const int n = (t % a.tiles_n) * kOutCols + part * kCols + lane, m = row0_of(t) + lane;
 #pragma unroll
       for (int i = 0; i < kCols / 32; ++i) {
         const bool in = n + i * 32 < a.n;
@@ -376,62 +382,62 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
       }
       next_xs = m < a.m ? __ldg(a.xscale + m) : 0.f;
     };
-    fetch(pair);
+    fetch(pair + half * pairs);
     bool ok = true;
-    uint32_t lt = 0;
-    for (int t = pair; t < tiles; t += pairs, ++lt) {
-      const uint32_t ab = lt & 1;
-      const int m = row_of(t), n0 = (t % a.tiles_n) * kOutCols + part * kCols;
-      const int cols = max(0, min(kCols, a.n - n0));
+    int turn = 0;  // of the two boxes
+    uint32_t use = 0;
+    for (int t = pair + half * pairs; t < tiles; t += 2 * pairs, ++use) {
+      const int m0 = row0_of(t), n0 = (t % a.tiles_n) * kOutCols + part * kCols;
+      const int cols = m0 < a.m ? max(0, min(kCols, a.n - n0)) : 0, rows = min(32, a.m - m0);
 #pragma unroll
-      for (int i = 0; i < kCols / 32; ++i) consts[i * 32 + lane] = next[2 * i], consts[64 + i * 32 + lane] = next[2 * i + 1];
+      for (int i = 0; i < kCols / 32; ++i) consts[i * 32 + lane] = next[2 * i], consts[128 + i * 32 + lane] = next[2 * i + 1];
       const float xs = next_xs;
-      fetch(t + pairs);
-      constexpr int kBox = kBoxCols<T, GATED>, kRowBytes = kBox * static_cast<int>(sizeof(T)), kChunks = kRowBytes / 16;
-      // place of a row's 16-byte chunk in the box, as the TMA's swizzle of 128- or 64-byte rows has it
-      auto at = [&](int r, int j) { return box + r * kRowBytes + ((kChunks == 8 ? j ^ (r & 7) : j ^ ((r >> 1) & 3)) << 4); };
-      const bool some = cols > 0 && m - lane < a.m;
-      // the box is free once its last store has read it; then the residual is brought there, whole lines at a time
-      auto residual_box = [&](int c) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      fetch(t + 2 * pairs);
+      // a box is free once the store before the last has read it; then the residual is brought there, whole lines at a time
+      auto take_box = [&](int c) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
         __syncwarp();
         if (!a.residual) return;
 #pragma unroll
-        for (int i = 0; i < kChunks; ++i) {
-          const int r = i * (32 / kChunks) + lane / kChunks, j = lane % kChunks, from = c + j * (16 / static_cast<int>(sizeof(T)));
-          const int bytes = m - lane + r < a.m ? max(0, min(16, (cols - from) * static_cast<int>(sizeof(T)))) : 0;
+        for (int i = 0; i < 4; ++i) {
+          const int r = i * 8 + lane / 4, from = c + (lane % 4) * kPer;
+          const int bytes = r < rows ? max(0, min(16, (cols - from) * static_cast<int>(sizeof(T)))) : 0;
           const T* res = static_cast<const T*>(a.residual);
-          serving::copy16(at(r, j), bytes ? res + (m - lane + r) * a.residual_rs + n0 + from : res, bytes);
+          serving::copy16(spread<64>(boxes + turn * 2048, r, lane % 4), bytes ? res + (m0 + r) * a.residual_rs + n0 + from : res, bytes);
         }
         serving::copy_commit();
       };
-      if (a.staged && some) residual_box(0);
+      if (a.staged && cols > 0) take_box(0);
       __syncwarp();
-      ok = ok && serving::wait_warp(&tfull[ab], (lt >> 1) & 1, a.err);
+      ok = ok && serving::wait_warp(&tfull[half], use & 1, a.err);
       tc_fence_after();
-      const uint32_t t_row = tmem + ab * 256 + (static_cast<uint32_t>(q * 32) << 16) + part * kCols;
+      const uint32_t t_row = tmem + half * 256 + (static_cast<uint32_t>(q * 32) << 16) + part * kCols;
       // the accumulator is free once its last columns are in registers; the arrival releases nothing beyond that (a release at
       // cluster scope would wait for the stores)
       auto give_back = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(tempty_leader[ab]) : "memory");
+        if (lane == 0) asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(tempty_leader) : "memory");
       };
       if (cols == 0) give_back();
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 32) {
-        uint32_t r[32], r2[GATED ? 32 : 1];
+      for (int c = 0; c < cols; c += kChunk) {
+        uint32_t r[kChunk], r2[GATED ? kChunk : 1];
         if (ok) {
-          tmem_ld32(t_row + c, r);
-          if constexpr (GATED) tmem_ld32(t_row + 128 + c, reinterpret_cast<uint32_t(&)[32]>(r2));
+          if constexpr (GATED) {
+            tmem_ld16(t_row + c, r);
+            tmem_ld16(t_row + 128 + c, r2);
+          } else {
+            tmem_ld32(t_row + c, r);
+          }
           tmem_ld_wait();
         }
-        if (c + 32 >= cols) give_back();
-        float v[32];
+        if (c + kChunk >= cols) give_back();
+        float v[kChunk];
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
+        for (int j = 0; j < kChunk; j += 4) {
           const float4 w4 = *reinterpret_cast<const float4*>(consts + c + j);
-          const float4 b4 = *reinterpret_cast<const float4*>(consts + 64 + c + j);
+          const float4 b4 = *reinterpret_cast<const float4*>(consts + 128 + c + j);
           const float w[4] = {w4.x, w4.y, w4.z, w4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -441,62 +447,70 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
             v[j + e] = y;
           }
         }
-        if (!some) continue;
         if (a.staged) {
-          constexpr int kIn = 4 / static_cast<int>(sizeof(T)), kPer = 4 * kIn;  // outputs of a word, of 16 bytes
-          const int first = c % kBox;
-          if (a.residual && first == 0) {
-            serving::copy_wait<0>();
-            __syncwarp();
-          }
+          constexpr int kSub = kChunk < kBox ? kChunk : kBox;  // columns that go to one box at once
 #pragma unroll
-          for (int j = 0; j < 32; j += kPer) {
-            uint4* place = reinterpret_cast<uint4*>(at(lane, (first + j) / kPer));
-            if (a.residual) {
-              const uint4 w = *place;
-              const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          for (int u = 0; u < kChunk; u += kSub) {
+            if (c + u >= cols) break;
+            const int first = (c + u) % kBox;
+            uint8_t* box = boxes + turn * 2048;
+            if (a.residual && first == 0) {
+              serving::copy_wait<0>();
+              __syncwarp();
+            }
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if constexpr (sizeof(T) == 4) {
-                  v[j + e] = __fadd_rn(v[j + e], __uint_as_float(u[e]));
-                } else {
-                  const float2 f = serving::unpack2<T>(u[e]);
-                  v[j + 2 * e] = __fadd_rn(v[j + 2 * e], f.x);
-                  v[j + 2 * e + 1] = __fadd_rn(v[j + 2 * e + 1], f.y);
+            for (int j = u; j < u + kSub; j += kPer) {
+              uint4* place = reinterpret_cast<uint4*>(spread<64>(box, lane, (first + j - u) / kPer));
+              if (!GATED && a.residual) {
+                const uint4 w = *place;
+                const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  if constexpr (sizeof(T) == 4) {
+                    v[j + e] = __fadd_rn(v[j + e], __uint_as_float(x[e]));
+                  } else {
+                    const float2 f = serving::unpack2<T>(x[e]);
+                    v[j + 2 * e] = __fadd_rn(v[j + 2 * e], f.x);
+                    v[j + 2 * e + 1] = __fadd_rn(v[j + 2 * e + 1], f.y);
+                  }
                 }
               }
-            }
-            uint32_t p[4];
+              uint32_t p[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (sizeof(T) == 4) p[e] = __float_as_uint(v[j + e]);
-              else p[e] = serving::pack2<T>(v[j + 2 * e], v[j + 2 * e + 1]);
+              for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(T) == 4) p[e] = __float_as_uint(v[j + e]);
+                else p[e] = serving::pack2<T>(v[j + 2 * e], v[j + 2 * e + 1]);
+              }
+              *place = make_uint4(p[0], p[1], p[2], p[3]);
             }
-            *place = make_uint4(p[0], p[1], p[2], p[3]);
+            if (first + kSub == kBox || c + u + kSub >= cols) {  // the box is complete (what is behind the last column TMA leaves out)
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (ok)
+                  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                                   reinterpret_cast<uint64_t>(&a.to)),
+                               "r"(n0 + c + u - first), "r"(m0), "r"(smem_u32(box))
+                               : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+              }
+              turn ^= 1;
+              __syncwarp();
+              if (c + u + kSub < cols) take_box(c + u + kSub);
+            }
           }
-          if (first + 32 == kBox || c + 32 >= cols) {  // the box is complete (what is behind the last column TMA leaves out)
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0 && ok)
-              asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;" ::"l"(
-                               reinterpret_cast<uint64_t>(&a.to)),
-                           "r"(n0 + c - first), "r"(m), "r"(smem_u32(box))
-                           : "memory");
-            __syncwarp();
-            if (c + 32 < cols) residual_box(c + 32);
-          }
-        } else {  // through the box as well, 32 columns in fp32, and on from there a row of them at a time
+        } else {  // through the boxes as well, a chunk in fp32, and on from there a row or two of it at a time
+          constexpr int kRow = kChunk * 4;
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(box + lane * 128 + (((j / 4) ^ (lane & 7)) << 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          for (int j = 0; j < kChunk; j += 4) *reinterpret_cast<float4*>(spread<kRow>(boxes, lane, j / 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
           __syncwarp();
-          if (ok && c + lane < cols) {
-            const int rows = min(32, a.m - (m - lane));
-            T* out = static_cast<T*>(a.out) + (m - lane) * a.out_rs + n0 + c + lane;
-            const T* res = static_cast<const T*>(a.residual) + (m - lane) * a.residual_rs + n0 + c + lane;
+          const int col = lane % kChunk;
+          if (ok && c + col < cols) {
+            T* out = static_cast<T*>(a.out) + m0 * a.out_rs + n0 + c + col;
+            const T* res = static_cast<const T*>(a.residual) + m0 * a.residual_rs + n0 + c + col;
 #pragma unroll 8
-            for (int i = 0; i < rows; ++i) {
-              float y = *reinterpret_cast<const float*>(box + i * 128 + (((lane / 4) ^ (i & 7)) << 4) + (lane % 4) * 4);
+            for (int i = lane / kChunk; i < rows; i += 32 / kChunk) {
+              float y = *reinterpret_cast<const float*>(spread<kRow>(boxes, i, col / 4) + (col % 4) * 4);
               if (a.residual) y = __fadd_rn(y, static_cast<float>(res[i * a.residual_rs]));
               put<T>(out + i * a.out_rs, y);
             }
@@ -505,7 +519,7 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
         __syncwarp();
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the box is read before the CTA ends
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the boxes are read before the CTA ends
     __syncwarp();
   }
   tc_fence_before();
