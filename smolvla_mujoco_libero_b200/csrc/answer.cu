@@ -83,9 +83,11 @@ int32_t launch_few(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStream_t s
   a.tiles_m = (d->m + MT - 1) / MT, a.tiles_n = (d->n + 127) / 128;
   const long long tiles = static_cast<long long>(a.tiles_m) * a.tiles_n;
   const int slices = (d->k + li8::kSlice - 1) / li8::kSlice;
-  // K is shared by as many CTAs as leave a tile one, at most one round over the SMs
+  // K is shared where a tile's parts keep 5 slices at least, within one round over the SMs: adding them up costs 1 us with one
+  // token and 3 with 128 (K = 4096, N = 4096, 1 token: 5.7 us, alone 9.6; 128 tokens 9.6 and 11.9; K = 960, N = 1600, 1 token:
+  // 4.5 us by 8, alone 4.1; 128 tokens 7.7 and 5.9)
   a.splits = 1;
-  while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.splits * 2 <= slices) a.splits *= 2;
+  while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.splits * 10 <= slices) a.splits *= 2;
   if (tiles * a.splits > 0x7fffffffll) return fail(SVLA_ERR_ARG, "svla_linear_i8: too many tiles");
   return launch_cluster(kern, dim3(static_cast<unsigned>(tiles * a.splits)), dim3(li8::kFewThreads), li8::Few<MT, GATED>::kBytes, st,
                         "linear_i8_few_kernel", static_cast<unsigned>(a.splits), a);
@@ -112,14 +114,16 @@ int32_t launch_many(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStream_t 
 
 template <typename T, bool GATED>
 int32_t launch_linear(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStream_t st) {
-  const bool many = d->impl == SVLA_LINEAR_MANY || (d->impl == SVLA_LINEAR_AUTO && d->m > 256);
-  if (many) return launch_many<T, GATED>(a, d, st);
+  // Up to 128 rows the weights are read once by either kernel, and the one for few rows takes 15 us for 128 x 49280 where the
+  // other takes 25.  Beyond, it moves twice the bytes per product and starts 3 us earlier: it is the faster one while its
+  // tiles fit one round over the SMs (few / many, us: 768 x 1600 x 960, 78 tiles, 5.9 / 9.0; 512 x 4096 x 4096, 128 tiles, 12.2 /
+  // 15.6; 768 x 4096 x 4096, 192 tiles, 16.5 / 16.2; 177 x 49280 x 960, 770 tiles, 26 / 24)
+  const long long tiles = (static_cast<long long>(d->m) + 127) / 128 * ((static_cast<long long>(d->n) + 127) / 128);
+  if (d->impl == SVLA_LINEAR_MANY || (d->impl == SVLA_LINEAR_AUTO && d->m > 128 && tiles > sm_count())) return launch_many<T, GATED>(a, d, st);
   if (d->m <= 16) return launch_few<T, 16, GATED>(a, d, st);
   if (d->m <= 32) return launch_few<T, 32, GATED>(a, d, st);
   if (d->m <= 64) return launch_few<T, 64, GATED>(a, d, st);
-  if (d->m <= 128 || GATED) return launch_few<T, 128, GATED>(a, d, st);
-  if constexpr (!GATED) return launch_few<T, 256, false>(a, d, st);
-  return SVLA_OK;
+  return launch_few<T, 128, GATED>(a, d, st);
 }
 
 template <typename T>

@@ -221,24 +221,44 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
     }
     __syncwarp();
     cluster_sync();
-    if (ok && in) {
-      const uint32_t base = smem_u32(parts) + lane_n * 4;
-      for (int c = split + part * a.splits; c < cols; c += 2 * a.splits) {
-        uint32_t sum = 0u, sum2 = 0u;
-#pragma unroll 8
-        for (int s = 0; s < a.splits; ++s) {
+    // a warp adds up a token's 128 outputs, four a lane: the parts of all CTAs are on their way at once
+    if (ok) {
+      const int n4 = n0 + (threadIdx.x & 31) * 4;
+      float w4[4], u4[4], b4[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bool there = n4 + e < a.n;
+        w4[e] = there ? __ldg(a.wscale + n4 + e) : 0.f;
+        u4[e] = GATED && there ? __ldg(a.wscale + a.n + n4 + e) : 0.f;
+        b4[e] = a.bias && there ? __ldg(a.bias + n4 + e) : -0.f;
+      }
+      const uint32_t base = smem_u32(parts) + (threadIdx.x & 31) * 16;
+      for (int c = split + warp * a.splits; c < cols; c += (kFewThreads / 32) * a.splits) {
+        uint32_t sum[4] = {0u, 0u, 0u, 0u}, sum2[4] = {0u, 0u, 0u, 0u};
+        auto add = [&](uint32_t (&to)[4], uint32_t from) {
+          uint32_t v[4];
+          asm volatile("ld.shared::cluster.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(from));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) to[e] += v[e];
+        };
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          if (s >= a.splits) break;
           const uint32_t from = mapa_shared(base + c * 512, s);
-          uint32_t v;
-          asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(from));
-          sum += v;
-          if constexpr (GATED) {
-            asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(from + MT * 512));
-            sum2 += v;
-          }
+          add(sum, from);
+          if constexpr (GATED) add(sum2, from + MT * 512);
         }
-        float v = value(sum, sum2, scales[c]);
-        if (a.residual) v = __fadd_rn(v, static_cast<float>(static_cast<const T*>(a.residual)[(m0 + c) * a.residual_rs + n]));
-        put<T>(static_cast<T*>(a.out) + (m0 + c) * a.out_rs + n, v);
+        T* out = static_cast<T*>(a.out) + (m0 + c) * a.out_rs + n4;
+        const T* res = static_cast<const T*>(a.residual) + (m0 + c) * a.residual_rs + n4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (n4 + e >= a.n) break;
+          float v = scaled(sum[e], scales[c], w4[e]);
+          if constexpr (GATED) v = __fmul_rn(silu(v), scaled(sum2[e], scales[c], u4[e]));
+          v = __fadd_rn(v, b4[e]);
+          if (a.residual) v = __fadd_rn(v, static_cast<float>(res[e]));
+          put<T>(out + e, v);
+        }
       }
     }
     __syncwarp();
@@ -254,9 +274,11 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
 
 namespace li8 {
 struct Many {
-  static constexpr int kStages = 4, kTile = 128 * kSlice, kStage = 2 * kTile;  // a CTA's rows of x and its half of w
-  static constexpr int kOut = kStages * kStage, kBoxes = 4096;  // each epilogue warp's two boxes of 32 rows x 64 bytes
-  static constexpr int kBar = kOut + 16 * kBoxes;
+  // A CTA's rows of x and its half of w.  A stage more is worth more than a second box per warp: K = 11008 in 236 us, with 4
+  // stages and two boxes 256 (K = 960, gated: 49 and 48)
+  static constexpr int kStages = 5, kTile = 128 * kSlice, kStage = 2 * kTile;
+  static constexpr int kOut = kStages * kStage, kBoxBytes = 2048;  // each epilogue warp's box of 32 rows x 64 bytes
+  static constexpr int kBar = kOut + 16 * kBoxBytes;
   static constexpr int kConst = kBar + 256;                    // each epilogue warp's 2 x 128 column constants
   static constexpr int kBytes = kConst + 16 * 256 * 4 + 1024;  // + alignment slack
   static_assert(kBytes <= 232448);
@@ -264,11 +286,8 @@ struct Many {
 constexpr int kManyThreads = 576;  // TMA, MMA, 2 x 8 warps of epilogue
 template <typename T>
 constexpr int kBoxCols = 64 / static_cast<int>(sizeof(T));
-// 16-byte chunk j of row r where rows of 64 or 128 bytes lie behind each other, spread over the banks as TMA's swizzles do
-template <int kRow>
-__device__ __forceinline__ uint8_t* spread(uint8_t* base, int r, int j) {
-  return base + r * kRow + ((kRow == 128 ? j ^ (r & 7) : j ^ ((r >> 1) & 3)) << 4);
-}
+// 16-byte chunk j of a box's row r: rows of 64 bytes, spread over the banks as TMA's swizzle of them does
+__device__ __forceinline__ uint8_t* chunk_of(uint8_t* box, int r, int j) { return box + r * 64 + ((j ^ ((r >> 1) & 3)) << 4); }
 }  // namespace li8
 
 // Tiles of 256 tokens x 256 weights (gated: 128 gates and their 128 ups) per CTA pair
@@ -366,7 +385,7 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
     const int q = warp & 3, part = ((warp - 2) / 4) & 1, half = (warp - 2) / 8;
     constexpr int kCols = kOutCols / 2, kChunk = GATED ? 16 : 32, kBox = kBoxCols<T>, kPer = 16 / static_cast<int>(sizeof(T));
     float* consts = reinterpret_cast<float*>(smem + C::kConst) + (warp - 2) * 256;  // scales, then biases or ups' scales
-    uint8_t* boxes = smem + C::kOut + (warp - 2) * C::kBoxes;
+    uint8_t* box = smem + C::kOut + (warp - 2) * C::kBoxBytes;
     const uint32_t tempty_leader = mapa_shared(smem_u32(&tempty[half]), 0);
     // a tile's constants: fetched one tile ahead
     float next[2 * kCols / 32], next_xs;
@@ -384,7 +403,6 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
     };
     fetch(pair + half * pairs);
     bool ok = true;
-    int turn = 0;  // of the two boxes
     uint32_t use = 0;
     for (int t = pair + half * pairs; t < tiles; t += 2 * pairs, ++use) {
       const int m0 = row0_of(t), n0 = (t % a.tiles_n) * kOutCols + part * kCols;
@@ -393,9 +411,9 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
       for (int i = 0; i < kCols / 32; ++i) consts[i * 32 + lane] = next[2 * i], consts[128 + i * 32 + lane] = next[2 * i + 1];
       const float xs = next_xs;
       fetch(t + 2 * pairs);
-      // a box is free once the store before the last has read it; then the residual is brought there, whole lines at a time
+      // the box is free once its last store has read it; then the residual is brought there, whole lines at a time
       auto take_box = [&](int c) {
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
         if (!a.residual) return;
 #pragma unroll
@@ -403,7 +421,7 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
           const int r = i * 8 + lane / 4, from = c + (lane % 4) * kPer;
           const int bytes = r < rows ? max(0, min(16, (cols - from) * static_cast<int>(sizeof(T)))) : 0;
           const T* res = static_cast<const T*>(a.residual);
-          serving::copy16(spread<64>(boxes + turn * 2048, r, lane % 4), bytes ? res + (m0 + r) * a.residual_rs + n0 + from : res, bytes);
+          serving::copy16(chunk_of(box, r, lane % 4), bytes ? res + (m0 + r) * a.residual_rs + n0 + from : res, bytes);
         }
         serving::copy_commit();
       };
@@ -453,14 +471,13 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
           for (int u = 0; u < kChunk; u += kSub) {
             if (c + u >= cols) break;
             const int first = (c + u) % kBox;
-            uint8_t* box = boxes + turn * 2048;
             if (a.residual && first == 0) {
               serving::copy_wait<0>();
               __syncwarp();
             }
 #pragma unroll
             for (int j = u; j < u + kSub; j += kPer) {
-              uint4* place = reinterpret_cast<uint4*>(spread<64>(box, lane, (first + j - u) / kPer));
+              uint4* place = reinterpret_cast<uint4*>(chunk_of(box, lane, (first + j - u) / kPer));
               if (!GATED && a.residual) {
                 const uint4 w = *place;
                 const uint32_t x[4] = {w.x, w.y, w.z, w.w};
@@ -494,32 +511,35 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
                                : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
               }
-              turn ^= 1;
               __syncwarp();
               if (c + u + kSub < cols) take_box(c + u + kSub);
             }
           }
-        } else {  // through the boxes as well, a chunk in fp32, and on from there a row or two of it at a time
-          constexpr int kRow = kChunk * 4;
+        } else {  // through the box as well, 16 columns in fp32 at a time, and on from there two rows of them at a time
 #pragma unroll
-          for (int j = 0; j < kChunk; j += 4) *reinterpret_cast<float4*>(spread<kRow>(boxes, lane, j / 4)) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-          __syncwarp();
-          const int col = lane % kChunk;
-          if (ok && c + col < cols) {
-            T* out = static_cast<T*>(a.out) + m0 * a.out_rs + n0 + c + col;
-            const T* res = static_cast<const T*>(a.residual) + m0 * a.residual_rs + n0 + c + col;
+          for (int u = 0; u < kChunk; u += 16) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4)
+              *reinterpret_cast<float4*>(chunk_of(box, lane, j / 4)) = make_float4(v[u + j], v[u + j + 1], v[u + j + 2], v[u + j + 3]);
+            __syncwarp();
+            const int col = lane % 16, n = n0 + c + u + col;
+            if (ok && c + u + col < cols) {
+              T* out = static_cast<T*>(a.out) + m0 * a.out_rs + n;
+              const T* res = static_cast<const T*>(a.residual) + m0 * a.residual_rs + n;
 #pragma unroll 8
-            for (int i = lane / kChunk; i < rows; i += 32 / kChunk) {
-              float y = *reinterpret_cast<const float*>(spread<kRow>(boxes, i, col / 4) + (col % 4) * 4);
-              if (a.residual) y = __fadd_rn(y, static_cast<float>(res[i * a.residual_rs]));
-              put<T>(out + i * a.out_rs, y);
+              for (int i = lane / 16; i < rows; i += 2) {
+                float y = *reinterpret_cast<const float*>(chunk_of(box, i, col / 4) + (col % 4) * 4);
+                if (a.residual) y = __fadd_rn(y, static_cast<float>(res[i * a.residual_rs]));
+                put<T>(out + i * a.out_rs, y);
+              }
             }
+            __syncwarp();
           }
         }
         __syncwarp();
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the boxes are read before the CTA ends
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the box is read before the CTA ends
     __syncwarp();
   }
   tc_fence_before();
