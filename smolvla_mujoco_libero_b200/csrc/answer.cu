@@ -16,31 +16,29 @@ int32_t check_dtype16(const char* who, int32_t dtype) {
 }
 
 // ---------------------------------------------------------------- quantised rows
-template <typename T, bool VEC, int W, int CH>
+template <typename T, bool VEC, int CH>
 int32_t launch_quant(const QuantRowsArgs& a, cudaStream_t st) {
-  const unsigned blocks = W == 1 ? static_cast<unsigned>((static_cast<long long>(a.m) + 3) / 4) : static_cast<unsigned>(a.m);
-  return launch(quant_rows_kernel<T, VEC, W, CH>, dim3(blocks), dim3(W == 1 ? 128 : W * 32), 0, st, "quant_rows_kernel", a);
-}
-
-template <typename T, bool VEC, int W>
-int32_t launch_quant_w(const QuantRowsArgs& a, cudaStream_t st) {
-  const int chunks = (a.k + W * 256 - 1) / (W * 256);
-  if constexpr (W <= 4) {  // (more warps take rows of more than 2 chunks only)
-    if (chunks <= 1) return launch_quant<T, VEC, W, 1>(a, st);
-    if (chunks == 2) return launch_quant<T, VEC, W, 2>(a, st);
+  static int resident[64][qrows::kMaxWarps + 1] = {{0}};  // blocks that fit an SM
+  auto kern = quant_rows_kernel<T, VEC, CH>;
+  const int warps = (a.k + CH * 256 - 1) / (CH * 256);
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return fail(SVLA_ERR_ARG, "device index %d out of range", dev);
+  if (resident[dev][warps] == 0) {
+    int n = 0;
+    cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, warps * 32, 0);
+    if (e != cudaSuccess) return fail(SVLA_ERR_CUDA, "cudaOccupancyMaxActiveBlocksPerMultiprocessor: %s", cudaGetErrorString(e));
+    resident[dev][warps] = n < 1 ? 1 : n;
   }
-  if (chunks == 3) return launch_quant<T, VEC, W, 3>(a, st);
-  return launch_quant<T, VEC, W, 4>(a, st);
+  const int blocks = resident[dev][warps] * sm_count();
+  return launch(kern, dim3(static_cast<unsigned>(a.m < blocks ? a.m : blocks)), dim3(warps * 32), 0, st, "quant_rows_kernel", a);
 }
 
 template <typename T, bool VEC>
 int32_t launch_quant_t(const QuantRowsArgs& a, cudaStream_t st) {
-  // as few warps as hold the row; four where the rows are fewer than the GPU's warps
-  if (a.k <= 1024 && a.m > 8 * sm_count()) return launch_quant_w<T, VEC, 1>(a, st);
-  if (a.k <= 4096) return launch_quant_w<T, VEC, 4>(a, st);
-  if (a.k <= 8192) return launch_quant_w<T, VEC, 8>(a, st);
-  if (a.k <= 16384) return launch_quant_w<T, VEC, 16>(a, st);
-  return launch_quant_w<T, VEC, 32>(a, st);
+  if (a.k <= 8192 && a.m <= 2 * sm_count()) return launch_quant<T, VEC, 1>(a, st);
+  if (a.k <= 16384) return launch_quant<T, VEC, 2>(a, st);
+  return launch_quant<T, VEC, 4>(a, st);
 }
 
 // ---------------------------------------------------------------- int8 products
