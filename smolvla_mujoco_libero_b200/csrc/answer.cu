@@ -37,7 +37,7 @@ int32_t launch_quant(const QuantRowsArgs& a, cudaStream_t st) {
 template <typename T, bool VEC>
 int32_t launch_quant_t(const QuantRowsArgs& a, cudaStream_t st) {
   if (a.k <= 8192 && a.m <= 2 * sm_count()) return launch_quant<T, VEC, 1>(a, st);
-  if (a.k <= 16384) return launch_quant<T, VEC, 2>(a, st);
+  if (a.k <= 8192) return launch_quant<T, VEC, 2>(a, st);
   return launch_quant<T, VEC, 4>(a, st);
 }
 

@@ -6,7 +6,8 @@
 // The floor is memory: x and residual once in, h, codes and values once out.  A row is held in registers from its load to its
 // codes, so every statistic (mean, centred squares, largest magnitude) is a pass over registers and a round of shuffles (and one
 // of shared memory, where a row has several warps).  A block owns a row at a time, two chunks of 8 elements per thread, and asks
-// for its next row before it works on this one.
+// for its next row before it works on this one.  Instructions come next: pairs of elements go through the packed fp32 pipe (with
+// scalar operations 8192 rows of 4096 with everything took 53 instructions an element and 73 us).
 //
 // Sums and statistics in fp32, of the unrounded h.  Quotients are correctly rounded (quotient() below), so without a norm the
 // codes are those of the definition bit for bit.  A row that holds no finite maximum (an infinity, a NaN) has scale NaN and codes 0:
@@ -33,17 +34,19 @@ struct QuantRowsArgs {
 };
 
 namespace qrows {
-__device__ __forceinline__ float max_nan(float a, float b) {
+// max(a, |b|, |c|), NaN where one is; a >= 0
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// d / s correctly rounded, r = 1 / s correctly rounded: P. Markstein's correction of a quotient (Computation of elementary
-// functions on the IBM RISC System/6000 processor, 1990); the caller keeps s within 2^+-60 and |d| below 2^8 s
-__device__ __forceinline__ float quotient(float d, float s, float r) {
-  const float q = __fmul_rn(d, r);
-  return __fmaf_rn(__fmaf_rn(-q, s, d), r, q);
+// d / s correctly rounded, r = 1 / s correctly rounded, minus_s = -s: P. Markstein's correction of a quotient (Computation of
+// elementary functions on the IBM RISC System/6000 processor, 1990); the caller keeps s within 2^+-60 and |d| below 2^8 s
+__device__ __forceinline__ float2 quotient(float2 d, float2 minus_s, float2 r) {
+  const float2 q = __fmul2_rn(d, r);
+  return __ffma2_rn(__ffma2_rn(q, minus_s, d), r, q);
 }
 
 // 8 elements from column c as they are stored; VEC: 16 bytes at once, otherwise element by element up to k (zeros behind it)
@@ -61,67 +64,69 @@ __device__ __forceinline__ uint4 raw8(const T* row, int c, int k) {
   }
 }
 template <typename T>
-__device__ __forceinline__ void unpack8(float (&v)[8], const uint4& w) {
-  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = serving::unpack2<T>(u[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
+__device__ __forceinline__ void unpack8(float2 (&v)[4], const uint4& w) {
+  v[0] = serving::unpack2<T>(w.x), v[1] = serving::unpack2<T>(w.y), v[2] = serving::unpack2<T>(w.z), v[3] = serving::unpack2<T>(w.w);
 }
-template <typename T>
-__device__ __forceinline__ T rounded(float x);
-template <>
-__device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <>
-__device__ __forceinline__ __half rounded<__half>(float x) { return __float2half_rn(x); }
-
 template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, const float (&v)[8], int c, int k) {
+__device__ __forceinline__ void store8(T* row, const float2 (&v)[4], int c, int k) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) u[i] = serving::pack2<T>(v[i].x, v[i].y);
   if constexpr (VEC) {
-    *reinterpret_cast<uint4*>(row + c) = make_uint4(serving::pack2<T>(v[0], v[1]), serving::pack2<T>(v[2], v[3]),
-                                                    serving::pack2<T>(v[4], v[5]), serving::pack2<T>(v[6], v[7]));
+    *reinterpret_cast<uint4*>(row + c) = make_uint4(u[0], u[1], u[2], u[3]);
   } else {
+    uint16_t* p = reinterpret_cast<uint16_t*>(row);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (c + e < k) row[c + e] = rounded<T>(v[e]);
+      if (c + e < k) p[c + e] = static_cast<uint16_t>(u[e / 2] >> (16 * (e % 2)));
   }
 }
 
-enum class Join { Add, Max };
-template <Join J>
-__device__ __forceinline__ float join(float a, float b) {
-  if constexpr (J == Join::Add) return __fadd_rn(a, b);
-  else return max_nan(a, b);
-}
-// over the block's threads; `part` is used by one reduction of every other row only
-template <Join J>
-__device__ __forceinline__ float reduce_block(float v, float* part) {
+// Over the block's threads: a warp's lanes, then the warps through `part`, which holds zeros behind them and is used by one
+// reduction of every other row only.
+__device__ __forceinline__ float add_block(float v, float* part) {
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v = join<J>(v, __shfl_xor_sync(0xffffffffu, v, d));
+  for (int d = 16; d > 0; d >>= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, d));
   const int warps = blockDim.x >> 5;
   if (warps > 1) {
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = part[0];
-    for (int i = 1; i < warps; ++i) v = join<J>(v, part[i]);  // the same order in every thread
+    v = 0.f;
+    for (int i = 0; i < warps; i += 4) {  // the same order in every thread
+      const float4 p = *reinterpret_cast<const float4*>(part + i);
+      v = __fadd_rn(v, __fadd_rn(__fadd_rn(p.x, p.y), __fadd_rn(p.z, p.w)));
+    }
   }
   return v;
+}
+// the largest of values >= 0, NaN where one is: as integers they compare alike, and a NaN (without its sign) is above infinity
+__device__ __forceinline__ float max_block(float v, float* part) {
+  unsigned u = __reduce_max_sync(0xffffffffu, __float_as_uint(v) & 0x7FFFFFFFu);
+  const int warps = blockDim.x >> 5;
+  if (warps > 1) {
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = __uint_as_float(u);
+    __syncthreads();
+    for (int i = 0; i < warps; i += 4) {
+      const uint4 p = *reinterpret_cast<const uint4*>(part + i);
+      u = max(max(u, max(p.x, p.y)), max(p.z, p.w));
+    }
+  }
+  return __uint_as_float(u);
 }
 
 // y / s: by the hardware's reciprocal (2^-22 or so) and Markstein's correction where s is within 2^+-100 (off by half a step and
 // 2^-43), by the division itself elsewhere
-__device__ __forceinline__ void divide8(float (&y)[8], const float (&s)[8]) {
-  float least = fabsf(s[0]), most = least;
+__device__ __forceinline__ void divide8(float2 (&y)[4], const float2 (&s)[4]) {
+  float least = fabsf(s[0].x), most = 0.f;
 #pragma unroll
-  for (int e = 1; e < 8; ++e) least = fminf(least, fabsf(s[e])), most = fmaxf(most, fabsf(s[e]));
+  for (int e = 0; e < 4; ++e) least = fminf(least, fminf(fabsf(s[e].x), fabsf(s[e].y))), most = max_abs(most, s[e].x, s[e].y);
   if (least > 7.9e-31f && most < 1.2e30f) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = quotient(y[e], s[e], rcp_approx(s[e]));
+    for (int e = 0; e < 4; ++e)
+      y[e] = quotient(y[e], make_float2(-s[e].x, -s[e].y), make_float2(rcp_approx(s[e].x), rcp_approx(s[e].y)));
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __fdiv_rn(y[e], s[e]);
+    for (int e = 0; e < 4; ++e) y[e] = make_float2(__fdiv_rn(y[e].x, s[e].x), __fdiv_rn(y[e].y, s[e].y));
   }
 }
 constexpr int kMaxWarps = 32;
@@ -129,9 +134,11 @@ constexpr int kMaxWarps = 32;
 
 // CH chunks of 8 elements per thread; the block's threads hold a row
 template <typename T, bool VEC, int CH>
-__global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a) {
+__global__ void __launch_bounds__(CH == 2 ? 512 : 1024) quant_rows_kernel(const QuantRowsArgs a) {
   using namespace qrows;
-  __shared__ float part[2][3][kMaxWarps];
+  __shared__ __align__(16) float part[2][3][kMaxWarps];
+  for (int i = threadIdx.x; i < 6 * kMaxWarps; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
   const int k = a.k;
@@ -147,21 +154,29 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a)
       if (a.residual) rr[i] = column(i) < k ? raw8<T, VEC>(r, column(i), k) : make_uint4(0u, 0u, 0u, 0u);
     }
   };
-  // whether element e of chunk i is one of the row's (whole chunks are, where they are read at once)
-  auto in = [&](int i, int e) { return VEC ? column(i) < k : column(i) + e < k; };
+  // a chunk's elements behind the row's end set to zero (where chunks are read whole, the chunk is in or out)
+  auto clip = [&](float2 (&v)[4], int i) {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (column(i) + 2 * e >= k) v[e].x = 0.f;
+        if (column(i) + 2 * e + 1 >= k) v[e].y = 0.f;
+      }
+    }
+  };
   fetch(blockIdx.x);
   int turn = 0;
   for (long long row = blockIdx.x; row < a.m; row += gridDim.x, turn ^= 1) {
-    float y[CH][8];
+    float2 y[CH][4];
 #pragma unroll
     for (int i = 0; i < CH; ++i) unpack8<T>(y[i], rx[i]);
     if (a.residual) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        float v[8];
+        float2 v[4];
         unpack8<T>(v, rr[i]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[i][e] = __fadd_rn(y[i][e], v[e]);
+        for (int e = 0; e < 4; ++e) y[i][e] = __fadd2_rn(y[i][e], v[e]);
       }
     }
     fetch(row + gridDim.x);
@@ -177,46 +192,58 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a)
       // Squares beyond fp32's range (components above 1e17 or so) are seen in their sum; the row is then scaled by 2^-80, which
       // a norm does not notice, and its statistics are taken again.  The choice is the row's, so its threads agree.
       for (int pass = 0; pass < 2; ++pass) {
+        float2 sum = both(0.f);
         if (a.bias) {
-          mean = 0.f;
 #pragma unroll
           for (int i = 0; i < CH; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mean = __fadd_rn(mean, y[i][e]);
-          mean = __fmul_rn(reduce_block<Join::Add>(mean, part[turn][0]), inv);
-        }
-        squares = 0.f;
+            for (int e = 0; e < 4; ++e) sum = __fadd2_rn(sum, y[i][e]);
+          mean = __fmul_rn(add_block(__fadd_rn(sum.x, sum.y), part[turn][0]), inv);
+          sum = both(0.f);
 #pragma unroll
-        for (int i = 0; i < CH; ++i)
+          for (int i = 0; i < CH; ++i) {
+            if (column(i) >= k) continue;
+            float2 d[4];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float d = in(i, e) ? __fsub_rn(y[i][e], mean) : 0.f;
-            squares = __fmaf_rn(d, d, squares);
+            for (int e = 0; e < 4; ++e) d[e] = __fadd2_rn(y[i][e], both(-mean));
+            clip(d, i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum = __ffma2_rn(d[e], d[e], sum);
           }
-        squares = reduce_block<Join::Add>(squares, part[turn][1]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < CH; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum = __ffma2_rn(y[i][e], y[i][e], sum);
+        }
+        squares = add_block(__fadd_rn(sum.x, sum.y), part[turn][1]);
         if (pass == 1 || squares < __int_as_float(0x7f800000)) break;
         constexpr float kDown = 8.271806125530277e-25f;  // 2^-80
 #pragma unroll
         for (int i = 0; i < CH; ++i)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[i][e] = __fmul_rn(y[i][e], kDown);
+          for (int e = 0; e < 4; ++e) y[i][e] = __fmul2_rn(y[i][e], both(kDown));
         eps = 0.f;
         __syncthreads();  // the partial sums are read before they are written again
       }
-      const float rstd = __frsqrt_rn(__fmaf_rn(squares, inv, eps));
+      const float2 rstd = both(__frsqrt_rn(__fmaf_rn(squares, inv, eps)));
       const T* w = static_cast<const T*>(a.weight);
       const T* b = static_cast<const T*>(a.bias);
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         if (column(i) >= k) continue;
-        float g[8];
+        float2 g[4];
+        if (a.bias) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[i][e] = __fadd2_rn(y[i][e], both(-mean));
+        }
         unpack8<T>(g, raw8<T, VEC>(w, column(i), k));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[i][e] = __fmul_rn(__fmul_rn(__fsub_rn(y[i][e], mean), rstd), g[e]);
+        for (int e = 0; e < 4; ++e) y[i][e] = __fmul2_rn(__fmul2_rn(y[i][e], rstd), g[e]);
         if (a.bias) {
           unpack8<T>(g, raw8<T, VEC>(b, column(i), k));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[i][e] = __fadd_rn(y[i][e], g[e]);
+          for (int e = 0; e < 4; ++e) y[i][e] = __fadd2_rn(y[i][e], g[e]);
         }
       }
     }
@@ -224,50 +251,56 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a)
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         if (column(i) >= k) continue;
-        float d[8];
+        float2 d[4];
         if constexpr (VEC) {
           const float4* s = reinterpret_cast<const float4*>(a.smooth + column(i));
           const float4 s0 = __ldg(s), s1 = __ldg(s + 1);
-          d[0] = s0.x, d[1] = s0.y, d[2] = s0.z, d[3] = s0.w, d[4] = s1.x, d[5] = s1.y, d[6] = s1.z, d[7] = s1.w;
+          d[0] = make_float2(s0.x, s0.y), d[1] = make_float2(s0.z, s0.w), d[2] = make_float2(s1.x, s1.y), d[3] = make_float2(s1.z, s1.w);
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] = in(i, e) ? __ldg(a.smooth + column(i) + e) : 1.f;
+          for (int e = 0; e < 4; ++e) {
+            const int c = column(i) + 2 * e;
+            d[e] = make_float2(c < k ? __ldg(a.smooth + c) : 1.f, c + 1 < k ? __ldg(a.smooth + c + 1) : 1.f);
+          }
         }
         divide8(y[i], d);
       }
     }
     float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
+    for (int i = 0; i < CH; ++i) {
+      clip(y[i], i);  // (0 * infinity behind the end is no element's)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (in(i, e)) top = max_nan(top, fabsf(y[i][e]));
-    top = reduce_block<Join::Max>(top, part[turn][2]);
+      for (int e = 0; e < 4; ++e) top = max_abs(top, y[i][e].x, y[i][e].y);
+    }
+    top = max_block(top, part[turn][2]);
     const bool finite = top < __int_as_float(0x7f800000);
     const float scale = finite ? __fdiv_rn(top, 127.f) : __int_as_float(0x7fc00000);
     if (threadIdx.x == 0) a.scale[row] = scale;
     const bool plain = scale > 8.6e-19f && scale < 1.2e18f;  // 2^+-60
-    const float r = plain ? __frcp_rn(scale) : 0.f;
+    const float2 r = both(plain ? __frcp_rn(scale) : 0.f);
     int8_t* codes = a.codes + row * a.codes_rs;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
       if (column(i) >= k) continue;
-      float t[8];  // the code in the low bits: adding 1.5 * 2^23 rounds to an integer, ties to even
+      constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits, ties to even
+      float2 t[4];
       if (plain) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = __fadd_rn(quotient(y[i][e], scale, r), 12582912.f);  // (at most 127 (1 + 2^-23))
+        for (int e = 0; e < 4; ++e) t[e] = __fadd2_rn(quotient(y[i][e], both(-scale), r), both(kRound));  // (at most 127 (1 + 2^-23))
       } else {
+        auto code = [&](float v) {
+          const float q = scale > 0.f ? __fdiv_rn(v, scale) : 0.f;  // (NaN: no)
+          return __fadd_rn(fminf(fmaxf(q, -127.f), 127.f), kRound);
+        };
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float q = scale > 0.f ? __fdiv_rn(y[i][e], scale) : 0.f;  // (NaN: no)
-          t[e] = __fadd_rn(fminf(fmaxf(q, -127.f), 127.f), 12582912.f);
-        }
+        for (int e = 0; e < 4; ++e) t[e] = make_float2(code(y[i][e].x), code(y[i][e].y));
       }
       uint32_t packed[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint32_t lo = __byte_perm(__float_as_uint(t[4 * h]), __float_as_uint(t[4 * h + 1]), 0x0040);
-        const uint32_t hi = __byte_perm(__float_as_uint(t[4 * h + 2]), __float_as_uint(t[4 * h + 3]), 0x0040);
+        const uint32_t lo = __byte_perm(__float_as_uint(t[2 * h].x), __float_as_uint(t[2 * h].y), 0x0040);
+        const uint32_t hi = __byte_perm(__float_as_uint(t[2 * h + 1].x), __float_as_uint(t[2 * h + 1].y), 0x0040);
         packed[h] = __byte_perm(lo, hi, 0x5410);
       }
       if constexpr (VEC) {
@@ -275,11 +308,11 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a)
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (in(i, e)) codes[column(i) + e] = static_cast<int8_t>(packed[e / 4] >> (8 * (e % 4)));
+          if (column(i) + e < k) codes[column(i) + e] = static_cast<int8_t>(packed[e / 4] >> (8 * (e % 4)));
       }
       if (a.values) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) t[e] = __fmul_rn(__fsub_rn(t[e], 12582912.f), scale);
+        for (int e = 0; e < 4; ++e) t[e] = __fmul2_rn(__fadd2_rn(t[e], both(-kRound)), both(scale));
         store8<T, VEC>(static_cast<T*>(a.values) + row * a.values_rs, t, column(i), k);
       }
     }
