@@ -96,7 +96,7 @@ def build_torch(force: bool = False) -> Path:
                     f'-DSVLA_TORCH_TAG="{torch_tag()}"',
                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
                     *[a for p in include for a in ("-isystem", str(p))], "-o", str(TORCH_OUT), str(TORCH_SRC),
-                    f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"], check=True)
+                    f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python"], check=True)
     return TORCH_OUT
 
 

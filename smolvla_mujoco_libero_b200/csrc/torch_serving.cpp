@@ -2,6 +2,7 @@
 // sample_tokens of ops.py): the tensors' checks, the outputs and the call of the C ABI.  In C++ because a single token's operators take less time on the GPU than an
 // interpreter needs to look at a dozen tensors: an append of one token, called again and again, takes 5.9 us, 12.5 with the
 // checks in Python and the call through ctypes (attention of one token 6.0 and 11.0).
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/extension.h>
@@ -278,6 +279,11 @@ struct Where {
   }
 };
 
+// an output from torch's allocator, without the dispatcher's way there (half a microsecond each)
+Tensor fresh(const Where& w, at::IntArrayRef sizes, at::ScalarType dtype) {
+  return Tensor(at::detail::empty_cuda(sizes, dtype, c10::Device(c10::kCUDA, static_cast<c10::DeviceIndex>(w.dev)), std::nullopt));
+}
+
 int32_t dtype_code(at::ScalarType t) {
   return t == at::kHalf ? SVLA_DT_HALF : t == at::kBFloat16 ? SVLA_DT_BF16 : t == at::kFloat ? SVLA_DT_FLOAT : -1;
 }
@@ -298,15 +304,15 @@ py::tuple quantize_rows(const Tensor& x, const Opt& weight, const Opt& bias, dou
     d.codes_rs = w.matrix(*codes, "codes", at::kChar, m, k, k);
   } else {  // rows 16 bytes apart, as the product takes them
     d.codes_rs = (k + 15) / 16 * 16;
-    codes = x.new_empty({m, d.codes_rs}, x.options().dtype(at::kChar));
+    codes = fresh(w, {m, d.codes_rs}, at::kChar);
     if (d.codes_rs != k) codes = codes->narrow(1, 0, k);
   }
   if (scale) w.vector(*scale, "scale", at::kFloat, m);
-  else scale = x.new_empty({m}, x.options().dtype(at::kFloat));
+  else scale = fresh(w, {m}, at::kFloat);
   if (sum) d.sum_rs = w.matrix(*sum, "sum", t, m, k, k);
-  else if (residual) sum = x.new_empty({m, k}), d.sum_rs = k;
+  else if (residual) sum = fresh(w, {m, k}, t), d.sum_rs = k;
   if (values) d.values_rs = w.matrix(*values, "values", t, m, k, k);
-  else if (want_values) values = x.new_empty({m, k}), d.values_rs = k;
+  else if (want_values) values = fresh(w, {m, k}, t), d.values_rs = k;
   d.x = x.const_data_ptr(), d.codes = static_cast<int8_t*>(codes->data_ptr()), d.scale = static_cast<float*>(scale->data_ptr());
   if (sum) d.sum = sum->data_ptr();
   if (values) d.values = values->data_ptr();
@@ -332,7 +338,7 @@ Tensor linear_i8_rows(const Tensor& x, const Tensor& xscale, const Tensor& weigh
   if (bias) d.bias = static_cast<const float*>(w.vector(*bias, "bias", at::kFloat, n));
   if (residual) d.residual_rs = w.matrix(*residual, "residual", dtype, m, n, n), d.residual = residual->const_data_ptr();
   if (out) d.out_rs = w.matrix(*out, "out", dtype, m, n, n);
-  else out = x.new_empty({m, n}, x.options().dtype(dtype)), d.out_rs = n;
+  else out = fresh(w, {m, n}, dtype), d.out_rs = n;
   d.x = static_cast<const int8_t*>(x.const_data_ptr()), d.w = static_cast<const int8_t*>(weight.const_data_ptr());
   d.out = out->data_ptr();
   d.m = i32(m, "the number of rows"), d.n = i32(n, "n"), d.k = i32(k, "k");
@@ -364,9 +370,9 @@ py::tuple sample_tokens(const Tensor& logits, const Tensor& u, const py::object&
   setting(w, top_p, "top_p", at::kFloat, batch, &d.top_p, &d.top_p_value);
   setting(w, min_p, "min_p", at::kFloat, batch, &d.min_p, &d.min_p_value);
   if (tokens) w.vector(*tokens, "tokens", at::kInt, batch);
-  else tokens = logits.new_empty({batch}, logits.options().dtype(at::kInt));
+  else tokens = fresh(w, {batch}, at::kInt);
   if (logprob) w.vector(*logprob, "logprob", at::kFloat, batch);
-  else logprob = logits.new_empty({batch}, logits.options().dtype(at::kFloat));
+  else logprob = fresh(w, {batch}, at::kFloat);
   d.logits = logits.const_data_ptr();
   d.tokens = static_cast<int32_t*>(tokens->data_ptr()), d.logprob = static_cast<float*>(logprob->data_ptr());
   d.batch = i32(batch, "the number of rows"), d.vocab = i32(vocab, "vocab"), d.dtype = dtype_code(t);
