@@ -23,6 +23,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "ptx.cuh"
 #include "serving_common.cuh"
 
@@ -46,7 +48,7 @@ using u64 = unsigned long long;
 constexpr int kThreads = 256, kWarps = kThreads / 32, kBinBits = 10, kBins = 1 << kBinBits, kFine = 4 * kBins, kList = 256, kMaxCtas = 8;
 constexpr double kUnit = 17592186044416.0;  // 2^44
 
-__device__ const double kPowers[64] = {  // 2^(j / 64)
+__device__ const double kPowers[64] = {  // 2^(j / 64); shared memory holds them times 2^44
     1.0, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
     1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
     1.0905077326652577, 1.102382583307841, 1.1143867425958924, 1.1265216186082418,
@@ -101,8 +103,8 @@ struct Weigh {
     p = fma(f, p, 0.010830424696239445);
     p = fma(f, p, 1.0);
     p *= powers[n & 63];
-    // times 2^(44 + n / 64), then rounded to an integer by adding 2^52
-    p = __hiloint2double(__double2hiint(p) + ((44 + (n >> 6)) << 20), __double2loint(p)) + 4503599627370496.0;
+    // times 2^(n / 64), whole octaves in the exponent, then rounded to an integer by adding 2^52
+    p = __hiloint2double(__double2hiint(p) + ((n << 14) & 0xFFF00000), __double2loint(p)) + 4503599627370496.0;
     return static_cast<u64>(__double_as_longlong(p));
   }
 };
@@ -227,6 +229,15 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// the larger ones of two pairs of 16-bit logits, NaN where one is
+template <typename T>
+__device__ __forceinline__ unsigned max2(unsigned a, unsigned b) {
+  unsigned r;
+  if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
 // the low bits that are 0 in every logit of the type, as fp32
 template <typename T>
 constexpr int kZeroBits = 0;
@@ -255,7 +266,7 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
   Block k{s, cluster_ctarank(), ctas, static_cast<int>(threadIdx.x), static_cast<int>(threadIdx.x & 31), static_cast<int>(threadIdx.x >> 5), 0u, 0u};
   const int tid = k.tid, lane = k.lane;
   const long long row = blockIdx.x / ctas;
-  if (tid < 64) s.powers[tid] = kPowers[tid];
+  if (tid < 64) s.powers[tid] = kPowers[tid] * kUnit;
   if (tid < 2) s.listed[tid] = 0u;
   pdl_wait();
   pdl_trigger();
@@ -279,12 +290,11 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
       for (int i = tid; i < done / kPer; i += kThreads) {
         const uint4 w = __ldcs(reinterpret_cast<const uint4*>(src) + i);
         reinterpret_cast<uint4*>(row_words)[i] = w;
-        const unsigned u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 l = logits_of<T>(u[e]);
-          top = max_nan(top, l.x);
-          if constexpr (kIn == 2) top = max_nan(top, l.y);
+        if constexpr (kIn == 1) {
+          top = max_nan(max_nan(top, max_nan(__uint_as_float(w.x), __uint_as_float(w.y))), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
+        } else {
+          const float2 l = logits_of<T>(max2<T>(max2<T>(w.x, w.y), max2<T>(w.z, w.w)));
+          top = max_nan(top, max_nan(l.x, l.y));
         }
       }
     }
@@ -313,18 +323,26 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
   // f(four logits, index of the first) over this thread's tokens; -infinity behind the last
   auto for_mine = [&](auto f) {
     constexpr int kGroup = 4 / kIn;
-#pragma unroll 1
-    for (int j = 0; j < a.words; j += kGroup) {
+    int j = 0;
+    for (; j + kGroup <= a.words; j += kGroup) {
       float l[4];
 #pragma unroll
       for (int e = 0; e < kGroup; ++e) {
-        const bool in = e == 0 || j + e < a.words;
-        const float2 v = logits_of<T>(in ? mine[j + e] : 0u);
-        l[e * kIn] = in ? v.x : -INFINITY;
-        if constexpr (kIn == 2) l[e * kIn + 1] = in ? v.y : -INFINITY;
+        const float2 v = logits_of<T>(mine[j + e]);
+        l[e * kIn] = v.x;
+        if constexpr (kIn == 2) l[e * kIn + 1] = v.y;
       }
       f(l, mine_first + j * kIn);
     }
+    float l[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (an odd number of words: there is a rest)
+#pragma unroll
+    for (int e = 0; e < kGroup - 1; ++e) {
+      if (j + e >= a.words) break;
+      const float2 v = logits_of<T>(mine[j + e]);
+      l[e * kIn] = v.x;
+      if constexpr (kIn == 2) l[e * kIn + 1] = v.y;
+    }
+    f(l, mine_first + j * kIn);
   };
   // a row without a finite largest logit or with a NaN, and settings that are none
   const bool bad = !(fabsf(top) < INFINITY) || !(temperature >= 0.f && temperature < INFINITY) || !(top_p >= 0.f) || !(min_p >= 0.f) || !(u >= 0.f && u <= 1.f);
