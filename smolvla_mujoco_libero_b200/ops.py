@@ -419,7 +419,7 @@ def quantize_rows(x: torch.Tensor, weight: torch.Tensor | None = None, bias: tor
                   residual: torch.Tensor | None = None, smooth: torch.Tensor | None = None, want_values: bool = False,
                   codes: torch.Tensor | None = None, scale: torch.Tensor | None = None, sum: torch.Tensor | None = None,
                   values: torch.Tensor | None = None) -> QuantizedRows:
-    """Rows of bf16 or fp16 x [rows, k] (any row stride) in int8 with a scale each: h = x + residual, its RMSNorm (``weight``) or
+    """Rows of bf16 or fp16 x [rows, k] (rows any distance apart, not overlapping) in int8 with a scale each: h = x + residual, its RMSNorm (``weight``) or
     LayerNorm (``weight`` and ``bias``), divided by ``smooth`` (fp32 [k]); scale = max |y| / 127, codes = round(y / scale).
     ``sum`` is h (there with a residual; it may be x or the residual itself), ``values`` what the codes stand for
     (``want_values``: the activations that a fake-quantised linear multiplies, deploy/linear_only_quant.py:140-162).  A row
@@ -529,3 +529,39 @@ def _paged_attention_op(q: torch.Tensor, cache: torch.Tensor, cu_q: torch.Tensor
 @_paged_attention_op.register_fake
 def _(q, cache, cu_q, kv_len, page_table, scale):
     return q.new_empty(q.shape)
+
+
+@torch.library.custom_op("svla::quantize_rows", mutates_args=())
+def _quantize_rows_op(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+                      residual: torch.Tensor | None, smooth: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    r = quantize_rows(x, weight, bias, eps, residual, smooth)
+    return r.codes, r.scale, x.new_empty(0, x.shape[1]) if r.sum is None else r.sum
+
+
+@_quantize_rows_op.register_fake
+def _(x, weight, bias, eps, residual, smooth):
+    m, k = x.shape
+    codes = x.new_empty(m, -(-k // 16) * 16, dtype=torch.int8)[:, :k]
+    return codes, x.new_empty(m, dtype=torch.float32), x.new_empty(0 if residual is None else m, k)
+
+
+@torch.library.custom_op("svla::linear_i8_rows", mutates_args=())
+def _linear_i8_rows_op(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, wscale: torch.Tensor,
+                       bias: torch.Tensor | None, residual: torch.Tensor | None, gated: bool, dtype: torch.dtype) -> torch.Tensor:
+    return linear_i8_rows(x, x_scale, weight, wscale, bias, residual, gated, dtype)
+
+
+@_linear_i8_rows_op.register_fake
+def _(x, x_scale, weight, wscale, bias, residual, gated, dtype):
+    return x.new_empty(x.shape[0], weight.shape[0] // 2 if gated else weight.shape[0], dtype=dtype)
+
+
+@torch.library.custom_op("svla::sample_tokens", mutates_args=())
+def _sample_tokens_op(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None, top_k: torch.Tensor | None,
+                      top_p: torch.Tensor | None, min_p: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+    return sample_tokens(logits, u, temperature, top_k, top_p, min_p)
+
+
+@_sample_tokens_op.register_fake
+def _(logits, u, temperature, top_k, top_p, min_p):
+    return logits.new_empty(logits.shape[0], dtype=torch.int32), logits.new_empty(logits.shape[0], dtype=torch.float32)
