@@ -19,12 +19,13 @@ int32_t launch_sample(SampleArgs& a, cudaStream_t st) {
   auto bytes = [](int words) { return static_cast<int>(sizeof(sample::Shared)) + words * sample::kThreads * 4; };
   if (int32_t rc = allow_smem(kern, bytes(words(kSampleVocab, sample::kMaxCtas)), configured)) return rc;
   // CTAs of about a thousand tokens or more each, up to 8, which is the fastest for what fits the GPU at once (one row of 49280
-  // tokens with top_k and top_p: 12.4 us, 13.8 with 4, 17.4 with 2); many rows of no more than 88 KB of shared memory per CTA
-  // have less to begin, to tell one another and to join with 4 (256 mixed rows 44 us, 66 with 8, 62 with 2; 512 rows
-  // without filters 51, 73 and 46)
+  // tokens with top_k and top_p: 12.6 us, 13.8 with 4, 17.4 with 2); many rows have less to begin, to tell one another and to join
+  // with as few as leave three CTAs to an SM (256 mixed rows in fp32: 45 us with 4, 62 with 2, 66 with 8; 512 rows without filters
+  // in bf16: 46 with 2, 50 with 4, 73 with 8)
   int ctas = 1;
   while (ctas < sample::kMaxCtas && a.vocab > 1024 * ctas) ctas *= 2;
-  if (ctas == 8 && 2ll * a.batch > sm_count() && bytes(words(a.vocab, 4)) <= 88 * 1024) ctas = 4;
+  if (2ll * a.batch > sm_count())
+    while (ctas > 2 && bytes(words(a.vocab, ctas / 2)) <= 75 * 1024) ctas /= 2;
   a.words = words(a.vocab, ctas);
   return launch_cluster(kern, dim3(static_cast<unsigned>(a.batch) * ctas), dim3(sample::kThreads), bytes(a.words), st, "sample_kernel",
                         static_cast<unsigned>(ctas), a);

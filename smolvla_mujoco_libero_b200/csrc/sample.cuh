@@ -68,8 +68,8 @@ __device__ const double kPowers[64] = {  // 2^(j / 64); shared memory holds them
 
 struct alignas(16) Shared {
   unsigned hist[4][kBins];  // at first kFine bins of tokens; later tokens, and the weights' bits 0-14, 15-29 and 30-44 (sums of 2^16 of them stay in 32 bits)
-  u64 list[kList], list_w[kList];
-  u64 own[kList];           // of this CTA, on their way to the list of CTA 0
+  u64 list[kList];
+  u64 list_w[kList];        // CTA 0's; before that, in every CTA, the tokens that go to CTA 0's list
   double powers[64];
   u64 exch[2][3];           // what the CTAs tell one another, in turn
   u64 warp_sum[2][kWarps];
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
         for (int e = 0; e < 4; ++e)
           if (l[e] >= from && l[e] <= to && keeps(l[e], i + e)) {
             const unsigned at = atomicAdd(&s.own_n, 1u);
-            if (at < kList) s.own[at] = place_of(l[e], i + e);
+            if (at < kList) s.list_w[at] = place_of(l[e], i + e);
           }
       });
       __syncthreads();
@@ -519,7 +519,7 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
       __syncthreads();
       if (n) {
         const unsigned at = s.own_at;
-        for (unsigned i = tid; i < n && at + i < kList; i += kThreads) remote_st(&s.list[at + i], 0, s.own[i]);
+        for (unsigned i = tid; i < n && at + i < kList; i += kThreads) remote_st(&s.list[at + i], 0, s.list_w[i]);
       }
       csync();
       const unsigned all = min(remote_ld(&s.listed[gather_turn], 0), static_cast<unsigned>(kList));
