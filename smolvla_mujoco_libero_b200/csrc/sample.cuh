@@ -9,10 +9,11 @@
 // A cluster of up to 8 CTAs holds a row in shared memory, read once from DRAM; every later pass is over shared memory, a
 // thread's tokens next to each other (an odd number of words: no bank conflicts), so thread order is index order.  Without
 // filters there is one pass of exponentials and a scan.  Filters need the place where a running count (top_k) or a running weight
-// (top_p), in falling order of the logits, reaches a limit: a histogram over 1024 bins of (max - l) / temperature, whose bins
-// the CTAs add up by shares through distributed shared memory, gives the bin.  Up to 256 tokens are then ranked by one CTA: all
-// that top_k leaves, and the token is found among them at once, or those of the bin.  A bin of more is divided again, by the bits
-// of its logits; one of equal logits is cut by index.
+// (top_p), in falling order of the logits, reaches a limit.  Tokens are counted in 4096 bins of (max - l) / temperature, whose bins
+// the CTAs add up by shares through distributed shared memory.  That gives the bin where top_k cuts; where all that is left is
+// up to 256 tokens, one CTA ranks them and finds the token at once.  Otherwise counts times weights at the bins' middles say
+// between which logits top_p cuts, one pass of exponentials gives the exact sums around them, and what lies between is noted:
+// up to 256 of them one CTA ranks, more are divided by the bits of their logits, equal ones are cut by index.
 //
 // The exponential, P. T. P. Tang's table-driven method (Table-driven implementation of the exponential function in IEEE
 // floating-point arithmetic, 1989) in 64 bits: (l - max) 64 log2(e) / temperature = n + f, 2^(n / 64) from a table of 64 and the
@@ -45,7 +46,8 @@ struct SampleArgs {
 
 namespace sample {
 using u64 = unsigned long long;
-constexpr int kThreads = 256, kWarps = kThreads / 32, kBinBits = 10, kBins = 1 << kBinBits, kFine = 4 * kBins, kList = 256, kMaxCtas = 8;
+constexpr int kThreads = 256, kWarps = kThreads / 32, kBinBits = 9, kBins = 1 << kBinBits, kFine = 8 * kBins, kList = 256, kMaxCtas = 8;
+constexpr int kNear = 4 * kBins * 2;
 constexpr double kUnit = 17592186044416.0;  // 2^44
 
 __device__ const double kPowers[64] = {  // 2^(j / 64); shared memory holds them times 2^44
@@ -67,7 +69,13 @@ __device__ const double kPowers[64] = {  // 2^(j / 64); shared memory holds them
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.978456026387951};
 
 struct alignas(16) Shared {
-  unsigned hist[4][kBins];  // at first kFine bins of tokens; later tokens, and the weights' bits 0-14, 15-29 and 30-44 (sums of 2^16 of them stay in 32 bits)
+  union {
+    unsigned fine[kFine];        // at first: tokens per bin
+    struct {
+      unsigned hist[4][kBins];   // then: tokens, and the weights' bits 0-14, 15-29 and 30-44 (sums of 2^16 of them stay in 32 bits)
+      unsigned short near[kNear];  // this CTA's tokens about the cut, by their places in its share
+    };
+  };
   u64 list[kList];
   u64 list_w[kList];        // CTA 0's; before that, in every CTA, the tokens that go to CTA 0's list
   double powers[64];
@@ -400,12 +408,12 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
   // the sum of all weights, 2^52 in front of each taken off at the end; what is raised to cut_l weighs nothing
   auto weight_of_all = [&](auto more) {
     u64 all = 0ull;
-    for_mine([&](const float (&l)[4], int) {
+    for_mine([&](const float (&l)[4], int i) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const u64 w = weigh.bits(fmaxf(l[e], cut_l));
         all += w;
-        more(l[e], w & 0xFFFFFFFFFFFFFull);
+        more(l, e, i, w & 0xFFFFFFFFFFFFFull);
       }
     });
     return all - static_cast<u64>((a.words * kIn + 3) / 4 * 4) * 0x4330000000000000ull;
@@ -429,7 +437,7 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
     // at first bins of 1 / 120 of the temperature: what is kept lies less than 33 (or one step of the logits) below the largest
     const float to_bin = fminf(120.f / temperature, 3.4028234663852886e38f);
     auto fine_bin = [&](float l) { return __float2int_rn(fminf(__fmul_rn(__fsub_rn(top, l), to_bin), static_cast<float>(kFine - 1))); };
-    unsigned* fine = &s.hist[0][0];
+    unsigned* fine = s.fine;
     int my_bin = 0, my_bins = 0;  // this thread's of this CTA's share of the bins
     auto share = [&](int bins) {
       const int per = bins / static_cast<int>(ctas), per_thread = max(4, per / kThreads);
@@ -438,6 +446,24 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
     auto clear = [&]() {
       for (int i = tid; i < kBins; i += kThreads) reinterpret_cast<uint4*>(&s.hist[0][0])[i] = make_uint4(0u, 0u, 0u, 0u);
       __syncthreads();
+    };
+    // f(logit, index) of this CTA's kept tokens from one logit to another: from the list of those about the cut, once it is
+    // there and holds them, or from all
+    int near_n = -1;
+    auto for_members = [&](float from, float to, auto f) {
+      if (near_n >= 0 && near_n <= kNear) {
+        for (int j = tid; j < near_n; j += kThreads) {
+          const int at = s.near[j];
+          const float l = static_cast<float>(reinterpret_cast<const T*>(row_words)[at]);
+          if (l >= from && l <= to && keeps(l, first + at)) f(l, first + at);
+        }
+      } else {
+        for_mine([&](const float (&l)[4], int i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (l[e] >= from && l[e] <= to && keeps(l[e], i + e)) f(l[e], i + e);
+        });
+      }
     };
     // the CTAs' histograms added up: each CTA's share of the bins lies in its own hist[0] (tokens) and hist[1], hist[2] (weight)
     u64 c_before = 0ull, w_before = 0ull, c_total = 0ull;  // tokens and weight before this thread's bins, tokens of all bins
@@ -493,25 +519,14 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
       csync();
       bin = static_cast<int>(s.found[0]), bin_n = s.found[1], bin_before = s.found[2];
     };
-    auto some = [](const float (&l)[4], float from, float to) {  // any of the four between the two
-      bool in = false;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) in |= l[e] >= from && l[e] <= to;
-      return in;
-    };
     // the tokens from one logit to another, as far as they are kept, to the list of CTA 0; -> how many there are, at most kList
     unsigned gather_turn = 0u;
     auto gather = [&](float from, float to) -> int {
       if (tid == 0) s.own_n = 0u;
       __syncthreads();
-      for_mine([&](const float (&l)[4], int i) {
-        if (!some(l, from, to)) return;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (l[e] >= from && l[e] <= to && keeps(l[e], i + e)) {
-            const unsigned at = atomicAdd(&s.own_n, 1u);
-            if (at < kList) s.list_w[at] = place_of(l[e], i + e);
-          }
+      for_members(from, to, [&](float l, int i) {
+        const unsigned at = atomicAdd(&s.own_n, 1u);
+        if (at < kList) s.list_w[at] = place_of(l, i);
       });
       __syncthreads();
       const unsigned n = min(s.own_n, static_cast<unsigned>(kList));
@@ -598,23 +613,16 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
         const int bits = 32 - __clz(hi - lo), shift = bits > kBinBits ? bits - kBinBits : 0;
         clear();
         share(kBins);
-        for_mine([&](const float (&l)[4], int i) {
-          if (!__any_sync(0xffffffffu, some(l, from, to))) return;
-          u64 w[4] = {0ull, 0ull, 0ull, 0ull};
-          if (!count)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = weigh(l[e]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (!(l[e] >= from && l[e] <= to && keeps(l[e], i + e))) continue;
-            const int b = static_cast<int>((hi - key_of(l[e])) >> shift);
-            atomicAdd(&s.hist[0][b], 1u);
-            if (count) continue;
-            atomicAdd(&s.hist[1][b], static_cast<unsigned>(w[e]) & 0x7FFFu);
-            atomicAdd(&s.hist[2][b], static_cast<unsigned>(w[e] >> 15) & 0x7FFFu);
-            atomicAdd(&s.hist[3][b], static_cast<unsigned>(w[e] >> 30));
-          }
+        for_members(from, to, [&](float l, int) {
+          const int b = static_cast<int>((hi - key_of(l)) >> shift);
+          atomicAdd(&s.hist[0][b], 1u);
+          if (count) return;
+          const u64 w = weigh(l);
+          atomicAdd(&s.hist[1][b], static_cast<unsigned>(w) & 0x7FFFu);
+          atomicAdd(&s.hist[2][b], static_cast<unsigned>(w >> 15) & 0x7FFFu);
+          atomicAdd(&s.hist[3][b], static_cast<unsigned>(w >> 30));
         });
+        __syncwarp();
         merge(!count);
         if (count) cross(need, c_before, count_of);
         else cross(need, w_before, weight_of);
@@ -629,7 +637,8 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
     auto highest_of = [&](int b) { return b <= 0 ? top : of_key(smallest(key_of(cut_l), key_of(top), [&](float l) { return fine_bin(l) < b; }) - 1u); };
 
     // tokens per bin
-    clear();
+    for (int i = tid; i < kFine / 4; i += kThreads) reinterpret_cast<uint4*>(fine)[i] = make_uint4(0u, 0u, 0u, 0u);
+    __syncthreads();
     share(kFine);
     for_mine([&](const float (&l)[4], int) {
 #pragma unroll
@@ -729,37 +738,55 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
     }
     if (cuts) resolve(true, static_cast<u64>(top_k) - bin_before, last_l, highest_of(last_bin), bin_n);
     if (by_weight) {
-      // exact sums: of all that is kept, and of what lies above the window
+      // exact sums: of all that is kept, and of what lies above the window; the window's tokens are noted
+      if (tid == 0) s.own_n = 0u;
+      __syncthreads();
+      auto note = [&](const float (&l)[4], int e, int i, u64 w) {
+        if (l[e] > to) sum += w;
+        else if (l[e] >= from) {
+          const unsigned at = atomicAdd(&s.own_n, 1u);
+          if (at < kNear) s.near[at] = static_cast<unsigned short>(i + e - first);
+        }
+      };
       u64 all = 0ull, t_all, t_above, below, none = 0ull;
       if (dense) {
-        all = weight_of_all([&](float l, u64 w) { sum += l > to ? w : 0ull; });
-      } else for_mine([&](const float (&l)[4], int i) {
-        if (!__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= cut_l)) return;
+        all = weight_of_all(note);
+      } else {
+        for_mine([&](const float (&l)[4], int i) {
+          if (!__any_sync(0xffffffffu, fmaxf(fmaxf(l[0], l[1]), fmaxf(l[2], l[3])) >= cut_l)) return;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const u64 w = weigh(l[e]);
-          all += keeps(l[e], i + e) ? w : 0ull;
-          if (l[e] > to) sum += w;
-        }
-      });
+          for (int e = 0; e < 4; ++e) {
+            const u64 w = weigh(l[e]);
+            if (!keeps(l[e], i + e)) continue;
+            all += w;
+            note(l, e, i, w);
+          }
+        });
+      }
+      __syncwarp();
       k.scan(all, t_all), k.scan(sum, t_above);
+      near_n = static_cast<int>(s.own_n);
       k.exchange(t_all, t_above, none);
       all = k.over_ctas(t_all, below);
       const u64 limit = larger(1ull, static_cast<u64>(ceil(static_cast<double>(top_p) * static_cast<double>(all))));
       resolve(false, limit - k.over_ctas(t_above, below), from, to, window);
-      for_mine([&](const float (&l)[4], int i) {
-        if (!__any_sync(0xffffffffu, some(l, from, to))) return;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const u64 w = weigh(l[e]);
-          sum += l[e] >= from && l[e] <= to && keeps(l[e], i + e) ? w : 0ull;
-        }
+      // what is kept of the window, added to the threads whose tokens it is: bits 0-21 and 22-44 of the weights
+      unsigned* extra = &s.hist[0][0];
+      for (int i = tid; i < 2 * kThreads; i += kThreads) extra[i] = 0u;
+      __syncthreads();
+      for_members(from, to, [&](float l, int i) {
+        const u64 w = weigh(l);
+        const int owner = (i - first) / (a.words * kIn);
+        atomicAdd(&extra[owner], static_cast<unsigned>(w) & 0x3FFFFFu);
+        atomicAdd(&extra[kThreads + owner], static_cast<unsigned>(w >> 22));
       });
+      __syncthreads();
+      sum += extra[tid] + (static_cast<u64>(extra[kThreads + tid]) << 22);
     }
   }
   if (!by_weight) {
     if (dense) {
-      sum = weight_of_all([](float, u64) {});
+      sum = weight_of_all([](const float (&)[4], int, int, u64) {});
     } else {
       for_mine([&](const float (&l)[4], int i) {
         // (a warp without any skips the exponentials)
