@@ -8,13 +8,17 @@
 // Few rows (linear_i8_few_kernel).  The floor is the weights' bytes, so the weights are the M side of the MMA (128 of them per
 // tile) and up to MT tokens its N side: no tensor time goes into empty rows, a lane of tensor memory is an output channel, and
 // a token's outputs leave in whole lines.  Where the tiles are fewer than the SMs, a cluster of up to 8 CTAs shares a tile's K
-// and adds its parts through distributed shared memory; whole numbers, so the order does not matter.
+// and adds its parts through distributed shared memory; whole numbers, so the order does not matter.  64 x 49280 x 960 to fp32:
+// 13.8 us, 4.4 TB/s (385 tiles in one round of three CTAs per SM; 27 us with 4 epilogue warps and two CTAs); one row by 1600 x 960:
+// 3.9 us, of which the launch is 2.
 //
 // Many rows (linear_i8_many_kernel).  Bound by the tensor pipe: CTA pairs compute 256 tokens x 256 weights (cta_group::2), which
 // halves the weights' way into each SM: an MMA of 128 x 256 x 32 per SM takes 128 cycles and 8 KB of shared memory, its operands
 // arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 8 epilogue warps for each.  Outputs leave through
 // shared memory and TMA stores: written by the threads that own a row each, every warp's store touches 32 lines, and the stores'
 // way through L1 took 8000 cycles per tile.
+// 8192 x 4096 x 11008: 231 us, 3.2 POPS (275 back to back, under the power cap); 11328 x 2560 x 960, gated: 49 us, 2.3 POPS, where a
+// tile has 8 slices of K only and its epilogue (two int32 conversions, an exponential and a reciprocal per output) takes as long.
 #pragma once
 
 #include <cuda_bf16.h>

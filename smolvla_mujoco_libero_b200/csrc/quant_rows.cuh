@@ -9,6 +9,9 @@
 // for its next row before it works on this one.  Instructions come next: pairs of elements go through the packed fp32 pipe (with
 // scalar operations 8192 rows of 4096 with everything took 53 instructions an element and 73 us).
 //
+// Measured: 11328 rows of 960, residual and RMSNorm, 18.5 us (5.3 TB/s); 8192 of 4096, residual and LayerNorm, 54 us (5.6 TB/s,
+// issue slots 68%); 11328 of 2560, smoothed, 31 us (4.6 TB/s; a hardware reciprocal per element, of which an SM does 16 a cycle).
+//
 // Sums and statistics in fp32, of the unrounded h.  Quotients are correctly rounded (quotient() below), so without a norm the
 // codes are those of the definition bit for bit.  A row that holds no finite maximum (an infinity, a NaN) has scale NaN and codes 0:
 // it stays visible in every product.
