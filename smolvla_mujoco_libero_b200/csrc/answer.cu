@@ -37,7 +37,7 @@ int32_t launch_quant(const QuantRowsArgs& a, cudaStream_t st) {
 template <typename T, bool VEC>
 int32_t launch_quant_t(const QuantRowsArgs& a, cudaStream_t st) {
   // by k alone, so that a row's sums are the same in any batch (one row of 960 with a chunk per thread: 2.1 us, with two 2.7)
-  if (a.k <= 8192) return launch_quant<T, VEC, 2>(a, st);
+  if (a.k <= 16384) return launch_quant<T, VEC, 2>(a, st);
   return launch_quant<T, VEC, 4>(a, st);
 }
 

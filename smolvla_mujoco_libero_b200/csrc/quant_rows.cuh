@@ -52,38 +52,103 @@ __device__ __forceinline__ float2 quotient(float2 d, float2 minus_s, float2 r) {
   return __ffma2_rn(__ffma2_rn(q, minus_s, d), r, q);
 }
 
-// 8 elements from column c as they are stored; VEC: 16 bytes at once, otherwise element by element up to k (zeros behind it)
+// 8 elements of a vector of all rows (weight, bias) from column c, zeros behind k.  VEC: 16 bytes at once.  Otherwise what the
+// address allows: 16 bytes, or the 4-byte words that hold an element, shifted by one where the vector begins inside a word.
 template <typename T, bool VEC>
 __device__ __forceinline__ uint4 raw8(const T* row, int c, int k) {
-  if constexpr (VEC) {
-    return *reinterpret_cast<const uint4*>(row + c);
-  } else {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-    uint32_t u[4];
+  if constexpr (VEC) return *reinterpret_cast<const uint4*>(row + c);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + c);
+  const int n = k - c;
+  if (n >= 8 && at % 16 == 0) return *reinterpret_cast<const uint4*>(at);
+  const uint32_t* p = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+  const int ahead = static_cast<int>(at & 2) / 2;  // 1: element 0 is the upper half of word 0
+  uint32_t w[5], u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      u[i] = (c + 2 * i < k ? p[c + 2 * i] : 0u) | (c + 2 * i + 1 < k ? static_cast<uint32_t>(p[c + 2 * i + 1]) << 16 : 0u);
-    return make_uint4(u[0], u[1], u[2], u[3]);
+  for (int i = 0; i < 5; ++i) w[i] = 2 * i - ahead < n && 2 * i - ahead < 8 ? p[i] : 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    u[i] = ahead ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+    if (2 * i + 1 >= n) u[i] = 2 * i < n ? u[i] & 0xFFFFu : 0u;
   }
+  return make_uint4(u[0], u[1], u[2], u[3]);
 }
 template <typename T>
 __device__ __forceinline__ void unpack8(float2 (&v)[4], const uint4& w) {
   v[0] = serving::unpack2<T>(w.x), v[1] = serving::unpack2<T>(w.y), v[2] = serving::unpack2<T>(w.z), v[3] = serving::unpack2<T>(w.w);
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* row, const float2 (&v)[4], int c, int k) {
-  uint32_t u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] = serving::pack2<T>(v[i].x, v[i].y);
-  if constexpr (VEC) {
-    *reinterpret_cast<uint4*>(row + c) = make_uint4(u[0], u[1], u[2], u[3]);
-  } else {
-    uint16_t* p = reinterpret_cast<uint16_t*>(row);
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c + e < k) p[c + e] = static_cast<uint16_t>(u[e / 2] >> (16 * (e % 2)));
-  }
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float2 (&v)[4]) {
+  return make_uint4(serving::pack2<T>(v[0].x, v[0].y), serving::pack2<T>(v[1].x, v[1].y), serving::pack2<T>(v[2].x, v[2].y),
+                    serving::pack2<T>(v[3].x, v[3].y));
 }
+
+// A warp's 256 elements of a row from column c0 on.  VEC: 16 bytes a lane.  Otherwise (k no multiple of 8, or rows that are
+// not 16-byte aligned) the 4-byte words that hold them, a word per lane after the other, and through shared memory to the lanes
+// that own them (11328 rows of 2561 with residual and RMSNorm: 108 us; 185 with words taken by the lanes that own them; 2560: 47).
+template <typename T, bool VEC>
+struct Piece;
+template <typename T>
+struct Piece<T, true> {
+  uint4 w;
+  __device__ __forceinline__ void fetch(const T* row, int c0, int k, int lane) {
+    w = c0 + lane * 8 < k ? *reinterpret_cast<const uint4*>(row + c0 + lane * 8) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ uint4 take(const T*, int, int, int, uint32_t*) const { return w; }
+  static __device__ __forceinline__ void put(T* row, int c0, int k, int lane, const uint4& v, uint32_t*) {
+    if (c0 + lane * 8 < k) *reinterpret_cast<uint4*>(row + c0 + lane * 8) = v;
+  }
+};
+template <typename T>
+struct Piece<T, false> {
+  uint32_t w[4], last;
+  // 1: the first element is the upper half of word 0
+  static __device__ __forceinline__ int ahead(const T* row, int c0) { return static_cast<int>(reinterpret_cast<uintptr_t>(row + c0) & 2) / 2; }
+  static __device__ __forceinline__ uint32_t* words(const T* row, int c0) {
+    return reinterpret_cast<uint32_t*>(reinterpret_cast<uintptr_t>(row + c0) & ~uintptr_t(3));
+  }
+  __device__ __forceinline__ void fetch(const T* row, int c0, int k, int lane) {
+    const int off = ahead(row, c0), n = min(256, k - c0);
+    const uint32_t* p = words(row, c0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = 2 * (j * 32 + lane) - off < n ? p[j * 32 + lane] : 0u;
+    last = off && n == 256 ? p[128] : 0u;
+  }
+  __device__ __forceinline__ uint4 take(const T* row, int c0, int k, int lane, uint32_t* stage) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) stage[j * 32 + lane] = w[j];
+    if (lane == 0) stage[128] = last;
+    __syncwarp();
+    const uint4 q = *reinterpret_cast<const uint4*>(stage + 4 * lane);
+    const uint32_t u[5] = {q.x, q.y, q.z, q.w, stage[4 * lane + 4]};
+    __syncwarp();
+    uint32_t v[4];
+    const int off = ahead(row, c0), n = k - c0 - lane * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = off ? __funnelshift_r(u[i], u[i + 1], 16) : u[i];
+      if (2 * i + 1 >= n) v[i] = 2 * i < n ? v[i] & 0xFFFFu : 0u;
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
+  static __device__ __forceinline__ void put(T* row, int c0, int k, int lane, const uint4& v, uint32_t* stage) {
+    *reinterpret_cast<uint4*>(stage + 4 * lane) = v;
+    __syncwarp();
+    const int off = ahead(row, c0), n = min(256, k - c0);
+    uint32_t* p = words(row, c0);
+#pragma unroll
+    for (int j = 0; j < 5; ++j) {
+      const int i = j * 32 + lane, e = 2 * i - off;  // the word's lower element
+      if (j == 4 && lane > 0) break;
+      if (e >= n || e + 1 < 0) continue;
+      const uint32_t lower = off ? (i > 0 ? stage[i - 1] >> 16 : 0u) : stage[i] & 0xFFFFu;
+      const uint32_t upper = off ? (i < 128 ? stage[i] << 16 : 0u) : stage[i] & 0xFFFF0000u;
+      if (e >= 0 && e + 1 < n) p[i] = lower | upper;
+      else if (e >= 0) *reinterpret_cast<uint16_t*>(p + i) = static_cast<uint16_t>(lower);
+      else *(reinterpret_cast<uint16_t*>(p + i) + 1) = static_cast<uint16_t>(upper >> 16);
+    }
+    __syncwarp();
+  }
+};
 
 // Over the block's threads: a warp's lanes, then the warps through `part`, which holds zeros behind them and is used by one
 // reduction of every other row only.
@@ -137,7 +202,7 @@ constexpr int kMaxWarps = 32;
 
 // CH chunks of 8 elements per thread; the block's threads hold a row
 template <typename T, bool VEC, int CH>
-__global__ void __launch_bounds__(CH == 2 ? 512 : 1024) quant_rows_kernel(const QuantRowsArgs a) {
+__global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a) {
   using namespace qrows;
   __shared__ __align__(16) float part[2][3][kMaxWarps];
   for (int i = threadIdx.x; i < 6 * kMaxWarps; i += blockDim.x) (&part[0][0][0])[i] = 0.f;
@@ -145,16 +210,20 @@ __global__ void __launch_bounds__(CH == 2 ? 512 : 1024) quant_rows_kernel(const 
   pdl_wait();
   pdl_trigger();
   const int k = a.k;
+  __shared__ __align__(16) uint32_t stages[VEC ? 1 : kMaxWarps][VEC ? 4 : 132];
+  uint32_t* stage = stages[VEC ? 0 : threadIdx.x >> 5];
+  const int lane = threadIdx.x & 31;
   auto column = [&](int i) { return (i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8; };
-  uint4 rx[CH], rr[CH];
+  auto column0 = [&](int i) { return (i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x) - lane) * 8; };  // lane 0's
+  Piece<T, VEC> rx[CH], rr[CH];
   auto fetch = [&](long long row) {
     if (row >= a.m) return;
     const T* x = static_cast<const T*>(a.x) + row * a.x_rs;
     const T* r = static_cast<const T*>(a.residual) + row * a.residual_rs;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      rx[i] = column(i) < k ? raw8<T, VEC>(x, column(i), k) : make_uint4(0u, 0u, 0u, 0u);
-      if (a.residual) rr[i] = column(i) < k ? raw8<T, VEC>(r, column(i), k) : make_uint4(0u, 0u, 0u, 0u);
+      rx[i].fetch(x, column0(i), k, lane);
+      if (a.residual) rr[i].fetch(r, column0(i), k, lane);
     }
   };
   // a chunk's elements behind the row's end set to zero (where chunks are read whole, the chunk is in or out)
@@ -172,22 +241,20 @@ __global__ void __launch_bounds__(CH == 2 ? 512 : 1024) quant_rows_kernel(const 
   for (long long row = blockIdx.x; row < a.m; row += gridDim.x, turn ^= 1) {
     float2 y[CH][4];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) unpack8<T>(y[i], rx[i]);
+    for (int i = 0; i < CH; ++i) unpack8<T>(y[i], rx[i].take(static_cast<const T*>(a.x) + row * a.x_rs, column0(i), k, lane, stage));
     if (a.residual) {
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         float2 v[4];
-        unpack8<T>(v, rr[i]);
+        unpack8<T>(v, rr[i].take(static_cast<const T*>(a.residual) + row * a.residual_rs, column0(i), k, lane, stage));
 #pragma unroll
         for (int e = 0; e < 4; ++e) y[i][e] = __fadd2_rn(y[i][e], v[e]);
       }
     }
     fetch(row + gridDim.x);
     if (a.sum) {
-      T* s = static_cast<T*>(a.sum) + row * a.sum_rs;
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
-        if (column(i) < k) store8<T, VEC>(s, y[i], column(i), k);
+      for (int i = 0; i < CH; ++i) Piece<T, VEC>::put(static_cast<T*>(a.sum) + row * a.sum_rs, column0(i), k, lane, pack8<T>(y[i]), stage);
     }
     if (a.weight) {
       const float inv = __fdiv_rn(1.f, static_cast<float>(k));
@@ -255,7 +322,7 @@ __global__ void __launch_bounds__(CH == 2 ? 512 : 1024) quant_rows_kernel(const 
       for (int i = 0; i < CH; ++i) {
         if (column(i) >= k) continue;
         float2 d[4];
-        if constexpr (VEC) {
+        if (VEC || (column(i) + 8 <= k && reinterpret_cast<uintptr_t>(a.smooth) % 16 == 0)) {
           const float4* s = reinterpret_cast<const float4*>(a.smooth + column(i));
           const float4 s0 = __ldg(s), s1 = __ldg(s + 1);
           d[0] = make_float2(s0.x, s0.y), d[1] = make_float2(s0.z, s0.w), d[2] = make_float2(s1.x, s1.y), d[3] = make_float2(s1.z, s1.w);
@@ -285,7 +352,6 @@ __global__ void __launch_bounds__(CH == 2 ? 512 : 1024) quant_rows_kernel(const 
     int8_t* codes = a.codes + row * a.codes_rs;
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      if (column(i) >= k) continue;
       constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer in the low bits, ties to even
       float2 t[4];
       if (plain) {
@@ -306,9 +372,9 @@ __global__ void __launch_bounds__(CH == 2 ? 512 : 1024) quant_rows_kernel(const 
         const uint32_t hi = __byte_perm(__float_as_uint(t[2 * h + 1].x), __float_as_uint(t[2 * h + 1].y), 0x0040);
         packed[h] = __byte_perm(lo, hi, 0x5410);
       }
-      if constexpr (VEC) {
+      if (column(i) + 8 <= k && (VEC || reinterpret_cast<uintptr_t>(codes) % 8 == 0)) {
         *reinterpret_cast<uint2*>(codes + column(i)) = make_uint2(packed[0], packed[1]);
-      } else {
+      } else if (!VEC) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (column(i) + e < k) codes[column(i) + e] = static_cast<int8_t>(packed[e / 4] >> (8 * (e % 4)));
@@ -316,7 +382,7 @@ __global__ void __launch_bounds__(CH == 2 ? 512 : 1024) quant_rows_kernel(const 
       if (a.values) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = __fmul2_rn(__fadd2_rn(t[e], both(-kRound)), both(scale));
-        store8<T, VEC>(static_cast<T*>(a.values) + row * a.values_rs, t, column(i), k);
+        Piece<T, VEC>::put(static_cast<T*>(a.values) + row * a.values_rs, column0(i), k, lane, pack8<T>(t), stage);
       }
     }
   }
