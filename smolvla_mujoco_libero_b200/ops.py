@@ -423,7 +423,7 @@ def quantize_rows(x: torch.Tensor, weight: torch.Tensor | None = None, bias: tor
     LayerNorm (``weight`` and ``bias``), divided by ``smooth`` (fp32 [k]); scale = max |y| / 127, codes = round(y / scale).
     ``sum`` is h (there with a residual; it may be x or the residual itself), ``values`` what the codes stand for
     (``want_values``: the activations that a fake-quantised linear multiplies, deploy/linear_only_quant.py:140-162).  A row
-    that is not finite gets scale NaN and codes 0.  The outputs may be given."""
+    that is not finite gets scale NaN and codes 0.  The outputs may be given; small new ones share an allocation."""
     return QuantizedRows(*L.serving().quantize_rows(x, weight, bias, eps, residual, smooth, want_values, codes, scale, sum, values))
 
 
@@ -534,8 +534,10 @@ def _(q, cache, cu_q, kv_len, page_table, scale):
 @torch.library.custom_op("svla::quantize_rows", mutates_args=())
 def _quantize_rows_op(x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
                       residual: torch.Tensor | None, smooth: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    r = quantize_rows(x, weight, bias, eps, residual, smooth)
-    return r.codes, r.scale, x.new_empty(0, x.shape[1]) if r.sum is None else r.sum
+    m, k = x.shape  # (outputs of their own: quantize_rows may put small ones into one allocation)
+    r = quantize_rows(x, weight, bias, eps, residual, smooth, codes=x.new_empty(m, -(-k // 16) * 16, dtype=torch.int8)[:, :k],
+                      scale=x.new_empty(m, dtype=torch.float32), sum=None if residual is None else x.new_empty(m, k))
+    return r.codes, r.scale, x.new_empty(0, k) if r.sum is None else r.sum
 
 
 @_quantize_rows_op.register_fake
