@@ -17,8 +17,9 @@
 // arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 8 epilogue warps for each.  Outputs leave through
 // shared memory and TMA stores: written by the threads that own a row each, every warp's store touches 32 lines, and the stores'
 // way through L1 took 8000 cycles per tile.
-// 8192 x 4096 x 11008: 231 us, 3.2 POPS (275 back to back, under the power cap); 11328 x 2560 x 960, gated: 49 us, 2.3 POPS, where a
-// tile has 8 slices of K only and its epilogue (two int32 conversions, an exponential and a reciprocal per output) takes as long.
+// 8192 x 4096 x 11008: 231 us, 3.2 POPS (275 back to back, under the power cap); 11328 x 2560 x 960, gated: 48 us, 2.3 POPS: a
+// tile has 8 slices of K only, and its epilogue (two int32 conversions, an exponential and a reciprocal per output) holds the
+// accumulator as long again (K = 128: 32 us).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -60,6 +61,17 @@ __device__ __forceinline__ float silu(float x) { return __fmul_rn(x, rcp_approx(
 
 __device__ __forceinline__ float scaled(uint32_t acc, float a, float b) {
   return __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(acc)), a), b);
+}
+
+// the same for pairs, through the packed fp32 pipe: each half rounds as the scalar operation does
+__device__ __forceinline__ float2 silu2(float2 x) {
+  const float2 z = __fmul2_rn(x, make_float2(-serving::kLog2e, -serving::kLog2e));
+  const float2 d = __fadd2_rn(make_float2(1.f, 1.f), make_float2(ex2_approx(z.x), ex2_approx(z.y)));
+  return __fmul2_rn(x, make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+}
+__device__ __forceinline__ float2 scaled2(uint32_t a0, uint32_t a1, float a, float2 b) {
+  const float2 v = make_float2(static_cast<float>(static_cast<int>(a0)), static_cast<float>(static_cast<int>(a1)));
+  return __fmul2_rn(__fmul2_rn(v, make_float2(a, a)), b);
 }
 
 template <int MT, bool GATED>
@@ -279,7 +291,7 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
 namespace li8 {
 struct Many {
   // A CTA's rows of x and its half of w.  A stage more is worth more than a second box per warp: K = 11008 in 236 us, with 4
-  // stages and two boxes 256 (K = 960, gated: 49 and 48)
+  // stages and two boxes 256 (K = 960, gated: 48 either way)
   static constexpr int kStages = 5, kTile = 128 * kSlice, kStage = 2 * kTile;
   static constexpr int kOut = kStages * kStage, kBoxBytes = 2048;  // each epilogue warp's box of 32 rows x 64 bytes
   static constexpr int kBar = kOut + 16 * kBoxBytes;
@@ -460,13 +472,13 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
         for (int j = 0; j < kChunk; j += 4) {
           const float4 w4 = *reinterpret_cast<const float4*>(consts + c + j);
           const float4 b4 = *reinterpret_cast<const float4*>(consts + 128 + c + j);
-          const float w[4] = {w4.x, w4.y, w4.z, w4.w}, b[4] = {b4.x, b4.y, b4.z, b4.w};
+          const float2 w[2] = {make_float2(w4.x, w4.y), make_float2(w4.z, w4.w)}, b[2] = {make_float2(b4.x, b4.y), make_float2(b4.z, b4.w)};
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float y = scaled(r[j + e], xs, w[e]);
-            if constexpr (GATED) y = __fmul_rn(silu(y), scaled(r2[GATED ? j + e : 0], xs, b[e]));
-            else y = __fadd_rn(y, b[e]);
-            v[j + e] = y;
+          for (int e = 0; e < 2; ++e) {
+            float2 y = scaled2(r[j + 2 * e], r[j + 2 * e + 1], xs, w[e]);
+            if constexpr (GATED) y = __fmul2_rn(silu2(y), scaled2(r2[GATED ? j + 2 * e : 0], r2[GATED ? j + 2 * e + 1 : 0], xs, b[e]));
+            else y = __fadd2_rn(y, b[e]);
+            v[j + 2 * e] = y.x, v[j + 2 * e + 1] = y.y;
           }
         }
         if (a.staged) {

@@ -10,7 +10,7 @@
 // scalar operations 8192 rows of 4096 with everything took 53 instructions an element and 73 us).
 //
 // Measured: 11328 rows of 960, residual and RMSNorm, 18.5 us (5.3 TB/s); 8192 of 4096, residual and LayerNorm, 54 us (5.6 TB/s,
-// issue slots 68%); 11328 of 2560, smoothed, 31 us (4.6 TB/s; a hardware reciprocal per element, of which an SM does 16 a cycle).
+// issue slots 68%); 11328 of 2560, smoothed, 31 us (4.6 TB/s, three bytes written for two read; the same without the reciprocals).
 //
 // Sums and statistics in fp32, of the unrounded h.  Quotients are correctly rounded (quotient() below), so without a norm the
 // codes are those of the definition bit for bit.  A row that holds no finite maximum (an infinity, a NaN) has scale NaN and codes 0:
