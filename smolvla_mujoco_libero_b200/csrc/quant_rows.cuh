@@ -131,6 +131,7 @@ struct Piece<T, false> {
     return make_uint4(v[0], v[1], v[2], v[3]);
   }
   static __device__ __forceinline__ void put(T* row, int c0, int k, int lane, const uint4& v, uint32_t* stage) {
+    if (c0 >= k) return;  // (at c0 = k word 0 holds element k - 1, which is another warp's, and what stands behind the row)
     *reinterpret_cast<uint4*>(stage + 4 * lane) = v;
     __syncwarp();
     const int off = ahead(row, c0), n = min(256, k - c0);
