@@ -438,9 +438,15 @@ __global__ void __launch_bounds__(sample::kThreads, 4) sample_kernel(const Sampl
   const bool dense = !by_count && min_p == 0.f && weigh(cut_l) == 0ull;
   u64 sum = 0ull;  // of this thread's kept tokens
   if (by_count || by_weight) {
-    // at first bins of 1 / 120 of the temperature: what is kept lies less than 33 (or one step of the logits) below the largest
-    const float to_bin = fminf(120.f / temperature, 3.4028234663852886e38f);
-    auto fine_bin = [&](float l) { return __float2int_rn(fminf(__fmul_rn(__fsub_rn(top, l), to_bin), static_cast<float>(kFine - 1))); };
+    // At first bins of 1 / 120 of the temperature: what is kept lies less than 33 (or one step of the logits) below the largest.
+    // Differences are taken in halves, so that those above 3.4e38 stay finite, where the temperature is above 1, and times 2^64
+    // where it is so small that 120 / temperature leaves fp32 (with larger logits than that allows, one step is more than 33
+    // temperatures and only equal logits are left: any bins do).
+    const float unit = temperature >= 1.f ? 0.5f : temperature < 5.421010862427522e-20f && fabsf(top) < 4.611686018427388e18f ? 18446744073709551616.f : 1.f;
+    const float to_bin = fminf(120.f / __fmul_rn(temperature, unit), 3.4028234663852886e38f), top_units = __fmul_rn(top, unit);
+    auto fine_bin = [&](float l) {
+      return __float2int_rn(fminf(__fmul_rn(__fmaf_rn(l, -unit, top_units), to_bin), static_cast<float>(kFine - 1)));
+    };
     unsigned* fine = s.fine;
     int my_bin = 0, my_bins = 0;  // this thread's of this CTA's share of the bins
     auto share = [&](int bins) {
