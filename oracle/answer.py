@@ -28,15 +28,20 @@ def rows_tolerance(x, weight=None, bias=None, eps=1e-5, residual=None, smooth=No
     A thread adds up at most 32 values, 5 rounds of shuffles join 32 threads and 31 additions as many warps: a statistic is off
     by at most 70 half steps (2^-24) of its magnitudes' sum, its root by half of that.  Beside it: the sum h, the square, the
     reciprocal root (2), the two products with it, the bias' sum, the quotient with smooth, the scale: 10 half steps.  LayerNorm's mean
-    is off by 72 half steps of mean |h|, which counts against the centred values: relative to the largest y it is 72 (mean |h| / std)
-    times the largest weight."""
+    is off by 72 half steps of mean |h|, e, which counts against the centred values: relative to the largest y it is 72 (mean |h| / std)
+    times the largest weight.  Where the mean is more than 4 deviations the mean of the centred values is taken off as well: it is
+    off by 72 half steps of their mean size (at most e above that of the exact ones), both centrings round, and a sum h
+    that was rounded is off by half a step of it."""
     half = 2.0 ** -24
     y, scale = rows(x, weight, bias, eps, residual, smooth)
     rel = torch.full_like(scale, (10 + (35 if weight is not None else 0)) * half)
     if bias is not None:
         h = x.double() + (residual.double() if residual is not None else 0)
         d = h - h.mean(-1, keepdim=True)
-        off = 72 * half * h.abs().mean(-1) / torch.sqrt(d.square().mean(-1) + eps)
+        e = 72 * half * h.abs().mean(-1)
+        again = half * (72 * (d.abs().mean(-1) + e) + d.abs().amax(-1) + e + (2 * h.abs().amax(-1) if residual is not None else 0))
+        far = h.mean(-1).square() > 17 * d.square().mean(-1)
+        off = torch.where(far, again, e) / torch.sqrt(d.square().mean(-1) + eps)
         w = weight.double().abs() / (smooth.double() if smooth is not None else 1)
         b = bias.double().abs() / (smooth.double() if smooth is not None else 1)
         # the bias may cancel most of a product: errors are relative to the parts
