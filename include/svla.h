@@ -387,7 +387,8 @@ int32_t svla_paged_attention(const svla_paged_attn_desc* desc, svla_stream_t str
 
 /* h = x + residual;  y = h, or its RMSNorm (weight), or its LayerNorm (weight and bias), divided by smooth;
  * scale[m] = max |y| / 127;  codes = round(y / scale) (ties to even);  sum = h;  values = codes * scale.
- * Statistics in fp32 of the unrounded h.  A row of zeros gets scale 0 and codes 0; one whose largest |y| is
+ * Statistics in fp32 of the unrounded h, over its whole range; where the root is of 0 (no spread and eps 0)
+ * the normalised values are 0.  A row of zeros gets scale 0 and codes 0; one whose largest |y| is
  * not finite gets scale NaN and codes 0 (and its products are NaN).  sum and values may be x or residual
  * itself (in place, same row stride).  Rows, and weight, bias and smooth, of any alignment; 16-byte aligned
  * ones of k a multiple of 8 are read 16 bytes at a time.  1 <= k <= 32768. */

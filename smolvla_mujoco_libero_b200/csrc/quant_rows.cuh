@@ -288,15 +288,17 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a)
           }
           squares = add_block(__fadd_rn(sum.x, sum.y), part[turn][1]);
         }
-        // Squares beyond fp32's range (components above 1e17 or so) are seen in their sum; the row is then scaled by 2^-80, which a
-        // norm does not notice, and its statistics are taken again.
-        if (!scaled && !(near && squares < __int_as_float(0x7f800000))) {
-          constexpr float kDown = 8.271806125530277e-25f;  // 2^-80
+        // Squares beyond fp32's range (components above 1e17 or so) are seen in their sum, those below it (with an eps as small)
+        // in what the root is taken of; the row is then scaled by 2^-80 or 2^80, which a norm does not notice, and its statistics
+        // are taken again.  (What is scaled up lies below 2^-32: centred, and not over 2^8 deviations.)
+        const bool over = !(near && squares < __int_as_float(0x7f800000));
+        if (!scaled && (over || __fmaf_rn(squares, inv, eps) < 8.3e-25f)) {
+          const float by = over ? 8.271806125530277e-25f : 1.2089258196146292e24f;
 #pragma unroll
           for (int i = 0; i < CH; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[i][e] = __fmul2_rn(y[i][e], both(kDown));
-          eps = __fmul_rn(__fmul_rn(eps, kDown), kDown);
+            for (int e = 0; e < 4; ++e) y[i][e] = __fmul2_rn(y[i][e], both(by));
+          eps = __fmul_rn(__fmul_rn(eps, by), by);
           scaled = true;
         } else if (const float variance = __fmul_rn(squares, inv);
                    !centred && (0.0625f * mean * mean > variance || (mean != 0.f && variance < 7.9e-31f))) {
