@@ -68,11 +68,12 @@ __device__ __forceinline__ float2 scaled2(uint32_t a0, uint32_t a1, float a, flo
 
 // x sigmoid(x) with the hardware's 2^z and reciprocal (2^-22 and 2^-23 relative).  z = -x log2(e) is rounded, which puts the
 // exponential off by 2^-24 |x|; outputs of 16 bits hide that.  For fp32 ones what z lacks, -x - z ln 2, comes in to first order
-// (11328 x 2560 x 960: 56 us, 55 without; 68 with expf and a division).  A sigmoid below 2^-126, x < -87.3, is 0.
+// (11328 x 2560 x 960: 56.7 us, 55 without; 68 with expf and a division).  A sigmoid below 2^-126, x < -87.3, is 0.
 template <typename T>
 __device__ __forceinline__ float2 silu2(float2 x) {
   if constexpr (sizeof(T) == 4) {
-    const float2 c = make_float2(fmaxf(x.x, -88.f), fmaxf(x.y, -88.f));  // 2^z stays finite (x itself carries a NaN on)
+    auto clamp = [](float v) { return fminf(fmaxf(v, -88.f), 128.f); };  // 2^z and what z lacks stay finite; beyond, 2^z is 0 or the sigmoid is
+    const float2 c = make_float2(clamp(x.x), clamp(x.y));                // (x itself carries a NaN on)
     const float2 z = __fmul2_rn(c, make_float2(-serving::kLog2e, -serving::kLog2e));
     float2 t = __ffma2_rn(z, make_float2(-0.6931471824645996f, -0.6931471824645996f), make_float2(-c.x, -c.y));
     t = __ffma2_rn(z, make_float2(1.9046542121259336e-09f, 1.9046542121259336e-09f), t);
@@ -88,7 +89,7 @@ __device__ __forceinline__ float2 silu2(float2 x) {
 template <typename T>
 __device__ __forceinline__ float silu(float x) {
   if constexpr (sizeof(T) == 4) {
-    const float c = fmaxf(x, -88.f), z = __fmul_rn(c, -serving::kLog2e);
+    const float c = fminf(fmaxf(x, -88.f), 128.f), z = __fmul_rn(c, -serving::kLog2e);
     const float t = __fmaf_rn(z, 1.9046542121259336e-09f, __fmaf_rn(z, -0.6931471824645996f, -c)), e = ex2_approx(z);
     return __fmul_rn(x, rcp_approx(__fadd_rn(1.f, __fmaf_rn(e, t, e))));
   } else {

@@ -28,3 +28,23 @@ def test_gated_products_of_large_gates(impl, m, k, shift):
     y = gate * torch.sigmoid(gate) * up
     off = (got - y).abs() / (10.1 * 2.0 ** -24 * y.abs() + (gate * up).abs() * 2.0 ** -126 + 1e-37)
     assert float(off.max()) <= 1, float(off.max())
+
+
+@pytest.mark.parametrize("impl", [L.LINEAR_FEW, L.LINEAR_MANY], ids=["few", "many"])
+@pytest.mark.parametrize("dtype", [FP32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("size", [1e3, 1e10, 1e25, 1e34, 1e36])
+def test_gates_beyond_the_exponential(impl, dtype, size):
+    """Gates from 1e3 to fp32's end, whose activation is the gate itself or 0; beyond that end an infinity, as the product's."""
+    m, n, k, g = 7, 64, 16, gen(3)
+    x, w = (torch.randint(1, 128, (r, k), generator=g, dtype=torch.int8) for r in (m, 2 * n))
+    w[:n:2] *= -1  # every other gate is negative
+    xs, ws = torch.ones(m), torch.cat([torch.full((n,), size), torch.full((n,), 1e-3 / size)])
+    gate, up = ((x.double() @ w.double().T) * ws.double()).chunk(2, -1)
+    finite = gate < torch.finfo(FP32).max
+    got = ops.linear_i8_rows(x.to(DEV), xs.to(DEV), w.to(DEV), ws.to(DEV), gated=True, dtype=dtype, impl=impl).double().cpu()
+    y = torch.where(gate > 0, gate * up, 0.0)
+    off = 2.0 ** -24 * 12 + (torch.finfo(dtype).eps / 2 if dtype != FP32 else 0)
+    live = finite & (gate > -torch.finfo(FP32).max)
+    assert bool(((got - y).abs() <= off * y.abs() + 1e-30)[live].all())
+    assert bool((got[~finite] == torch.inf).all())
+    assert size > 1e25 or bool(live.all())  # (sums reach 16 127^2 = 2.6e5)
