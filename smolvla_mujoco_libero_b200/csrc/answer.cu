@@ -103,7 +103,7 @@ int32_t launch_many(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStream_t 
   if (tiles > 0x7fffffffll / 2) return fail(SVLA_ERR_ARG, "svla_linear_i8: too many tiles");
   const int size = static_cast<int>(sizeof(T));
   auto by_16 = [&](const void* p, int64_t rs) { return aligned(p, 16) && rs * size % 16 == 0; };
-  a.staged = d->n * size % 16 == 0 && by_16(a.out, a.out_rs) && (!a.residual || by_16(a.residual, a.residual_rs));
+  a.staged = static_cast<int64_t>(d->n) * size % 16 == 0 && by_16(a.out, a.out_rs) && (!a.residual || by_16(a.residual, a.residual_rs));
   if (a.staged) if (int32_t rc = make_tmap_out(&a.to, d, size)) return rc;
   const long long pairs = sm_count() / 2;
   return launch_cluster(kern, dim3(static_cast<unsigned>(2 * (tiles < pairs ? tiles : pairs))), dim3(li8::kManyThreads),
@@ -174,7 +174,8 @@ int32_t svla_linear_i8(const svla_linear_i8_desc* d, svla_stream_t stream) {
   if (d->m < 0 || d->n < 0) return fail(SVLA_ERR_ARG, "%s: negative m or n", who);
   // fewer than 2^17 products of two codes (of -128 too) stay below 2^31
   if (d->k < 1 || d->k >= 131072) return fail(SVLA_ERR_ARG, "%s: k must be 1 to 131071 (got %d)", who, d->k);
-  if (d->n > 0x3fffffff) return fail(SVLA_ERR_ARG, "%s: n must stay below 2^30", who);
+  // (tiles' counts and origins, and two weight rows per gated output, in 31 bits)
+  if (d->m > 0x3fffffff || d->n > 0x3fffffff) return fail(SVLA_ERR_ARG, "%s: m and n must stay below 2^30 (got %d and %d)", who, d->m, d->n);
   if (d->impl < SVLA_LINEAR_AUTO || d->impl > SVLA_LINEAR_MANY) return fail(SVLA_ERR_ARG, "%s: bad impl %d", who, d->impl);
   if (d->gated && (d->bias || d->residual)) return fail(SVLA_ERR_ARG, "%s: a gated product takes no bias and no residual", who);
   if (d->m == 0 || d->n == 0) return SVLA_OK;
