@@ -63,6 +63,14 @@ void check(int32_t rc, const char* who) {
   if (rc) py::module_::import("smolvla_mujoco_libero_b200._lib").attr("check")(rc, who);
 }
 
+// a caller's tensor that a kernel writes has a new version, as after torch's own in-place operations: a graph that saved it notices
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+void written(const Opt& t) {
+  if (t) written(*t);
+}
+
 int32_t i32(int64_t x, const char* what) {
   if (x > std::numeric_limits<int32_t>::max()) refuse(what, " does not fit 31 bits (", x, ")");
   return static_cast<int32_t>(x);
@@ -196,6 +204,7 @@ py::object kv_append(const Tensor& cache, const Tensor& k, const Tensor& v, cons
     d.hkv = ca.heads, d.head_dim = i32(c.d, "head_dim"), d.dtype = c.code();
     d.bits = ca.bits, d.page_size = ca.page, d.n_pages = ca.n_pages, d.max_pages = ca.max_pages;
     check(calls.append(&d, c.stream()), "svla_kv_append");
+    written(cache), written(q_out), written(k_out), written(v_out);
   }
   if (want_rows) return py::make_tuple(q_out, *k_out, *v_out);
   return py::cast(q_out);
@@ -218,6 +227,7 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   d.head_dim = i32(c.d, "head_dim"), d.dtype = c.code(), d.causal = causal;
   d.scale = f32_scale(scale), d.impl = impl;
   check(calls.packed(&d, c.stream()), "svla_packed_attention");
+  written(out);
   return *out;
 }
 
@@ -246,6 +256,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& cache, const Tensor& cu_q,
   d.page_table = static_cast<const int32_t*>(page_table.const_data_ptr()), d.page_table_rs = ca.table_rs;
   d.q_rs = rq.rs, d.scale = f32_scale(scale);
   check(calls.paged(&d, c.stream()), "svla_paged_attention");
+  written(out), written(workspace);
   return *out;
 }
 
@@ -351,6 +362,7 @@ py::tuple quantize_rows(const Tensor& x, const Opt& weight, const Opt& bias, dou
   if (values) d.values = values->data_ptr();
   d.m = i32(m, "the number of rows"), d.k = i32(k, "k"), d.dtype = dtype_code(t), d.eps = static_cast<float>(eps);
   check(calls.quant_rows(&d, w.stream()), "svla_quant_rows");
+  written(codes), written(scale), written(sum), written(values);
   return py::make_tuple(*codes, *scale, sum, values);
 }
 
@@ -377,6 +389,7 @@ Tensor linear_i8_rows(const Tensor& x, const Tensor& xscale, const Tensor& weigh
   d.m = i32(m, "the number of rows"), d.n = i32(n, "n"), d.k = i32(k, "k");
   d.dtype = dtype_code(dtype), d.gated = gated, d.impl = impl;
   check(calls.linear(&d, w.stream()), "svla_linear_i8");
+  written(out);
   return *out;
 }
 
@@ -410,6 +423,7 @@ py::tuple sample_tokens(const Tensor& logits, const Tensor& u, const py::object&
   d.tokens = static_cast<int32_t*>(tokens->data_ptr()), d.logprob = static_cast<float*>(logprob->data_ptr());
   d.batch = i32(batch, "the number of rows"), d.vocab = i32(vocab, "vocab"), d.dtype = dtype_code(t);
   check(calls.sample(&d, w.stream()), "svla_sample_tokens");
+  written(tokens), written(logprob);
   return py::make_tuple(*tokens, *logprob);
 }
 

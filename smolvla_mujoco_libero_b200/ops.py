@@ -3,7 +3,8 @@
 Each function checks devices / dtypes / contiguity, allocates its outputs with torch (the only allocation in
 this layer), and launches on torch's current CUDA stream through ctypes.  The most used ops are also
 registered as ``torch.ops.svla.*`` custom ops.  Nothing here computes on the CPU: a missing library or a
-CPU tensor raises.
+CPU tensor raises.  Nothing here is differentiable: inputs that require grad are taken as their values, and
+results carry no graph.
 """
 
 from __future__ import annotations
