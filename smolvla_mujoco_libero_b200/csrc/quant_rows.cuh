@@ -131,16 +131,17 @@ struct Piece<T, false> {
     return make_uint4(v[0], v[1], v[2], v[3]);
   }
   static __device__ __forceinline__ void put(T* row, int c0, int k, int lane, const uint4& v, uint32_t* stage) {
-    if (c0 >= k) return;  // (at c0 = k word 0 holds element k - 1, which is another warp's, and what stands behind the row)
     *reinterpret_cast<uint4*>(stage + 4 * lane) = v;
     __syncwarp();
-    const int off = ahead(row, c0), n = min(256, k - c0);
+    // A piece behind the row's end stores nothing.  (One that begins there would store its word 0 otherwise, which holds element
+    // k - 1, another warp's, and what stands behind the row; a return in this place: 11328 rows of 961 50 us, so 46.)
+    const int n = min(256, k - c0), off = n > 0 ? ahead(row, c0) : 0;
     uint32_t* p = words(row, c0);
 #pragma unroll
     for (int j = 0; j < 5; ++j) {
-      const int i = j * 32 + lane, e = 2 * i - off;  // the word's lower element
+      const int i = j * 32 + lane, e = 2 * i - off;  // the word's lower element, -1 at least
       if (j == 4 && lane > 0) break;
-      if (e >= n || e + 1 < 0) continue;
+      if (e >= n) continue;
       const uint32_t lower = off ? (i > 0 ? stage[i - 1] >> 16 : 0u) : stage[i] & 0xFFFFu;
       const uint32_t upper = off ? (i < 128 ? stage[i] << 16 : 0u) : stage[i] & 0xFFFF0000u;
       if (e >= 0 && e + 1 < n) p[i] = lower | upper;
@@ -259,12 +260,11 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a)
     }
     if (a.weight) {
       const float inv = __fdiv_rn(1.f, static_cast<float>(k));
-      float squares = 0.f, eps = a.eps;
+      float power, eps = a.eps;  // what the root is taken of
       // One round over the row, and another for a few: the choices are the row's, so its threads agree, and each is made once.
-      bool scaled = false, centred = false;
-      for (;;) {
+      for (bool scaled = false, centred = false;;) {
         float2 sum = both(0.f);
-        float mean = 0.f;
+        float mean = 0.f, squares = __int_as_float(0x7f800000);
         if (a.bias) {
 #pragma unroll
           for (int i = 0; i < CH; ++i)
@@ -273,46 +273,47 @@ __global__ void __launch_bounds__(1024) quant_rows_kernel(const QuantRowsArgs a)
           mean = __fdiv_rn(add_block(__fadd_rn(sum.x, sum.y), part[turn][0]), static_cast<float>(k));
           sum = both(0.f);
         }
-        const bool near = !a.bias || fabsf(mean) < 1.2676506002282294e30f;  // 2^100: centring does not overflow
-        if (near || scaled) {
+        if (fabsf(mean) < 1.2676506002282294e30f || scaled) {  // (from 2^100 on centring might overflow)
+          if (a.bias) {
 #pragma unroll
-          for (int i = 0; i < CH; ++i) {
-            if (column(i) >= k) continue;
-            if (a.bias) {
+            for (int i = 0; i < CH; ++i) {
+              if (column(i) >= k) continue;
 #pragma unroll
               for (int e = 0; e < 4; ++e) y[i][e] = __fadd2_rn(y[i][e], both(-mean));
               clip(y[i], i);
             }
+          }
+#pragma unroll
+          for (int i = 0; i < CH; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum = __ffma2_rn(y[i][e], y[i][e], sum);
-          }
           squares = add_block(__fadd_rn(sum.x, sum.y), part[turn][1]);
         }
-        // Squares beyond fp32's range (components above 1e17 or so) are seen in their sum, those below it (with an eps as small)
-        // in what the root is taken of; the row is then scaled by 2^-80 or 2^80, which a norm does not notice, and its statistics
-        // are taken again.  (What is scaled up lies below 2^-32: centred, and not over 2^8 deviations.)
-        const bool over = !(near && squares < __int_as_float(0x7f800000));
-        if (!scaled && (over || __fmaf_rn(squares, inv, eps) < 8.3e-25f)) {
-          const float by = over ? 8.271806125530277e-25f : 1.2089258196146292e24f;
+        const float variance = __fmul_rn(squares, inv);
+        power = __fmaf_rn(squares, inv, eps);
+        const bool fits = power >= 8.3e-25f && power < __int_as_float(0x7f800000), far = mean != 0.f && 0.0625f * mean * mean >= variance;
+        if (fits && !far) break;
+        if (!fits && !scaled) {
+          // Squares beyond fp32's range (components above 1e17 or so), or below it with an eps as small: the row is scaled by 2^-80
+          // or 2^80, which a norm does not notice.  (What is scaled up lies below 2^-32: centred, and not over 2^8 deviations.)
+          const float by = power < 1.f ? 1.2089258196146292e24f : 8.271806125530277e-25f;
 #pragma unroll
           for (int i = 0; i < CH; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[i][e] = __fmul2_rn(y[i][e], both(by));
           eps = __fmul_rn(__fmul_rn(eps, by), by);
           scaled = true;
-        } else if (const float variance = __fmul_rn(squares, inv);
-                   !centred && (0.0625f * mean * mean > variance || (mean != 0.f && variance < 7.9e-31f))) {
-          // A mean of more than 4 deviations (or squares too small to tell): as a sum of large numbers it is off by a step of
-          // them or more, so the mean of what is left is taken off as well (8192 rows of 4096 with all, every one
-          // such a row: 65 us, none: 54; the sum of what is left taken beside the squares of every row: 62)
+        } else if (far && !centred) {
+          // A mean of more than 4 deviations: as a sum of large numbers it is off by a step of them or more, so the mean of what is
+          // left is taken off as well (8192 rows of 4096 with all, every one such a row: 64 us, none: 53; the sum of what is left
+          // taken beside the squares of every row: 62)
           centred = true;
         } else {
           break;
         }
         __syncthreads();  // the partial sums are read before they are written again
       }
-      const float power = __fmaf_rn(squares, inv, eps);  // 0: every y is
-      const float2 rstd = both(power == 0.f ? 0.f : __frsqrt_rn(power));
+      const float2 rstd = both(power == 0.f ? 0.f : __frsqrt_rn(power));  // 0: every y is
       const T* w = static_cast<const T*>(a.weight);
       const T* b = static_cast<const T*>(a.bias);
 #pragma unroll
