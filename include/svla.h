@@ -408,8 +408,9 @@ typedef struct svla_quant_rows_desc {
 } svla_quant_rows_desc;
 int32_t svla_quant_rows(const svla_quant_rows_desc* desc, svla_stream_t stream);
 
-/* out[m, n] = xscale[m] * wscale[n] * sum_k x[m, k] w[n, k] + bias[n] + residual[m, n], the sum exact, the rest in
- * fp32, rounded once.  gated: w and wscale hold 2 n rows, the gate's n first, and out = silu(gate) * up.
+/* out[m, n] = ((sum_k x[m, k] w[n, k]) * xscale[m]) * wscale[n] + bias[n] + residual[m, n], the sum exact, the rest in
+ * fp32 in this order (an xscale times a sum beyond fp32 is infinite), rounded once to the output's type.  gated: w
+ * and wscale hold 2 n rows, the gate's n first, and out = silu(gate) * up.
  * x and w 16-byte aligned with row strides that are multiples of 16 bytes (k itself may be any number below
  * 2^17: what stands behind a row's k is not read).  m and n below 2^30.  out may be residual (in place, same row
  * stride). */

@@ -81,9 +81,9 @@ int32_t launch_few(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStream_t s
   a.tiles_m = (d->m + MT - 1) / MT, a.tiles_n = (d->n + 127) / 128;
   const long long tiles = static_cast<long long>(a.tiles_m) * a.tiles_n;
   const int slices = (d->k + li8::kSlice - 1) / li8::kSlice;
-  // K is shared where a tile's parts keep 5 slices at least, within one round over the SMs: adding them up costs 1 us with one
-  // token and 3 with 128 (K = 4096, N = 4096, 1 token: 5.7 us, alone 9.6; 128 tokens 9.6 and 11.9; K = 960, N = 1600, 1 token:
-  // 4.5 us by 8, alone 4.1; 128 tokens 7.7 and 5.9)
+  // K is shared where a tile's parts keep 5 slices at least, within one round over the SMs: adding them up costs half a us with one
+  // token and 2 with 128 (K = 4096, N = 4096, 1 token: 6.8 us, alone 11.4; 128 tokens 10.9 and 15.4; K = 960, N = 1600, 1 token:
+  // 4.4 us by 8, alone 4.0; 128 tokens 7.5 and 5.8)
   a.splits = 1;
   while (a.splits < 8 && tiles * a.splits * 2 <= sm_count() && a.splits * 10 <= slices) a.splits *= 2;
   if (tiles * a.splits > 0x7fffffffll) return fail(SVLA_ERR_ARG, "svla_linear_i8: too many tiles");
@@ -112,10 +112,10 @@ int32_t launch_many(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStream_t 
 
 template <typename T, bool GATED>
 int32_t launch_linear(LinearI8Args& a, const svla_linear_i8_desc* d, cudaStream_t st) {
-  // Up to 128 rows the weights are read once by either kernel, and the one for few rows takes 15 us for 128 x 49280 where the
-  // other takes 25.  Beyond, it moves twice the bytes per product and starts 3 us earlier: it is the faster one while its
-  // tiles fit one round over the SMs (few / many, us: 768 x 1600 x 960, 78 tiles, 5.9 / 9.0; 512 x 4096 x 4096, 128 tiles, 12.2 /
-  // 15.6; 768 x 4096 x 4096, 192 tiles, 16.5 / 16.2; 177 x 49280 x 960, 770 tiles, 26 / 24)
+  // Up to 128 rows the weights are read once by either kernel, and the one for few rows takes 17.8 us for 128 x 49280 x 960 where
+  // the other takes 22.4.  Beyond, it moves twice the bytes per product and starts 3 us earlier: it is the faster one while its
+  // tiles fit one round over the SMs (few / many, us: 768 x 1600 x 960, 78 tiles, 6.0 / 8.8; 512 x 4096 x 4096, 128 tiles, 15.7 /
+  // 16.3; 768 x 4096 x 4096, 192 tiles, 17.2 / 16.8; 177 x 49280 x 960, 770 tiles, 26.1 / 21.8; 49280 columns in fp32)
   const long long tiles = (static_cast<long long>(d->m) + 127) / 128 * ((static_cast<long long>(d->n) + 127) / 128);
   if (d->impl == SVLA_LINEAR_MANY || (d->impl == SVLA_LINEAR_AUTO && d->m > 128 && tiles > sm_count())) return launch_many<T, GATED>(a, d, st);
   if (d->m <= 16) return launch_few<T, 16, GATED>(a, d, st);

@@ -9,7 +9,7 @@
 // tile) and up to MT tokens its N side: no tensor time goes into empty rows, a lane of tensor memory is an output channel, and
 // a token's outputs leave in whole lines.  Where the tiles are fewer than the SMs, a cluster of up to 8 CTAs shares a tile's K
 // and adds its parts through distributed shared memory; whole numbers, so the order does not matter.  64 x 49280 x 960 to fp32:
-// 13.8 us, 4.4 TB/s (385 tiles in one round of three CTAs per SM; 27 us with 4 epilogue warps and two CTAs); one row by 1600 x 960:
+// 13.7 us, 4.4 TB/s (385 tiles in one round of three CTAs per SM; 27 us with 4 epilogue warps and two CTAs); one row by 1600 x 960:
 // 3.9 us, of which the launch is 2.
 //
 // Many rows (linear_i8_many_kernel).  Bound by the tensor pipe: CTA pairs compute 256 tokens x 256 weights (cta_group::2), which
@@ -17,9 +17,11 @@
 // arrive at 64 bytes a cycle.  Persistent, accumulators double-buffered (all 512 columns), 8 epilogue warps for each.  Outputs leave through
 // shared memory and TMA stores: written by the threads that own a row each, every warp's store touches 32 lines, and the stores'
 // way through L1 took 8000 cycles per tile.
-// 8192 x 4096 x 11008: 231 us, 3.2 POPS (275 back to back, under the power cap); 11328 x 2560 x 960, gated: 48 us, 2.3 POPS: a
-// tile has 8 slices of K only, and its epilogue (two int32 conversions, an exponential and a reciprocal per output) holds the
-// accumulator as long again (K = 128: 32 us).
+// 8192 x 4096 x 11008: 220 us, 3.3 POPS; in fp16 with a residual 241, called again and again, under the power cap, 286.
+// 11328 x 2560 x 960, gated: 47 us, 2.4 POPS, 31.5 with K = 128: a tile has 8 slices of K only, and its epilogue holds the accumulator
+// longer than they take.  No pipe is at its limit there (tensor 54%, issue slots 49%, exponentials and reciprocals 32%): a warp waits
+// for its columns, works, waits for its box to be read.  Not gated, where outputs are twice as many per tile: 11328 x 960 x 960 16.8 us,
+// 1600 columns 24.4, 2560 31.5 (2.43, 4.26 and 6.08 tiles per pair, in 3, 5 and 7 rounds).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -313,8 +315,8 @@ __global__ void __launch_bounds__(li8::kFewThreads) linear_i8_few_kernel(const _
 
 namespace li8 {
 struct Many {
-  // A CTA's rows of x and its half of w.  A stage more is worth more than a second box per warp: K = 11008 in 236 us, with 4
-  // stages and two boxes 256 (K = 960, gated: 48 either way)
+  // A CTA's rows of x and its half of w.  A stage more is worth more than a second box per warp (4 stages and two boxes
+  // took 8% longer with K = 11008, as long with K = 960, gated)
   static constexpr int kStages = 5, kTile = 128 * kSlice, kStage = 2 * kTile;
   static constexpr int kOut = kStages * kStage, kBoxBytes = 2048;  // each epilogue warp's box of 32 rows x 64 bytes
   static constexpr int kBar = kOut + 16 * kBoxBytes;
@@ -420,7 +422,8 @@ __global__ void __launch_bounds__(li8::kManyThreads, 1) linear_i8_many_kernel(co
     }
   } else {
     // Warps 2-9 take the even tiles and 10-17 the odd ones, so that one half's exponentials run beside the other's stores; of a
-    // tile, two warps per lane quarter have half of the columns each
+    // tile, two warps per lane quarter have half of the columns each.  (Gated products gain by it, 68 us to 49 when it was
+    // brought in; plain ones of short K lose: 11328 x 5120 x 128 took 37.7 us with all 16 warps on a tile and takes 40.7.)
     const int q = warp & 3, part = ((warp - 2) / 4) & 1, half = (warp - 2) / 8;
     constexpr int kCols = kOutCols / 2, kChunk = GATED ? 16 : 32, kBox = kBoxCols<T>, kPer = 16 / static_cast<int>(sizeof(T));
     float* consts = reinterpret_cast<float*>(smem + C::kConst) + (warp - 2) * 256;  // scales, then biases or ups' scales

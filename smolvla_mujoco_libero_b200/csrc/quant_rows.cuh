@@ -9,8 +9,9 @@
 // for its next row before it works on this one.  Instructions come next: pairs of elements go through the packed fp32 pipe (with
 // scalar operations 8192 rows of 4096 with everything took 53 instructions an element and 73 us).
 //
-// Measured: 11328 rows of 960, residual and RMSNorm, 18.5 us (5.3 TB/s); 8192 of 4096, residual and LayerNorm, 54 us (5.6 TB/s,
-// issue slots 68%); 11328 of 2560, smoothed, 31 us (4.6 TB/s, three bytes written for two read; the same without the reciprocals).
+// Measured: 11328 rows of 960, residual and RMSNorm, 17.7 us (5.5 TB/s); 8192 of 4096, residual and LayerNorm, 53 us (5.7 TB/s,
+// issue slots 71%); 11328 of 2560, smoothed, 31.3 us (4.6 TB/s): without the smoothing it takes 25.0, with a product in the
+// quotients' place 26.6, and with the divisors held in registers from row to row 38.
 //
 // Sums and statistics in fp32, of the unrounded h.  Quotients are correctly rounded (quotient() below), so without a norm the
 // codes are those of the definition bit for bit.  A row that holds no finite maximum (an infinity, a NaN) has scale NaN and codes 0:
@@ -84,7 +85,8 @@ __device__ __forceinline__ uint4 pack8(const float2 (&v)[4]) {
 
 // A warp's 256 elements of a row from column c0 on.  VEC: 16 bytes a lane.  Otherwise (k no multiple of 8, or rows that are
 // not 16-byte aligned) the 4-byte words that hold them, a word per lane after the other, and through shared memory to the lanes
-// that own them (11328 rows of 2561 with residual and RMSNorm: 108 us; 185 with words taken by the lanes that own them; 2560: 47).
+// that own them (11328 rows of 2561 with residual and RMSNorm: 116 us; 2560: 47.6; words taken by the lanes that own them took 1.7
+// times as long).
 template <typename T, bool VEC>
 struct Piece;
 template <typename T>

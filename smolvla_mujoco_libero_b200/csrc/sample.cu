@@ -19,9 +19,9 @@ int32_t launch_sample(SampleArgs& a, cudaStream_t st) {
   auto bytes = [](int words) { return static_cast<int>(sizeof(sample::Shared)) + words * sample::kThreads * 4; };
   if (int32_t rc = allow_smem(kern, bytes(words(kSampleVocab, sample::kMaxCtas)), configured)) return rc;
   // CTAs of about a thousand tokens or more each, up to 8, which is the fastest for what fits the GPU at once (one row of 49280
-  // tokens with top_k and top_p: 12.6 us, 13.8 with 4, 17.4 with 2); many rows have less to begin, to tell one another and to join
-  // with as few as leave three CTAs to an SM (256 mixed rows in fp32: 45 us with 4, 62 with 2, 66 with 8; 512 rows without filters
-  // in bf16: 46 with 2, 50 with 4, 73 with 8)
+  // tokens with top_k and top_p: 12.8 us, 14.7 with 4, 18.9 with 2; 64 bf16 rows of 131072 with top_p: 60.4, 66.3 with 4); many rows
+  // have less to begin, to tell one another and to join with as few as leave three CTAs to an SM (256 mixed rows in fp32: 45 us
+  // with 4, 62 with 2, 54 with 8; 512 rows without filters in bf16: 44 with 2, 49 with 4, 69 with 8)
   int ctas = 1;
   while (ctas < sample::kMaxCtas && a.vocab > 1024 * ctas) ctas *= 2;
   if (2ll * a.batch > sm_count())

@@ -20,7 +20,7 @@
 // exponent, 2^(f / 64) by the polynomial of degree 4 through Chebyshev's points (4.9e-15 relative, a twelfth of a unit at the
 // most likely token): 10 operations in 64 bits, of which an SM does 64 a cycle.
 //
-// Measured: one row of 49280, top_k and top_p, 12.6 us; 256 rows with settings of their own 45; 512 rows (bf16) without filters
+// Measured: one row of 49280, top_k and top_p, 12.8 us; 256 rows with settings of their own 45; 512 rows (bf16) without filters
 // 44; 64 rows of 131072 (bf16), top_p keeping thousands, 60.  A CTA's life is a chain of load, joins between CTAs and scans
 // with 2 to 4 CTAs per SM to fill it: issue slots are 40 to 50% busy, the 64-bit pipe 33% without filters.
 #pragma once

@@ -442,7 +442,7 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tens
                   top_k: torch.Tensor | int | None = None, top_p: torch.Tensor | float | None = None,
                   min_p: torch.Tensor | float | None = None, tokens: torch.Tensor | None = None,
                   logprob: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-    """One token per row of logits [batch, vocab] (bf16, fp16 or fp32, any row stride), drawn with u [batch] (fp32 in [0, 1]), and
+    """One token per row of logits [batch, vocab] (bf16, fp16 or fp32, rows any distance apart, not overlapping), drawn with u [batch] (fp32 in [0, 1]), and
     its log-probability among the tokens that the settings keep: (int32 [batch], fp32 [batch]).  Settings are fp32 (``top_k``:
     int32) tensors [batch], numbers for all rows, or None; temperature 0 takes the largest logit.  svla.h has the definition.  Rows
     without a finite largest logit, and settings that are none, give token -1 and NaN."""
